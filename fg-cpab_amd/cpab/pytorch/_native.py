@@ -19,6 +19,7 @@ _lib = None
 _load_error = None
 
 _c_int, _c_i64, _c_f32, _c_vp = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
+_c_f64 = ctypes.c_double
 
 # name -> (restype, argtypes); must match include/cpab_hip.h
 _SIGNATURES = {
@@ -75,6 +76,24 @@ _SIGNATURES = {
     "cpab_interp_backward_workspace_size": (_c_i64, [_c_int, _c_i64, _c_i64, _c_vp]),
     "cpab_interp_backward_ws": (_c_int, [_c_int, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp,
                                          _c_vp, _c_vp, _c_vp, _c_i64, _c_vp]),
+    "cpab_recurrence_carries": (_c_i64, [_c_int, _c_i64, _c_i64, _c_i64]),
+    "cpab_recurrence_workspace_size": (_c_i64, [_c_int, _c_i64, _c_i64, _c_i64, _c_int]),
+    "cpab_recurrence_forward": (_c_int, [_c_int, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp, _c_vp,
+                                         _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64,
+                                         _c_vp]),
+    "cpab_recurrence_backward": (_c_int, [_c_int, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp,
+                                          _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_vp,
+                                          _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_vp]),
+    "cpab_rms_norm_forward": (_c_int, [_c_int, _c_int, _c_int, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp,
+                                       _c_i64, _c_vp, _c_f32, _c_vp, _c_vp, _c_vp, _c_vp]),
+    "cpab_rms_norm_e4m3": (_c_int, [_c_int, _c_int, _c_int, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp,
+                                    _c_i64, _c_vp, _c_f32, _c_vp, _c_vp, _c_vp, _c_vp]),
+    "cpab_rms_norm_backward_workspace_size": (_c_i64, [_c_i64, _c_i64]),
+    "cpab_rms_norm_backward": (_c_int, [_c_int, _c_int, _c_int, _c_i64, _c_i64, _c_vp, _c_i64,
+                                        _c_vp, _c_vp, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp,
+                                        _c_vp, _c_vp, _c_i64, _c_vp]),
+    "cpab_adamw_step": (_c_int, [_c_int, _c_int, _c_i64, _c_vp, _c_i64, _c_f64, _c_f64, _c_f64,
+                                 _c_f64, _c_f64, ctypes.c_uint32, _c_vp]),
 }
 
 

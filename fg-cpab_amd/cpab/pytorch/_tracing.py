@@ -31,13 +31,17 @@ class _Recorded(torch.autograd.Function):
             ctx.args = [a.detach().requires_grad_(need) if isinstance(a, torch.Tensor) else a
                         for a, need in zip(args, ctx.needs_input_grad[1:])]
             ctx.out = function(*ctx.args)
-        return ctx.out.detach()
+        if isinstance(ctx.out, torch.Tensor):
+            return ctx.out.detach()
+        return tuple(o.detach() for o in ctx.out)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
+    def backward(ctx, *grads):
         wanted = [i for i, need in enumerate(ctx.needs_input_grad[1:]) if need]
-        grads = torch.autograd.grad(ctx.out, [ctx.args[i] for i in wanted], grad,
-                                    retain_graph=True, allow_unused=True)
+        outs = (ctx.out,) if isinstance(ctx.out, torch.Tensor) else ctx.out
+        kept = [(o, g) for o, g in zip(outs, grads) if o.requires_grad]
+        grads = torch.autograd.grad([o for o, _ in kept], [ctx.args[i] for i in wanted],
+                                    [g for _, g in kept], retain_graph=True, allow_unused=True)
         found = dict(zip(wanted, grads))
         return (None, *(found.get(i) for i in range(len(ctx.args))))

@@ -19,11 +19,12 @@
 
 #include "../../include/cpab_hip.h"
 #include "cpab_device.hpp"
+#include "capi_common.hpp"
 #include "cpab_launch.hpp"
 
-namespace {
+namespace cpab {
 
-thread_local std::string g_last_error;
+static thread_local std::string g_last_error;
 
 int fail(int code, const char* fmt, ...) {
   char buf[1024];
@@ -39,6 +40,14 @@ int check_hip(hipError_t e, const char* what) {
   if (e == hipSuccess) return CPAB_OK;
   return fail(CPAB_ERR_DEVICE, "%s: HIP error %d (%s)", what, (int)e, hipGetErrorString(e));
 }
+
+}  // namespace cpab
+
+namespace {
+
+using cpab::check_hip;
+using cpab::fail;
+using cpab::g_last_error;
 
 struct DeviceInfo {
   int cus = 0;
@@ -109,17 +118,6 @@ int check_points(int64_t nP, int64_t n_theta, int ndim) {
   (void)ndim;
   return CPAB_OK;
 }
-
-#define CPAB_REQUIRE(ptr) \
-  do { if (!(ptr)) return fail(CPAB_ERR_INVALID, "%s must not be NULL", #ptr); } while (0)
-
-// Per-cell tables are read as 8- and 16-byte vectors; every float array must
-// be at least float-aligned.
-#define CPAB_ALIGNED(ptr, bytes)                                                      \
-  do {                                                                                \
-    if ((ptr) && (reinterpret_cast<uintptr_t>(ptr) % (bytes)) != 0)                  \
-      return fail(CPAB_ERR_INVALID, "%s must be %d-byte aligned", #ptr, (int)(bytes)); \
-  } while (0)
 
 // ---- launch-shape policy ---------------------------------------------------
 // Fixed per problem shape and device (CU count, LDS per workgroup); each
@@ -662,6 +660,8 @@ int image_shape(int ndim, int64_t n_batch, int64_t C, const int64_t* in_size,
 
 }  // namespace
 
+int cpab::compute_units() { return device_info().cus; }
+
 extern "C" {
 
 const char* cpab_last_error_string(void) { return g_last_error.c_str(); }
@@ -670,8 +670,8 @@ const char* cpab_last_error_string(void) { return g_last_error.c_str(); }
 // (cpab_backward_project; projection arguments of the chain and
 // transform_data backwards).  200: the fused transform_data entry points take
 // the uniform grid's per-axis coordinates instead of the meshgrid.  402:
-// cpab_transform_data_backward_data.
-int cpab_abi_version(void) { return 402; }
+// cpab_transform_data_backward_data.  403: the operators around the transform.
+int cpab_abi_version(void) { return 403; }
 
 int cpab_affine(int ndim, int64_t n_theta, int nC, int d, const float* theta,
                 const int32_t* row_ptr, const int32_t* col_idx, const float* vals, float* As,

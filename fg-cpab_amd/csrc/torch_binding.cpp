@@ -8,61 +8,11 @@
 // of 16 x 10,000 1D points (35 us of kernels) took 122 us with the functions as
 // torch.autograd.Function over ctypes and takes 67 here; 32 x 784 2D points 132
 // and 75, 16 x 60,001 2D points in 20 steps 137 and 90.
-#include <torch/extension.h>
-
-#include <ATen/ops/empty.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPCachingAllocator.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-
-#include <sstream>
-#include <stdexcept>
-#include <string>
-#include <vector>
-
-#include "cpab_hip.h"
+#include "torch_common.hpp"
 
 namespace {
 
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
-[[noreturn]] void fail(const std::string& msg) { throw std::runtime_error(msg); }
-
-void check(int rc, const char* what) {
-  if (rc != 0) fail(std::string(what) + " failed: " + cpab_last_error_string());
-}
-
-std::string shape_of(const Tensor& t) {   // as str(tuple(t.shape))
-  std::ostringstream s;
-  s << "(";
-  for (int64_t k = 0; k < t.dim(); ++k) s << (k ? ", " : "") << t.size(k);
-  s << (t.dim() == 1 ? ",)" : ")");
-  return s.str();
-}
-
-std::string dtype_of(const Tensor& t) {
-  return std::string("torch.") + c10::getDtypeNames(t.scalar_type()).first;
-}
-
-const float* in(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
-float* out(Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
-
-Tensor empty(at::IntArrayRef size, const Tensor& like) {
-  return at::empty(size, at::TensorOptions().device(like.device()).dtype(at::kFloat));
-}
-
-// Device memory used by this call alone: back in torch's caching allocator,
-// for work queued behind it on the current stream, when the call returns.
-at::DataPtr scratch(int64_t bytes) {
-  return c10::hip::HIPCachingAllocator::get()->allocate((size_t)(bytes > 0 ? bytes : 1));
-}
-
-void* stream_of(const Tensor& t) {
-  return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream();
-}
+using namespace cpab_torch;
 
 // The tables of basis_tables() (transformer.py) and the solver's parameters as
 // they are at the call; kept from forward to backward.
@@ -125,19 +75,6 @@ void keep(AutogradContext* ctx, const c10::intrusive_ptr<Call>& c) {
       c10::IValue::make_capsule(c10::static_intrusive_pointer_cast<torch::CustomClassHolder>(c));
 }
 
-// torch.autograd.function.once_differentiable: the gradients cannot be
-// differentiated again.
-variable_list once(variable_list grads, const Tensor& grad_out) {
-  if (!at::GradMode::is_enabled() || !grad_out.requires_grad()) return grads;
-  for (Tensor& g : grads)
-    if (g.defined()) g = g.detach().set_requires_grad(true);
-  torch::autograd::DelayedError err(
-      "trying to differentiate twice a function that was marked with @once_differentiable",
-      (int64_t)grads.size());
-  return err.apply(std::move(grads));
-}
-
-Tensor plain(const Tensor& t) { return t.detach().contiguous(); }
 Tensor grad_of(const Tensor& g) { return g.detach().to(at::kFloat).contiguous(); }
 
 // Shape and type checks shared by the point transforms; theta of one stage.
@@ -455,9 +392,12 @@ Tensor interp(int64_t ndim, const Tensor& data, const Tensor& grid, std::vector<
 
 }  // namespace
 
+void sequence_functions(py::module& m);   // torch_sequence.cpp
+
 PYBIND11_MODULE(_cpab_torch, m) {
   m.def("grid", &grid);
   m.def("chain", &chain);
   m.def("image", &image);
   m.def("interp", &interp);
+  sequence_functions(m);
 }

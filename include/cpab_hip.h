@@ -48,7 +48,8 @@ const char* cpab_last_error_string(void);
 /* ABI version (major*100 + minor).  400: the transform_data entry points take
  * seed_grad.  401: the deterministic mode (cpab_set_deterministic and the
  * workspace sizes and cpab_interp_backward_ws that go with it).  402:
- * cpab_transform_data_backward_data. */
+ * cpab_transform_data_backward_data.  403: the operators around the transform
+ * (cpab_recurrence_*, cpab_rms_norm_*, cpab_adamw_step). */
 int cpab_abi_version(void);
 
 /* A = B theta per theta: As[b, r] = sum_k vals[k] * theta[b, col_idx[k]] over
@@ -344,6 +345,122 @@ int cpab_interp_backward_ws(int ndim, int64_t B, int64_t C, const int64_t* in_si
  * recorded launches of one kernel and forgets them. */
 void cpab_profile_enable(int on);
 int cpab_profile_read(const char* kernel, double* total_ms, int64_t* launches);
+
+/* ---------------------------------------------------------------------------
+ * Operators around the transform (no reference counterpart): the parts of a
+ * network that reads long signals and gives theta, and the step that moves its
+ * weights.  Their arrays hold 32-bit floats (CPAB_F32) or bfloat16 (CPAB_BF16)
+ * as `dtype` says, with no alignment beyond the type's; everything computed is
+ * held in 32 bits and rounded to the array's type when it is stored.  Nothing is
+ * allocated; a call with nothing to do returns CPAB_OK.
+ * ------------------------------------------------------------------------- */
+#define CPAB_F32 0
+#define CPAB_BF16 1
+
+/* Gated linear recurrence over B rows of T samples of C channels:
+ *   a_t = sigmoid(f_t),  h_t = a_t h_{t-1} + (1 - a_t) x_t,
+ *   y_t = h_t g_t sigmoid(g_t)   (y_t = h_t where g is NULL),
+ * for t < lengths[b] (T where lengths is NULL; clamped to [0, T]); behind a row's
+ * end y is 0, the state stays, and x, f and g are not used.  x, f, g: [B, T, C] at
+ * strides[0..5] (elements: x's over B and over T, then f's and g's), channels
+ * contiguous; h0 [B, C] float32, the state before the first sample (NULL: zeros);
+ * lengths [B] int32, or int64 where lengths64 is set; y [B, T, C] contiguous;
+ * h_last [B, C] float32, the state after each row's last sample.
+ * carries: NULL, or cpab_recurrence_carries(...) floats that the backward of the
+ * same sizes takes.  workspace: cpab_recurrence_workspace_size(...) bytes,
+ * 16-byte aligned. */
+int64_t cpab_recurrence_carries(int dtype, int64_t B, int64_t T, int64_t C);
+int64_t cpab_recurrence_workspace_size(int dtype, int64_t B, int64_t T, int64_t C, int backward);
+int cpab_recurrence_forward(int dtype, int64_t B, int64_t T, int64_t C, const void* x,
+                            const void* f, const void* g, const int64_t* strides,
+                            const float* h0, const void* lengths, int lengths64, void* y,
+                            float* h_last, float* carries, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
+/* Backward of cpab_recurrence_forward with the same x, f, g, strides, h0 and
+ * lengths and the carries that it wrote: grad_y [B, T, C] and grad_h_last [B, C]
+ * float32 (either may be NULL: zeros) give grad_x, grad_f, grad_g [B, T, C]
+ * contiguous and grad_h0 [B, C] float32 (each may be NULL; grad_g only with g). */
+int cpab_recurrence_backward(int dtype, int64_t B, int64_t T, int64_t C, const void* x,
+                             const void* f, const void* g, const int64_t* strides,
+                             const float* h0, const void* lengths, int lengths64,
+                             const float* carries, const void* grad_y, const float* grad_h_last,
+                             void* grad_x, void* grad_f, void* grad_g, float* grad_h0,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Root-mean-square norm of each of `rows` rows of C values, with the addition of
+ * the residual before it:
+ *   r = x + residual (x where residual is NULL),  s = 1 / sqrt(mean(r^2) + eps),
+ *   y = r s weight.
+ * x rows at x_stride elements, residual rows (of residual_dtype: dtype or
+ * CPAB_F32) at residual_stride; weight [C] of weight_dtype; y [rows, C]
+ * contiguous; residual_out [rows, C] contiguous of residual_dtype, r rounded to it
+ * (the norm is taken of r before that; NULL without a residual);
+ * rstd NULL or [rows]: s, which the backward takes. */
+int cpab_rms_norm_forward(int dtype, int residual_dtype, int weight_dtype, int64_t rows, int64_t C,
+                          const void* x, int64_t x_stride, const void* residual,
+                          int64_t residual_stride, const void* weight, float eps, void* y,
+                          void* residual_out, float* rstd, void* stream);
+
+/* The same with y in 8 bits: q [rows, C], OCP E4M3 values nearest to y / scale, and
+ * scale [rows] = max |y| / 448 over the row (1 where that is 0). */
+int cpab_rms_norm_e4m3(int dtype, int residual_dtype, int weight_dtype, int64_t rows, int64_t C,
+                       const void* x, int64_t x_stride, const void* residual,
+                       int64_t residual_stride, const void* weight, float eps, void* q,
+                       float* scale, void* residual_out, void* stream);
+
+/* Backward of cpab_rms_norm_forward: from r [rows, C] at r_stride (residual_out, of
+ * residual_dtype; x itself, of dtype, where there was no residual: pass
+ * residual_dtype = dtype), rstd, grad_y [rows, C] of dtype at grad_y_stride and
+ * grad_residual_out [rows, C] of residual_dtype at grad_residual_stride (NULL:
+ * zeros), with u = weight grad_y:
+ *   grad_r = s (u - r s^2 mean(u r)) + grad_residual_out,
+ * stored as grad_x (of dtype; may be NULL) and grad_residual (of residual_dtype;
+ * may be NULL), and grad_weight [C] of weight_dtype (may be NULL), the sum over
+ * the rows of grad_y r s in an order that depends on the sizes alone.
+ * workspace: cpab_rms_norm_backward_workspace_size(rows, C) bytes. */
+int64_t cpab_rms_norm_backward_workspace_size(int64_t rows, int64_t C);
+int cpab_rms_norm_backward(int dtype, int residual_dtype, int weight_dtype, int64_t rows, int64_t C,
+                           const void* r, int64_t r_stride, const float* rstd, const void* weight,
+                           const void* grad_y, int64_t grad_y_stride,
+                           const void* grad_residual_out, int64_t grad_residual_stride,
+                           void* grad_x, void* grad_residual, void* grad_weight, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/* One tensor of an AdamW step: n values of the parameter and its gradient (of the
+ * step's dtype), the first and second moments, and (may be NULL) the float32 master
+ * values that the step moves in the parameter's place, of which the parameter is
+ * then the rounding.  state_bits 32: exp_avg and exp_avg_sq are float32 [n], the
+ * scales unused.  state_bits 8: exp_avg holds the first moment and exp_avg_sq the
+ * second moment's square root as OCP E4M3 values [n], each 32 of them with one
+ * power-of-two scale (E8M0: 2^(byte - 127)) in exp_avg_scale / exp_avg_sq_scale
+ * [ceil(n / 32)]. */
+typedef struct {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  void* exp_avg_scale;
+  void* exp_avg_sq_scale;
+  float* master;
+  int64_t n;
+} cpab_adamw_tensor;
+
+/* AdamW step number `step` (from 1) over n_tensors tensors (an array in host
+ * memory, read before the call returns):
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   p = p (1 - lr weight_decay)
+ *       - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps).
+ * 8-bit states: the scale of 32 values is the least power of two (from 2^-127)
+ * with max |x| <= 448 scale over those that are finite; x / scale is rounded up or
+ * down at random, in proportion, from 32 random bits for each value:
+ *   w = mix(i + key),  key = mix(mix(seed xor step * 0x9E3779B1) + tensor),
+ * i the value's index in its tensor, tensor the tensor's in the array; the moment
+ * adds the low 16 bits below the last place kept, and the root the high 16.  A
+ * root above 0 is at least the smallest positive code; what is not finite is NaN. */
+int cpab_adamw_step(int dtype, int state_bits, int64_t n_tensors, const cpab_adamw_tensor* tensors,
+                    int64_t step, double lr, double beta1, double beta2, double eps,
+                    double weight_decay, uint32_t seed, void* stream);
 
 #ifdef __cplusplus
 }
