@@ -26,8 +26,7 @@ int size_of(int dtype) { return dtype == CPAB_F32 ? 4 : 2; }
 #define CPAB_TRY(call) \
   do { const int rc_ = (call); if (rc_ != CPAB_OK) return rc_; } while (0)
 
-// Workgroups are counted in 32 bits: values of one array below 2^37, rows and
-// channels below 2^31.
+// Values of one array below 2^37, rows and channels below 2^31.
 constexpr int64_t kMaxValues = 1LL << 37, kMaxCount = (1LL << 31) - 1;
 
 int check_recurrence(int dtype, int64_t B, int64_t T, int64_t C) {
@@ -36,7 +35,8 @@ int check_recurrence(int dtype, int64_t B, int64_t T, int64_t C) {
     return fail(CPAB_ERR_INVALID, "negative size (B=%lld, T=%lld, C=%lld)", (long long)B,
                 (long long)T, (long long)C);
   if (B > kMaxCount || T > kMaxCount || C > kMaxCount ||
-      (double)B * (double)(T > 0 ? T : 1) * (double)C >= (double)kMaxValues)
+      (double)B * (double)(T > 0 ? T : 1) * (double)C >= (double)kMaxValues ||
+      (B > 0 && C > 0 && !cpab::recurrence_fits(dtype, B, T, C)))
     return fail(CPAB_ERR_INVALID, "recurrence of %lld x %lld x %lld values is too large",
                 (long long)B, (long long)T, (long long)C);
   return CPAB_OK;

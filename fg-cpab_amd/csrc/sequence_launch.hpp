@@ -18,6 +18,8 @@ struct Recurrence {
   const void* lengths;
   int lengths64;
 };
+// Whether the launches' lanes can be counted in 32 bits, as a grid's are.
+bool recurrence_fits(int dtype, int64_t B, int64_t T, int64_t C);
 int64_t recurrence_carries(int dtype, int64_t B, int64_t T, int64_t C);
 int64_t recurrence_workspace(int dtype, int64_t B, int64_t T, int64_t C, bool backward);
 hipError_t launch_recurrence_forward(int dtype, const Recurrence& r, void* y, float* h_last,
