@@ -36,7 +36,7 @@ int check_recurrence(int dtype, int64_t B, int64_t T, int64_t C) {
                 (long long)T, (long long)C);
   if (B > kMaxCount || T > kMaxCount || C > kMaxCount ||
       (double)B * (double)(T > 0 ? T : 1) * (double)C >= (double)kMaxValues ||
-      (B > 0 && C > 0 && !cpab::recurrence_fits(dtype, B, T, C)))
+      (B > 0 && C > 0 && !cpab::recurrence_fits(dtype, B, T, C, 0)))
     return fail(CPAB_ERR_INVALID, "recurrence of %lld x %lld x %lld values is too large",
                 (long long)B, (long long)T, (long long)C);
   return CPAB_OK;
@@ -54,7 +54,15 @@ int fill_recurrence(int dtype, int64_t B, int64_t T, int64_t C, const void* x, c
   *r = cpab::Recurrence{};
   r->B = B; r->T = T; r->C = C;
   r->x = x; r->f = f; r->g = g;
-  if (strides) {
+  if (strides && T > 0) {
+    int64_t most = 0;
+    for (int k = 0; k < (g ? 6 : 4); ++k) {
+      if (strides[k] < 0) return fail(CPAB_ERR_INVALID, "strides must not be negative");
+      if (k % 2 == 1 && strides[k] > most) most = strides[k];
+    }
+    if (!cpab::recurrence_fits(dtype, B, T, C, most))
+      return fail(CPAB_ERR_INVALID, "samples %lld values apart are too far for 32-bit offsets",
+                  (long long)most);
     r->xb = strides[0]; r->xt = strides[1];
     r->fb = strides[2]; r->ft = strides[3];
     if (g) { r->gb = strides[4]; r->gt = strides[5]; }

@@ -17,16 +17,18 @@ __device__ __forceinline__ T from_float(float v) {
   return (T)v;   // bfloat16: to nearest, ties to even
 }
 
-// sigmoid(v) and sigmoid(-v) = 1 - sigmoid(v), each to a few units in its last
-// place: with e = exp(-|v|) they are 1 / (1 + e) and e / (1 + e), and nothing is
-// subtracted from 1.
+// sigmoid(v) and sigmoid(-v) = 1 - sigmoid(v): with e = exp(-|v|) the smaller is
+// e / (1 + e), to a few units in its last place (and |v| units from the scaling of exp's
+// argument), and 1 less that the larger, off by half a unit and the smaller's share:
+// gates near 1, whose products run over hundreds of samples, come nearer so than by the
+// approximate reciprocal.
 struct Gate {
   float pos, neg;
 };
 __device__ __forceinline__ Gate sigmoids(float v) {
   const float e = __expf(-fabsf(v));
-  const float big = __builtin_amdgcn_rcpf(1.0f + e);
-  const float small = e * big;
+  const float small = e * __builtin_amdgcn_rcpf(1.0f + e);
+  const float big = 1.0f - small;
   return v < 0.0f ? Gate{small, big} : Gate{big, small};
 }
 

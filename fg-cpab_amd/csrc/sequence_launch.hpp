@@ -9,6 +9,8 @@
 
 namespace cpab {
 
+int compute_units();   // of the current device (capi.cpp)
+
 // Sizes and inputs of a gated recurrence; strides in elements.
 struct Recurrence {
   int64_t B, T, C;
@@ -18,8 +20,9 @@ struct Recurrence {
   const void* lengths;
   int lengths64;
 };
-// Whether the launches' lanes can be counted in 32 bits, as a grid's are.
-bool recurrence_fits(int dtype, int64_t B, int64_t T, int64_t C);
+// Whether the launches' lanes can be counted in 32 bits, as a grid's are, and a tile's
+// samples, at most `stride` values apart, be reached by offsets of 31.
+bool recurrence_fits(int dtype, int64_t B, int64_t T, int64_t C, int64_t stride);
 int64_t recurrence_carries(int dtype, int64_t B, int64_t T, int64_t C);
 int64_t recurrence_workspace(int dtype, int64_t B, int64_t T, int64_t C, bool backward);
 hipError_t launch_recurrence_forward(int dtype, const Recurrence& r, void* y, float* h_last,

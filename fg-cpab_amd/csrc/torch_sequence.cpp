@@ -19,10 +19,12 @@ bool has_type(const Tensor& t) {
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor of(const Maybe& t) { return t.has_value() ? *t : Tensor(); }
 
-// `t` with its last dimension contiguous, detached; no copy where it is already.
-Tensor rows_of(const Tensor& t) {
+// [B, T, C] with its channels contiguous, detached; no copy where they are already
+// (and its samples not so far apart that a tile's offsets pass 32 bits).
+Tensor samples_of(const Tensor& t) {
   const Tensor d = t.detach();
-  return d.dim() == 0 || d.size(-1) <= 1 || d.stride(-1) == 1 ? d : d.contiguous();
+  return (d.size(2) <= 1 || d.stride(2) == 1) && d.stride(1) <= (1 << 15) + 4 * d.size(2)
+             ? d : d.contiguous();
 }
 
 // A gradient as the kernels take it, or none.
@@ -62,7 +64,8 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
                                const Maybe& maybe_lengths, bool keep) {
     const c10::OptionalDeviceGuard guard(x_.device());
     const Tensor g_ = of(maybe_g), h0_ = of(maybe_h0), lengths = of(maybe_lengths);
-    const Tensor x = rows_of(x_), f = rows_of(f_), g = g_.defined() ? rows_of(g_) : Tensor();
+    const Tensor x = samples_of(x_), f = samples_of(f_),
+                 g = g_.defined() ? samples_of(g_) : Tensor();
     const Tensor h0 = h0_.defined() ? plain(h0_) : Tensor();
     const int64_t B = x.size(0), T = x.size(1), C = x.size(2);
     Tensor y = at::empty({B, T, C}, x.options()), h = empty({B, C}, x), carries;
