@@ -1,19 +1,28 @@
 // Root-mean-square norm with the residual's addition, to the input's type or to
 // 8 bits with a scale per row, and its gradient.
 //
-// s = 1 / sqrt(mean(r^2) + eps), y = r s w.  Backward, with u = w dy:
-//   dr = s (u - r s^2 mean(u r)) + dr_out,  dw = sum over rows of dy r s.
+// s = 1 / sqrt(mean(r^2) + eps), y = r s w.  Backward, with u = w dy and n = r s:
+//   dr = s (u - n mean(u n)) + dr_out,  dw = sum over rows of dy n.
+//
+// Bound by memory: each value is read once and written once.  A row is held in the
+// registers of `tpr` lanes (a power of two, so that a narrow row does not leave a wave
+// idle and a wide one is spread over many), in pieces of V neighbouring values (16
+// bytes); the sums go over the lanes by shuffles and, beyond a wave, LDS.  Rows wider
+// than the registers of the largest workgroup are read again from the cache instead.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
+#include "cpab_launch.hpp"
 #include "sequence_device.hpp"
 #include "sequence_launch.hpp"
 
 namespace cpab {
 namespace {
 
-constexpr int kLanes = 256;
+constexpr int kMaxLanes = 1024;   // of a workgroup
+constexpr int kMinBlock = 256;
 
 struct Sum {
   __device__ float operator()(float a, float b) const { return a + b; }
@@ -22,94 +31,374 @@ struct Max {   // a NaN stays
   __device__ float operator()(float a, float b) const { return a != a || a > b ? a : b; }
 };
 
-// The same value in every lane of the workgroup; `room` holds a float per wave.
+// The same value in each of a row's `tpr` lanes; `room` holds a float for each wave.
+// Called by every lane of the workgroup.
 template <typename Op>
-__device__ float over_workgroup(float v, float* room, Op op) {
-  for (int d = 1; d < 64; d *= 2) v = op(v, __shfl_xor(v, d));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = room[0];
-  for (int w = 1; w < (int)blockDim.x >> 6; ++w) v = op(v, room[w]);
+__device__ __forceinline__ float over_row(float v, int tpr, float* room, Op op) {
+  const int most = min(tpr, 64);
+  for (int d = 1; d < most; d *= 2) v = op(v, __shfl_xor(v, d));
+  if (tpr > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = v;
+    __syncthreads();
+    const int waves = tpr >> 6, first = (threadIdx.x >> 6) & ~(waves - 1);
+    v = room[first];
+    for (int w = 1; w < waves; ++w) v = op(v, room[first + w]);
+  }
   return v;
 }
 
-__device__ __forceinline__ uint8_t to_e4m3(float v) {   // |v| <= 448 or NaN
-  return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false) & 0xff);
+__device__ __forceinline__ uint32_t to_e4m3(float v) {   // |v| <= 448 or NaN
+  return __builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false) & 0xff;
+}
+// v / sc, inv = 1 / sc: the product's rounding taken back, so that what lies between two
+// 8-bit values falls to the nearer.
+__device__ __forceinline__ float divided(float v, float sc, float inv) {
+  const float z = v * inv;
+  return fmaf(fmaf(-z, sc, v), inv, z);
+}
+__device__ __forceinline__ float within_e4m3(float v) {
+  return fabsf(v) > 448.0f ? copysignf(448.0f, v) : v;
 }
 
-template <typename T, typename R, typename W>
-__global__ void __launch_bounds__(kLanes)
-rms_norm_forward_kernel(RmsNorm n, T* y, uint8_t* q, float* scale, R* residual_out, float* rstd) {
-  __shared__ float room[kLanes / 64];
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(n.x) + row * n.x_stride;
-  const R* res = n.residual ? static_cast<const R*>(n.residual) + row * n.residual_stride : nullptr;
-  const W* w = static_cast<const W*>(n.weight);
-  const auto value = [&](int64_t c) { return to_float(x[c]) + (res ? to_float(res[c]) : 0.0f); };
-  float sum = 0.0f;
-  for (int64_t c = threadIdx.x; c < n.C; c += kLanes) {
-    const float r = value(c);
-    sum = fmaf(r, r, sum);
+// V neighbouring values at any alignment of theirs.
+template <int BYTES, int ALIGN>
+struct Piece {
+  typedef uint32_t Wide __attribute__((ext_vector_type(BYTES >= 4 ? BYTES / 4 : 1)));
+  typedef typename std::conditional<BYTES >= 4, Wide, typename std::conditional<BYTES == 2, uint16_t, uint8_t>::type>::type Bits;
+  typedef Bits __attribute__((aligned(ALIGN))) Unit;
+};
+template <int V, typename T>
+__device__ __forceinline__ void load(const T* p, float out[V]) {
+  constexpr int kAll = V * (int)sizeof(T), kBytes = kAll < 16 ? kAll : 16, kEach = kBytes / (int)sizeof(T);
+  typedef Piece<kBytes, sizeof(T)> P;
+#pragma unroll
+  for (int k = 0; k < V / kEach; ++k) {
+    struct { T v[kEach]; } raw;
+    const typename P::Bits bits = reinterpret_cast<const typename P::Unit*>(p)[k];
+    __builtin_memcpy(&raw, &bits, sizeof(raw));
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) out[k * kEach + e] = to_float(raw.v[e]);
   }
-  sum = over_workgroup(sum, room, Sum());
-  const float s = 1.0f / sqrtf(sum / (float)n.C + n.eps);
-  if (rstd && threadIdx.x == 0) rstd[row] = s;
-  float inv = 0.0f;
-  if (q) {
-    float top = 0.0f;
-    for (int64_t c = threadIdx.x; c < n.C; c += kLanes)
-      top = Max()(fabsf(value(c) * s * to_float(w[c])), top);
-    top = over_workgroup(top, room, Max());
-    const float sc = top == 0.0f ? 1.0f : top / 448.0f;
-    if (threadIdx.x == 0) scale[row] = sc;
-    inv = 1.0f / sc;
+}
+template <int V, typename T>
+__device__ __forceinline__ void store(T* p, const float in[V]) {
+  constexpr int kAll = V * (int)sizeof(T), kBytes = kAll < 16 ? kAll : 16, kEach = kBytes / (int)sizeof(T);
+  typedef Piece<kBytes, sizeof(T)> P;
+#pragma unroll
+  for (int k = 0; k < V / kEach; ++k) {
+    struct { T v[kEach]; } raw;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) raw.v[e] = from_float<T>(in[k * kEach + e]);
+    typename P::Bits bits;
+    __builtin_memcpy(&bits, &raw, sizeof(raw));
+    reinterpret_cast<typename P::Unit*>(p)[k] = bits;
   }
-  for (int64_t c = threadIdx.x; c < n.C; c += kLanes) {
-    const float r = value(c), v = r * s * to_float(w[c]);
-    if (q) {
-      const float z = v * inv;
-      q[row * n.C + c] = to_e4m3(fabsf(z) > 448.0f ? copysignf(448.0f, z) : z);
-    } else {
-      y[row * n.C + c] = from_float<T>(v);
+}
+template <int V>
+__device__ __forceinline__ void store_e4m3(uint8_t* p, const float in[V]) {
+  if constexpr (V == 1) {
+    *p = (uint8_t)to_e4m3(in[0]);
+  } else {
+    typedef Piece<V, 1> P;
+    uint32_t words[V / 4];
+#pragma unroll
+    for (int k = 0; k < V / 4; ++k) {
+      int w = __builtin_amdgcn_cvt_pk_fp8_f32(in[4 * k], in[4 * k + 1], 0, false);
+      w = __builtin_amdgcn_cvt_pk_fp8_f32(in[4 * k + 2], in[4 * k + 3], w, true);
+      words[k] = (uint32_t)w;
     }
-    if (residual_out) residual_out[row * n.C + c] = from_float<R>(r);
+    typename P::Bits bits;
+    __builtin_memcpy(&bits, words, sizeof(words));
+    *reinterpret_cast<typename P::Unit*>(p) = bits;
   }
 }
 
-template <typename T, typename R, typename W>
-__global__ void __launch_bounds__(kLanes)
-rms_norm_backward_kernel(RmsNormGrad n, T* dx, R* dres) {
-  __shared__ float room[kLanes / 64];
-  const int64_t row = blockIdx.x;
-  const R* r = static_cast<const R*>(n.r) + row * n.r_stride;
-  const T* dy = static_cast<const T*>(n.grad_y) + row * n.grad_y_stride;
-  const R* dout = n.grad_out ? static_cast<const R*>(n.grad_out) + row * n.grad_out_stride : nullptr;
-  const W* w = static_cast<const W*>(n.weight);
-  const float s = n.rstd[row];
-  float sum = 0.0f;
-  for (int64_t c = threadIdx.x; c < n.C; c += kLanes)
-    sum = fmaf(to_float(dy[c]) * to_float(w[c]), to_float(r[c]) * s, sum);
-  const float mean = over_workgroup(sum, room, Sum()) / (float)n.C;
-  for (int64_t c = threadIdx.x; c < n.C; c += kLanes) {
-    const float u = to_float(dy[c]) * to_float(w[c]);
-    const float d = s * (u - to_float(r[c]) * s * mean) + (dout ? to_float(dout[c]) : 0.0f);
-    if (dx) dx[row * n.C + c] = from_float<T>(d);
-    if (dres) dres[row * n.C + c] = from_float<R>(d);
+// Where a lane's piece `k` lies.  The last piece of a row that V does not divide is moved
+// back to end with the row; `again` of its first values are another lane's too, and are
+// not summed a second time (stored they are, the same).  V <= C.
+struct Place {
+  int64_t at;
+  int again;   // V or more: no piece
+  __device__ Place(int k, int tpr, int lane, int V, int64_t C) {
+    const int64_t from = ((int64_t)k * tpr + lane) * V;
+    at = min(from, C - V);
+    again = (int)min(from - at, (int64_t)V);
+  }
+};
+
+template <typename T, typename R, typename W, bool EIGHT, int V, int CH>
+__global__ void __launch_bounds__(kMaxLanes)
+rms_norm_forward_kernel(RmsNorm n, T* y, uint8_t* q, float* scale, R* residual_out, float* rstd,
+                        int tpr) {
+  __shared__ float room[kMaxLanes / 64];
+  const int lane = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr;
+  const int per = blockDim.x / tpr;
+  const int64_t rounds = (n.rows + per - 1) / per;
+  float w[CH][V];
+#pragma unroll
+  for (int k = 0; k < CH; ++k) {
+    const Place p(k, tpr, lane, V, n.C);
+    if (p.again < V) load<V>(static_cast<const W*>(n.weight) + p.at, w[k]);
+  }
+  for (int64_t round = blockIdx.x; round < rounds; round += gridDim.x) {
+    const bool live = round * per + group < n.rows;
+    const int64_t row = min(round * per + group, n.rows - 1);
+    const T* x = static_cast<const T*>(n.x) + row * n.x_stride;
+    const R* res = static_cast<const R*>(n.residual) + row * n.residual_stride;
+    float r[CH][V];
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const Place p(k, tpr, lane, V, n.C);
+      if (p.again < V) load<V>(x + p.at, r[k]);
+    }
+    if (n.residual) {
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        const Place p(k, tpr, lane, V, n.C);
+        if (p.again >= V) continue;
+        float more[V];
+        load<V>(res + p.at, more);
+#pragma unroll
+        for (int e = 0; e < V; ++e) r[k][e] += more[e];
+      }
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const Place p(k, tpr, lane, V, n.C);
+      if (p.again >= V) continue;
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum += e >= p.again ? r[k][e] * r[k][e] : 0.0f;
+      if (residual_out && live) store<V>(residual_out + row * n.C + p.at, r[k]);
+    }
+    sum = over_row(sum, tpr, room, Sum());
+    const float s = 1.0f / sqrtf(sum / (float)n.C + n.eps);
+    if (rstd && live && lane == 0) rstd[row] = s;
+    float top = 0.0f;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const Place p(k, tpr, lane, V, n.C);
+      if (p.again >= V) continue;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        r[k][e] = r[k][e] * s * w[k][e];
+        if (EIGHT) top = Max()(fabsf(r[k][e]), top);
+      }
+      if (!EIGHT && live) store<V>(y + row * n.C + p.at, r[k]);
+    }
+    if (!EIGHT) continue;
+    top = over_row(top, tpr, room, Max());
+    const float sc = top == 0.0f ? 1.0f : top / 448.0f;
+    if (live && lane == 0) scale[row] = sc;
+    const float inv = 1.0f / sc;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const Place p(k, tpr, lane, V, n.C);
+      if (p.again >= V) continue;
+#pragma unroll
+      for (int e = 0; e < V; ++e) r[k][e] = within_e4m3(divided(r[k][e], sc, inv));
+      if (live) store_e4m3<V>(q + row * n.C + p.at, r[k]);
+    }
   }
 }
 
-// grad_weight, a lane per channel.
-template <typename T, typename R, typename W>
-__global__ void __launch_bounds__(kLanes) rms_norm_weight_kernel(RmsNormGrad n, W* dw) {
-  const int64_t c = blockIdx.x * (int64_t)kLanes + threadIdx.x;
-  if (c >= n.C) return;
-  const R* r = static_cast<const R*>(n.r) + c;
-  const T* dy = static_cast<const T*>(n.grad_y) + c;
+// Each workgroup takes every gridDim.x-th round of rows and adds up its part of dw in
+// registers; the parts, [gridDim.x, C], are joined by the next kernel in their order.
+template <typename T, typename R, typename W, int V, int CH>
+__global__ void __launch_bounds__(kMaxLanes)
+rms_norm_backward_kernel(RmsNormGrad n, T* dx, R* dres, float* parts, int tpr) {
+  __shared__ float room[kMaxLanes / 64];
+  extern __shared__ float sums[];   // [per - 1][tpr][CH][V], where rows share a workgroup
+  const int lane = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr;
+  const int per = blockDim.x / tpr;
+  const int64_t rounds = (n.rows + per - 1) / per;
+  float w[CH][V], dw[CH][V];
+#pragma unroll
+  for (int k = 0; k < CH; ++k) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) dw[k][e] = 0.0f;
+    const Place p(k, tpr, lane, V, n.C);
+    if (p.again < V) load<V>(static_cast<const W*>(n.weight) + p.at, w[k]);
+  }
+  for (int64_t round = blockIdx.x; round < rounds; round += gridDim.x) {
+    const bool live = round * per + group < n.rows;
+    const int64_t row = min(round * per + group, n.rows - 1);
+    const R* r = static_cast<const R*>(n.r) + row * n.r_stride;
+    const T* dy = static_cast<const T*>(n.grad_y) + row * n.grad_y_stride;
+    const R* dout = static_cast<const R*>(n.grad_out) + row * n.grad_out_stride;
+    const float s = n.rstd[row];
+    float v[CH][V], u[CH][V];
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const Place p(k, tpr, lane, V, n.C);
+      if (p.again >= V) continue;
+      load<V>(r + p.at, v[k]);
+      load<V>(dy + p.at, u[k]);
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const Place p(k, tpr, lane, V, n.C);
+      if (p.again >= V) continue;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[k][e] *= s;
+        if (live) dw[k][e] = fmaf(u[k][e], v[k][e], dw[k][e]);
+        u[k][e] *= w[k][e];
+        sum += e >= p.again ? u[k][e] * v[k][e] : 0.0f;
+      }
+    }
+    if (!dx && !dres) continue;
+    const float mean = over_row(sum, tpr, room, Sum()) / (float)n.C;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const Place p(k, tpr, lane, V, n.C);
+      if (p.again >= V || !live) continue;
+      float d[V] = {};
+      if (n.grad_out) load<V>(dout + p.at, d);
+#pragma unroll
+      for (int e = 0; e < V; ++e) d[e] += s * (u[k][e] - v[k][e] * mean);
+      if (dx) store<V>(dx + row * n.C + p.at, d);
+      if (dres) store<V>(dres + row * n.C + p.at, d);
+    }
+  }
+  if (!parts) return;
+  if (per > 1) {
+    // the other rows' lanes of the same channels, in their order
+    if (group > 0) {
+#pragma unroll
+      for (int k = 0; k < CH; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          sums[((group - 1) * CH * V + k * V + e) * tpr + lane] = dw[k][e];
+    }
+    __syncthreads();
+    if (group > 0) return;
+    for (int g = 0; g < per - 1; ++g)
+#pragma unroll
+      for (int k = 0; k < CH; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) dw[k][e] += sums[(g * CH * V + k * V + e) * tpr + lane];
+  }
+#pragma unroll
+  for (int k = 0; k < CH; ++k) {
+    const Place p(k, tpr, lane, V, n.C);
+    if (p.again < V) store<V>(parts + (int64_t)blockIdx.x * n.C + p.at, dw[k]);
+  }
+}
+
+// dw[c] = the sum of `count` parts.  A workgroup has 16 channels and 64 runs of parts,
+// joined over a wave's four and then the 16 waves.  Latency counts (4 MB of parts for
+// 32768 x 1024: 4.8 us with 64 channels and 16 runs).
+template <typename W>
+__global__ void __launch_bounds__(1024)
+rms_norm_weight_kernel(const float* parts, int count, int64_t C, W* dw) {
+  __shared__ float sums[16][16];
+  const int lane = threadIdx.x & 15, run = threadIdx.x >> 4;
+  const int64_t c = blockIdx.x * (int64_t)16 + lane;
   float sum = 0.0f;
-  for (int64_t row = 0; row < n.rows; ++row)
-    sum = fmaf(to_float(dy[row * n.grad_y_stride]), to_float(r[row * n.r_stride]) * n.rstd[row], sum);
+  if (c < C)
+#pragma unroll 8
+    for (int k = run; k < count; k += 64) sum += parts[k * C + c];
+  sum += __shfl_xor(sum, 16);
+  sum += __shfl_xor(sum, 32);
+  if ((run & 3) == 0) sums[run >> 2][lane] = sum;
+  __syncthreads();
+  if (run > 0 || c >= C) return;
+#pragma unroll
+  for (int k = 1; k < 16; ++k) sum += sums[k][lane];
   dw[c] = from_float<W>(sum);
+}
+
+// ---- rows of any width: read once for each sum and once for the result -------------
+
+template <typename T, typename R, typename W, bool EIGHT>
+__global__ void __launch_bounds__(kMaxLanes)
+rms_norm_wide_forward_kernel(RmsNorm n, T* y, uint8_t* q, float* scale, R* residual_out, float* rstd) {
+  __shared__ float room[kMaxLanes / 64];
+  const W* w = static_cast<const W*>(n.weight);
+  for (int64_t row = blockIdx.x; row < n.rows; row += gridDim.x) {
+    const T* x = static_cast<const T*>(n.x) + row * n.x_stride;
+    const R* res = n.residual ? static_cast<const R*>(n.residual) + row * n.residual_stride : nullptr;
+    const auto value = [&](int64_t c) { return to_float(x[c]) + (res ? to_float(res[c]) : 0.0f); };
+    float sum = 0.0f;
+    for (int64_t c = threadIdx.x; c < n.C; c += kMaxLanes) sum += value(c) * value(c);
+    sum = over_row(sum, kMaxLanes, room, Sum());
+    const float s = 1.0f / sqrtf(sum / (float)n.C + n.eps);
+    if (rstd && threadIdx.x == 0) rstd[row] = s;
+    float sc = 1.0f, inv = 1.0f;
+    if (EIGHT) {
+      float top = 0.0f;
+      for (int64_t c = threadIdx.x; c < n.C; c += kMaxLanes)
+        top = Max()(fabsf(value(c) * s * to_float(w[c])), top);
+      top = over_row(top, kMaxLanes, room, Max());
+      sc = top == 0.0f ? 1.0f : top / 448.0f;
+      if (threadIdx.x == 0) scale[row] = sc;
+      inv = 1.0f / sc;
+    }
+    for (int64_t c = threadIdx.x; c < n.C; c += kMaxLanes) {
+      const float r = value(c), v = r * s * to_float(w[c]);
+      if (EIGHT)
+        q[row * n.C + c] = (uint8_t)to_e4m3(within_e4m3(divided(v, sc, inv)));
+      else
+        y[row * n.C + c] = from_float<T>(v);
+      if (residual_out) residual_out[row * n.C + c] = from_float<R>(r);
+    }
+  }
+}
+
+// parts [gridDim.x, C]: this workgroup's rows' part of dw, zero before.
+template <typename T, typename R, typename W>
+__global__ void __launch_bounds__(kMaxLanes)
+rms_norm_wide_backward_kernel(RmsNormGrad n, T* dx, R* dres, float* parts) {
+  __shared__ float room[kMaxLanes / 64];
+  const W* w = static_cast<const W*>(n.weight);
+  float* part = parts ? parts + (int64_t)blockIdx.x * n.C : nullptr;
+  for (int64_t row = blockIdx.x; row < n.rows; row += gridDim.x) {
+    const R* r = static_cast<const R*>(n.r) + row * n.r_stride;
+    const T* dy = static_cast<const T*>(n.grad_y) + row * n.grad_y_stride;
+    const R* dout = n.grad_out ? static_cast<const R*>(n.grad_out) + row * n.grad_out_stride : nullptr;
+    const float s = n.rstd[row];
+    float sum = 0.0f;
+    for (int64_t c = threadIdx.x; c < n.C; c += kMaxLanes) {
+      const float g = to_float(dy[c]), v = to_float(r[c]) * s;
+      sum += g * to_float(w[c]) * v;
+      if (part) part[c] += g * v;   // the lane's own channels
+    }
+    if (!dx && !dres) continue;
+    const float mean = over_row(sum, kMaxLanes, room, Sum()) / (float)n.C;
+    for (int64_t c = threadIdx.x; c < n.C; c += kMaxLanes) {
+      const float u = to_float(dy[c]) * to_float(w[c]);
+      const float d = s * (u - to_float(r[c]) * s * mean) + (dout ? to_float(dout[c]) : 0.0f);
+      if (dx) dx[row * n.C + c] = from_float<T>(d);
+      if (dres) dres[row * n.C + c] = from_float<R>(d);
+    }
+  }
+}
+
+// How a launch lays rows on lanes.
+struct Layout {
+  int V, CH, tpr, block;
+  int64_t rounds;   // of rows, one workgroup each
+  bool wide;
+};
+Layout layout(int dtype, int64_t rows, int64_t C) {
+  Layout l;
+  l.V = dtype == CPAB_F32 ? 4 : 8;
+  if (C < l.V) l.V = 1;
+  const int64_t pieces = (C + l.V - 1) / l.V;
+  // two pieces a lane where there are that many (32768 x 1024 bfloat16, backward: 46.6 us,
+  // 51.3 with one, 144 with four, whose registers spill)
+  l.tpr = 8;
+  while (l.tpr < kMaxLanes && (int64_t)l.tpr * 2 < pieces) l.tpr *= 2;
+  const int64_t each = (pieces + l.tpr - 1) / l.tpr;
+  l.CH = each <= 1 ? 1 : each <= 2 ? 2 : 4;
+  l.wide = each > 4;
+  l.block = std::max(l.tpr, kMinBlock);
+  const int per = l.block / l.tpr;
+  l.rounds = (rows + per - 1) / per;
+  return l;
 }
 
 // f(T(), R(), W()) for the arrays' types.
@@ -120,35 +409,92 @@ void with_types(int dtype, int residual, int weight, F f) {
     return weight == CPAB_F32 ? f(bf16(), 0.0f, 0.0f) : f(bf16(), 0.0f, bf16());
   return weight == CPAB_F32 ? f(bf16(), bf16(), 0.0f) : f(bf16(), bf16(), bf16());
 }
+// f(V, CH) as constants.
+template <typename T, typename F>
+void with_layout(const Layout& l, F f) {
+  constexpr int V = 16 / (int)sizeof(T);
+  typedef std::integral_constant<int, V> Many;
+  typedef std::integral_constant<int, 1> One;
+  if (l.V == 1) return f(One(), One());   // C < V: at most 8 lanes' worth
+  if (l.CH == 1) return f(Many(), One());
+  if (l.CH == 2) return f(Many(), std::integral_constant<int, 2>());
+  f(Many(), std::integral_constant<int, 4>());
+}
+
+// Workgroups that take rounds of rows in turn, their weights in registers: `waves` to a
+// compute unit.  Forward 64, twice what runs at once (16384 x 8192 bfloat16 to 8 bits:
+// 186 us, 5.0 TB/s as a large copy; 218 with 32, 208 with a workgroup for each round);
+// backward 16 (32768 x 1024: 46.6 and 4.8 us for dw's parts, 51 and 4.0 with 12, 49 and
+// 8.2 with 32).
+int64_t workgroups(int64_t rounds, int block, int waves) {
+  return std::max<int64_t>(1, std::min<int64_t>(rounds, (int64_t)compute_units() * waves * 64 / block));
+}
 
 }  // namespace
 
 hipError_t launch_rms_norm_forward(const RmsNorm& n, void* y, float* scale, void* residual_out,
                                    float* rstd, hipStream_t st) {
+  const Layout l = layout(n.dtype, n.rows, n.C);
   with_types(n.dtype, n.residual_dtype, n.weight_dtype, [&](auto t, auto r, auto w) {
     typedef decltype(t) T;
     typedef decltype(r) R;
     typedef decltype(w) W;
-    rms_norm_forward_kernel<T, R, W><<<(unsigned)n.rows, kLanes, 0, st>>>(
-        n, scale ? nullptr : (T*)y, scale ? (uint8_t*)y : nullptr, scale, (R*)residual_out, rstd);
+    const auto out = [&](auto eight) {
+      constexpr bool E = decltype(eight)::value;
+      if (l.wide) {
+        rms_norm_wide_forward_kernel<T, R, W, E>
+            <<<(unsigned)workgroups(n.rows, kMaxLanes, 32), kMaxLanes, 0, st>>>(
+                n, (T*)y, (uint8_t*)y, scale, (R*)residual_out, rstd);
+        return;
+      }
+      with_layout<T>(l, [&](auto v, auto ch) {
+        rms_norm_forward_kernel<T, R, W, E, decltype(v)::value, decltype(ch)::value>
+            <<<(unsigned)workgroups(l.rounds, l.block, 64), l.block, 0, st>>>(
+                n, (T*)y, (uint8_t*)y, scale, (R*)residual_out, rstd, l.tpr);
+      });
+    };
+    scale ? out(std::true_type()) : out(std::false_type());
   });
   return hipGetLastError();
 }
 
-int64_t rms_norm_backward_workspace(int64_t, int64_t) { return 0; }
+// Workgroups of the backward: the fewer, the fewer parts of dw to join.
+static int64_t backward_parts(int dtype, int64_t rows, int64_t C) {
+  const Layout l = layout(dtype, rows, C);
+  return l.wide ? workgroups(rows, kMaxLanes, 16) : workgroups(l.rounds, l.block, 16);
+}
+
+int64_t rms_norm_backward_workspace(int64_t rows, int64_t C) {
+  return std::max(backward_parts(CPAB_F32, rows, C), backward_parts(CPAB_BF16, rows, C)) * C * 4;
+}
 
 hipError_t launch_rms_norm_backward(const RmsNormGrad& n, void* grad_x, void* grad_residual,
-                                    void* grad_weight, void*, hipStream_t st) {
+                                    void* grad_weight, void* workspace, hipStream_t st) {
+  const Layout l = layout(n.dtype, n.rows, n.C);
+  const int64_t count = backward_parts(n.dtype, n.rows, n.C);
+  float* parts = grad_weight ? static_cast<float*>(workspace) : nullptr;
+  if (parts && (l.wide || n.rows == 0)) {
+    const hipError_t e = launch_fill(parts, count * n.C, 0.0f, st);
+    if (e != hipSuccess) return e;
+  }
   with_types(n.dtype, n.residual_dtype, n.weight_dtype, [&](auto t, auto r, auto w) {
     typedef decltype(t) T;
     typedef decltype(r) R;
     typedef decltype(w) W;
-    if (grad_x || grad_residual)
-      rms_norm_backward_kernel<T, R, W><<<(unsigned)n.rows, kLanes, 0, st>>>(n, (T*)grad_x,
-                                                                            (R*)grad_residual);
-    if (grad_weight)
-      rms_norm_weight_kernel<T, R, W><<<(unsigned)((n.C + kLanes - 1) / kLanes), kLanes, 0, st>>>(
-          n, (W*)grad_weight);
+    if (n.rows > 0 && l.wide) {
+      rms_norm_wide_backward_kernel<T, R, W><<<(unsigned)count, kMaxLanes, 0, st>>>(
+          n, (T*)grad_x, (R*)grad_residual, parts);
+    } else if (n.rows > 0) {
+      with_layout<T>(l, [&](auto v, auto ch) {
+        constexpr int V = decltype(v)::value, CH = decltype(ch)::value;
+        const size_t lds = (size_t)(l.block / l.tpr - 1) * l.tpr * CH * V * 4;
+        rms_norm_backward_kernel<T, R, W, V, CH><<<(unsigned)count, l.block, lds, st>>>(
+            n, (T*)grad_x, (R*)grad_residual, parts, l.tpr);
+      });
+    }
+    if (parts)
+      rms_norm_weight_kernel<W><<<(unsigned)((n.C + 15) / 16), 1024, 0, st>>>(parts, (int)count, n.C,
+                                                                             (W*)grad_weight);
   });
   return hipGetLastError();
 }
