@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "sequence_device.hpp"
 #include "sequence_launch.hpp"
@@ -56,70 +57,176 @@ __device__ __forceinline__ float round_at_random(float a, uint32_t r) {
 __device__ __forceinline__ float from_e4m3(uint8_t v) {
   return __builtin_amdgcn_cvt_f32_fp8((int)v, 0);
 }
-// z an E4M3 value, or NaN.
-__device__ __forceinline__ uint8_t to_e4m3(float z) {
-  return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(z, z, 0, false) & 0xff);
-}
-
 // The weight after a step, from the new moments and the root of the second.
 __device__ __forceinline__ float moved(const AdamW& a, float w, float m, float root) {
   return w * a.decay - a.rate * m / (root * a.root + a.eps);
 }
 
-// A lane per value; 32 lanes share a scale.
-template <typename T, bool EIGHT>
-__global__ void __launch_bounds__(kLanes)
-adamw_kernel(cpab_adamw_tensor t, AdamW a, uint32_t key) {
-  const int64_t i = blockIdx.x * (int64_t)kLanes + threadIdx.x;
-  const bool in = i < t.n;
-  T* p = static_cast<T*>(t.param);
-  float g = 0.0f, m = 0.0f, v = 0.0f, w = 0.0f;
-  if (in) {
-    g = to_float(static_cast<const T*>(t.grad)[i]);
-    w = t.master ? t.master[i] : to_float(p[i]);
-    if (EIGHT) {
-      m = from_e4m3(static_cast<const uint8_t*>(t.exp_avg)[i]) *
-          power_of_two((int)static_cast<const uint8_t*>(t.exp_avg_scale)[i / kGroup] - 127);
-      v = from_e4m3(static_cast<const uint8_t*>(t.exp_avg_sq)[i]) *
-          power_of_two((int)static_cast<const uint8_t*>(t.exp_avg_sq_scale)[i / kGroup] - 127);
-      v *= v;
-    } else {
-      m = static_cast<const float*>(t.exp_avg)[i];
-      v = static_cast<const float*>(t.exp_avg_sq)[i];
-    }
+// N values at any alignment of theirs, N * sizeof(T) a power of two up to 16 bytes.
+template <typename T, int N>
+struct Pack {
+  static constexpr int kBytes = N * (int)sizeof(T);
+  typedef uint32_t Words __attribute__((ext_vector_type(kBytes / 4)));
+  typedef Words __attribute__((aligned(sizeof(T)))) Unit;
+  T v[N];
+  __device__ __forceinline__ static Pack load(const T* p) {
+    return __builtin_bit_cast(Pack, (Words)*reinterpret_cast<const Unit*>(p));
   }
+  __device__ __forceinline__ void store(T* p) const {
+    *reinterpret_cast<Unit*>(p) = __builtin_bit_cast(Words, *this);
+  }
+};
+
+constexpr int kEach = 4;                       // values of a lane
+constexpr int kSpan = kLanes * kEach;          // of a workgroup
+constexpr int kTensors = 48;                   // of a launch: 64 bytes of arguments each
+
+// The tensors of a launch and where each one's spans begin among the launch's.
+struct Batch {
+  cpab_adamw_tensor t[kTensors];
+  uint32_t first[kTensors + 1];
+  uint32_t ordinal;   // of the first tensor, in the step's list
+};
+
+// Four E4M3 values, or NaN.
+__device__ __forceinline__ Pack<uint8_t, kEach> pack_e4m3(const float z[kEach]) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], w, true);
+  return __builtin_bit_cast(Pack<uint8_t, kEach>, w);
+}
+
+// One value's step: the new moments, their root, and the moved weight.
+__device__ __forceinline__ void advance(const AdamW& a, float g, float& m, float& v, float& root,
+                                        float& w) {
   m = a.beta1 * m + a.rest1 * g;
   v = a.beta2 * v + a.rest2 * g * g;
-  const float root = sqrtf(v);
-  if (in) {
-    w = moved(a, w, m, root);
-    p[i] = from_float<T>(w);
-    if (t.master) t.master[i] = w;
+  root = sqrtf(v);
+  w = moved(a, w, m, root);
+}
+
+// A span of a tensor to a workgroup, four neighbouring values to a lane; eight lanes hold
+// the 32 that share a scale.
+template <typename T, bool EIGHT, bool MASTER>
+__global__ void __launch_bounds__(kLanes) adamw_kernel(Batch batch, int count, AdamW a) {
+  // the tensor of this span: the last that begins at or before it
+  int lo = 0, hi = count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (batch.first[mid] <= blockIdx.x) lo = mid; else hi = mid - 1;
   }
-  if (!EIGHT) {
-    if (in) {
-      static_cast<float*>(t.exp_avg)[i] = m;
-      static_cast<float*>(t.exp_avg_sq)[i] = v;
+  const cpab_adamw_tensor& t = batch.t[lo];
+  const int64_t at = (int64_t)(blockIdx.x - batch.first[lo]) * kSpan + threadIdx.x * kEach;
+  const int here = (int)max((int64_t)0, min((int64_t)kEach, t.n - at));   // values of this lane
+  T* p = static_cast<T*>(t.param) + at;
+  const T* gp = static_cast<const T*>(t.grad) + at;
+  float* wp = MASTER ? t.master + at : nullptr;
+  float g[kEach] = {}, w[kEach] = {}, m[kEach] = {}, v[kEach] = {}, root[kEach];
+  float* mp = static_cast<float*>(t.exp_avg) + at;
+  float* vp = static_cast<float*>(t.exp_avg_sq) + at;
+  uint8_t* m8 = static_cast<uint8_t*>(t.exp_avg) + at;
+  uint8_t* v8 = static_cast<uint8_t*>(t.exp_avg_sq) + at;
+  uint8_t* ms = static_cast<uint8_t*>(t.exp_avg_scale) + at / kGroup;
+  uint8_t* vs = static_cast<uint8_t*>(t.exp_avg_sq_scale) + at / kGroup;
+  if (here == kEach) {
+    const auto gs = Pack<T, kEach>::load(gp);
+    if (MASTER) {
+      const auto ws = Pack<float, kEach>::load(wp);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) w[e] = ws.v[e];
+    } else {
+      const auto ws = Pack<T, kEach>::load(p);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) w[e] = to_float(ws.v[e]);
     }
-    return;
+    if (EIGHT) {
+      const auto mq = Pack<uint8_t, kEach>::load(m8), vq = Pack<uint8_t, kEach>::load(v8);
+      const float mk = power_of_two((int)*ms - 127), vk = power_of_two((int)*vs - 127);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        m[e] = from_e4m3(mq.v[e]) * mk;
+        v[e] = from_e4m3(vq.v[e]) * vk;
+      }
+    } else {
+      const auto mq = Pack<float, kEach>::load(mp), vq = Pack<float, kEach>::load(vp);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) m[e] = mq.v[e], v[e] = vq.v[e];
+    }
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) g[e] = to_float(gs.v[e]);
+  } else if (here > 0) {   // a tensor's end
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      if (e >= here) continue;
+      g[e] = to_float(gp[e]);
+      w[e] = MASTER ? wp[e] : to_float(p[e]);
+      m[e] = EIGHT ? from_e4m3(m8[e]) * power_of_two((int)*ms - 127) : mp[e];
+      v[e] = EIGHT ? from_e4m3(v8[e]) * power_of_two((int)*vs - 127) : vp[e];
+    }
   }
-  const bool fine_m = fabsf(m) < INFINITY, fine_v = root < INFINITY;
-  float top_m = fine_m ? fabsf(m) : 0.0f, top_v = fine_v ? root : 0.0f;
-  for (int d = 1; d < kGroup; d *= 2) {
-    top_m = fmaxf(top_m, __shfl_xor(top_m, d));
-    top_v = fmaxf(top_v, __shfl_xor(top_v, d));
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    if (EIGHT) v[e] *= v[e];
+    advance(a, g[e], m[e], v[e], root[e], w[e]);
   }
-  if (!in) return;
-  const int km = scale_exponent(top_m), kv = scale_exponent(top_v);
-  const uint32_t bits = mix((uint32_t)i + key);
-  const float am = round_at_random(fabsf(m) * power_of_two(-km), bits & 0xffffu);
-  float av = round_at_random(root * power_of_two(-kv), bits >> 16);
-  if (root > 0.0f) av = fmaxf(av, 0.001953125f);
-  static_cast<uint8_t*>(t.exp_avg)[i] = to_e4m3(fine_m ? copysignf(am, m) : NAN);
-  static_cast<uint8_t*>(t.exp_avg_sq)[i] = to_e4m3(fine_v ? av : NAN);
-  if (i % kGroup == 0) {
-    static_cast<uint8_t*>(t.exp_avg_scale)[i / kGroup] = (uint8_t)(km + 127);
-    static_cast<uint8_t*>(t.exp_avg_sq_scale)[i / kGroup] = (uint8_t)(kv + 127);
+  Pack<T, kEach> po;
+  Pack<float, kEach> wo, mo, vo;
+  Pack<uint8_t, kEach> mq, vq;
+  int km = 0, kv = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e)
+    po.v[e] = from_float<T>(w[e]), wo.v[e] = w[e], mo.v[e] = m[e], vo.v[e] = v[e];
+  if (EIGHT) {
+    float top_m = 0.0f, top_v = 0.0f;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      top_m = fmaxf(top_m, fabsf(m[e]) < INFINITY ? fabsf(m[e]) : 0.0f);
+      top_v = fmaxf(top_v, root[e] < INFINITY ? root[e] : 0.0f);
+    }
+    for (int d = 1; d < kGroup / kEach; d *= 2) {
+      top_m = fmaxf(top_m, __shfl_xor(top_m, d));
+      top_v = fmaxf(top_v, __shfl_xor(top_v, d));
+    }
+    km = scale_exponent(top_m), kv = scale_exponent(top_v);
+    const float im = power_of_two(-km), iv = power_of_two(-kv);
+    const uint32_t key = mix(a.key + batch.ordinal + (uint32_t)lo);
+    float am[kEach], av[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const uint32_t bits = mix((uint32_t)at + e + key);
+      am[e] = copysignf(round_at_random(fabsf(m[e]) * im, bits & 0xffffu), m[e]);
+      av[e] = round_at_random(root[e] * iv, bits >> 16);
+      if (root[e] > 0.0f) av[e] = fmaxf(av[e], 0.001953125f);
+      if (!(fabsf(m[e]) < INFINITY)) am[e] = NAN;
+      if (!(root[e] < INFINITY)) av[e] = NAN;
+    }
+    mq = pack_e4m3(am);
+    vq = pack_e4m3(av);
+  }
+  if (here == kEach) {
+    po.store(p);
+    if (MASTER) wo.store(wp);
+    if (EIGHT) {
+      mq.store(m8);
+      vq.store(v8);
+    } else {
+      mo.store(mp);
+      vo.store(vp);
+    }
+  } else if (here > 0) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      if (e >= here) continue;
+      p[e] = po.v[e];
+      if (MASTER) wp[e] = wo.v[e];
+      if (EIGHT)
+        m8[e] = mq.v[e], v8[e] = vq.v[e];
+      else
+        mp[e] = mo.v[e], vp[e] = vo.v[e];
+    }
+  }
+  if (EIGHT && here > 0 && at % kGroup == 0) {
+    *ms = (uint8_t)(km + 127);
+    *vs = (uint8_t)(kv + 127);
   }
 }
 
@@ -129,19 +236,37 @@ uint32_t adamw_mix(uint32_t z) { return mix(z); }
 
 hipError_t launch_adamw(int dtype, int state_bits, int64_t n_tensors,
                         const cpab_adamw_tensor* tensors, const AdamW& a, hipStream_t s) {
-  for (int64_t k = 0; k < n_tensors; ++k) {
-    const cpab_adamw_tensor& t = tensors[k];
-    if (t.n == 0) continue;
-    const unsigned blocks = (unsigned)((t.n + kLanes - 1) / kLanes);
-    const uint32_t key = mix(a.key + (uint32_t)k);
-    if (dtype == CPAB_F32)
-      state_bits == 8 ? adamw_kernel<float, true><<<blocks, kLanes, 0, s>>>(t, a, key)
-                      : adamw_kernel<float, false><<<blocks, kLanes, 0, s>>>(t, a, key);
-    else
-      state_bits == 8 ? adamw_kernel<bf16, true><<<blocks, kLanes, 0, s>>>(t, a, key)
-                      : adamw_kernel<bf16, false><<<blocks, kLanes, 0, s>>>(t, a, key);
+  constexpr int64_t kMost = kAdamWMost / kSpan;   // a launch's lanes are counted in 32 bits
+  for (int64_t k = 0; k < n_tensors;) {
+    Batch batch;
+    batch.ordinal = (uint32_t)k;
+    const bool master = tensors[k].master != nullptr;
+    int count = 0;
+    int64_t spans = 0;
+    for (; k < n_tensors && count < kTensors && (tensors[k].master != nullptr) == master; ++k, ++count) {
+      const int64_t more = (tensors[k].n + kSpan - 1) / kSpan;
+      if (spans + more > kMost) break;
+      batch.t[count] = tensors[k];
+      batch.first[count] = (uint32_t)spans;
+      spans += more;
+    }
+    if (count == 0) return hipErrorInvalidValue;   // capi_sequence.cpp lets none so large in
+    if (spans == 0) continue;
+    const auto launch = [&](auto t, auto eight, auto with) {
+      adamw_kernel<decltype(t), decltype(eight)::value, decltype(with)::value>
+          <<<(unsigned)spans, kLanes, 0, s>>>(batch, count, a);
+    };
+    const auto masters = [&](auto t, auto eight) {
+      master ? launch(t, eight, std::true_type()) : launch(t, eight, std::false_type());
+    };
+    const auto states = [&](auto t) {
+      state_bits == 8 ? masters(t, std::true_type()) : masters(t, std::false_type());
+    };
+    dtype == CPAB_F32 ? states(0.0f) : states(bf16());
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
   }
-  return hipGetLastError();
+  return hipSuccess;
 }
 
 }  // namespace cpab

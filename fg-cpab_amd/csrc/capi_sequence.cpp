@@ -240,7 +240,7 @@ int cpab_adamw_step(int dtype, int state_bits, int64_t n_tensors, const cpab_ada
   bool any = false;
   for (int64_t k = 0; k < n_tensors; ++k) {
     const cpab_adamw_tensor& t = tensors[k];
-    if (t.n < 0 || t.n >= kMaxValues)
+    if (t.n < 0 || t.n > cpab::kAdamWMost)
       return fail(CPAB_ERR_INVALID, "tensor %lld has %lld values", (long long)k, (long long)t.n);
     if (t.n == 0) continue;
     any = true;

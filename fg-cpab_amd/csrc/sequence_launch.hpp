@@ -69,6 +69,7 @@ struct AdamW {
   float eps;
   uint32_t key;                       // mix(seed xor step * 0x9E3779B1)
 };
+constexpr int64_t kAdamWMost = (1LL << 34) - 1024;   // values of one tensor
 hipError_t launch_adamw(int dtype, int state_bits, int64_t n_tensors,
                         const cpab_adamw_tensor* tensors, const AdamW& a, hipStream_t s);
 uint32_t adamw_mix(uint32_t z);
