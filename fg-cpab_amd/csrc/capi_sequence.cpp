@@ -262,6 +262,7 @@ int cpab_adamw_step(int dtype, int state_bits, int64_t n_tensors, const cpab_ada
   a.rate = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
   a.root = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
   a.eps = (float)eps;
+  a.cached = true;
   a.key = cpab::adamw_mix(seed ^ ((uint32_t)step * 0x9E3779B1u));
   return check_hip(cpab::launch_adamw(dtype, state_bits, n_tensors, tensors, a, as_stream(stream)),
                    "cpab_adamw_step");

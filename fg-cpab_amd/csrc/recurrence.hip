@@ -42,8 +42,10 @@ namespace {
 constexpr int kBlock = 512;   // lanes of a workgroup, at most
 constexpr int kWindow = 64;   // tiles that a look-back sees: a lane of a wave to each
 
-// Samples of a lane: what registers hold at four waves to a SIMD.
-constexpr int forward_steps(int) { return 16; }
+// Samples of a lane: what registers hold at four waves to a SIMD; forward one, where the
+// samples are few and their latency counts (64 x 1 x 512 bfloat16: 6.0 us with 16).
+constexpr int kForwardSteps = 16, kFewSamples = 16;
+int forward_steps(int64_t T) { return T <= kFewSamples ? 1 : kForwardSteps; }
 constexpr int backward_steps(int V) { return 16 / V; }
 
 // How a launch cuts [B, T, C] into tiles.
@@ -231,7 +233,10 @@ __device__ __forceinline__ void store(T* base, uint32_t off, const float in[V]) 
   for (int v = 0; v < V; ++v) raw[v] = from_float<T>(in[v]);
   auto p = (__attribute__((address_space(1))) char*)base;
   asm volatile("" : "+s"(p));
-  *(__attribute__((address_space(1))) Unit*)(p + off) = __builtin_bit_cast(Unit, raw);
+  // past the second-level cache, which the inputs need (16 x 10,000 x 64 in 32 bits, forward
+  // and backward: 33 and 49 us, 39 and 58 through it)
+  __builtin_nontemporal_store((Unit)__builtin_bit_cast(Unit, raw),
+                              (__attribute__((address_space(1))) Unit*)(p + off));
 }
 
 // Bytes from a tile's first sample to channel c of its sample t; below 2^31
@@ -249,11 +254,10 @@ __device__ __forceinline__ unsigned take_tile(unsigned* counter, unsigned* room)
   return (unsigned)__builtin_amdgcn_readfirstlane((int)*room);
 }
 
-template <typename T, int V, bool GATE>
+template <typename T, int V, bool GATE, int L>
 __global__ void __launch_bounds__(kBlock, 4)
 recurrence_forward_kernel(Recurrence r, Tiling s, T* y, float* h_last, float* carries,
                           Tiling back, Word* words, unsigned* flags, unsigned* counter) {
-  constexpr int L = forward_steps(V);
   extern __shared__ char room[];
   __shared__ unsigned mine_of;
   __shared__ int nearest;
@@ -510,7 +514,7 @@ int channels(int dtype, int64_t C) { return dtype == CPAB_BF16 && C > 1 ? 2 : 1;
 
 Tiling tiling(int dtype, int64_t B, int64_t T, int64_t C, bool backward) {
   Tiling s;
-  const int V = channels(dtype, C), L = backward ? backward_steps(V) : forward_steps(V);
+  const int V = channels(dtype, C), L = backward ? backward_steps(V) : forward_steps(T);
   // 32 lanes of 4 bytes are a cache line across, and the more segments the fewer tiles
   // for a state to pass (one row of 131,072 x 512, bfloat16, forward: 147 us, 234 with 64
   // lanes, 159 with 16; 8 x 4096 x 1280 forward and backward 235, 232 and 300).
@@ -564,7 +568,7 @@ struct Room {
 bool recurrence_fits(int dtype, int64_t B, int64_t T, int64_t C, int64_t stride) {
   for (const bool backward : {false, true}) {
     const Tiling s = tiling(dtype, B, T, C, backward);
-    const int V = channels(dtype, C), L = backward ? backward_steps(V) : forward_steps(V);
+    const int V = channels(dtype, C), L = backward ? backward_steps(V) : forward_steps(T);
     if ((double)s.tiles * (double)s.across * (double)B * s.block >= 4294967296.0) return false;
     if (((double)s.segs * L * (double)std::max(stride, C) + (double)C) * 4 >= 2147483648.0) return false;
   }
@@ -588,9 +592,12 @@ hipError_t launch_recurrence_forward(int dtype, const Recurrence& r, void* y, fl
   const int V = channels(dtype, r.C);
   with_shape(dtype, V, r.g != nullptr, [&](auto t, auto vs, auto gate) {
     typedef decltype(t) T;
-    recurrence_forward_kernel<T, decltype(vs)::value, decltype(gate)::value>
-        <<<s.tiles * s.chains, s.block, lds_bytes(s, V), st>>>(r, s, (T*)y, h_last, carries, back,
-                                                          room.words, room.flags, room.counter);
+    constexpr int W = decltype(vs)::value;
+    constexpr bool G = decltype(gate)::value;
+    const auto k = forward_steps(r.T) == 1 ? recurrence_forward_kernel<T, W, G, 1>
+                                           : recurrence_forward_kernel<T, W, G, kForwardSteps>;
+    k<<<s.tiles * s.chains, s.block, lds_bytes(s, V), st>>>(r, s, (T*)y, h_last, carries, back,
+                                                            room.words, room.flags, room.counter);
   });
   return hipGetLastError();
 }

@@ -68,6 +68,7 @@ struct AdamW {
   float root;                         // 1 / sqrt(1 - beta2^step)
   float eps;
   uint32_t key;                       // mix(seed xor step * 0x9E3779B1)
+  bool cached;                        // the parameters are stored through the caches
 };
 constexpr int64_t kAdamWMost = (1LL << 34) - 1024;   // values of one tensor
 hipError_t launch_adamw(int dtype, int state_bits, int64_t n_tensors,
