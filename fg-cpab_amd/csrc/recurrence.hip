@@ -54,11 +54,13 @@ struct Tiling {
   unsigned tiles, across, chains;   // tiles along T and C; across * B
 };
 
-__device__ __forceinline__ int64_t row_length(const Recurrence& r, int64_t b) {
-  if (!r.lengths) return r.T;
-  const int64_t n = r.lengths64 ? static_cast<const int64_t*>(r.lengths)[b]
-                                : (int64_t)static_cast<const int32_t*>(r.lengths)[b];
-  return n < 0 ? 0 : (n > r.T ? r.T : n);
+// Samples of row b (T below 2^31), the same in every lane for the compiler too.
+__device__ __forceinline__ int row_length(const Recurrence& r, int64_t b) {
+  int64_t n = r.T;
+  if (r.lengths)
+    n = r.lengths64 ? static_cast<const int64_t*>(r.lengths)[b]
+                    : (int64_t)static_cast<const int32_t*>(r.lengths)[b];
+  return __builtin_amdgcn_readfirstlane((int)(n < 0 ? 0 : (n > r.T ? r.T : n)));
 }
 
 // ---- a tile's map or state as one 64-bit word ------------------------------------
@@ -76,6 +78,14 @@ __device__ __forceinline__ float word_B(Word w) { return __uint_as_float((uint32
 __device__ __forceinline__ float word_A(Word w) {
   return __uint_as_float((uint32_t)(w >> 32) & 0x7fffffffu);
 }
+// A barrier for what lanes hand each other in LDS: unlike __syncthreads it does not wait
+// for a wave's stores to memory.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 constexpr unsigned kHasMap = 1, kHasState = 2;   // a tile's flag
 template <typename W>
 __device__ __forceinline__ void publish(W* at, W w) {
@@ -93,70 +103,87 @@ struct Join {
   const Tiling& s;
   float2* agg;     // LDS [segs][lanes * V]: the segments' (A, B)
   Word* window;    // LDS [kWindow][lanes * V]: the tiles before, newest first
+  float* entry;    // LDS [lanes * V]: the state before the tile
   int* nearest;    // LDS: how many tiles back the nearest state is
   int seg, lane;
 
   __device__ Join(const Tiling& t, char* room, int* one, int sg, int ln)
       : s(t), agg(reinterpret_cast<float2*>(room)),
-        window(reinterpret_cast<Word*>(agg + t.segs * t.lanes * V)), nearest(one), seg(sg), lane(ln) {}
+        window(reinterpret_cast<Word*>(agg + t.segs * t.lanes * V)),
+        entry(reinterpret_cast<float*>(window + min(kWindow, (int)t.tiles) * t.lanes * V)),
+        nearest(one), seg(sg), lane(ln) {}
   __device__ float2& at(int sg, int v) const { return agg[(sg * s.lanes + lane) * V + v]; }
+  // f(k-th (A, B)) for `count` segments from `first` in steps of `dir`, read four ahead:
+  // a step waits for a multiplication then, and not for LDS (16 segments in 1.0 us).
+  template <typename F>
+  __device__ __forceinline__ void segments(int first, int count, int dir, F f) const {
+    for (int k = 0; k < count; k += 4) {
+      float2 m[4][V];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int v = 0; v < V; ++v) m[q][v] = at(first + min(k + q, count - 1) * dir, v);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (k + q < count) f(m[q]);
+    }
+  }
   // Of the whole tile, segments taken from `first` in steps of `dir`.
   __device__ void whole(int first, int dir, float A[V], float B[V]) const {
 #pragma unroll
     for (int v = 0; v < V; ++v) A[v] = 1.0f, B[v] = 0.0f;
-#pragma unroll 2
-    for (int k = 0, sg = first; k < s.segs; ++k, sg += dir)
+    segments(first, s.segs, dir, [&](const float2 m[V]) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float2 m = at(sg, v);
-        B[v] = fmaf(m.x, B[v], m.y);
-        A[v] *= m.x;
+        B[v] = fmaf(m[v].x, B[v], m[v].y);
+        A[v] *= m[v].x;
       }
+    });
   }
   // h: from the state before the tile to that before a segment, over `count` segments
   // from `first` in steps of `dir`.
   __device__ void to_segment(int first, int count, int dir, float h[V]) const {
-#pragma unroll 2
-    for (int k = 0, sg = first; k < count; ++k, sg += dir)
+    segments(first, count, dir, [&](const float2 m[V]) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float2 m = at(sg, v);
-        h[v] = fmaf(m.x, h[v], m.y);
-      }
+      for (int v = 0; v < V; ++v) h[v] = fmaf(m[v].x, h[v], m[v].y);
+    });
   }
   // h: the state before tile `number`, given as the state before tile 0.  (A, B): the
-  // tile's own, used in segment 0; `follows`: tiles come after it.  Tile k's words of this
-  // lane's channels at words[k * stride], its flag at flags[k].
+  // tile's own, used in segment 0; `follows`: tiles come after it.  The chain's flags and
+  // words, tile by tile: lanes' words next to each other, [tiles][V][lanes].
   __device__ void state_before(int number, bool follows, const float A[V], const float B[V],
-                               Word* words, int64_t stride, unsigned* flags, float h[V]) const {
+                               Word* words, unsigned* flags, float h[V]) const {
+    const auto word = [&](int tile, int v) {
+      return words + ((int64_t)tile * V + v) * s.lanes + lane;
+    };
     const bool first = threadIdx.x == 0;
     if (number > 0) {
       if (seg == 0 && follows) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) publish(words + number * stride + v, map_word(A[v], B[v]));
+        for (int v = 0; v < V; ++v) publish(word(number, v), map_word(A[v], B[v]));
         if (first) publish(flags + number, kHasMap);
       }
-      if (threadIdx.x < 64) {
+      if (threadIdx.x >= blockDim.x - 64) {   // the last wave, beside the first
         // lane k: the tile k + 1 before; what lies before tile 0 is not asked
-        const int mine = number - 1 - (int)threadIdx.x;
+        const int mine = number - 1 - (int)(threadIdx.x & 63);
         for (;;) {
           const unsigned f = mine >= 0 ? peek(flags + mine) : kHasMap;
           const uint64_t state = __ballot(f == kHasState), any = __ballot(f != 0);
           const int k = __builtin_ctzll(state | 1ull << 63);
           if ((state >> k & 1) && !(~any & ((1ull << k) - 1))) {
-            if (first) *nearest = k;
+            if ((threadIdx.x & 63) == 0) *nearest = k;
             break;
           }
           __builtin_amdgcn_s_sleep(2);
         }
       }
-      __syncthreads();
+      lds_barrier();
       const int k = *nearest;
       // the flags are no more than a hint: a word says itself what it is
       for (int q = seg; q <= k; q += s.segs)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          Word* at = words + (number - 1 - q) * stride + v;
+          Word* at = word(number - 1 - q, v);
           Word w = peek(at);
           while (w == 0 || (q == k && !is_state(w))) {
             __builtin_amdgcn_s_sleep(1);
@@ -164,21 +191,39 @@ struct Join {
           }
           window[(q * s.lanes + lane) * V + v] = w;
         }
-      __syncthreads();
+      lds_barrier();
+      // one segment's lanes apply them, for all
+      if (seg == 0) {
+        for (int q = k; q >= 0; q -= 4) {   // read four ahead, as segments()
+          Word w[4][V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = word_B(window[(k * s.lanes + lane) * V + v]);
-      for (int q = k - 1; q >= 0; --q)
+          for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          // a tile may have come to its state since: that is then the one to take
-          const Word w = window[(q * s.lanes + lane) * V + v];
-          h[v] = is_state(w) ? word_B(w) : fmaf(word_A(w), h[v], word_B(w));
+            for (int v = 0; v < V; ++v) w[e][v] = window[(max(q - e, 0) * s.lanes + lane) * V + v];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (e > q) continue;
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+              // a tile may have come to its state since: that is then the one to take
+              h[v] = is_state(w[e][v]) ? word_B(w[e][v])
+                                       : fmaf(word_A(w[e][v]), h[v], word_B(w[e][v]));
+          }
         }
+      }
+    }
+    if (number > 0) {
+      if (seg == 0)
+#pragma unroll
+        for (int v = 0; v < V; ++v) entry[lane * V + v] = h[v];
+      lds_barrier();
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[v] = entry[lane * V + v];
     }
     if (seg == 0 && follows) {
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        publish(words + number * stride + v, state_word(fmaf(A[v], h[v], B[v])));
+        publish(word(number, v), state_word(fmaf(A[v], h[v], B[v])));
       if (first) publish(flags + number, kHasState);
     }
   }
@@ -210,33 +255,35 @@ struct Raw {
     return raw;
   }
 };
-// `base` is the same for the workgroup's lanes and `off` a lane's 32-bit offset in
-// bytes.  The empty assembly keeps the base in scalar registers of its own: added up
-// before, each sample of each array would take two vector registers of addresses (170
-// for the backward where 106 do).
+// A pointer that is the same for the workgroup's lanes and walks from sample to sample;
+// a lane adds its 32-bit offset.
+template <typename T>
+struct Walk {
+  __attribute__((address_space(1))) char* p;
+  int64_t step;
+  __device__ __forceinline__ Walk(const T* from, int64_t stride)
+      : p((__attribute__((address_space(1))) char*)from), step(stride * (int64_t)sizeof(T)) {}
+  __device__ __forceinline__ void next() { p += step; }
+};
 template <typename T, int V>
-__device__ __forceinline__ Raw<T, V> load(const T* base, uint32_t off) {
+__device__ __forceinline__ Raw<T, V> load(const Walk<T>& w, uint32_t off) {
   typedef typename Raw<T, V>::Unit Unit;
-  auto p = (const __attribute__((address_space(1))) char*)base;
-  asm volatile("" : "+s"(p));
-  const typename Raw<T, V>::Bits bits = *(const __attribute__((address_space(1))) Unit*)(p + off);
+  const typename Raw<T, V>::Bits bits = *(const __attribute__((address_space(1))) Unit*)(w.p + off);
   Raw<T, V> raw;
 #pragma unroll
   for (int k = 0; k < Raw<T, V>::kWords; ++k) raw.w[k] = (uint32_t)((uint64_t)bits >> (32 * k));
   return raw;
 }
 template <typename T, int V>
-__device__ __forceinline__ void store(T* base, uint32_t off, const float in[V]) {
+__device__ __forceinline__ void store(const Walk<T>& w, uint32_t off, const float in[V]) {
   typedef typename Raw<T, V>::Unit Unit;
   T raw[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) raw[v] = from_float<T>(in[v]);
-  auto p = (__attribute__((address_space(1))) char*)base;
-  asm volatile("" : "+s"(p));
   // past the second-level cache, which the inputs need (16 x 10,000 x 64 in 32 bits, forward
   // and backward: 33 and 49 us, 39 and 58 through it)
   __builtin_nontemporal_store((Unit)__builtin_bit_cast(Unit, raw),
-                              (__attribute__((address_space(1))) Unit*)(p + off));
+                              (__attribute__((address_space(1))) Unit*)(w.p + off));
 }
 
 // Bytes from a tile's first sample to channel c of its sample t; below 2^31
@@ -248,10 +295,13 @@ __device__ __forceinline__ uint32_t offset(int t, int64_t stride, int64_t c) {
 
 // This workgroup's tile: by a ticket where tiles wait for others, else its index.
 __device__ __forceinline__ unsigned take_tile(unsigned* counter, unsigned* room) {
-  if (!counter) return blockIdx.x;
-  if (threadIdx.x == 0) *room = atomicAdd(counter, 1u);
-  __syncthreads();
-  return (unsigned)__builtin_amdgcn_readfirstlane((int)*room);
+  unsigned mine = blockIdx.x;
+  if (counter) {
+    if (threadIdx.x == 0) *room = atomicAdd(counter, 1u);
+    lds_barrier();
+    mine = *room;
+  }
+  return (unsigned)__builtin_amdgcn_readfirstlane((int)mine);
 }
 
 template <typename T, int V, bool GATE, int L>
@@ -274,16 +324,16 @@ recurrence_forward_kernel(Recurrence r, Tiling s, T* y, float* h_last, float* ca
     const int64_t ts = t0 + seg * L;
     const int rest = (int)min((int64_t)L, r.T - ts);   // of the lane's samples those in T,
     const int live = (int)min((int64_t)L, n - ts);     // and those in the row (none: <= 0)
-    T* out = y + (b * r.T + t0) * r.C;
+    Walk<T> out(y + (b * r.T + t0) * r.C, r.C);
     const uint32_t at = offset<T>(seg * L, r.C, c);
     // a tile that is whole, the usual one, needs no question at each sample
     const auto work = [&](auto whole) {
       constexpr bool full = decltype(whole)::value;
       float a[L][V], u[L][V];
       Raw<T, V> rf[L], rx[L], g[L];   // no sample: a gate that keeps the state
-      const T* x = static_cast<const T*>(r.x) + b * r.xb + t0 * r.xt;
-      const T* f = static_cast<const T*>(r.f) + b * r.fb + t0 * r.ft;
-      const T* gp = GATE ? static_cast<const T*>(r.g) + b * r.gb + t0 * r.gt : nullptr;
+      Walk<T> x(static_cast<const T*>(r.x) + b * r.xb + t0 * r.xt, r.xt);
+      Walk<T> f(static_cast<const T*>(r.f) + b * r.fb + t0 * r.ft, r.ft);
+      Walk<T> gp(GATE ? static_cast<const T*>(r.g) + b * r.gb + t0 * r.gt : nullptr, r.gt);
       const uint32_t atx = offset<T>(seg * L, r.xt, c), atf = offset<T>(seg * L, r.ft, c);
       const uint32_t atg = offset<T>(seg * L, r.gt, c);
 #pragma unroll
@@ -291,10 +341,12 @@ recurrence_forward_kernel(Recurrence r, Tiling s, T* y, float* h_last, float* ca
         rf[j] = Raw<T, V>::all(INFINITY);
         rx[j] = g[j] = Raw<T, V>::all(0.0f);
         if (full || j < live) {
-          rf[j] = load<T, V>(f + j * r.ft, atf);
-          rx[j] = load<T, V>(x + j * r.xt, atx);
-          if (GATE) g[j] = load<T, V>(gp + j * r.gt, atg);
+          rf[j] = load<T, V>(f, atf);
+          rx[j] = load<T, V>(x, atx);
+          if (GATE) g[j] = load<T, V>(gp, atg);
         }
+        f.next(), x.next();
+        if (GATE) gp.next();
       }
       float A[V], B[V];
 #pragma unroll
@@ -314,12 +366,14 @@ recurrence_forward_kernel(Recurrence r, Tiling s, T* y, float* h_last, float* ca
       float h[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) h[v] = r.h0 ? r.h0[b * r.C + c + v] : 0.0f;
-      __syncthreads();
+      lds_barrier();
       const bool follows = t1 < n;   // a live tile comes after this one
+      if (threadIdx.x < 64) __builtin_amdgcn_s_setprio(3);   // others' tiles wait for this wave
       if (seg == 0 && follows) join.whole(0, 1, A, B);
       if (s.tiles > 1)
-        join.state_before((int)tile, follows, A, B, words + b * r.C + c, r.B * r.C,
+        join.state_before((int)tile, follows, A, B, words + (int64_t)chain * s.tiles * s.lanes * V,
                           flags + chain * s.tiles, h);
+      __builtin_amdgcn_s_setprio(0);
       join.to_segment(0, seg, 1, h);
       if (carries) {   // where a tile of the backward begins, at the start of a segment
         const int span = back.segs * backward_steps(V);
@@ -338,9 +392,10 @@ recurrence_forward_kernel(Recurrence r, Tiling s, T* y, float* h_last, float* ca
           o[v] = GATE ? h[v] * (g[j][v] * sigmoids(g[j][v]).pos) : h[v];
         }
         if (full || j < live)
-          store<T, V>(out + j * r.C, at, o);
+          store<T, V>(out, at, o);
         else if (j < rest)
-          store<T, V>(out + j * r.C, at, none);
+          store<T, V>(out, at, none);
+        out.next();
       }
       if (!follows && seg == s.segs - 1) {
 #pragma unroll
@@ -348,7 +403,8 @@ recurrence_forward_kernel(Recurrence r, Tiling s, T* y, float* h_last, float* ca
       }
     };
     if (t0 >= n && tile > 0) {   // behind the row's end
-      for (int j = 0; j < rest; ++j) store<T, V>(out + j * r.C, at, none);
+      for (int j = 0; j < L; ++j, out.next())
+        if (j < rest) store<T, V>(out, at, none);
     } else if (t1 <= n) {
       work(std::true_type());
     } else {
@@ -381,9 +437,10 @@ recurrence_backward_kernel(Recurrence r, Tiling s, const float* carries, const T
     const auto work = [&](auto whole) {
       constexpr bool full = decltype(whole)::value;
       Raw<T, V> rf[L], x[L], g[L], rd[L];
-      const T* xp = static_cast<const T*>(r.x) + b * r.xb + t0 * r.xt;
-      const T* fp = static_cast<const T*>(r.f) + b * r.fb + t0 * r.ft;
-      const T* gp = GATE ? static_cast<const T*>(r.g) + b * r.gb + t0 * r.gt : nullptr;
+      Walk<T> xp(static_cast<const T*>(r.x) + b * r.xb + t0 * r.xt, r.xt);
+      Walk<T> fp(static_cast<const T*>(r.f) + b * r.fb + t0 * r.ft, r.ft);
+      Walk<T> gp(GATE ? static_cast<const T*>(r.g) + b * r.gb + t0 * r.gt : nullptr, r.gt);
+      Walk<T> dyp(dy + row, r.C), dgp(dg + row, r.C);
       const uint32_t atx = offset<T>(seg * L, r.xt, c), atf = offset<T>(seg * L, r.ft, c);
       const uint32_t atg = offset<T>(seg * L, r.gt, c);
 #pragma unroll
@@ -391,11 +448,13 @@ recurrence_backward_kernel(Recurrence r, Tiling s, const float* carries, const T
         rf[j] = Raw<T, V>::all(INFINITY);
         x[j] = g[j] = rd[j] = Raw<T, V>::all(0.0f);
         if (full || j < live) {
-          rf[j] = load<T, V>(fp + j * r.ft, atf);
-          x[j] = load<T, V>(xp + j * r.xt, atx);
-          if (GATE) g[j] = load<T, V>(gp + j * r.gt, atg);
-          if (dy) rd[j] = load<T, V>(dy + row + j * r.C, at);
+          rf[j] = load<T, V>(fp, atf);
+          x[j] = load<T, V>(xp, atx);
+          if (GATE) g[j] = load<T, V>(gp, atg);
+          if (dy) rd[j] = load<T, V>(dyp, at);
         }
+        fp.next(), xp.next(), dyp.next();
+        if (GATE) gp.next();
       }
       float A[V], B[V], h[V];
 #pragma unroll
@@ -414,7 +473,7 @@ recurrence_backward_kernel(Recurrence r, Tiling s, const float* carries, const T
       }
 #pragma unroll
       for (int v = 0; v < V; ++v) join.at(seg, v) = make_float2(A[v], B[v]);
-      __syncthreads();
+      lds_barrier();
       join.to_segment(0, seg, 1, h);
       // Through the samples: dg; k the gate's complement, f (h_{t-1} - x) a (1 - a), d
       // what reaches h_t.  The gates are computed again (two registers a value less
@@ -443,10 +502,11 @@ recurrence_backward_kernel(Recurrence r, Tiling s, const float* carries, const T
         }
         if (GATE && dg) {
           if (full || j < live)
-            store<T, V>(dg + row + j * r.C, at, o);
+            store<T, V>(dgp, at, o);
           else if (j < rest)
-            store<T, V>(dg + row + j * r.C, at, none);
+            store<T, V>(dgp, at, none);
         }
+        if (GATE) dgp.next();
       }
       // what a segment hands to the sample before it: A (what it is handed) + B
 #pragma unroll
@@ -455,21 +515,24 @@ recurrence_backward_kernel(Recurrence r, Tiling s, const float* carries, const T
       for (int j = L - 1; j >= 0; --j)
 #pragma unroll
         for (int v = 0; v < V; ++v) B[v] = (1.0f - k[j][v]) * (B[v] + d[j][v]);
-      __syncthreads();
+      lds_barrier();
 #pragma unroll
       for (int v = 0; v < V; ++v) join.at(seg, v) = make_float2(A[v], B[v]);
       float l[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) l[v] = dh_last ? dh_last[b * r.C + c + v] : 0.0f;
-      __syncthreads();
+      lds_barrier();
+      if (threadIdx.x < 64) __builtin_amdgcn_s_setprio(3);
       if (seg == 0 && tile > 0) join.whole(s.segs - 1, -1, A, B);
       if (s.tiles > 1) {
         const int span = s.segs * L;
         const int after = n > 0 ? (int)((n - 1) / span) - (int)tile : 0;   // live tiles after it
-        join.state_before(after, tile > 0, A, B, words + b * r.C + c, r.B * r.C,
+        join.state_before(after, tile > 0, A, B, words + (int64_t)chain * s.tiles * s.lanes * V,
                           flags + chain * s.tiles, l);
       }
+      __builtin_amdgcn_s_setprio(0);
       join.to_segment(s.segs - 1, s.segs - 1 - seg, -1, l);
+      Walk<T> dxp(dx + row + (L - 1) * r.C, -r.C), dfp(df + row + (L - 1) * r.C, -r.C);
 #pragma unroll
       for (int j = L - 1; j >= 0; --j) {
         float ox[V], of[V];
@@ -482,9 +545,10 @@ recurrence_backward_kernel(Recurrence r, Tiling s, const float* carries, const T
         }
         const bool in = full || j < live;
         if (full || j < rest) {
-          if (dx) store<T, V>(dx + row + j * r.C, at, in ? ox : none);
-          if (df) store<T, V>(df + row + j * r.C, at, in ? of : none);
+          if (dx) store<T, V>(dxp, at, in ? ox : none);
+          if (df) store<T, V>(dfp, at, in ? of : none);
         }
+        dxp.next(), dfp.next();
       }
       if (dh0 && tile == 0 && seg == 0) {
 #pragma unroll
@@ -492,10 +556,12 @@ recurrence_backward_kernel(Recurrence r, Tiling s, const float* carries, const T
       }
     };
     if (t0 >= n && tile > 0) {
-      for (int j = 0; j < rest; ++j) {
-        if (dx) store<T, V>(dx + row + j * r.C, at, none);
-        if (df) store<T, V>(df + row + j * r.C, at, none);
-        if (GATE && dg) store<T, V>(dg + row + j * r.C, at, none);
+      Walk<T> dxp(dx + row, r.C), dfp(df + row, r.C), dgp(dg + row, r.C);
+      for (int j = 0; j < L; ++j, dxp.next(), dfp.next(), dgp.next()) {
+        if (j >= rest) continue;
+        if (dx) store<T, V>(dxp, at, none);
+        if (df) store<T, V>(dfp, at, none);
+        if (GATE && dg) store<T, V>(dgp, at, none);
       }
     } else if (t1 <= n) {
       work(std::true_type());
@@ -518,7 +584,7 @@ Tiling tiling(int dtype, int64_t B, int64_t T, int64_t C, bool backward) {
   // 32 lanes of 4 bytes are a cache line across, and the more segments the fewer tiles
   // for a state to pass (one row of 131,072 x 512, bfloat16, forward: 147 us, 234 with 64
   // lanes, 159 with 16; 8 x 4096 x 1280 forward and backward 235, 232 and 300).
-  s.lanes = pow2_at_least((C + V - 1) / V, 32);
+  s.lanes = std::max(8, pow2_at_least((C + V - 1) / V, 32));
   // as many segments as the samples fill, up to the workgroup's lanes
   s.segs = pow2_at_least((T + L - 1) / L, kBlock / s.lanes);
   s.segs = std::max(s.segs, 64 / s.lanes);
@@ -531,7 +597,7 @@ Tiling tiling(int dtype, int64_t B, int64_t T, int64_t C, bool backward) {
 
 size_t lds_bytes(const Tiling& s, int V) {
   const size_t row = (size_t)s.lanes * V * sizeof(float2);
-  return s.segs * row + (s.tiles > 1 ? std::min<size_t>(kWindow, s.tiles) * row : 0);
+  return s.segs * row + (s.tiles > 1 ? std::min<size_t>(kWindow, s.tiles) * row + row / 2 : 0);
 }
 
 // f(T(), V, GATE) for the call's types, as constants.
@@ -545,21 +611,21 @@ void with_shape(int dtype, int V, bool gate, F f) {
   gate ? types(std::true_type()) : types(std::false_type());
 }
 
-// The workspace: a ticket counter (16 bytes), a word for each tile and channel, and a
-// flag for each tile.
+// The workspace: a ticket counter (16 bytes), a word for each channel of each tile, and
+// a flag for each tile.
 struct Room {
   unsigned *counter = nullptr, *flags = nullptr;
   Word* words = nullptr;
-  hipError_t clear(const Tiling& s, const Recurrence& r, void* workspace, hipStream_t st) {
+  hipError_t clear(const Tiling& s, int V, void* workspace, hipStream_t st) {
     if (s.tiles == 1) return hipSuccess;
     counter = static_cast<unsigned*>(workspace);
     words = static_cast<Word*>(workspace) + 2;
-    flags = reinterpret_cast<unsigned*>(words + (int64_t)s.tiles * r.B * r.C);
-    return launch_fill(static_cast<float*>(workspace), bytes(s, r.B, r.C) / 4, 0.0f, st);
+    flags = reinterpret_cast<unsigned*>(words + (int64_t)s.tiles * s.chains * s.lanes * V);
+    return launch_fill(static_cast<float*>(workspace), bytes(s, V) / 4, 0.0f, st);
   }
-  static int64_t bytes(const Tiling& s, int64_t B, int64_t C) {
+  static int64_t bytes(const Tiling& s, int V) {
     if (s.tiles == 1) return 0;
-    return 16 + (int64_t)s.tiles * (B * C * (int64_t)sizeof(Word) + (int64_t)s.chains * 4);
+    return 16 + (int64_t)s.tiles * s.chains * (s.lanes * V * (int64_t)sizeof(Word) + 4);
   }
 };
 
@@ -580,16 +646,16 @@ int64_t recurrence_carries(int dtype, int64_t B, int64_t T, int64_t C) {
 }
 
 int64_t recurrence_workspace(int dtype, int64_t B, int64_t T, int64_t C, bool backward) {
-  return Room::bytes(tiling(dtype, B, T, C, backward), B, C);
+  return Room::bytes(tiling(dtype, B, T, C, backward), channels(dtype, C));
 }
 
 hipError_t launch_recurrence_forward(int dtype, const Recurrence& r, void* y, float* h_last,
                                      float* carries, void* workspace, hipStream_t st) {
   const Tiling s = tiling(dtype, r.B, r.T, r.C, false), back = tiling(dtype, r.B, r.T, r.C, true);
-  Room room;
-  const hipError_t e = room.clear(s, r, workspace, st);
-  if (e != hipSuccess) return e;
   const int V = channels(dtype, r.C);
+  Room room;
+  const hipError_t e = room.clear(s, V, workspace, st);
+  if (e != hipSuccess) return e;
   with_shape(dtype, V, r.g != nullptr, [&](auto t, auto vs, auto gate) {
     typedef decltype(t) T;
     constexpr int W = decltype(vs)::value;
@@ -611,10 +677,10 @@ hipError_t launch_recurrence_backward(int dtype, const Recurrence& r, const floa
     return hipMemcpyAsync(dh0, dh_last, r.B * r.C * 4, hipMemcpyDeviceToDevice, st);
   }
   const Tiling s = tiling(dtype, r.B, r.T, r.C, true);
-  Room room;
-  const hipError_t e = room.clear(s, r, workspace, st);
-  if (e != hipSuccess) return e;
   const int V = channels(dtype, r.C);
+  Room room;
+  const hipError_t e = room.clear(s, V, workspace, st);
+  if (e != hipSuccess) return e;
   with_shape(dtype, V, r.g != nullptr, [&](auto t, auto vs, auto gate) {
     typedef decltype(t) T;
     recurrence_backward_kernel<T, decltype(vs)::value, decltype(gate)::value>
