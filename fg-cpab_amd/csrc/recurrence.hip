@@ -97,135 +97,135 @@ __device__ __forceinline__ W peek(W* at) {
 }
 
 // What joins a workgroup's segments and the tiles.  Tiles are numbered from 0 in the
-// order in which a row's state travels (forward: time, backward: against it).
+// order in which a row's state travels (forward: time, backward: against it).  A tile's
+// channels are its `slots`, at most a wave of them: the first wave has a lane to each.
 template <int V>
 struct Join {
   const Tiling& s;
-  float2* agg;     // LDS [segs][lanes * V]: the segments' (A, B)
-  Word* window;    // LDS [kWindow][lanes * V]: the tiles before, newest first
-  float* entry;    // LDS [lanes * V]: the state before the tile
+  int slots, seg, lane;
+  float2* agg;     // LDS [segs][slots]: the segments' (A, B)
+  Word* window;    // LDS [kWindow][slots]: the tiles before, newest first
+  float* entry;    // LDS [slots]: the state before the tile
   int* nearest;    // LDS: how many tiles back the nearest state is
-  int seg, lane;
 
   __device__ Join(const Tiling& t, char* room, int* one, int sg, int ln)
-      : s(t), agg(reinterpret_cast<float2*>(room)),
-        window(reinterpret_cast<Word*>(agg + t.segs * t.lanes * V)),
-        entry(reinterpret_cast<float*>(window + min(kWindow, (int)t.tiles) * t.lanes * V)),
-        nearest(one), seg(sg), lane(ln) {}
-  __device__ float2& at(int sg, int v) const { return agg[(sg * s.lanes + lane) * V + v]; }
-  // f(k-th (A, B)) for `count` segments from `first` in steps of `dir`, read four ahead:
-  // a step waits for a multiplication then, and not for LDS (16 segments in 1.0 us).
-  template <typename F>
-  __device__ __forceinline__ void segments(int first, int count, int dir, F f) const {
-    for (int k = 0; k < count; k += 4) {
-      float2 m[4][V];
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int v = 0; v < V; ++v) m[q][v] = at(first + min(k + q, count - 1) * dir, v);
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (k + q < count) f(m[q]);
-    }
-  }
-  // Of the whole tile, segments taken from `first` in steps of `dir`.
-  __device__ void whole(int first, int dir, float A[V], float B[V]) const {
-#pragma unroll
-    for (int v = 0; v < V; ++v) A[v] = 1.0f, B[v] = 0.0f;
-    segments(first, s.segs, dir, [&](const float2 m[V]) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        B[v] = fmaf(m[v].x, B[v], m[v].y);
-        A[v] *= m[v].x;
-      }
-    });
-  }
+      : s(t), slots(t.lanes * V), seg(sg), lane(ln), agg(reinterpret_cast<float2*>(room)),
+        window(reinterpret_cast<Word*>(agg + t.segs * slots)),
+        entry(reinterpret_cast<float*>(window + min(kWindow, (int)t.tiles) * slots)), nearest(one) {}
+  __device__ float2& at(int sg, int v) const { return agg[sg * slots + lane * V + v]; }
   // h: from the state before the tile to that before a segment, over `count` segments
   // from `first` in steps of `dir`.
   __device__ void to_segment(int first, int count, int dir, float h[V]) const {
-    segments(first, count, dir, [&](const float2 m[V]) {
+#pragma unroll 2
+    for (int k = 0, sg = first; k < count; ++k, sg += dir)
 #pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = fmaf(m[v].x, h[v], m[v].y);
-    });
+      for (int v = 0; v < V; ++v) {
+        const float2 m = at(sg, v);
+        h[v] = fmaf(m.x, h[v], m.y);
+      }
   }
-  // h: the state before tile `number`, given as the state before tile 0.  (A, B): the
-  // tile's own, used in segment 0; `follows`: tiles come after it.  The chain's flags and
-  // words, tile by tile: lanes' words next to each other, [tiles][V][lanes].
-  __device__ void state_before(int number, bool follows, const float A[V], const float B[V],
-                               Word* words, unsigned* flags, float h[V]) const {
-    const auto word = [&](int tile, int v) {
-      return words + ((int64_t)tile * V + v) * s.lanes + lane;
-    };
-    const bool first = threadIdx.x == 0;
-    if (number > 0) {
-      if (seg == 0 && follows) {
+  // (A, B) of the whole tile in a slot, segments taken from `first` in steps of `dir`,
+  // read four ahead: a step waits for a multiplication then, and not for LDS.
+  __device__ float2 whole(int slot, int first, int dir) const {
+    float2 all = make_float2(1.0f, 0.0f);
+    for (int k = 0; k < s.segs; k += 4) {
+      float2 m[4];
 #pragma unroll
-        for (int v = 0; v < V; ++v) publish(word(number, v), map_word(A[v], B[v]));
-        if (first) publish(flags + number, kHasMap);
-      }
-      if (threadIdx.x >= blockDim.x - 64) {   // the last wave, beside the first
-        // lane k: the tile k + 1 before; what lies before tile 0 is not asked
-        const int mine = number - 1 - (int)(threadIdx.x & 63);
-        for (;;) {
-          const unsigned f = mine >= 0 ? peek(flags + mine) : kHasMap;
-          const uint64_t state = __ballot(f == kHasState), any = __ballot(f != 0);
-          const int k = __builtin_ctzll(state | 1ull << 63);
-          if ((state >> k & 1) && !(~any & ((1ull << k) - 1))) {
-            if ((threadIdx.x & 63) == 0) *nearest = k;
-            break;
-          }
-          __builtin_amdgcn_s_sleep(2);
-        }
-      }
-      lds_barrier();
-      const int k = *nearest;
-      // the flags are no more than a hint: a word says itself what it is
-      for (int q = seg; q <= k; q += s.segs)
+      for (int q = 0; q < 4; ++q) m[q] = agg[(first + min(k + q, s.segs - 1) * dir) * slots + slot];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          Word* at = word(number - 1 - q, v);
-          Word w = peek(at);
-          while (w == 0 || (q == k && !is_state(w))) {
-            __builtin_amdgcn_s_sleep(1);
-            w = peek(at);
-          }
-          window[(q * s.lanes + lane) * V + v] = w;
-        }
-      lds_barrier();
-      // one segment's lanes apply them, for all
-      if (seg == 0) {
-        for (int q = k; q >= 0; q -= 4) {   // read four ahead, as segments()
-          Word w[4][V];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int v = 0; v < V; ++v) w[e][v] = window[(max(q - e, 0) * s.lanes + lane) * V + v];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (e > q) continue;
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-              // a tile may have come to its state since: that is then the one to take
-              h[v] = is_state(w[e][v]) ? word_B(w[e][v])
-                                       : fmaf(word_A(w[e][v]), h[v], word_B(w[e][v]));
-          }
-        }
+      for (int q = 0; q < 4; ++q) {
+        if (k + q >= s.segs) continue;
+        all.y = fmaf(m[q].x, all.y, m[q].y);
+        all.x *= m[q].x;
       }
     }
-    if (number > 0) {
+    return all;
+  }
+  // h: the state before tile `number`, given as the state before tile 0; the segments'
+  // (A, B) are in LDS, taken as in whole().  `follows`: tiles come after it.  The chain's
+  // words, [tiles][slots], and flags, tile by tile.  Called by every lane.
+  __device__ void state_before(int number, bool follows, int segment, int dir, Word* words,
+                               unsigned* flags, float h[V]) const {
+    const int slot = threadIdx.x;
+    const bool carries = slot < slots;
+    Word* own = words + (int64_t)number * slots + slot;
+    if (number == 0) {
+      if (!follows) return;
       if (seg == 0)
 #pragma unroll
         for (int v = 0; v < V; ++v) entry[lane * V + v] = h[v];
       lds_barrier();
-#pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = entry[lane * V + v];
+      if (carries) {
+        const float2 all = whole(slot, segment, dir);
+        publish(own, state_word(fmaf(all.x, entry[slot], all.y)));
+        if (slot == 0) publish(flags, kHasState);
+      }
+      return;
     }
-    if (seg == 0 && follows) {
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        publish(word(number, v), state_word(fmaf(A[v], h[v], B[v])));
-      if (first) publish(flags + number, kHasState);
+    // other tiles wait for this wave
+    if (slot < 64) __builtin_amdgcn_s_setprio(3);
+    float2 all;
+    if (carries && follows) {
+      all = whole(slot, segment, dir);
+      publish(own, map_word(all.x, all.y));
+      if (slot == 0) publish(flags + number, kHasMap);
     }
+    if (threadIdx.x >= blockDim.x - 64) {   // the last wave, beside the first
+      // lane k: the tile k + 1 before; what lies before tile 0 is not asked
+      const int mine = number - 1 - (int)(threadIdx.x & 63);
+      for (;;) {
+        const unsigned f = mine >= 0 ? peek(flags + mine) : kHasMap;
+        const uint64_t state = __ballot(f == kHasState), any = __ballot(f != 0);
+        const int k = __builtin_ctzll(state | 1ull << 63);
+        if ((state >> k & 1) && !(~any & ((1ull << k) - 1))) {
+          if ((threadIdx.x & 63) == 0) *nearest = k;
+          break;
+        }
+        __builtin_amdgcn_s_sleep(2);
+      }
+    }
+    lds_barrier();
+    // Words of the tiles up to the nearest state, two of each lane on their way at once.
+    // The flags are no more than a hint: a word says itself what it is.
+    const int k = *nearest, count = (k + 1) * slots, lanes = blockDim.x;
+    const Word* newest = words + (int64_t)(number - 1) * slots;
+    const auto ready = [&](Word w, int i) { return w != 0 && (i < k * slots || is_state(w)); };
+    const auto from = [&](int i) {   // tile i / slots back, slot i % slots
+      return const_cast<Word*>(newest) - (i & -slots) + (i & (slots - 1));
+    };
+    for (int i = threadIdx.x; i < count; i += 2 * lanes) {
+      const bool two = i + lanes < count;
+      Word w = peek(from(i)), x = two ? peek(from(i + lanes)) : 0;
+      while (!ready(w, i)) w = peek(from(i));
+      window[i] = w;
+      if (!two) continue;
+      while (!ready(x, i + lanes)) x = peek(from(i + lanes));
+      window[i + lanes] = x;
+    }
+    lds_barrier();
+    if (carries) {
+      float state = 0.0f;
+      for (int q = k; q >= 0; q -= 4) {   // read four ahead, as in whole()
+        Word w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = window[max(q - e, 0) * slots + slot];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (e > q) continue;
+          // a tile may have come to its state since: that is then the one to take
+          state = is_state(w[e]) ? word_B(w[e]) : fmaf(word_A(w[e]), state, word_B(w[e]));
+        }
+      }
+      entry[slot] = state;
+      if (follows) {
+        publish(own, state_word(fmaf(all.x, state, all.y)));
+        if (slot == 0) publish(flags + number, kHasState);
+      }
+    }
+    __builtin_amdgcn_s_setprio(0);
+    lds_barrier();
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = entry[lane * V + v];
   }
 };
 
@@ -368,12 +368,9 @@ recurrence_forward_kernel(Recurrence r, Tiling s, T* y, float* h_last, float* ca
       for (int v = 0; v < V; ++v) h[v] = r.h0 ? r.h0[b * r.C + c + v] : 0.0f;
       lds_barrier();
       const bool follows = t1 < n;   // a live tile comes after this one
-      if (threadIdx.x < 64) __builtin_amdgcn_s_setprio(3);   // others' tiles wait for this wave
-      if (seg == 0 && follows) join.whole(0, 1, A, B);
       if (s.tiles > 1)
-        join.state_before((int)tile, follows, A, B, words + (int64_t)chain * s.tiles * s.lanes * V,
+        join.state_before((int)tile, follows, 0, 1, words + (int64_t)chain * s.tiles * join.slots,
                           flags + chain * s.tiles, h);
-      __builtin_amdgcn_s_setprio(0);
       join.to_segment(0, seg, 1, h);
       if (carries) {   // where a tile of the backward begins, at the start of a segment
         const int span = back.segs * backward_steps(V);
@@ -522,15 +519,12 @@ recurrence_backward_kernel(Recurrence r, Tiling s, const float* carries, const T
 #pragma unroll
       for (int v = 0; v < V; ++v) l[v] = dh_last ? dh_last[b * r.C + c + v] : 0.0f;
       lds_barrier();
-      if (threadIdx.x < 64) __builtin_amdgcn_s_setprio(3);
-      if (seg == 0 && tile > 0) join.whole(s.segs - 1, -1, A, B);
       if (s.tiles > 1) {
         const int span = s.segs * L;
         const int after = n > 0 ? (int)((n - 1) / span) - (int)tile : 0;   // live tiles after it
-        join.state_before(after, tile > 0, A, B, words + (int64_t)chain * s.tiles * s.lanes * V,
-                          flags + chain * s.tiles, l);
+        join.state_before(after, tile > 0, s.segs - 1, -1,
+                          words + (int64_t)chain * s.tiles * join.slots, flags + chain * s.tiles, l);
       }
-      __builtin_amdgcn_s_setprio(0);
       join.to_segment(s.segs - 1, s.segs - 1 - seg, -1, l);
       Walk<T> dxp(dx + row + (L - 1) * r.C, -r.C), dfp(df + row + (L - 1) * r.C, -r.C);
 #pragma unroll
