@@ -54,7 +54,8 @@ class AdamW(torch.optim.Optimizer):
         lr, betas, eps, weight_decay: as torch.optim.AdamW
         state_bits: 32, or 8: the moments in 8 bits (2.1 bytes a parameter, not 8)
         master_weights: bool, keep 32-bit values of bfloat16 parameters, which
-            otherwise lose steps smaller than their rounding
+            otherwise lose steps smaller than their rounding (taken from the parameters
+            at the first step; a parameter set by hand afterwards is not seen)
         seed: int, of the 8-bit states' random rounding
     """
 
@@ -102,7 +103,7 @@ class AdamW(torch.optim.Optimizer):
                 state = self.state[p]
                 if not state:
                     state.update(self._new_state(p, group))
-                state["step"] += 1
+                state["step"] = int(state["step"]) + 1
                 key = (p.dtype, p.device, state["step"], "master" in state)
                 if key not in calls:
                     calls[key] = ([], [], [], ordinal)

@@ -24,9 +24,12 @@
 // without waiting: every wait ends.
 //
 // One wave of a workgroup polls, and only a flag to each tile; the words of the channels
-// are read once, when the flags say that they are there.  (All lanes polling the words
-// took the memory's bandwidth from the samples: 8 x 4096 x 1280 bfloat16, forward and
-// backward, 87 and 153 us, where the tiles alone take 78 and 126.)
+// are read once, when the flags say that they are there (all lanes polling the words took
+// the memory's bandwidth from the samples).
+//
+// Bound by memory: 8 x 4096 x 1280 bfloat16 forward 74 us and backward 143, 4.5 and 4.1
+// TB/s of what has to be read and written; 72 and 128 without the look-back.  With few
+// chains the look-back counts: one row of 131,072 x 512, forward, 124 us, 104 without.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -281,7 +284,7 @@ __device__ __forceinline__ void store(const Walk<T>& w, uint32_t off, const floa
 #pragma unroll
   for (int v = 0; v < V; ++v) raw[v] = from_float<T>(in[v]);
   // past the second-level cache, which the inputs need (16 x 10,000 x 64 in 32 bits, forward
-  // and backward: 33 and 49 us, 39 and 58 through it)
+  // and backward, through it and past it: 39 and 58 us, 33 and 49)
   __builtin_nontemporal_store((Unit)__builtin_bit_cast(Unit, raw),
                               (__attribute__((address_space(1))) Unit*)(w.p + off));
 }
@@ -576,8 +579,10 @@ Tiling tiling(int dtype, int64_t B, int64_t T, int64_t C, bool backward) {
   Tiling s;
   const int V = channels(dtype, C), L = backward ? backward_steps(V) : forward_steps(T);
   // 32 lanes of 4 bytes are a cache line across, and the more segments the fewer tiles
-  // for a state to pass (one row of 131,072 x 512, bfloat16, forward: 147 us, 234 with 64
-  // lanes, 159 with 16; 8 x 4096 x 1280 forward and backward 235, 232 and 300).
+  // for a state to pass (8 x 4096 x 1280 bfloat16, forward and backward: 74 and 143 us, with
+  // 16 lanes 93 and 192, in half as many segments 87 and 143; one row of 131,072 x 512,
+  // forward, 124, 141 and 188; 16 x 10,000 x 64 in 32 bits 33 and 47, 39 and 64, 46 and 51).
+  // At least 8, so that a few channels do not make thousands of segments.
   s.lanes = std::max(8, pow2_at_least((C + V - 1) / V, 32));
   // as many segments as the samples fill, up to the workgroup's lanes
   s.segs = pow2_at_least((T + L - 1) / L, kBlock / s.lanes);

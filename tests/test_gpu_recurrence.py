@@ -189,6 +189,45 @@ def test_in_pieces(cuda):
     check(torch.cat(parts, 1), so.f64(y), bound * so.f64(g).abs() + 40 * U * so.f64(y).abs(), "y")
 
 
+@pytest.mark.parametrize("dtype,C", [(torch.float32, 40), (torch.bfloat16, 130)])
+def test_hundreds_of_tiles_in_pieces(cuda, dtype, C):
+    # a state passes hundreds of tiles: against the same signal read in short pieces,
+    # whose states and gradients autograd hands on.  Both sides carry the bounds above
+    # (twice); bfloat16 gradients half a unit each besides.
+    B, T = 2, 70001
+    lengths = [T, 33333]
+    x, f, g, h0, n = make(cuda, dtype, B, T, C, lengths=lengths, seed=17)
+    x, f, g = (torch.nan_to_num(t, 0.0, 0.0, 0.0) for t in (x, f, g))
+    x, f = x.clamp(-8, 8), f.clamp(-8, 8)
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    dy = torch.randn(B, T, C, device=cuda, generator=gen).to(dtype)
+    dh = torch.randn(B, C, device=cuda, generator=gen)
+    one = [t.detach().requires_grad_() for t in (x, f, g, h0)]
+    y, h = cpab.gated_recurrence(*one, n)
+    grads = torch.autograd.grad((y, h), one, (dy, dh))
+    two = [t.detach().requires_grad_() for t in (x, f, g, h0)]
+    s, parts, step = two[3], [], 3001
+    for t in range(0, T, step):
+        p, s = cpab.gated_recurrence(*(v[:, t:t + step] for v in two[:3]), s, (n - t).clamp(min=0))
+        parts.append(p)
+    want = torch.autograd.grad((torch.cat(parts, 1), s), two, (dy, dh))
+    M = float(max(x.abs().max(), h0.abs().max()))
+    N = so.recurrence_memory(so.f64(f), T)
+    unit = 2 * so.UNIT[dtype] if dtype != torch.float32 else 0.0
+    eh = 36 * U * N * M
+    silu = so.f64(g).abs()
+    check(h, so.f64(s), eh, "h")
+    ry = so.f64(torch.cat(parts, 1))
+    check(y, ry, eh * silu + (80 * U + unit) * ry.abs() + 1e-38, "y")
+    L = float((dy.float() * g.float() * torch.sigmoid(g.float())).abs().max()) * N + float(dh.abs().max())
+    el = 36 * U * N * L
+    for k, (a, b) in enumerate(zip(grads, want)):
+        b = so.f64(b)
+        scale = (el, 0.25 * (2 * M * el + 4 * L * eh + 160 * U * M * L),
+                 so.f64(dy).abs() * (1.1 * eh + 120 * U * M * (1 + silu)), el)[k]
+        check(a, b, scale + (unit + 80 * U) * b.abs() + 1e-38, f"grad {k}")
+
+
 def test_same_call_same_bits(cuda):
     x, f, g, h0, _ = make(cuda, torch.float32, 2, 3000, 65, seed=8)
     leaves = [t.detach().requires_grad_() for t in (x, f, g, h0)]
