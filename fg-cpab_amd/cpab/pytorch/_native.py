@@ -90,7 +90,7 @@ _SIGNATURES = {
                                     _c_i64, _c_vp, _c_f32, _c_vp, _c_vp, _c_vp, _c_vp]),
     "cpab_rms_norm_backward_workspace_size": (_c_i64, [_c_i64, _c_i64]),
     "cpab_rms_norm_backward": (_c_int, [_c_int, _c_int, _c_int, _c_i64, _c_i64, _c_vp, _c_i64,
-                                        _c_vp, _c_vp, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp,
+                                        _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp,
                                         _c_vp, _c_vp, _c_i64, _c_vp]),
     "cpab_adamw_step": (_c_int, [_c_int, _c_int, _c_i64, _c_vp, _c_i64, _c_f64, _c_f64, _c_f64,
                                  _c_f64, _c_f64, ctypes.c_uint32, _c_vp]),

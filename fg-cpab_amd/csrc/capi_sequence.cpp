@@ -200,7 +200,8 @@ int64_t cpab_rms_norm_backward_workspace_size(int64_t rows, int64_t C) {
 }
 
 int cpab_rms_norm_backward(int dtype, int residual_dtype, int weight_dtype, int64_t rows, int64_t C,
-                           const void* r, int64_t r_stride, const float* rstd, const void* weight,
+                           const void* r, int64_t r_stride, const void* added,
+                           int64_t added_stride, const float* rstd, const void* weight,
                            const void* grad_y, int64_t grad_y_stride,
                            const void* grad_residual_out, int64_t grad_residual_stride,
                            void* grad_x, void* grad_residual, void* grad_weight, void* workspace,
@@ -210,14 +211,15 @@ int cpab_rms_norm_backward(int dtype, int residual_dtype, int weight_dtype, int6
   if (rows > 0) {
     CPAB_REQUIRE(r); CPAB_REQUIRE(rstd); CPAB_REQUIRE(weight); CPAB_REQUIRE(grad_y);
   }
-  CPAB_TYPED(r, residual_dtype); CPAB_ALIGNED(rstd, 4); CPAB_TYPED(weight, weight_dtype);
+  CPAB_TYPED(r, residual_dtype); CPAB_TYPED(added, residual_dtype); CPAB_ALIGNED(rstd, 4); CPAB_TYPED(weight, weight_dtype);
   CPAB_TYPED(grad_y, dtype); CPAB_TYPED(grad_residual_out, residual_dtype);
   CPAB_TYPED(grad_x, dtype); CPAB_TYPED(grad_residual, residual_dtype);
   CPAB_TYPED(grad_weight, weight_dtype);
   CPAB_TRY(check_workspace(workspace, workspace_bytes,
                            grad_weight ? cpab::rms_norm_backward_workspace(rows, C) : 0));
-  const cpab::RmsNormGrad n{dtype, residual_dtype, weight_dtype, rows, C, r, r_stride, rstd, weight,
-                            grad_y, grad_y_stride, grad_residual_out, grad_residual_stride};
+  const cpab::RmsNormGrad n{dtype, residual_dtype, weight_dtype, rows, C, r, r_stride, added,
+                            added_stride, rstd, weight, grad_y, grad_y_stride, grad_residual_out,
+                            grad_residual_stride};
   return check_hip(cpab::launch_rms_norm_backward(n, grad_x, grad_residual, grad_weight, workspace,
                                                   as_stream(stream)),
                    "cpab_rms_norm_backward");

@@ -4,6 +4,10 @@
 // s = 1 / sqrt(mean(r^2) + eps), y = r s w.  Backward, with u = w dy and n = r s:
 //   dr = s (u - n mean(u n)) + dr_out,  dw = sum over rows of dy n.
 //
+// The forward's norm is of r before it is rounded to the residual's type; the backward
+// takes the rounded r, or, for a weight of 32 bits whose gradient would show that
+// rounding (0.0017 of its value), x and the residual again.
+//
 // Bound by memory: each value is read once and written once.  A row is held in the
 // registers of `tpr` lanes (a power of two, so that a narrow row does not leave a wave
 // idle and a wide one is spread over many), in pieces of V neighbouring values (16
@@ -51,15 +55,23 @@ __device__ __forceinline__ float over_row(float v, int tpr, float* room, Op op) 
 __device__ __forceinline__ uint32_t to_e4m3(float v) {   // |v| <= 448 or NaN
   return __builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false) & 0xff;
 }
-// v / sc, inv = 1 / sc: the product's rounding taken back, so that what lies between two
-// 8-bit values falls to the nearer.
-__device__ __forceinline__ float divided(float v, float sc, float inv) {
-  const float z = v * inv;
-  return fmaf(fmaf(-z, sc, v), inv, z);
-}
-__device__ __forceinline__ float within_e4m3(float v) {
-  return fabsf(v) > 448.0f ? copysignf(448.0f, v) : v;
-}
+// A row in 8 bits.  s cancels between y and its scale: with z = r w, y / scale is
+// z / (max |z| / 448), two roundings from the definition, and the scale max |z| s / 448.
+struct Eight {
+  float scale, by, inv;
+  __device__ Eight(float top, float s) {   // top = max |z|
+    const float y = top * s;
+    scale = y == 0.0f ? 1.0f : y / 448.0f;
+    by = y == 0.0f ? 1.0f : top / 448.0f;
+    inv = y == 0.0f ? 0.0f : 1.0f / by;
+  }
+  // z / by, the product's rounding taken back, so that what lies between two 8-bit
+  // values falls to the nearer.
+  __device__ __forceinline__ float value(float z) const {
+    const float q = z * inv, v = fmaf(fmaf(-q, by, z), inv, q);
+    return fabsf(v) > 448.0f ? copysignf(448.0f, v) : v;
+  }
+};
 
 // V neighbouring values at any alignment of theirs.
 template <int BYTES, int ALIGN>
@@ -182,22 +194,21 @@ rms_norm_forward_kernel(RmsNorm n, T* y, uint8_t* q, float* scale, R* residual_o
       if (p.again >= V) continue;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        r[k][e] = r[k][e] * s * w[k][e];
+        r[k][e] = EIGHT ? r[k][e] * w[k][e] : r[k][e] * s * w[k][e];
         if (EIGHT) top = Max()(fabsf(r[k][e]), top);
       }
       if (!EIGHT && live) store<V>(y + row * n.C + p.at, r[k]);
     }
     if (!EIGHT) continue;
     top = over_row(top, tpr, room, Max());
-    const float sc = top == 0.0f ? 1.0f : top / 448.0f;
-    if (live && lane == 0) scale[row] = sc;
-    const float inv = 1.0f / sc;
+    const Eight by(top, s);
+    if (live && lane == 0) scale[row] = by.scale;
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       const Place p(k, tpr, lane, V, n.C);
       if (p.again >= V) continue;
 #pragma unroll
-      for (int e = 0; e < V; ++e) r[k][e] = within_e4m3(divided(r[k][e], sc, inv));
+      for (int e = 0; e < V; ++e) r[k][e] = by.value(r[k][e]);
       if (live) store_e4m3<V>(q + row * n.C + p.at, r[k]);
     }
   }
@@ -235,6 +246,18 @@ rms_norm_backward_kernel(RmsNormGrad n, T* dx, R* dres, float* parts, int tpr) {
       if (p.again >= V) continue;
       load<V>(r + p.at, v[k]);
       load<V>(dy + p.at, u[k]);
+    }
+    if (n.added) {
+      const R* more = static_cast<const R*>(n.added) + row * n.added_stride;
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        const Place p(k, tpr, lane, V, n.C);
+        if (p.again >= V) continue;
+        float a[V];
+        load<V>(more + p.at, a);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[k][e] += a[e];
+      }
     }
     float sum = 0.0f;
 #pragma unroll
@@ -327,22 +350,20 @@ rms_norm_wide_forward_kernel(RmsNorm n, T* y, uint8_t* q, float* scale, R* resid
     sum = over_row(sum, kMaxLanes, room, Sum());
     const float s = 1.0f / sqrtf(sum / (float)n.C + n.eps);
     if (rstd && threadIdx.x == 0) rstd[row] = s;
-    float sc = 1.0f, inv = 1.0f;
+    float top = 0.0f;
     if (EIGHT) {
-      float top = 0.0f;
       for (int64_t c = threadIdx.x; c < n.C; c += kMaxLanes)
-        top = Max()(fabsf(value(c) * s * to_float(w[c])), top);
+        top = Max()(fabsf(value(c) * to_float(w[c])), top);
       top = over_row(top, kMaxLanes, room, Max());
-      sc = top == 0.0f ? 1.0f : top / 448.0f;
-      if (threadIdx.x == 0) scale[row] = sc;
-      inv = 1.0f / sc;
     }
+    const Eight by(top, s);
+    if (EIGHT && threadIdx.x == 0) scale[row] = by.scale;
     for (int64_t c = threadIdx.x; c < n.C; c += kMaxLanes) {
-      const float r = value(c), v = r * s * to_float(w[c]);
+      const float r = value(c);
       if (EIGHT)
-        q[row * n.C + c] = (uint8_t)to_e4m3(within_e4m3(divided(v, sc, inv)));
+        q[row * n.C + c] = (uint8_t)to_e4m3(by.value(r * to_float(w[c])));
       else
-        y[row * n.C + c] = from_float<T>(v);
+        y[row * n.C + c] = from_float<T>(r * s * to_float(w[c]));
       if (residual_out) residual_out[row * n.C + c] = from_float<R>(r);
     }
   }
@@ -359,10 +380,12 @@ rms_norm_wide_backward_kernel(RmsNormGrad n, T* dx, R* dres, float* parts) {
     const R* r = static_cast<const R*>(n.r) + row * n.r_stride;
     const T* dy = static_cast<const T*>(n.grad_y) + row * n.grad_y_stride;
     const R* dout = n.grad_out ? static_cast<const R*>(n.grad_out) + row * n.grad_out_stride : nullptr;
+    const R* more = n.added ? static_cast<const R*>(n.added) + row * n.added_stride : nullptr;
+    const auto value = [&](int64_t c) { return to_float(r[c]) + (more ? to_float(more[c]) : 0.0f); };
     const float s = n.rstd[row];
     float sum = 0.0f;
     for (int64_t c = threadIdx.x; c < n.C; c += kMaxLanes) {
-      const float g = to_float(dy[c]), v = to_float(r[c]) * s;
+      const float g = to_float(dy[c]), v = value(c) * s;
       sum += g * to_float(w[c]) * v;
       if (part) part[c] += g * v;   // the lane's own channels
     }
@@ -370,7 +393,7 @@ rms_norm_wide_backward_kernel(RmsNormGrad n, T* dx, R* dres, float* parts) {
     const float mean = over_row(sum, kMaxLanes, room, Sum()) / (float)n.C;
     for (int64_t c = threadIdx.x; c < n.C; c += kMaxLanes) {
       const float u = to_float(dy[c]) * to_float(w[c]);
-      const float d = s * (u - to_float(r[c]) * s * mean) + (dout ? to_float(dout[c]) : 0.0f);
+      const float d = s * (u - value(c) * s * mean) + (dout ? to_float(dout[c]) : 0.0f);
       if (dx) dx[row * n.C + c] = from_float<T>(d);
       if (dres) dres[row * n.C + c] = from_float<R>(d);
     }

@@ -50,6 +50,8 @@ struct RmsNormGrad {
   int64_t rows, C;
   const void* r;
   int64_t r_stride;
+  const void* added;   // to r, in 32 bits; may be NULL
+  int64_t added_stride;
   const float* rstd;
   const void* weight;
   const void* grad_y;

@@ -174,7 +174,13 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
                                 ptr(w), (float)eps, ptr(y), ptr(sum), out(rstd), stream_of(x)),
           "cpab_rms_norm_forward");
     ctx->set_materialize_grads(false);
-    if (keep) ctx->save_for_backward({sum.defined() ? sum : x, w, rstd});
+    // the rounded sum; or its parts, where its rounding would show in a 32-bit gradient
+    const bool parts = sum.defined() && sum.scalar_type() != at::kFloat &&
+                       w.scalar_type() == at::kFloat && weight_.requires_grad();
+    if (keep && parts)
+      ctx->save_for_backward({x, w, rstd, res});
+    else if (keep)
+      ctx->save_for_backward({sum.defined() ? sum : x, w, rstd, Tensor()});
     ctx->saved_data["dtype"] = (int64_t)x.scalar_type();
     if (sum.defined()) return {y, sum};
     return {y};
@@ -185,7 +191,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     {
       const at::NoGradGuard no_grad;
       const auto saved = ctx->get_saved_variables();
-      const Tensor &r_ = saved[0], &w = saved[1], &rstd = saved[2];
+      const Tensor &r_ = saved[0], &w = saved[1], &rstd = saved[2], &added = saved[3];
       const c10::OptionalDeviceGuard guard(r_.device());
       const bool residual = grads.size() > 1;
       const auto dtype = (at::ScalarType)ctx->saved_data["dtype"].toInt();
@@ -208,8 +214,8 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
       at::DataPtr ws;
       if (bytes > 0) ws = scratch(bytes);
       check(cpab_rms_norm_backward(dtype == at::kFloat ? CPAB_F32 : CPAB_BF16, type_of(r),
-                                   type_of(w), rows, C, ptr(r), r.stride(0), in(rstd), ptr(w),
-                                   ptr(dy), dy.stride(0), ptr(dout),
+                                   type_of(w), rows, C, ptr(r), r.stride(0), ptr(added),
+                                   added.defined() ? added.stride(0) : 0, in(rstd), ptr(w), ptr(dy), dy.stride(0), ptr(dout),
                                    dout.defined() ? dout.stride(0) : 0, ptr(dx),
                                    same ? nullptr : ptr(dres), ptr(dw), ws.get(), bytes,
                                    stream_of(r)),

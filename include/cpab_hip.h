@@ -418,10 +418,14 @@ int cpab_rms_norm_e4m3(int dtype, int residual_dtype, int weight_dtype, int64_t 
  * stored as grad_x (of dtype; may be NULL) and grad_residual (of residual_dtype;
  * may be NULL), and grad_weight [C] of weight_dtype (may be NULL), the sum over
  * the rows of grad_y r s in an order that depends on the sizes alone.
+ * With `added` (rows of residual_dtype at added_stride; may be NULL), r and it are added
+ * in 32 bits: x and the residual, of one type, in place of a sum that was rounded to it,
+ * whose rounding a grad_weight of 32 bits would show.
  * workspace: cpab_rms_norm_backward_workspace_size(rows, C) bytes. */
 int64_t cpab_rms_norm_backward_workspace_size(int64_t rows, int64_t C);
 int cpab_rms_norm_backward(int dtype, int residual_dtype, int weight_dtype, int64_t rows, int64_t C,
-                           const void* r, int64_t r_stride, const float* rstd, const void* weight,
+                           const void* r, int64_t r_stride, const void* added,
+                           int64_t added_stride, const float* rstd, const void* weight,
                            const void* grad_y, int64_t grad_y_stride,
                            const void* grad_residual_out, int64_t grad_residual_stride,
                            void* grad_x, void* grad_residual, void* grad_weight, void* workspace,

@@ -194,6 +194,28 @@ def test_parts_of_the_gradient(cuda):
         torch.testing.assert_close(t.grad.float(), 2 * g.float(), rtol=2 ** -7, atol=0)
 
 
+@pytest.mark.parametrize("rows,C", [(37, 100), (700, 513), (3, 40001)])
+def test_weight_of_32_bits_beside_16(cuda, rows, C):
+    # its gradient does not show the rounding of a 16-bit residual: the bound of a
+    # 32-bit sum of the terms
+    x, w, res = make(cuda, BF16, rows, C, BF16, F32, 8)
+    leaves = [t.detach().requires_grad_() for t in (x, w, res)]
+    dy = torch.randn(rows, C, generator=torch.Generator().manual_seed(4)).bfloat16().to(cuda)
+    out = cpab.rms_norm(*leaves)
+    got = torch.autograd.grad(out, leaves, (dy, torch.zeros_like(out[1])))
+    X, W, R, DY = (so.f64(t) for t in (x, w, res, dy))
+    _, rr, s = so.rms_norm(X, W, R)
+    want = so.rms_norm_grads(X, W, R, 1e-6, DY, None)
+    size = (DY * rr * s).abs().sum(0)
+    check(got[1], want[1], ((rows + 8) * U + (C / 128 + 16) * U) * size + U * want[1].abs(), "grad weight")
+    # the inputs are what is kept then: changed in place they are refused
+    out = cpab.rms_norm(*leaves)
+    with torch.no_grad():
+        leaves[2].mul_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out[0].sum().backward()
+
+
 def test_gradient_against_differences(cuda):
     # central differences of the kernel's own forward; with a step of 2^-7 the
     # third-order term is under 2^-12 of the derivative's scale
@@ -262,6 +284,20 @@ def test_side_stream_and_graph(cuda):
             torch.cuda.synchronize()
             assert torch.equal(q.view(torch.uint8), want[0].view(torch.uint8))
             assert torch.equal(scale, want[1]) and torch.equal(t, want[2])
+
+
+def test_nothing_is_left_behind(cuda):
+    # the sum is an output and kept for the backward: neither a dropped graph nor a used
+    # one holds it
+    x, w, r = make(cuda, BF16, 500, 1000, BF16, BF16, 9)
+    leaves = [t.detach().requires_grad_() for t in (x, w, r)]
+    dy = torch.ones_like(x)
+    torch.autograd.grad(cpab.rms_norm(*leaves), leaves, (dy, dy))
+    before = torch.cuda.memory_allocated()
+    for _ in range(5):
+        cpab.rms_norm(*leaves)
+        torch.autograd.grad(cpab.rms_norm(*leaves), leaves, (dy, dy))
+    assert torch.cuda.memory_allocated() == before
 
 
 def test_refusals(cuda):

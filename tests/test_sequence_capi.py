@@ -101,7 +101,8 @@ def _check_norm():
     _refused(lib.cpab_rms_norm_e4m3(0, 0, 0, 2, 4, P, 4, P, 4, P, 1e-6, P, None, P, None), "scale")
 
     def backward(rows=2, C=4, r=P, rstd=P, dw=None):
-        return lib.cpab_rms_norm_backward(0, 0, 0, rows, C, r, 4, rstd, P, P, 4, P, 4, P, P, dw, None, 0, None)
+        return lib.cpab_rms_norm_backward(0, 0, 0, rows, C, r, 4, None, 0, rstd, P, P, 4, P, 4, P, P, dw, None, 0,
+                                          None)
     _refused(backward(r=None), "r must not be NULL")
     _refused(backward(rstd=None), "rstd")
     need = lib.cpab_rms_norm_backward_workspace_size(100000, 64)
