@@ -215,10 +215,11 @@ rms_norm_forward_kernel(RmsNorm n, T* y, uint8_t* q, float* scale, R* residual_o
 }
 
 // Each workgroup takes every gridDim.x-th round of rows and adds up its part of dw in
-// registers; the parts, [gridDim.x, C], are joined by the next kernel in their order.
+// registers; the parts, [gridDim.x, C], are joined by the next kernel in their order, and
+// the part of a workgroup that is alone is the whole, `direct`.
 template <typename T, typename R, typename W, int V, int CH>
 __global__ void __launch_bounds__(kMaxLanes)
-rms_norm_backward_kernel(RmsNormGrad n, T* dx, R* dres, float* parts, int tpr) {
+rms_norm_backward_kernel(RmsNormGrad n, T* dx, R* dres, float* parts, W* direct, int tpr) {
   __shared__ float room[kMaxLanes / 64];
   extern __shared__ float sums[];   // [per - 1][tpr][CH][V], where rows share a workgroup
   const int lane = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr;
@@ -286,7 +287,7 @@ rms_norm_backward_kernel(RmsNormGrad n, T* dx, R* dres, float* parts, int tpr) {
       if (dres) store<V>(dres + row * n.C + p.at, d);
     }
   }
-  if (!parts) return;
+  if (!parts && !direct) return;
   if (per > 1) {
     // the other rows' lanes of the same channels, in their order
     if (group > 0) {
@@ -307,7 +308,11 @@ rms_norm_backward_kernel(RmsNormGrad n, T* dx, R* dres, float* parts, int tpr) {
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
     const Place p(k, tpr, lane, V, n.C);
-    if (p.again < V) store<V>(parts + (int64_t)blockIdx.x * n.C + p.at, dw[k]);
+    if (p.again >= V) continue;
+    if (direct)
+      store<V>(direct + p.at, dw[k]);
+    else
+      store<V>(parts + (int64_t)blockIdx.x * n.C + p.at, dw[k]);
   }
 }
 
@@ -481,21 +486,42 @@ hipError_t launch_rms_norm_forward(const RmsNorm& n, void* y, float* scale, void
   return hipGetLastError();
 }
 
-// Workgroups of the backward: the fewer, the fewer parts of dw to join.
-static int64_t backward_parts(int dtype, int64_t rows, int64_t C) {
-  const Layout l = layout(dtype, rows, C);
-  return l.wide ? workgroups(rows, kMaxLanes, 16) : workgroups(l.rounds, l.block, 16);
+// The backward's layout, with dw.  Rows that one workgroup goes through in four rounds are
+// one workgroup's, which saves the second launch (its host time, 6 us of 71 a pass).
+static Layout backward_layout(int dtype, int64_t rows, int64_t C) {
+  Layout l = layout(dtype, rows, C);
+  const int most = l.tpr < 64 ? 512 : kMaxLanes;   // 64 KiB of LDS for the other rows' sums
+  if (!l.wide && rows <= 4 * (most / l.tpr)) {
+    while (l.block < most && l.rounds > 1) {
+      l.block *= 2;
+      l.rounds = (rows + l.block / l.tpr - 1) / (l.block / l.tpr);
+    }
+  }
+  return l;
+}
+// Its workgroups: the fewer, the fewer parts of dw to join.
+static int64_t backward_parts(const Layout& l, int64_t rows) {
+  if (l.wide) return workgroups(rows, kMaxLanes, 16);
+  return l.rounds <= 4 ? 1 : workgroups(l.rounds, l.block, 16);
 }
 
 int64_t rms_norm_backward_workspace(int64_t rows, int64_t C) {
-  return std::max(backward_parts(CPAB_F32, rows, C), backward_parts(CPAB_BF16, rows, C)) * C * 4;
+  int64_t most = 0;
+  for (const int dtype : {CPAB_F32, CPAB_BF16}) {
+    const Layout l = backward_layout(dtype, rows, C);
+    const int64_t parts = backward_parts(l, rows);
+    if (l.wide || rows == 0 || parts > 1) most = std::max(most, parts);
+  }
+  return most * C * 4;
 }
 
 hipError_t launch_rms_norm_backward(const RmsNormGrad& n, void* grad_x, void* grad_residual,
                                     void* grad_weight, void* workspace, hipStream_t st) {
-  const Layout l = layout(n.dtype, n.rows, n.C);
-  const int64_t count = backward_parts(n.dtype, n.rows, n.C);
-  float* parts = grad_weight ? static_cast<float*>(workspace) : nullptr;
+  const Layout l = grad_weight ? backward_layout(n.dtype, n.rows, n.C) : layout(n.dtype, n.rows, n.C);
+  const int64_t count = grad_weight ? backward_parts(l, n.rows)
+                                    : workgroups(l.wide ? n.rows : l.rounds, l.wide ? kMaxLanes : l.block, 64);
+  const bool alone = grad_weight && !l.wide && n.rows > 0 && count == 1;
+  float* parts = grad_weight && !alone ? static_cast<float*>(workspace) : nullptr;
   if (parts && (l.wide || n.rows == 0)) {
     const hipError_t e = launch_fill(parts, count * n.C, 0.0f, st);
     if (e != hipSuccess) return e;
@@ -512,7 +538,7 @@ hipError_t launch_rms_norm_backward(const RmsNormGrad& n, void* grad_x, void* gr
         constexpr int V = decltype(v)::value, CH = decltype(ch)::value;
         const size_t lds = (size_t)(l.block / l.tpr - 1) * l.tpr * CH * V * 4;
         rms_norm_backward_kernel<T, R, W, V, CH><<<(unsigned)count, l.block, lds, st>>>(
-            n, (T*)grad_x, (R*)grad_residual, parts, l.tpr);
+            n, (T*)grad_x, (R*)grad_residual, parts, alone ? (W*)grad_weight : nullptr, l.tpr);
       });
     }
     if (parts)

@@ -27,9 +27,9 @@ Tensor samples_of(const Tensor& t) {
              ? d : d.contiguous();
 }
 
-// A gradient as the kernels take it, or none.
-Tensor grad_like(const Tensor& g, const Tensor& like) {
-  return g.defined() ? g.detach().to(like.scalar_type()) : Tensor();
+// A gradient of type `type`, or none.
+Tensor grad_of(const Tensor& g, at::ScalarType type) {
+  return !g.defined() || g.scalar_type() == type ? g : g.to(type);
 }
 
 bool any_grad(std::initializer_list<Tensor> ts) {
@@ -94,8 +94,9 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
                    &carries = saved[5];
       const c10::OptionalDeviceGuard guard(x.device());
       const int64_t B = x.size(0), T = x.size(1), C = x.size(2);
-      Tensor dy = grad_like(grads[0], x), dh = grads[1].defined() ? plain(grads[1].to(at::kFloat)) : Tensor();
+      Tensor dy = grad_of(grads[0], x.scalar_type()), dh = grad_of(grads[1], at::kFloat);
       if (dy.defined()) dy = dy.contiguous();
+      if (dh.defined()) dh = dh.contiguous();
       if (ctx->needs_input_grad(0)) dx = at::empty({B, T, C}, x.options());
       if (ctx->needs_input_grad(1)) df = at::empty({B, T, C}, x.options());
       // inputs that were not given have no place among those that may need a gradient
@@ -151,7 +152,7 @@ variable_list recurrence(const Tensor& x, const Tensor& f, const Maybe& g_, cons
 
 // [rows, C] with one stride over the rows, without a copy where that is possible.
 Tensor as_rows(const Tensor& t, int64_t C) {
-  const Tensor d = t.detach();
+  const Tensor d = t.requires_grad() ? t.detach() : t;
   const Tensor m = t.dim() == 2 ? d : d.reshape({-1, C});
   return C <= 1 || m.stride(1) == 1 ? m : m.contiguous();
 }
@@ -203,9 +204,9 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
       const bool same = dtype == r.scalar_type();
       const auto shape = grads[0].defined() ? grads[0].sizes().vec() : grads[1].sizes().vec();
       const auto options = r.options().dtype(dtype);
-      Tensor dy = grads[0].defined() ? as_rows(grads[0].to(dtype), C) : at::zeros({rows, C}, options);
+      Tensor dy = grads[0].defined() ? as_rows(grad_of(grads[0], dtype), C) : at::zeros({rows, C}, options);
       Tensor dout;
-      if (residual && grads[1].defined()) dout = as_rows(grads[1].to(r.scalar_type()), C);
+      if (residual && grads[1].defined()) dout = as_rows(grad_of(grads[1], r.scalar_type()), C);
       // one gradient for both where they have one type
       if (want_x || (want_res && same)) dx = at::empty(shape, options);
       if (want_res) dres = same ? dx : at::empty(shape, r.options());

@@ -8,6 +8,8 @@ products and the store a unit each.  So y carries e = (C / 128 + 16) u of its va
 the mean of u r s carries (C / 64 + 20) u of the mean of |u r s|, and a term of the
 weight's gradient 8 u before `rows` are added in some order: rows u of the sum of the
 terms' sizes.  r of 16 bits, as it is kept for the backward, is off by 2^-8."""
+import time
+
 import pytest
 import torch
 
@@ -292,12 +294,16 @@ def test_nothing_is_left_behind(cuda):
     x, w, r = make(cuda, BF16, 500, 1000, BF16, BF16, 9)
     leaves = [t.detach().requires_grad_() for t in (x, w, r)]
     dy = torch.ones_like(x)
-    torch.autograd.grad(cpab.rms_norm(*leaves), leaves, (dy, dy))
     before = torch.cuda.memory_allocated()
     for _ in range(5):
         cpab.rms_norm(*leaves)
         torch.autograd.grad(cpab.rms_norm(*leaves), leaves, (dy, dy))
-    assert torch.cuda.memory_allocated() == before
+    # the engine's thread lets go of the last pass's tensors a little after grad returns
+    for _ in range(100):
+        if torch.cuda.memory_allocated() <= before:
+            break
+        time.sleep(0.01)
+    assert torch.cuda.memory_allocated() <= before
 
 
 def test_refusals(cuda):
