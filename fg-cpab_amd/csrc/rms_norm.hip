@@ -487,7 +487,8 @@ hipError_t launch_rms_norm_forward(const RmsNorm& n, void* y, float* scale, void
 }
 
 // The backward's layout, with dw.  Rows that one workgroup goes through in four rounds are
-// one workgroup's, which saves the second launch (its host time, 6 us of 71 a pass).
+// one workgroup's, which saves the second launch: 64 x 1024 bfloat16, forward and backward,
+// 37 us a pass and 41 with it (32 x 4096, nearer the limit: 39.7 and 40.8).
 static Layout backward_layout(int dtype, int64_t rows, int64_t C) {
   Layout l = layout(dtype, rows, C);
   const int most = l.tpr < 64 ? 512 : kMaxLanes;   // 64 KiB of LDS for the other rows' sums

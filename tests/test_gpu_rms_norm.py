@@ -10,8 +10,6 @@ weight's gradient 8 u before `rows` are added in some order: rows u of the sum o
 terms' sizes.  r of 16 bits, as it is kept for the backward, is off by 2^-8."""
 import time
 
-import time
-
 import pytest
 import torch
 
