@@ -32,6 +32,13 @@ Tensor grad_of(const Tensor& g, at::ScalarType type) {
   return !g.defined() || g.scalar_type() == type ? g : g.to(type);
 }
 
+// Whether a gradient came at all: a function behind an output may have none to give.
+bool any_defined(const variable_list& grads) {
+  for (const Tensor& g : grads)
+    if (g.defined()) return true;
+  return false;
+}
+
 bool any_grad(std::initializer_list<Tensor> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor& t : ts)
@@ -86,6 +93,7 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
   }
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    if (!any_defined(grads)) return variable_list(6);
     Tensor dx, df, dg, dh0;
     {
       const at::NoGradGuard no_grad;
@@ -188,6 +196,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
   }
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    if (!any_defined(grads)) return variable_list(5);
     Tensor dx, dres, dw;
     {
       const at::NoGradGuard no_grad;

@@ -405,3 +405,21 @@ def test_empty(cuda):
         gx, gh = torch.autograd.grad((y, h), (x, h0), (torch.ones_like(y), torch.ones_like(h)))
         assert gx.shape == shape and (gh == 1).all()
     assert np.isfinite(float(h.sum()))
+
+class NoGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *outputs):
+        return sum(t.float().sum() for t in outputs)
+
+    @staticmethod
+    def backward(ctx, g):
+        return (None,) * len(ctx.needs_input_grad)
+
+
+def test_no_gradient_comes(cuda):
+    # what stands behind the outputs has no gradient to give: then neither has the scan
+    leaves = [torch.randn(2, 9, 4, device=cuda).requires_grad_() for _ in range(3)]
+    leaves.append(torch.randn(2, 4, device=cuda).requires_grad_())
+    out = cpab.gated_recurrence(*leaves)
+    grads = torch.autograd.grad(NoGradient.apply(*out), leaves, allow_unused=True)
+    assert all(g is None for g in grads)

@@ -329,3 +329,23 @@ def test_no_rows(cuda):
     y = cpab.rms_norm(x, w)
     gx, gw = torch.autograd.grad(y.sum(), (x, w))
     assert y.shape == (0, 8) and gx.shape == (0, 8) and (gw == 0).all()
+
+class NoGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *outputs):
+        return sum(t.float().sum() for t in outputs)
+
+    @staticmethod
+    def backward(ctx, g):
+        return (None,) * len(ctx.needs_input_grad)
+
+
+@pytest.mark.parametrize("residual", [False, True])
+def test_no_gradient_comes(cuda, residual):
+    # what stands behind the outputs has no gradient to give: then neither has the norm
+    x, r = (torch.randn(5, 8, device=cuda).requires_grad_() for _ in range(2))
+    w = torch.ones(8, device=cuda).requires_grad_()
+    out = cpab.rms_norm(x, w, r) if residual else (cpab.rms_norm(x, w),)
+    leaves = (x, w, r)[:3 if residual else 2]
+    grads = torch.autograd.grad(NoGradient.apply(*out), leaves, allow_unused=True)
+    assert all(g is None for g in grads)
