@@ -55,19 +55,25 @@ __device__ __forceinline__ float over_row(float v, int tpr, float* room, Op op) 
 __device__ __forceinline__ uint32_t to_e4m3(float v) {   // |v| <= 448 or NaN
   return __builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false) & 0xff;
 }
-// A row in 8 bits.  s cancels between y and its scale: with z = r w, y / scale is
-// z / (max |z| / 448), two roundings from the definition, and the scale max |z| s / 448.
+// A row in 8 bits.  s cancels between y and its scale: with s = m 2^k, m in [1, 2), and
+// z = (r 2^k) w, of y's size and one rounding from y / m, y / scale is
+// z / (max |z| / 448), two roundings from the definition, and the scale max |z| m / 448.
+__device__ __forceinline__ float power_of(float s) {   // 2^k; 0 and infinity stay, NaN is infinity
+  return __uint_as_float(__float_as_uint(s) & 0x7f800000u);
+}
 struct Eight {
-  float scale, by, inv;
+  float scale, up, by, inv;
   __device__ Eight(float top, float s) {   // top = max |z|
-    const float y = top * s;
+    const float y = top * __uint_as_float((__float_as_uint(s) & 0x7fffffu) | 0x3f800000u);
     scale = y == 0.0f ? 1.0f : y / 448.0f;
-    by = y == 0.0f ? 1.0f : top / 448.0f;
+    up = top < 0x1p-100f ? 0x1p100f : 1.0f;   // or 1 / by would pass the largest float
+    by = y == 0.0f ? 1.0f : top * up / 448.0f;
     inv = y == 0.0f ? 0.0f : 1.0f / by;
   }
   // z / by, the product's rounding taken back, so that what lies between two 8-bit
   // values falls to the nearer.
   __device__ __forceinline__ float value(float z) const {
+    z *= up;
     const float q = z * inv, v = fmaf(fmaf(-q, by, z), inv, q);
     return fabsf(v) > 448.0f ? copysignf(448.0f, v) : v;
   }
@@ -185,7 +191,7 @@ rms_norm_forward_kernel(RmsNorm n, T* y, uint8_t* q, float* scale, R* residual_o
       if (residual_out && live) store<V>(residual_out + row * n.C + p.at, r[k]);
     }
     sum = over_row(sum, tpr, room, Sum());
-    const float s = 1.0f / sqrtf(sum / (float)n.C + n.eps);
+    const float s = 1.0f / sqrtf(sum / (float)n.C + n.eps), by_s = EIGHT ? power_of(s) : s;
     if (rstd && live && lane == 0) rstd[row] = s;
     float top = 0.0f;
 #pragma unroll
@@ -194,7 +200,7 @@ rms_norm_forward_kernel(RmsNorm n, T* y, uint8_t* q, float* scale, R* residual_o
       if (p.again >= V) continue;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        r[k][e] = EIGHT ? r[k][e] * w[k][e] : r[k][e] * s * w[k][e];
+        r[k][e] = r[k][e] * by_s * w[k][e];
         if (EIGHT) top = Max()(fabsf(r[k][e]), top);
       }
       if (!EIGHT && live) store<V>(y + row * n.C + p.at, r[k]);
@@ -353,12 +359,12 @@ rms_norm_wide_forward_kernel(RmsNorm n, T* y, uint8_t* q, float* scale, R* resid
     float sum = 0.0f;
     for (int64_t c = threadIdx.x; c < n.C; c += kMaxLanes) sum += value(c) * value(c);
     sum = over_row(sum, kMaxLanes, room, Sum());
-    const float s = 1.0f / sqrtf(sum / (float)n.C + n.eps);
+    const float s = 1.0f / sqrtf(sum / (float)n.C + n.eps), by_s = EIGHT ? power_of(s) : s;
     if (rstd && threadIdx.x == 0) rstd[row] = s;
     float top = 0.0f;
     if (EIGHT) {
       for (int64_t c = threadIdx.x; c < n.C; c += kMaxLanes)
-        top = Max()(fabsf(value(c) * to_float(w[c])), top);
+        top = Max()(fabsf(value(c) * by_s * to_float(w[c])), top);
       top = over_row(top, kMaxLanes, room, Max());
     }
     const Eight by(top, s);
@@ -366,9 +372,9 @@ rms_norm_wide_forward_kernel(RmsNorm n, T* y, uint8_t* q, float* scale, R* resid
     for (int64_t c = threadIdx.x; c < n.C; c += kMaxLanes) {
       const float r = value(c);
       if (EIGHT)
-        q[row * n.C + c] = (uint8_t)to_e4m3(by.value(r * to_float(w[c])));
+        q[row * n.C + c] = (uint8_t)to_e4m3(by.value(r * by_s * to_float(w[c])));
       else
-        y[row * n.C + c] = from_float<T>(r * s * to_float(w[c]));
+        y[row * n.C + c] = from_float<T>(r * by_s * to_float(w[c]));
       if (residual_out) residual_out[row * n.C + c] = from_float<R>(r);
     }
   }

@@ -130,6 +130,26 @@ def test_zero_rows_and_tiny_ones(cuda):
     assert (cpab.rms_norm(z, w[:4]) == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("C", [100, 20000])
+@pytest.mark.parametrize("size,weight,eps", [(1e-37, 1.0, 1e-6), (1e-15, 1e-27, 1e-32),
+                                             (1e-19, 1e19, 1e-30), (1e17, 1e22, 1e-6), (1.0, 1e-33, 1e-6)])
+def test_8_bits_of_sizes_at_the_types_ends(cuda, dtype, C, size, weight, eps):
+    # rows whose norm and scale 32 bits hold as normal numbers, and r, r w or its inverse not
+    # in between: the bounds of compare(), and what rounding below 2^-126 adds to r w
+    x = (torch.randn(3, C, device=cuda) * size).to(dtype)
+    w = ((torch.rand(C, device=cuda) + 0.5) * weight).to(dtype)
+    q, scale = cpab.rms_norm(x, w, eps=eps, out_dtype=E4M3)
+    ry = so.rms_norm(so.f64(x), so.f64(w), None, eps)[0]
+    e = (C / 128 + 16) * U
+    top = ry.abs().amax(-1) / 448
+    assert (top > 2.0 ** -126).all()
+    check(scale, top, (e + 4 * U) * top + 2.0 ** -148, "scale")
+    value = so.f64(q.float()) * so.f64(scale)[:, None]
+    check(value, ry, (2.0 ** -4 + 4 * e) * ry.abs() + 2.0 ** -10 * so.f64(scale)[:, None] * (1 + e), "8 bits")
+    assert (so.f64(q.float()).abs() <= 448).all()
+
+
 def test_not_finite_rows(cuda):
     x = torch.randn(6, 70, device=cuda)
     w = torch.ones(70, device=cuda)
