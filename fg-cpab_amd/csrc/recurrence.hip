@@ -318,98 +318,98 @@ recurrence_forward_kernel(Recurrence r, Tiling s, T* y, float* h_last, float* ca
   const Join<V> join(s, room, &nearest, seg, lane);
   const float none[V] = {};
   const unsigned mine = take_tile(counter, &mine_of);
-    const unsigned tile = mine / s.chains, chain = mine - tile * s.chains;
-    const unsigned block = chain / s.across;
-    const int64_t b = block;
-    // lanes beyond the last channels repeat those
-    const int64_t c = min((int64_t)((chain - block * s.across) * s.lanes + lane) * V, r.C - V);
-    const int64_t n = row_length(r, b), t0 = (int64_t)tile * (s.segs * L), t1 = t0 + s.segs * L;
-    const int64_t ts = t0 + seg * L;
-    const int rest = (int)min((int64_t)L, r.T - ts);   // of the lane's samples those in T,
-    const int live = (int)min((int64_t)L, n - ts);     // and those in the row (none: <= 0)
-    Walk<T> out(y + (b * r.T + t0) * r.C, r.C);
-    const uint32_t at = offset<T>(seg * L, r.C, c);
-    // a tile that is whole, the usual one, needs no question at each sample
-    const auto work = [&](auto whole) {
-      constexpr bool full = decltype(whole)::value;
-      float a[L][V], u[L][V];
-      Raw<T, V> rf[L], rx[L], g[L];   // no sample: a gate that keeps the state
-      Walk<T> x(static_cast<const T*>(r.x) + b * r.xb + t0 * r.xt, r.xt);
-      Walk<T> f(static_cast<const T*>(r.f) + b * r.fb + t0 * r.ft, r.ft);
-      Walk<T> gp(GATE ? static_cast<const T*>(r.g) + b * r.gb + t0 * r.gt : nullptr, r.gt);
-      const uint32_t atx = offset<T>(seg * L, r.xt, c), atf = offset<T>(seg * L, r.ft, c);
-      const uint32_t atg = offset<T>(seg * L, r.gt, c);
+  const unsigned tile = mine / s.chains, chain = mine - tile * s.chains;
+  const unsigned block = chain / s.across;
+  const int64_t b = block;
+  // lanes beyond the last channels repeat those
+  const int64_t c = min((int64_t)((chain - block * s.across) * s.lanes + lane) * V, r.C - V);
+  const int64_t n = row_length(r, b), t0 = (int64_t)tile * (s.segs * L), t1 = t0 + s.segs * L;
+  const int64_t ts = t0 + seg * L;
+  const int rest = (int)min((int64_t)L, r.T - ts);   // of the lane's samples those in T,
+  const int live = (int)min((int64_t)L, n - ts);     // and those in the row (none: <= 0)
+  Walk<T> out(y + (b * r.T + t0) * r.C, r.C);
+  const uint32_t at = offset<T>(seg * L, r.C, c);
+  // a tile that is whole, the usual one, needs no question at each sample
+  const auto work = [&](auto whole) {
+    constexpr bool full = decltype(whole)::value;
+    float a[L][V], u[L][V];
+    Raw<T, V> rf[L], rx[L], g[L];   // no sample: a gate that keeps the state
+    Walk<T> x(static_cast<const T*>(r.x) + b * r.xb + t0 * r.xt, r.xt);
+    Walk<T> f(static_cast<const T*>(r.f) + b * r.fb + t0 * r.ft, r.ft);
+    Walk<T> gp(GATE ? static_cast<const T*>(r.g) + b * r.gb + t0 * r.gt : nullptr, r.gt);
+    const uint32_t atx = offset<T>(seg * L, r.xt, c), atf = offset<T>(seg * L, r.ft, c);
+    const uint32_t atg = offset<T>(seg * L, r.gt, c);
 #pragma unroll
-      for (int j = 0; j < L; ++j) {
-        rf[j] = Raw<T, V>::all(INFINITY);
-        rx[j] = g[j] = Raw<T, V>::all(0.0f);
-        if (full || j < live) {
-          rf[j] = load<T, V>(f, atf);
-          rx[j] = load<T, V>(x, atx);
-          if (GATE) g[j] = load<T, V>(gp, atg);
-        }
-        f.next(), x.next();
-        if (GATE) gp.next();
+    for (int j = 0; j < L; ++j) {
+      rf[j] = Raw<T, V>::all(INFINITY);
+      rx[j] = g[j] = Raw<T, V>::all(0.0f);
+      if (full || j < live) {
+        rf[j] = load<T, V>(f, atf);
+        rx[j] = load<T, V>(x, atx);
+        if (GATE) g[j] = load<T, V>(gp, atg);
       }
-      float A[V], B[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) A[v] = 1.0f, B[v] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < L; ++j)
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const Gate k = sigmoids(rf[j][v]);
-          a[j][v] = k.pos;
-          u[j][v] = k.neg * rx[j][v];
-          B[v] = fmaf(k.pos, B[v], u[j][v]);
-          A[v] *= k.pos;
-        }
-#pragma unroll
-      for (int v = 0; v < V; ++v) join.at(seg, v) = make_float2(A[v], B[v]);
-      float h[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = r.h0 ? r.h0[b * r.C + c + v] : 0.0f;
-      lds_barrier();
-      const bool follows = t1 < n;   // a live tile comes after this one
-      if (s.tiles > 1)
-        join.state_before((int)tile, follows, 0, 1, words + (int64_t)chain * s.tiles * join.slots,
-                          flags + chain * s.tiles, h);
-      join.to_segment(0, seg, 1, h);
-      if (carries) {   // where a tile of the backward begins, at the start of a segment
-        const int span = back.segs * backward_steps(V);
-        if (ts % span == 0 && ts < r.T)
-#pragma unroll
-          for (int v = 0; v < V; ++v)
-            carries[(b * (int64_t)back.tiles + ts / span) * r.C + c + v] = h[v];
-      }
-#pragma unroll
-      for (int j = 0; j < L; ++j) {
-        float o[V];
-        if (GATE) g[j].hold();
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          h[v] = fmaf(a[j][v], h[v], u[j][v]);
-          o[v] = GATE ? h[v] * (g[j][v] * sigmoids(g[j][v]).pos) : h[v];
-        }
-        if (full || j < live)
-          store<T, V>(out, at, o);
-        else if (j < rest)
-          store<T, V>(out, at, none);
-        out.next();
-      }
-      if (!follows && seg == s.segs - 1) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) h_last[b * r.C + c + v] = h[v];
-      }
-    };
-    if (t0 >= n && tile > 0) {   // behind the row's end
-      for (int j = 0; j < L; ++j, out.next())
-        if (j < rest) store<T, V>(out, at, none);
-    } else if (t1 <= n) {
-      work(std::true_type());
-    } else {
-      work(std::false_type());
+      f.next(), x.next();
+      if (GATE) gp.next();
     }
+    float A[V], B[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) A[v] = 1.0f, B[v] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < L; ++j)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const Gate k = sigmoids(rf[j][v]);
+        a[j][v] = k.pos;
+        u[j][v] = k.neg * rx[j][v];
+        B[v] = fmaf(k.pos, B[v], u[j][v]);
+        A[v] *= k.pos;
+      }
+#pragma unroll
+    for (int v = 0; v < V; ++v) join.at(seg, v) = make_float2(A[v], B[v]);
+    float h[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = r.h0 ? r.h0[b * r.C + c + v] : 0.0f;
+    lds_barrier();
+    const bool follows = t1 < n;   // a live tile comes after this one
+    if (s.tiles > 1)
+      join.state_before((int)tile, follows, 0, 1, words + (int64_t)chain * s.tiles * join.slots,
+                        flags + chain * s.tiles, h);
+    join.to_segment(0, seg, 1, h);
+    if (carries) {   // where a tile of the backward begins, at the start of a segment
+      const int span = back.segs * backward_steps(V);
+      if (ts % span == 0 && ts < r.T)
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          carries[(b * (int64_t)back.tiles + ts / span) * r.C + c + v] = h[v];
+    }
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      float o[V];
+      if (GATE) g[j].hold();
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        h[v] = fmaf(a[j][v], h[v], u[j][v]);
+        o[v] = GATE ? h[v] * (g[j][v] * sigmoids(g[j][v]).pos) : h[v];
+      }
+      if (full || j < live)
+        store<T, V>(out, at, o);
+      else if (j < rest)
+        store<T, V>(out, at, none);
+      out.next();
+    }
+    if (!follows && seg == s.segs - 1) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) h_last[b * r.C + c + v] = h[v];
+    }
+  };
+  if (t0 >= n && tile > 0) {   // behind the row's end
+    for (int j = 0; j < L; ++j, out.next())
+      if (j < rest) store<T, V>(out, at, none);
+  } else if (t1 <= n) {
+    work(std::true_type());
+  } else {
+    work(std::false_type());
+  }
 }
 
 template <typename T, int V, bool GATE>
@@ -425,146 +425,146 @@ recurrence_backward_kernel(Recurrence r, Tiling s, const float* carries, const T
   const Join<V> join(s, room, &nearest, seg, lane);
   const float none[V] = {};
   const unsigned mine = take_tile(counter, &mine_of);
-    const unsigned order = mine / s.chains, chain = mine - order * s.chains;
-    const unsigned tile = s.tiles - 1 - order, block = chain / s.across;
-    const int64_t b = block;
-    const int64_t c = min((int64_t)((chain - block * s.across) * s.lanes + lane) * V, r.C - V);
-    const int64_t n = row_length(r, b), t0 = (int64_t)tile * (s.segs * L), t1 = t0 + s.segs * L;
-    const int64_t ts = t0 + seg * L;
-    const int rest = (int)min((int64_t)L, r.T - ts), live = (int)min((int64_t)L, n - ts);
-    const int64_t row = (b * r.T + t0) * r.C;
-    const uint32_t at = offset<T>(seg * L, r.C, c);
-    const auto work = [&](auto whole) {
-      constexpr bool full = decltype(whole)::value;
-      Raw<T, V> rf[L], x[L], g[L], rd[L];
-      Walk<T> xp(static_cast<const T*>(r.x) + b * r.xb + t0 * r.xt, r.xt);
-      Walk<T> fp(static_cast<const T*>(r.f) + b * r.fb + t0 * r.ft, r.ft);
-      Walk<T> gp(GATE ? static_cast<const T*>(r.g) + b * r.gb + t0 * r.gt : nullptr, r.gt);
-      Walk<T> dyp(dy + row, r.C), dgp(dg + row, r.C);
-      const uint32_t atx = offset<T>(seg * L, r.xt, c), atf = offset<T>(seg * L, r.ft, c);
-      const uint32_t atg = offset<T>(seg * L, r.gt, c);
+  const unsigned order = mine / s.chains, chain = mine - order * s.chains;
+  const unsigned tile = s.tiles - 1 - order, block = chain / s.across;
+  const int64_t b = block;
+  const int64_t c = min((int64_t)((chain - block * s.across) * s.lanes + lane) * V, r.C - V);
+  const int64_t n = row_length(r, b), t0 = (int64_t)tile * (s.segs * L), t1 = t0 + s.segs * L;
+  const int64_t ts = t0 + seg * L;
+  const int rest = (int)min((int64_t)L, r.T - ts), live = (int)min((int64_t)L, n - ts);
+  const int64_t row = (b * r.T + t0) * r.C;
+  const uint32_t at = offset<T>(seg * L, r.C, c);
+  const auto work = [&](auto whole) {
+    constexpr bool full = decltype(whole)::value;
+    Raw<T, V> rf[L], x[L], g[L], rd[L];
+    Walk<T> xp(static_cast<const T*>(r.x) + b * r.xb + t0 * r.xt, r.xt);
+    Walk<T> fp(static_cast<const T*>(r.f) + b * r.fb + t0 * r.ft, r.ft);
+    Walk<T> gp(GATE ? static_cast<const T*>(r.g) + b * r.gb + t0 * r.gt : nullptr, r.gt);
+    Walk<T> dyp(dy + row, r.C), dgp(dg + row, r.C);
+    const uint32_t atx = offset<T>(seg * L, r.xt, c), atf = offset<T>(seg * L, r.ft, c);
+    const uint32_t atg = offset<T>(seg * L, r.gt, c);
 #pragma unroll
-      for (int j = 0; j < L; ++j) {
-        rf[j] = Raw<T, V>::all(INFINITY);
-        x[j] = g[j] = rd[j] = Raw<T, V>::all(0.0f);
-        if (full || j < live) {
-          rf[j] = load<T, V>(fp, atf);
-          x[j] = load<T, V>(xp, atx);
-          if (GATE) g[j] = load<T, V>(gp, atg);
-          if (dy) rd[j] = load<T, V>(dyp, at);
-        }
-        fp.next(), xp.next(), dyp.next();
-        if (GATE) gp.next();
+    for (int j = 0; j < L; ++j) {
+      rf[j] = Raw<T, V>::all(INFINITY);
+      x[j] = g[j] = rd[j] = Raw<T, V>::all(0.0f);
+      if (full || j < live) {
+        rf[j] = load<T, V>(fp, atf);
+        x[j] = load<T, V>(xp, atx);
+        if (GATE) g[j] = load<T, V>(gp, atg);
+        if (dy) rd[j] = load<T, V>(dyp, at);
       }
-      float A[V], B[V], h[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) A[v] = 1.0f, B[v] = 0.0f;
-#pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = carries[(b * (int64_t)s.tiles + tile) * r.C + c + v];
-#pragma unroll
-      for (int j = 0; j < L; ++j) {
-        rf[j].hold(), x[j].hold();
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const Gate q = sigmoids(rf[j][v]);
-          B[v] = fmaf(q.pos, B[v], q.neg * x[j][v]);
-          A[v] *= q.pos;
-        }
-      }
-#pragma unroll
-      for (int v = 0; v < V; ++v) join.at(seg, v) = make_float2(A[v], B[v]);
-      lds_barrier();
-      join.to_segment(0, seg, 1, h);
-      // Through the samples: dg; k the gate's complement, f (h_{t-1} - x) a (1 - a), d
-      // what reaches h_t.  The gates are computed again (two registers a value less
-      // across the join), and from here on a is 1 - k, off by a rounding of 1 as l is.
-      float k[L][V], f[L][V], d[L][V];
-#pragma unroll
-      for (int j = 0; j < L; ++j) {
-        float o[V];
-        rf[j].hold(), x[j].hold(), rd[j].hold();
-        if (GATE) g[j].hold();
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const Gate q = sigmoids(rf[j][v]);
-          k[j][v] = q.neg;
-          f[j][v] = (h[v] - x[j][v]) * (q.pos * q.neg);
-          h[v] = fmaf(q.pos, h[v], q.neg * x[j][v]);
-          if (GATE) {
-            const Gate z = sigmoids(g[j][v]);
-            o[v] = rd[j][v] * h[v] * z.pos * fmaf(g[j][v], z.neg, 1.0f);
-            d[j][v] = rd[j][v] * (g[j][v] * z.pos);
-          } else {
-            d[j][v] = rd[j][v];
-          }
-          // here and not where it is used: the parts would take more registers
-          asm volatile("" : "+v"(f[j][v]), "+v"(d[j][v]));
-        }
-        if (GATE && dg) {
-          if (full || j < live)
-            store<T, V>(dgp, at, o);
-          else if (j < rest)
-            store<T, V>(dgp, at, none);
-        }
-        if (GATE) dgp.next();
-      }
-      // what a segment hands to the sample before it: A (what it is handed) + B
-#pragma unroll
-      for (int v = 0; v < V; ++v) B[v] = 0.0f;
-#pragma unroll
-      for (int j = L - 1; j >= 0; --j)
-#pragma unroll
-        for (int v = 0; v < V; ++v) B[v] = (1.0f - k[j][v]) * (B[v] + d[j][v]);
-      lds_barrier();
-#pragma unroll
-      for (int v = 0; v < V; ++v) join.at(seg, v) = make_float2(A[v], B[v]);
-      float l[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) l[v] = dh_last ? dh_last[b * r.C + c + v] : 0.0f;
-      lds_barrier();
-      if (s.tiles > 1) {
-        const int span = s.segs * L;
-        const int after = n > 0 ? (int)((n - 1) / span) - (int)tile : 0;   // live tiles after it
-        join.state_before(after, tile > 0, s.segs - 1, -1,
-                          words + (int64_t)chain * s.tiles * join.slots, flags + chain * s.tiles, l);
-      }
-      join.to_segment(s.segs - 1, s.segs - 1 - seg, -1, l);
-      Walk<T> dxp(dx + row + (L - 1) * r.C, -r.C), dfp(df + row + (L - 1) * r.C, -r.C);
-#pragma unroll
-      for (int j = L - 1; j >= 0; --j) {
-        float ox[V], of[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          l[v] += d[j][v];
-          ox[v] = k[j][v] * l[v];
-          of[v] = l[v] * f[j][v];
-          l[v] *= 1.0f - k[j][v];
-        }
-        const bool in = full || j < live;
-        if (full || j < rest) {
-          if (dx) store<T, V>(dxp, at, in ? ox : none);
-          if (df) store<T, V>(dfp, at, in ? of : none);
-        }
-        dxp.next(), dfp.next();
-      }
-      if (dh0 && tile == 0 && seg == 0) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) dh0[b * r.C + c + v] = l[v];
-      }
-    };
-    if (t0 >= n && tile > 0) {
-      Walk<T> dxp(dx + row, r.C), dfp(df + row, r.C), dgp(dg + row, r.C);
-      for (int j = 0; j < L; ++j, dxp.next(), dfp.next(), dgp.next()) {
-        if (j >= rest) continue;
-        if (dx) store<T, V>(dxp, at, none);
-        if (df) store<T, V>(dfp, at, none);
-        if (GATE && dg) store<T, V>(dgp, at, none);
-      }
-    } else if (t1 <= n) {
-      work(std::true_type());
-    } else {
-      work(std::false_type());
+      fp.next(), xp.next(), dyp.next();
+      if (GATE) gp.next();
     }
+    float A[V], B[V], h[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) A[v] = 1.0f, B[v] = 0.0f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = carries[(b * (int64_t)s.tiles + tile) * r.C + c + v];
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      rf[j].hold(), x[j].hold();
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const Gate q = sigmoids(rf[j][v]);
+        B[v] = fmaf(q.pos, B[v], q.neg * x[j][v]);
+        A[v] *= q.pos;
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) join.at(seg, v) = make_float2(A[v], B[v]);
+    lds_barrier();
+    join.to_segment(0, seg, 1, h);
+    // Through the samples: dg; k the gate's complement, f (h_{t-1} - x) a (1 - a), d
+    // what reaches h_t.  The gates are computed again (two registers a value less
+    // across the join), and from here on a is 1 - k, off by a rounding of 1 as l is.
+    float k[L][V], f[L][V], d[L][V];
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      float o[V];
+      rf[j].hold(), x[j].hold(), rd[j].hold();
+      if (GATE) g[j].hold();
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const Gate q = sigmoids(rf[j][v]);
+        k[j][v] = q.neg;
+        f[j][v] = (h[v] - x[j][v]) * (q.pos * q.neg);
+        h[v] = fmaf(q.pos, h[v], q.neg * x[j][v]);
+        if (GATE) {
+          const Gate z = sigmoids(g[j][v]);
+          o[v] = rd[j][v] * h[v] * z.pos * fmaf(g[j][v], z.neg, 1.0f);
+          d[j][v] = rd[j][v] * (g[j][v] * z.pos);
+        } else {
+          d[j][v] = rd[j][v];
+        }
+        // here and not where it is used: the parts would take more registers
+        asm volatile("" : "+v"(f[j][v]), "+v"(d[j][v]));
+      }
+      if (GATE && dg) {
+        if (full || j < live)
+          store<T, V>(dgp, at, o);
+        else if (j < rest)
+          store<T, V>(dgp, at, none);
+      }
+      if (GATE) dgp.next();
+    }
+    // what a segment hands to the sample before it: A (what it is handed) + B
+#pragma unroll
+    for (int v = 0; v < V; ++v) B[v] = 0.0f;
+#pragma unroll
+    for (int j = L - 1; j >= 0; --j)
+#pragma unroll
+      for (int v = 0; v < V; ++v) B[v] = (1.0f - k[j][v]) * (B[v] + d[j][v]);
+    lds_barrier();
+#pragma unroll
+    for (int v = 0; v < V; ++v) join.at(seg, v) = make_float2(A[v], B[v]);
+    float l[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) l[v] = dh_last ? dh_last[b * r.C + c + v] : 0.0f;
+    lds_barrier();
+    if (s.tiles > 1) {
+      const int span = s.segs * L;
+      const int after = n > 0 ? (int)((n - 1) / span) - (int)tile : 0;   // live tiles after it
+      join.state_before(after, tile > 0, s.segs - 1, -1,
+                        words + (int64_t)chain * s.tiles * join.slots, flags + chain * s.tiles, l);
+    }
+    join.to_segment(s.segs - 1, s.segs - 1 - seg, -1, l);
+    Walk<T> dxp(dx + row + (L - 1) * r.C, -r.C), dfp(df + row + (L - 1) * r.C, -r.C);
+#pragma unroll
+    for (int j = L - 1; j >= 0; --j) {
+      float ox[V], of[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        l[v] += d[j][v];
+        ox[v] = k[j][v] * l[v];
+        of[v] = l[v] * f[j][v];
+        l[v] *= 1.0f - k[j][v];
+      }
+      const bool in = full || j < live;
+      if (full || j < rest) {
+        if (dx) store<T, V>(dxp, at, in ? ox : none);
+        if (df) store<T, V>(dfp, at, in ? of : none);
+      }
+      dxp.next(), dfp.next();
+    }
+    if (dh0 && tile == 0 && seg == 0) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) dh0[b * r.C + c + v] = l[v];
+    }
+  };
+  if (t0 >= n && tile > 0) {
+    Walk<T> dxp(dx + row, r.C), dfp(df + row, r.C), dgp(dg + row, r.C);
+    for (int j = 0; j < L; ++j, dxp.next(), dfp.next(), dgp.next()) {
+      if (j >= rest) continue;
+      if (dx) store<T, V>(dxp, at, none);
+      if (df) store<T, V>(dfp, at, none);
+      if (GATE && dg) store<T, V>(dgp, at, none);
+    }
+  } else if (t1 <= n) {
+    work(std::true_type());
+  } else {
+    work(std::false_type());
+  }
 }
 
 int pow2_at_least(int64_t n, int most) {
