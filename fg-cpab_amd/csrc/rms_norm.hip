@@ -70,10 +70,9 @@ struct Eight {
     by = y == 0.0f ? 1.0f : top * up / 448.0f;
     inv = y == 0.0f ? 0.0f : 1.0f / by;
   }
-  // z / by, the product's rounding taken back, so that what lies between two 8-bit
-  // values falls to the nearer.
+  // z / by, of z times `up`, the product's rounding taken back, so that what lies between
+  // two 8-bit values falls to the nearer.
   __device__ __forceinline__ float value(float z) const {
-    z *= up;
     const float q = z * inv, v = fmaf(fmaf(-q, by, z), inv, q);
     return fabsf(v) > 448.0f ? copysignf(448.0f, v) : v;
   }
@@ -209,6 +208,12 @@ rms_norm_forward_kernel(RmsNorm n, T* y, uint8_t* q, float* scale, R* residual_o
     top = over_row(top, tpr, room, Max());
     const Eight by(top, s);
     if (live && lane == 0) scale[row] = by.scale;
+    if (by.up != 1.0f) {   // hardly ever
+#pragma unroll
+      for (int k = 0; k < CH; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) r[k][e] *= by.up;
+    }
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       const Place p(k, tpr, lane, V, n.C);
@@ -372,7 +377,7 @@ rms_norm_wide_forward_kernel(RmsNorm n, T* y, uint8_t* q, float* scale, R* resid
     for (int64_t c = threadIdx.x; c < n.C; c += kMaxLanes) {
       const float r = value(c);
       if (EIGHT)
-        q[row * n.C + c] = (uint8_t)to_e4m3(by.value(r * by_s * to_float(w[c])));
+        q[row * n.C + c] = (uint8_t)to_e4m3(by.value(r * by_s * to_float(w[c]) * by.up));
       else
         y[row * n.C + c] = from_float<T>(r * by_s * to_float(w[c]));
       if (residual_out) residual_out[row * n.C + c] = from_float<R>(r);
