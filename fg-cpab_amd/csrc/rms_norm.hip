@@ -9,8 +9,8 @@
 // rounding (0.0017 of its value), x and the residual again.
 //
 // Bound by memory: each value is read once and written once.  A row is held in the
-// registers of `tpr` lanes (a power of two, so that a narrow row does not leave a wave
-// idle and a wide one is spread over many), in pieces of V neighbouring values (16
+// registers of `tpr` lanes (a part of a wave, so that a narrow row does not leave one
+// idle, or several waves), in pieces of V neighbouring values (16
 // bytes); the sums go over the lanes by shuffles and, beyond a wave, LDS.  Rows wider
 // than the registers of the largest workgroup are read again from the cache instead.
 #include <hip/hip_runtime.h>
@@ -45,7 +45,7 @@ __device__ __forceinline__ float over_row(float v, int tpr, float* room, Op op) 
     __syncthreads();
     if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = v;
     __syncthreads();
-    const int waves = tpr >> 6, first = (threadIdx.x >> 6) & ~(waves - 1);
+    const int waves = tpr >> 6, first = (int)(threadIdx.x >> 6) / waves * waves;
     v = room[first];
     for (int w = 1; w < waves; ++w) v = op(v, room[first + w]);
   }
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kMaxLanes)
 rms_norm_forward_kernel(RmsNorm n, T* y, uint8_t* q, float* scale, R* residual_out, float* rstd,
                         int tpr) {
   __shared__ float room[kMaxLanes / 64];
-  const int lane = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr;
+  const int group = threadIdx.x / tpr, lane = threadIdx.x - group * tpr;
   const int per = blockDim.x / tpr;
   const int64_t rounds = (n.rows + per - 1) / per;
   float w[CH][V];
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kMaxLanes)
 rms_norm_backward_kernel(RmsNormGrad n, T* dx, R* dres, float* parts, W* direct, int tpr) {
   __shared__ float room[kMaxLanes / 64];
   extern __shared__ float sums[];   // [per - 1][tpr][CH][V], where rows share a workgroup
-  const int lane = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr;
+  const int group = threadIdx.x / tpr, lane = threadIdx.x - group * tpr;
   const int per = blockDim.x / tpr;
   const int64_t rounds = (n.rows + per - 1) / per;
   float w[CH][V], dw[CH][V];
@@ -418,24 +418,44 @@ rms_norm_wide_backward_kernel(RmsNormGrad n, T* dx, R* dres, float* parts) {
 
 // How a launch lays rows on lanes.
 struct Layout {
-  int V, CH, tpr, block;
-  int64_t rounds;   // of rows, one workgroup each
+  int V, CH, tpr, block;   // tpr: a power of two up to a wave, or whole waves
+  int64_t rounds;          // of rows, one workgroup each
   bool wide;
 };
-Layout layout(int dtype, int64_t rows, int64_t C) {
+// Few lanes with several pieces each leave few idle where a width is not a power of two,
+// and make more workgroups to a compute unit; the registers bound what a lane holds, the
+// backward's most.  2^27 values, us, by the most pieces to a lane (2, 3, 4):
+//   forward to 8 bits, float32    333: 285, 201, 201    4096: 227, 226, 176
+//                      bfloat16   333: 140, 118, 117    4096: 112, 112, 119
+//   backward,          float32    333: 346, 304, 304    4096: 284, 285, 292
+//                      bfloat16   333: 178, 227, 226    4096: 158, 157, 395
+// In the forward 32 values to a lane come before 1024 lanes, of which one workgroup alone
+// finds room (16384, 8 bits: 190 us in 32 bits, 245 with 16; bfloat16 129 and 173).
+Layout layout(int dtype, int64_t rows, int64_t C, bool backward) {
   Layout l;
-  l.V = dtype == CPAB_F32 ? 4 : 8;
+  const bool f32 = dtype == CPAB_F32;
+  l.V = f32 ? 4 : 8;
+  const int most = (f32 ? 4 : 3) - backward, cap = backward ? 4 : 32 / l.V;
   if (C < l.V) l.V = 1;
   const int64_t pieces = (C + l.V - 1) / l.V;
-  // two pieces a lane where there are that many (32768 x 1024 bfloat16, backward: 46.6 us,
-  // 51.3 with one, 144 with four, whose registers spill)
-  l.tpr = 8;
-  while (l.tpr < kMaxLanes && (int64_t)l.tpr * 2 < pieces) l.tpr *= 2;
+  const auto lanes = [&](int each) {
+    int n = 8;
+    while (n < kMaxLanes && (int64_t)n * each < pieces) n *= 2;
+    return n;
+  };
+  l.tpr = lanes(most);
+  if (l.tpr == kMaxLanes) l.tpr = lanes(backward ? most : cap);
   const int64_t each = (pieces + l.tpr - 1) / l.tpr;
-  l.CH = each <= 1 ? 1 : each <= 2 ? 2 : 4;
-  l.wide = each > 4;
-  l.block = std::max(l.tpr, kMinBlock);
-  const int per = l.block / l.tpr;
+  l.wide = each > cap;
+  l.CH = (int)std::min<int64_t>(each <= 4 ? each : each <= 6 ? 6 : 8, cap);
+  if (backward && !f32 && l.CH == 2 && l.tpr > 64 && 3 * pieces < 4 * (int64_t)l.tpr && pieces <= kMaxLanes) {
+    // less than two thirds of the pieces that the lanes have room for: one piece a lane, as
+    // many waves as that takes (4200: 160 us, 201; 5000: 160, 189; 6000, not so: 179, 172)
+    l.CH = 1;
+    l.tpr = (int)((pieces + 63) / 64 * 64);
+  }
+  const int per = std::max(1, kMinBlock / l.tpr);
+  l.block = l.tpr * per;
   l.rounds = (rows + per - 1) / per;
   return l;
 }
@@ -449,15 +469,20 @@ void with_types(int dtype, int residual, int weight, F f) {
   return weight == CPAB_F32 ? f(bf16(), bf16(), 0.0f) : f(bf16(), bf16(), bf16());
 }
 // f(V, CH) as constants.
-template <typename T, typename F>
+template <typename T, bool BACKWARD, typename F>
 void with_layout(const Layout& l, F f) {
   constexpr int V = 16 / (int)sizeof(T);
-  typedef std::integral_constant<int, V> Many;
+  const auto many = [&](auto ch) { f(std::integral_constant<int, V>(), ch); };
   typedef std::integral_constant<int, 1> One;
   if (l.V == 1) return f(One(), One());   // C < V: at most 8 lanes' worth
-  if (l.CH == 1) return f(Many(), One());
-  if (l.CH == 2) return f(Many(), std::integral_constant<int, 2>());
-  f(Many(), std::integral_constant<int, 4>());
+  if (l.CH == 1) return many(One());
+  if (l.CH == 2) return many(std::integral_constant<int, 2>());
+  if (l.CH == 3) return many(std::integral_constant<int, 3>());
+  if constexpr (V == 4 && !BACKWARD) {
+    if (l.CH == 6) return many(std::integral_constant<int, 6>());
+    if (l.CH == 8) return many(std::integral_constant<int, 8>());
+  }
+  many(std::integral_constant<int, 4>());
 }
 
 // Workgroups that take rounds of rows in turn, their weights in registers: `waves` to a
@@ -473,7 +498,7 @@ int64_t workgroups(int64_t rounds, int block, int waves) {
 
 hipError_t launch_rms_norm_forward(const RmsNorm& n, void* y, float* scale, void* residual_out,
                                    float* rstd, hipStream_t st) {
-  const Layout l = layout(n.dtype, n.rows, n.C);
+  const Layout l = layout(n.dtype, n.rows, n.C, false);
   with_types(n.dtype, n.residual_dtype, n.weight_dtype, [&](auto t, auto r, auto w) {
     typedef decltype(t) T;
     typedef decltype(r) R;
@@ -486,7 +511,7 @@ hipError_t launch_rms_norm_forward(const RmsNorm& n, void* y, float* scale, void
                 n, (T*)y, (uint8_t*)y, scale, (R*)residual_out, rstd);
         return;
       }
-      with_layout<T>(l, [&](auto v, auto ch) {
+      with_layout<T, false>(l, [&](auto v, auto ch) {
         rms_norm_forward_kernel<T, R, W, E, decltype(v)::value, decltype(ch)::value>
             <<<(unsigned)workgroups(l.rounds, l.block, 64), l.block, 0, st>>>(
                 n, (T*)y, (uint8_t*)y, scale, (R*)residual_out, rstd, l.tpr);
@@ -501,10 +526,10 @@ hipError_t launch_rms_norm_forward(const RmsNorm& n, void* y, float* scale, void
 // one workgroup's, which saves the second launch: 64 x 1024 bfloat16, forward and backward,
 // 37 us a pass and 41 with it (32 x 4096, nearer the limit: 39.7 and 40.8).
 static Layout backward_layout(int dtype, int64_t rows, int64_t C) {
-  Layout l = layout(dtype, rows, C);
+  Layout l = layout(dtype, rows, C, true);
   const int most = l.tpr < 64 ? 512 : kMaxLanes;   // 64 KiB of LDS for the other rows' sums
   if (!l.wide && rows <= 4 * (most / l.tpr)) {
-    while (l.block < most && l.rounds > 1) {
+    while (2 * l.block <= most && l.rounds > 1) {
       l.block *= 2;
       l.rounds = (rows + l.block / l.tpr - 1) / (l.block / l.tpr);
     }
@@ -529,7 +554,7 @@ int64_t rms_norm_backward_workspace(int64_t rows, int64_t C) {
 
 hipError_t launch_rms_norm_backward(const RmsNormGrad& n, void* grad_x, void* grad_residual,
                                     void* grad_weight, void* workspace, hipStream_t st) {
-  const Layout l = grad_weight ? backward_layout(n.dtype, n.rows, n.C) : layout(n.dtype, n.rows, n.C);
+  const Layout l = grad_weight ? backward_layout(n.dtype, n.rows, n.C) : layout(n.dtype, n.rows, n.C, true);
   const int64_t count = grad_weight ? backward_parts(l, n.rows)
                                     : workgroups(l.wide ? n.rows : l.rounds, l.wide ? kMaxLanes : l.block, 64);
   const bool alone = grad_weight && !l.wide && n.rows > 0 && count == 1;
@@ -546,7 +571,7 @@ hipError_t launch_rms_norm_backward(const RmsNormGrad& n, void* grad_x, void* gr
       rms_norm_wide_backward_kernel<T, R, W><<<(unsigned)count, kMaxLanes, 0, st>>>(
           n, (T*)grad_x, (R*)grad_residual, parts);
     } else if (n.rows > 0) {
-      with_layout<T>(l, [&](auto v, auto ch) {
+      with_layout<T, true>(l, [&](auto v, auto ch) {
         constexpr int V = decltype(v)::value, CH = decltype(ch)::value;
         const size_t lds = (size_t)(l.block / l.tpr - 1) * l.tpr * CH * V * 4;
         rms_norm_backward_kernel<T, R, W, V, CH><<<(unsigned)count, l.block, lds, st>>>(

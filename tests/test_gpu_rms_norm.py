@@ -1,9 +1,10 @@
 """Root-mean-square norm against its definition in 64 bits.
 
-Bounds, from the arithmetic (u = 2^-24).  A lane adds at most C / 64 squares one after
-the other and a tree the lanes' sums: the mean of squares carries (C / 64 + 12) u at
-most, its root half of that and the root's and division's roundings 3 u; r, the two
-products and the store a unit each.  So y carries e = (C / 128 + 16) u of its value
+Bounds, from the arithmetic (u = 2^-24).  A lane adds C / 64 squares, or in narrow rows
+up to 24, one after the other (growing sums: half as many units) and a tree the lanes'
+sums: the mean of squares carries (C / 64 + 20) u at most, its root half of that and the
+root's and division's roundings 3 u; r, the two products and the store a unit each.  So y
+carries e = (C / 128 + 16) u of its value
 (and 16-bit outputs half a unit of their last place, at most 2^-8 of the value, besides).  In the backward
 the mean of u r s carries (C / 64 + 20) u of the mean of |u r s|, and a term of the
 weight's gradient 8 u before `rows` are added in some order: rows u of the sum of the
@@ -97,6 +98,15 @@ def test_widths(cuda, dtype, C, rows):
 @pytest.mark.parametrize("rows,C", [(1, 8192), (3, 16384), (2, 16383), (2, 20000), (1, 40001), (3, 4100)])
 def test_wide_rows(cuda, dtype, rows, C):
     compare(cuda, dtype, rows, C, residual=dtype, seed=1)
+
+
+@pytest.mark.parametrize("dtype,C", [(F32, 20), (F32, 100), (F32, 600), (F32, 1536), (F32, 5000), (F32, 9000),
+                                     (F32, 12288), (F32, 16389), (F32, 32768), (BF16, 180), (BF16, 1040),
+                                     (BF16, 2100), (BF16, 4200), (BF16, 5000), (BF16, 7168), (BF16, 8200),
+                                     (BF16, 14000), (BF16, 24600)])
+@pytest.mark.parametrize("rows", [1, 3, 19, 130])
+def test_widths_between_the_powers_of_two(cuda, dtype, C, rows):
+    compare(cuda, dtype, rows, C, residual=dtype, seed=4)
 
 
 @pytest.mark.parametrize("rows,C", [(1000, 64), (4099, 32), (700, 513), (20000, 8), (9000, 128)])
