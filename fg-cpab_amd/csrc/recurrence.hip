@@ -582,8 +582,16 @@ Tiling tiling(int dtype, int64_t B, int64_t T, int64_t C, bool backward) {
   // for a state to pass (8 x 4096 x 1280 bfloat16, forward and backward: 74 and 143 us, with
   // 16 lanes 93 and 192, in half as many segments 87 and 143; one row of 131,072 x 512,
   // forward, 124, 141 and 188; 16 x 10,000 x 64 in 32 bits 33 and 47, 39 and 64, 46 and 51).
-  // At least 8, so that a few channels do not make thousands of segments.
-  s.lanes = std::max(8, pow2_at_least((C + V - 1) / V, 32));
+  // At least 8, so that a few channels do not make thousands of segments.  Rows of 32-bit
+  // values that are not whole lines have the line at a tile's edge read twice and written
+  // in two parts: 64 lanes, where there is work enough, beside each step too, that half as
+  // many segments do not tell (forward and backward, us, 32 and 64 lanes: 32 x 1000 x 300 157 and 126, 4 x 8000 x
+  // 1111 588 and 442, 1 x 40,000 x 300 183 and 160;  1 x 40,000 x 200 122 and 123, forward 47
+  // and 54;  64 x 200 x 300 78 and 87;  whole lines, 4 x 26,204 x 160, 131 and 144).  A wave
+  // cannot have a lane to each of twice as many channels of 16 bits.
+  const bool edges = dtype == CPAB_F32 && C % 32 != 0 && T > kFewSamples && B * C >= 300 &&
+                     B * T * C > (1 << 23);
+  s.lanes = std::max(8, pow2_at_least((C + V - 1) / V, edges ? 64 : 32));
   // as many segments as the samples fill, up to the workgroup's lanes
   s.segs = pow2_at_least((T + L - 1) / L, kBlock / s.lanes);
   s.segs = std::max(s.segs, 64 / s.lanes);

@@ -117,6 +117,37 @@ def test_long_and_wide(cuda, dtype, B, T, C):
     compare(cuda, dtype, B, T, C, seed=2)
 
 
+@pytest.mark.parametrize("B,T,C", [(12, 2600, 300), (9, 1000, 1111)])
+def test_rows_that_are_not_whole_lines(cuda, B, T, C):
+    # such rows are laid out in another way where there are many: the whole batch against
+    # its rows a few at a time, whose layout the other tests hold to the definition; either
+    # is within compare()'s bounds, so they are within twice those of each other
+    lengths = [T - 7 * k * k for k in range(B)]
+    x, f, g, h0, n = make(cuda, torch.float32, B, T, C, lengths=lengths, seed=3)
+    dy, dh = torch.randn(B, T, C, device=cuda), torch.randn(B, C, device=cuda)
+
+    def run(rows):
+        leaves = [t[rows].detach().requires_grad_() for t in (x, f, g, h0)]
+        out = cpab.gated_recurrence(*leaves, n[rows])
+        return (*out, *torch.autograd.grad(out, leaves, (dy[rows], dh[rows])))
+
+    whole = run(slice(None))
+    few = [torch.cat(t) for t in zip(*(run(slice(k, k + 3)) for k in range(0, B, 3)))]
+    X, F, G = (so.padding_zeroed(so.f64(t), n.cpu()) for t in (x, f, g))
+    y, h, gx, gf, gg, gh = (so.f64(t) for t in few)
+    M, N = max(float(X.abs().max()), float(h0.abs().max())), so.recurrence_memory(F, T)
+    L = float((so.f64(dy) * G * torch.sigmoid(G)).abs().max()) * N + float(dh.abs().max())
+    eh, el, a, s = 18 * U * N * M, 18 * U * N * L, torch.sigmoid(F), torch.sigmoid(G)
+    for what, got, want, bound in (
+            ("h", whole[1], h, eh), ("y", whole[0], y, eh * G.abs() + 40 * U * y.abs() + 1e-38),
+            ("grad x", whole[2], gx, (1 - a) * el + 40 * U * gx.abs() + 1e-38),
+            ("grad f", whole[3], gf, a * (1 - a) * (2 * M * el + 2 * L * eh + 80 * U * M * L) + 1e-38),
+            ("grad g", whole[4], gg, so.f64(dy).abs() * ((s * (1 + G * (1 - s))).abs() * eh
+                                                        + 60 * U * M * (1 + G.abs())) + 1e-38),
+            ("grad h0", whole[5], gh, el + 20 * U * gh.abs())):
+        check(got, want, 2 * torch.as_tensor(bound), what)
+
+
 @pytest.mark.parametrize("gate,start", [(True, False), (False, True), (False, False)])
 @pytest.mark.parametrize("T", [1, 37, 520])
 def test_without_gate_or_start(cuda, gate, start, T):
