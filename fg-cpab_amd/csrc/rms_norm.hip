@@ -4,9 +4,10 @@
 // s = 1 / sqrt(mean(r^2) + eps), y = r s w.  Backward, with u = w dy and n = r s:
 //   dr = s (u - n mean(u n)) + dr_out,  dw = sum over rows of dy n.
 //
-// The forward's norm is of r before it is rounded to the residual's type; the backward
-// takes the rounded r, or, for a weight of 32 bits whose gradient would show that
-// rounding (0.0017 of its value), x and the residual again.
+// The forward's norm is of r before it is rounded to the residual's type, and the backward
+// is its gradient: where that type has 16 bits it takes x and the residual again and not the
+// rounded r, whose rounding the gradients would show beside their own (the weight's is
+// 0.0017 from 64 bits so, 0.0024 from the rounded r, for a quarter more to read and write).
 //
 // Bound by memory: each value is read once and written once.  A row is held in the
 // registers of `tpr` lanes (a part of a wave, so that a narrow row does not leave one

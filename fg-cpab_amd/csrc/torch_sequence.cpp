@@ -183,9 +183,8 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
                                 ptr(w), (float)eps, ptr(y), ptr(sum), out(rstd), stream_of(x)),
           "cpab_rms_norm_forward");
     ctx->set_materialize_grads(false);
-    // the rounded sum; or its parts, where its rounding would show in a 32-bit gradient
-    const bool parts = sum.defined() && sum.scalar_type() != at::kFloat &&
-                       w.scalar_type() == at::kFloat && weight_.requires_grad();
+    // the sum; or its parts, where it was rounded to 16 bits
+    const bool parts = sum.defined() && sum.scalar_type() != at::kFloat;
     if (keep && parts)
       ctx->save_for_backward({x, w, rstd, res});
     else if (keep)

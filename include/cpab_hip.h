@@ -420,7 +420,7 @@ int cpab_rms_norm_e4m3(int dtype, int residual_dtype, int weight_dtype, int64_t 
  * the rows of grad_y r s in an order that depends on the sizes alone.
  * With `added` (rows of residual_dtype at added_stride; may be NULL), r and it are added
  * in 32 bits: x and the residual, of one type, in place of a sum that was rounded to it,
- * whose rounding a grad_weight of 32 bits would show.
+ * whose rounding the gradients would show.
  * workspace: cpab_rms_norm_backward_workspace_size(rows, C) bytes. */
 int64_t cpab_rms_norm_backward_workspace_size(int64_t rows, int64_t C);
 int cpab_rms_norm_backward(int dtype, int residual_dtype, int weight_dtype, int64_t rows, int64_t C,
