@@ -475,9 +475,10 @@ recurrence_backward_kernel(Recurrence r, Tiling s, const float* carries, const T
     for (int v = 0; v < V; ++v) join.at(seg, v) = make_float2(A[v], B[v]);
     lds_barrier();
     join.to_segment(0, seg, 1, h);
-    // Through the samples: dg; k the gate's complement, f (h_{t-1} - x) a (1 - a), d
-    // what reaches h_t.  The gates are computed again (two registers a value less
-    // across the join), and from here on a is 1 - k, off by a rounding of 1 as l is.
+    // Through the samples: dg; k the gate, folded, f (h_{t-1} - x) a (1 - a), d what
+    // reaches h_t.  The gates are computed again (two registers a value less across the
+    // join) and kept folded: l may come to a sample through closed gates alone, so a has to
+    // be held to its own last places, as 1 - a has.
     float k[L][V], f[L][V], d[L][V];
 #pragma unroll
     for (int j = 0; j < L; ++j) {
@@ -486,8 +487,8 @@ recurrence_backward_kernel(Recurrence r, Tiling s, const float* carries, const T
       if (GATE) g[j].hold();
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const Gate q = sigmoids(rf[j][v]);
-        k[j][v] = q.neg;
+        k[j][v] = folded(rf[j][v]);
+        const Gate q = unfolded(k[j][v]);
         f[j][v] = (h[v] - x[j][v]) * (q.pos * q.neg);
         h[v] = fmaf(q.pos, h[v], q.neg * x[j][v]);
         if (GATE) {
@@ -514,7 +515,7 @@ recurrence_backward_kernel(Recurrence r, Tiling s, const float* carries, const T
 #pragma unroll
     for (int j = L - 1; j >= 0; --j)
 #pragma unroll
-      for (int v = 0; v < V; ++v) B[v] = (1.0f - k[j][v]) * (B[v] + d[j][v]);
+      for (int v = 0; v < V; ++v) B[v] = unfolded(k[j][v]).pos * (B[v] + d[j][v]);
     lds_barrier();
 #pragma unroll
     for (int v = 0; v < V; ++v) join.at(seg, v) = make_float2(A[v], B[v]);
@@ -535,10 +536,11 @@ recurrence_backward_kernel(Recurrence r, Tiling s, const float* carries, const T
       float ox[V], of[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
+        const Gate q = unfolded(k[j][v]);
         l[v] += d[j][v];
-        ox[v] = k[j][v] * l[v];
+        ox[v] = q.neg * l[v];
         of[v] = l[v] * f[j][v];
-        l[v] *= 1.0f - k[j][v];
+        l[v] *= q.pos;
       }
       const bool in = full || j < live;
       if (full || j < rest) {

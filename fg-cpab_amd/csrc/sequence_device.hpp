@@ -25,11 +25,16 @@ __device__ __forceinline__ T from_float(float v) {
 struct Gate {
   float pos, neg;
 };
-__device__ __forceinline__ Gate sigmoids(float v) {
+// Both in one register: the smaller, under v's sign, which says which of the two it is.
+// The larger alone would not do: 1 less it keeps nothing of a smaller below 2^-24.
+__device__ __forceinline__ float folded(float v) {
   const float e = __expf(-fabsf(v));
-  const float small = e * __builtin_amdgcn_rcpf(1.0f + e);
-  const float big = 1.0f - small;
-  return v < 0.0f ? Gate{small, big} : Gate{big, small};
+  return copysignf(e * __builtin_amdgcn_rcpf(1.0f + e), v);
 }
+__device__ __forceinline__ Gate unfolded(float half) {
+  const float small = fabsf(half), big = 1.0f - small;
+  return __float_as_int(half) < 0 ? Gate{small, big} : Gate{big, small};
+}
+__device__ __forceinline__ Gate sigmoids(float v) { return unfolded(folded(v)); }
 
 }  // namespace cpab
