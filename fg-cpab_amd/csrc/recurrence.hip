@@ -358,7 +358,7 @@ recurrence_forward_kernel(Recurrence r, Tiling s, T* y, float* h_last, float* ca
     for (int j = 0; j < L; ++j)
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const Gate k = sigmoids(rf[j][v]);
+        const Gate k = sigmoids<T>(rf[j][v]);
         a[j][v] = k.pos;
         u[j][v] = k.neg * rx[j][v];
         B[v] = fmaf(k.pos, B[v], u[j][v]);
@@ -389,7 +389,7 @@ recurrence_forward_kernel(Recurrence r, Tiling s, T* y, float* h_last, float* ca
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         h[v] = fmaf(a[j][v], h[v], u[j][v]);
-        o[v] = GATE ? h[v] * (g[j][v] * sigmoids(g[j][v]).pos) : h[v];
+        o[v] = GATE ? h[v] * (g[j][v] * sigmoids<T>(g[j][v]).pos) : h[v];
       }
       if (full || j < live)
         store<T, V>(out, at, o);
@@ -466,7 +466,7 @@ recurrence_backward_kernel(Recurrence r, Tiling s, const float* carries, const T
       rf[j].hold(), x[j].hold();
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const Gate q = sigmoids(rf[j][v]);
+        const Gate q = sigmoids<T>(rf[j][v]);
         B[v] = fmaf(q.pos, B[v], q.neg * x[j][v]);
         A[v] *= q.pos;
       }
@@ -487,12 +487,12 @@ recurrence_backward_kernel(Recurrence r, Tiling s, const float* carries, const T
       if (GATE) g[j].hold();
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        k[j][v] = folded(rf[j][v]);
+        k[j][v] = folded<T>(rf[j][v]);
         const Gate q = unfolded(k[j][v]);
         f[j][v] = (h[v] - x[j][v]) * (q.pos * q.neg);
         h[v] = fmaf(q.pos, h[v], q.neg * x[j][v]);
         if (GATE) {
-          const Gate z = sigmoids(g[j][v]);
+          const Gate z = sigmoids<T>(g[j][v]);
           o[v] = rd[j][v] * h[v] * z.pos * fmaf(g[j][v], z.neg, 1.0f);
           d[j][v] = rd[j][v] * (g[j][v] * z.pos);
         } else {
