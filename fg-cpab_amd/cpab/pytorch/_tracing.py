@@ -6,6 +6,8 @@ nothing wrote.  While a trace is recorded the call goes through a Python autogra
 function instead, which the tracer keeps as one operation and runs again with the
 traced module's inputs (and which ``torch.jit.save`` refuses to export).
 """
+import threading
+
 import torch
 
 __all__ = ["recorded"]
@@ -23,12 +25,23 @@ def recorded(function, *args):
 
 
 class _Recorded(torch.autograd.Function):
-    """A native function with a graph of its own, held from forward to backward."""
+    """A native function with a graph of its own, held from forward to backward, where the
+    caller's gradients are on (``needs_input_grad`` does not tell: a parameter asks for one
+    under ``torch.no_grad()`` too)."""
+
+    _caller = threading.local()
+
+    @classmethod
+    def apply(cls, *args):
+        # what a trace runs again as well, each time in its caller's mode
+        cls._caller.grad = torch.is_grad_enabled()
+        return super().apply(*args)
 
     @staticmethod
     def forward(ctx, function, *args):
-        with torch.enable_grad():
-            ctx.args = [a.detach().requires_grad_(need) if isinstance(a, torch.Tensor) else a
+        grad = _Recorded._caller.grad
+        with torch.set_grad_enabled(grad):
+            ctx.args = [a.detach().requires_grad_(grad and need) if isinstance(a, torch.Tensor) else a
                         for a, need in zip(args, ctx.needs_input_grad[1:])]
             ctx.out = function(*ctx.args)
         if isinstance(ctx.out, torch.Tensor):
