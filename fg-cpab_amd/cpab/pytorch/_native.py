@@ -77,6 +77,7 @@ _SIGNATURES = {
     "cpab_interp_backward_ws": (_c_int, [_c_int, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp,
                                          _c_vp, _c_vp, _c_vp, _c_i64, _c_vp]),
     "cpab_recurrence_carries": (_c_i64, [_c_int, _c_i64, _c_i64, _c_i64]),
+    "cpab_recurrence_max_stride": (_c_i64, [_c_int, _c_i64, _c_i64, _c_i64]),
     "cpab_recurrence_workspace_size": (_c_i64, [_c_int, _c_i64, _c_i64, _c_i64, _c_int]),
     "cpab_recurrence_forward": (_c_int, [_c_int, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp, _c_vp,
                                          _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64,

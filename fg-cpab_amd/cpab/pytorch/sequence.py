@@ -25,7 +25,9 @@ def gated_recurrence(x, f, g=None, h0=None, lengths=None):
 
     Arguments:
         x, f, g: [B, T, C] float32 or bfloat16 of one type; slices of one
-            projection's output are read where they lie (any strides over B and T)
+            projection's output and [T, B, C] in memory are read where they lie (any
+            strides over B and T, while the samples of a tile, up to 1024, span less than 2^31
+            bytes; others, and channels that are not neighbours, are copied first)
         h0: [B, C] float32, the state before the first sample (default: zeros)
         lengths: [B] int32 or int64, samples in each row (default: T; clamped to
             [0, T]).  Behind a row's end y is 0 and the state stays; what the inputs

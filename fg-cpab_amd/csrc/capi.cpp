@@ -671,7 +671,8 @@ const char* cpab_last_error_string(void) { return g_last_error.c_str(); }
 // transform_data backwards).  200: the fused transform_data entry points take
 // the uniform grid's per-axis coordinates instead of the meshgrid.  402:
 // cpab_transform_data_backward_data.  403: the operators around the transform.
-int cpab_abi_version(void) { return 403; }
+// 404: cpab_recurrence_max_stride.
+int cpab_abi_version(void) { return 404; }
 
 int cpab_affine(int ndim, int64_t n_theta, int nC, int d, const float* theta,
                 const int32_t* row_ptr, const int32_t* col_idx, const float* vals, float* As,

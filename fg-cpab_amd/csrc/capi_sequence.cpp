@@ -36,7 +36,7 @@ int check_recurrence(int dtype, int64_t B, int64_t T, int64_t C) {
                 (long long)T, (long long)C);
   if (B > kMaxCount || T > kMaxCount || C > kMaxCount ||
       (double)B * (double)(T > 0 ? T : 1) * (double)C >= (double)kMaxValues ||
-      (B > 0 && C > 0 && !cpab::recurrence_fits(dtype, B, T, C, 0)))
+      (B > 0 && C > 0 && !cpab::recurrence_fits(dtype, B, T, C)))
     return fail(CPAB_ERR_INVALID, "recurrence of %lld x %lld x %lld values is too large",
                 (long long)B, (long long)T, (long long)C);
   return CPAB_OK;
@@ -60,12 +60,15 @@ int fill_recurrence(int dtype, int64_t B, int64_t T, int64_t C, const void* x, c
       if (strides[k] < 0) return fail(CPAB_ERR_INVALID, "strides must not be negative");
       if (k % 2 == 1 && strides[k] > most) most = strides[k];
     }
-    if (!cpab::recurrence_fits(dtype, B, T, C, most))
-      return fail(CPAB_ERR_INVALID, "samples %lld values apart are too far for 32-bit offsets",
-                  (long long)most);
-    r->xb = strides[0]; r->xt = strides[1];
-    r->fb = strides[2]; r->ft = strides[3];
-    if (g) { r->gb = strides[4]; r->gt = strides[5]; }
+    r->xb = strides[0]; r->fb = strides[2];
+    if (g) r->gb = strides[4];
+    if (T > 1) {
+      if (most > cpab::recurrence_max_stride(dtype, B, T, C))
+        return fail(CPAB_ERR_INVALID, "samples %lld values apart are too far for 32-bit offsets",
+                    (long long)most);
+      r->xt = strides[1]; r->ft = strides[3];
+      if (g) r->gt = strides[5];
+    }
   }
   r->h0 = h0;
   r->lengths = lengths;
@@ -127,6 +130,11 @@ extern "C" {
 int64_t cpab_recurrence_carries(int dtype, int64_t B, int64_t T, int64_t C) {
   if (check_recurrence(dtype, B, T, C) != CPAB_OK) return 0;
   return cpab::recurrence_carries(dtype, B, T, C);
+}
+
+int64_t cpab_recurrence_max_stride(int dtype, int64_t B, int64_t T, int64_t C) {
+  if (check_recurrence(dtype, B, T, C) != CPAB_OK) return 0;
+  return T > 1 ? cpab::recurrence_max_stride(dtype, B, T, C) : INT64_MAX;
 }
 
 int64_t cpab_recurrence_workspace_size(int dtype, int64_t B, int64_t T, int64_t C, int backward) {

@@ -289,8 +289,8 @@ __device__ __forceinline__ void store(const Walk<T>& w, uint32_t off, const floa
                               (__attribute__((address_space(1))) Unit*)(w.p + off));
 }
 
-// Bytes from a tile's first sample to channel c of its sample t; below 2^31
-// (recurrence_fits).
+// Bytes from a tile's first sample to channel c of its sample t; below 2^31 for the samples
+// that there are (recurrence_max_stride), and not used for others.
 template <typename T>
 __device__ __forceinline__ uint32_t offset(int t, int64_t stride, int64_t c) {
   return (uint32_t)((uint32_t)t * (uint32_t)stride + (uint32_t)c) * (uint32_t)sizeof(T);
@@ -640,14 +640,21 @@ struct Room {
 
 }  // namespace
 
-bool recurrence_fits(int dtype, int64_t B, int64_t T, int64_t C, int64_t stride) {
+int64_t recurrence_max_stride(int dtype, int64_t B, int64_t T, int64_t C) {
+  int64_t span = 2;   // samples of a tile, those that there are
+  for (const bool backward : {false, true}) {
+    const int L = backward ? backward_steps(channels(dtype, C)) : forward_steps(T);
+    span = std::max(span, std::min<int64_t>(tiling(dtype, B, T, C, backward).segs * L, T));
+  }
+  return ((1LL << 31) / (dtype == CPAB_F32 ? 4 : 2) - 1 - C) / (span - 1);
+}
+
+bool recurrence_fits(int dtype, int64_t B, int64_t T, int64_t C) {
   for (const bool backward : {false, true}) {
     const Tiling s = tiling(dtype, B, T, C, backward);
-    const int V = channels(dtype, C), L = backward ? backward_steps(V) : forward_steps(T);
     if ((double)s.tiles * (double)s.across * (double)B * s.block >= 4294967296.0) return false;
-    if (((double)s.segs * L * (double)std::max(stride, C) + (double)C) * 4 >= 2147483648.0) return false;
   }
-  return true;
+  return T <= 1 || recurrence_max_stride(dtype, B, T, C) >= C;   // y's samples
 }
 
 int64_t recurrence_carries(int dtype, int64_t B, int64_t T, int64_t C) {

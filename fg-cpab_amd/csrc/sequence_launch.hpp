@@ -20,9 +20,12 @@ struct Recurrence {
   const void* lengths;
   int lengths64;
 };
-// Whether the launches' lanes can be counted in 32 bits, as a grid's are, and a tile's
-// samples, at most `stride` values apart, be reached by offsets of 31.
-bool recurrence_fits(int dtype, int64_t B, int64_t T, int64_t C, int64_t stride);
+// The most values from an input's sample to the next that a tile's samples are reached over
+// with offsets of 31 bits.
+int64_t recurrence_max_stride(int dtype, int64_t B, int64_t T, int64_t C);
+// Whether that holds for the outputs, and the launches' lanes can be counted in 32 bits, as
+// a grid's are.
+bool recurrence_fits(int dtype, int64_t B, int64_t T, int64_t C);
 int64_t recurrence_carries(int dtype, int64_t B, int64_t T, int64_t C);
 int64_t recurrence_workspace(int dtype, int64_t B, int64_t T, int64_t C, bool backward);
 hipError_t launch_recurrence_forward(int dtype, const Recurrence& r, void* y, float* h_last,

@@ -19,11 +19,13 @@ bool has_type(const Tensor& t) {
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor of(const Maybe& t) { return t.has_value() ? *t : Tensor(); }
 
-// [B, T, C] with its channels contiguous, detached; no copy where they are already
-// (and its samples not so far apart that a tile's offsets pass 32 bits).
+// [B, T, C] with its channels contiguous, detached; no copy where they are already and its
+// samples no further apart than the kernels reach.
 Tensor samples_of(const Tensor& t) {
   const Tensor d = t.detach();
-  return (d.size(2) <= 1 || d.stride(2) == 1) && d.stride(1) <= (1 << 15) + 4 * d.size(2)
+  const int64_t B = d.size(0), T = d.size(1), C = d.size(2);
+  return (C <= 1 || d.stride(2) == 1) &&
+                 (T <= 1 || d.stride(1) <= cpab_recurrence_max_stride(type_of(d), B, T, C))
              ? d : d.contiguous();
 }
 

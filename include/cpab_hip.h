@@ -49,7 +49,8 @@ const char* cpab_last_error_string(void);
  * seed_grad.  401: the deterministic mode (cpab_set_deterministic and the
  * workspace sizes and cpab_interp_backward_ws that go with it).  402:
  * cpab_transform_data_backward_data.  403: the operators around the transform
- * (cpab_recurrence_*, cpab_rms_norm_*, cpab_adamw_step). */
+ * (cpab_recurrence_*, cpab_rms_norm_*, cpab_adamw_step).  404:
+ * cpab_recurrence_max_stride. */
 int cpab_abi_version(void);
 
 /* A = B theta per theta: As[b, r] = sum_k vals[k] * theta[b, col_idx[k]] over
@@ -366,10 +367,13 @@ int cpab_profile_read(const char* kernel, double* total_ms, int64_t* launches);
  * contiguous; h0 [B, C] float32, the state before the first sample (NULL: zeros);
  * lengths [B] int32, or int64 where lengths64 is set; y [B, T, C] contiguous;
  * h_last [B, C] float32, the state after each row's last sample.
+ * Samples of x, f and g lie at most cpab_recurrence_max_stride(...) values apart: with
+ * others of the tile that a workgroup takes they are reached over less than 2^31 bytes.
  * carries: NULL, or cpab_recurrence_carries(...) floats that the backward of the
  * same sizes takes.  workspace: cpab_recurrence_workspace_size(...) bytes,
  * 16-byte aligned. */
 int64_t cpab_recurrence_carries(int dtype, int64_t B, int64_t T, int64_t C);
+int64_t cpab_recurrence_max_stride(int dtype, int64_t B, int64_t T, int64_t C);
 int64_t cpab_recurrence_workspace_size(int dtype, int64_t B, int64_t T, int64_t C, int backward);
 int cpab_recurrence_forward(int dtype, int64_t B, int64_t T, int64_t C, const void* x,
                             const void* f, const void* g, const int64_t* strides,
