@@ -39,7 +39,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
         seed: int, of the random rounding of 8-bit states (a call's result depends on
             its arguments alone)
 
-    The step's number is part of the launch: a step captured in a graph keeps it.
+    The tensors that it writes do not overlap; one that comes twice is refused.  The
+    step's number is part of the launch: a step captured in a graph keeps it.
     """
     torch_binding().adamw(params, grads, exp_avgs, exp_avg_sqs, int(step), float(lr),
                           float(betas[0]), float(betas[1]), float(eps), float(weight_decay),

@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <memory>
+#include <new>
 
 #include "capi_common.hpp"
 #include "sequence_launch.hpp"
@@ -85,6 +87,31 @@ int check_workspace(const void* workspace, int64_t have, int64_t need) {
                 (long long)need);
   return CPAB_OK;
 }
+
+// Addresses, `most` at most, that are to come once each.
+class Once {
+ public:
+  explicit Once(int64_t most) {
+    while (mask_ + 1 < 2 * most) mask_ = 2 * mask_ + 1;
+    if (mask_ >= kFew) many_.reset(new (std::nothrow) uintptr_t[mask_ + 1]());
+  }
+  bool room() const { return mask_ < kFew || many_; }
+  bool add(const void* p) {   // false: it came before
+    const uintptr_t key = reinterpret_cast<uintptr_t>(p);
+    uintptr_t* table = many_ ? many_.get() : few_;
+    int64_t at = (int64_t)(key * 0x9E3779B97F4A7C15u >> 32) & mask_;
+    for (; table[at]; at = (at + 1) & mask_)
+      if (table[at] == key) return false;
+    table[at] = key;
+    return true;
+  }
+
+ private:
+  static constexpr int64_t kFew = 1024;
+  int64_t mask_ = 63;
+  uintptr_t few_[kFew] = {};
+  std::unique_ptr<uintptr_t[]> many_;
+};
 
 int check_norm(int dtype, int residual_dtype, int weight_dtype, int64_t rows, int64_t C) {
   CPAB_TRY(check_dtype("dtype", dtype));
@@ -240,6 +267,7 @@ int cpab_adamw_step(int dtype, int state_bits, int64_t n_tensors, const cpab_ada
   if (state_bits != 32 && state_bits != 8)
     return fail(CPAB_ERR_INVALID, "state_bits must be 32 or 8, got %d", state_bits);
   if (n_tensors < 0) return fail(CPAB_ERR_INVALID, "negative number of tensors");
+  if (n_tensors > kMaxCount) return fail(CPAB_ERR_INVALID, "%lld tensors are too many", (long long)n_tensors);
   if (step < 1) return fail(CPAB_ERR_INVALID, "step must be at least 1, got %lld", (long long)step);
   if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0))
     return fail(CPAB_ERR_INVALID, "beta1 and beta2 must be in [0, 1), got %g and %g", beta1, beta2);
@@ -248,6 +276,8 @@ int cpab_adamw_step(int dtype, int state_bits, int64_t n_tensors, const cpab_ada
                 lr, eps, weight_decay);
   if (n_tensors > 0) CPAB_REQUIRE(tensors);
   bool any = false;
+  Once once(6 * n_tensors);
+  if (!once.room()) return fail(CPAB_ERR_INVALID, "no memory to look %lld tensors over", (long long)n_tensors);
   for (int64_t k = 0; k < n_tensors; ++k) {
     const cpab_adamw_tensor& t = tensors[k];
     if (t.n < 0 || t.n > cpab::kAdamWMost)
@@ -261,6 +291,13 @@ int cpab_adamw_step(int dtype, int state_bits, int64_t n_tensors, const cpab_ada
     } else {
       CPAB_ALIGNED(t.exp_avg, 4); CPAB_ALIGNED(t.exp_avg_sq, 4);
     }
+    // two workgroups would move it at once
+    void* const master = t.master;
+    for (void* p : {t.param, t.exp_avg, t.exp_avg_sq, master, state_bits == 8 ? t.exp_avg_scale : nullptr,
+                    state_bits == 8 ? t.exp_avg_sq_scale : nullptr})
+      if (p && !once.add(p))
+        return fail(CPAB_ERR_INVALID, "an array of tensor %lld comes twice among those that the step writes",
+                    (long long)k);
   }
   if (!any) return CPAB_OK;
   cpab::AdamW a;

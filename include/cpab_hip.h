@@ -442,7 +442,8 @@ int cpab_rms_norm_backward(int dtype, int residual_dtype, int weight_dtype, int6
  * scales unused.  state_bits 8: exp_avg holds the first moment and exp_avg_sq the
  * second moment's square root as OCP E4M3 values [n], each 32 of them with one
  * power-of-two scale (E8M0: 2^(byte - 127)) in exp_avg_scale / exp_avg_sq_scale
- * [ceil(n / 32)]. */
+ * [ceil(n / 32)].  The arrays that a step writes do not overlap; one that comes twice is
+ * refused. */
 typedef struct {
   void* param;
   const void* grad;
