@@ -92,34 +92,49 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        # what is refused is refused before anything moves, or is not counted
+        for group in self.param_groups:
+            for p in group["params"]:
+                assert p.grad is None or not p.grad.is_sparse, 'AdamW does not take sparse gradients'
         ordinal = 0
         for group in self.param_groups:
             # one call for the parameters of one type and device that took as many steps
             calls = {}
-            for p in group["params"]:
-                ordinal += 1
-                if p.grad is None:
-                    continue
-                assert not p.grad.is_sparse, 'AdamW does not take sparse gradients'
-                state = self.state[p]
-                if not state:
-                    state.update(self._new_state(p, group))
-                state["step"] = int(state["step"]) + 1
-                key = (p.dtype, p.device, state["step"], "master" in state)
-                if key not in calls:
-                    calls[key] = ([], [], [], ordinal)
-                calls[key][0].append(p)
-                calls[key][1].append(p.grad)
-                calls[key][2].append(state)
-            for (_, _, step, master), (params, grads, states, first) in calls.items():
-                lists = {k: [s[k] for s in states] for k in ("exp_avg", "exp_avg_sq")}
-                eight = group["state_bits"] == 8
-                scales = [[s[k + "_scale"] for s in states] if eight else None for k in lists]
-                adamw_step(params, grads, lists["exp_avg"], lists["exp_avg_sq"], step, group["lr"],
-                           group["betas"], group["eps"], group["weight_decay"], *scales,
-                           [s["master"] for s in states] if master else None,
-                           group["seed"] + 7919 * first)
+            try:
+                for p in group["params"]:
+                    ordinal += 1
+                    if p.grad is None:
+                        continue
+                    state = self.state[p]
+                    if not state:
+                        state.update(self._new_state(p, group))
+                    state["step"] = int(state["step"]) + 1
+                    key = (p.dtype, p.device, state["step"], "master" in state)
+                    if key not in calls:
+                        calls[key] = ([], [], [], ordinal)
+                    calls[key][0].append(p)
+                    calls[key][1].append(p.grad)
+                    calls[key][2].append(state)
+                for key in list(calls):
+                    self._call(group, key, *calls[key])
+                    del calls[key]
+            except Exception:
+                for _, _, states, _ in calls.values():
+                    for state in states:
+                        state["step"] -= 1
+                raise
         return loss
+
+    @staticmethod
+    def _call(group, key, params, grads, states, first):
+        _, _, step, master = key
+        lists = {k: [s[k] for s in states] for k in ("exp_avg", "exp_avg_sq")}
+        eight = group["state_bits"] == 8
+        scales = [[s[k + "_scale"] for s in states] if eight else None for k in lists]
+        adamw_step(params, grads, lists["exp_avg"], lists["exp_avg_sq"], step, group["lr"],
+                   group["betas"], group["eps"], group["weight_decay"], *scales,
+                   [s["master"] for s in states] if master else None,
+                   group["seed"] + 7919 * first)
 
     def load_state_dict(self, state_dict):
         """As torch's, but the states keep their own types (torch casts them to the
