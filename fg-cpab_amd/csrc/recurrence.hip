@@ -28,8 +28,9 @@
 // the memory's bandwidth from the samples).
 //
 // Bound by memory: 8 x 4096 x 1280 bfloat16 forward 74 us and backward 143, 4.5 and 4.1
-// TB/s of what has to be read and written; 72 and 128 without the look-back.  With few
-// chains the look-back counts: one row of 131,072 x 512, forward, 124 us, 104 without.
+// TB/s of what has to be read and written (a profile's 77 and 147; 69 and 132 without the
+// look-back).  With few chains the look-back counts: one row of 131,072 x 512, forward, 127
+// us, 99 without; 16 ragged rows of 10,000 x 64 in 32 bits 32 and 45, 28 and 42 without.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -587,12 +588,15 @@ Tiling tiling(int dtype, int64_t B, int64_t T, int64_t C, bool backward) {
   // At least 8, so that a few channels do not make thousands of segments.  Rows of 32-bit
   // values that are not whole lines have the line at a tile's edge read twice and written
   // in two parts: 64 lanes, where there is work enough, beside each step too, that half as
-  // many segments do not tell (forward and backward, us, 32 and 64 lanes: 32 x 1000 x 300 157 and 126, 4 x 8000 x
-  // 1111 588 and 442, 1 x 40,000 x 300 183 and 160;  1 x 40,000 x 200 122 and 123, forward 47
-  // and 54;  64 x 200 x 300 78 and 87;  whole lines, 4 x 26,204 x 160, 131 and 144).  A wave
-  // cannot have a lane to each of twice as many channels of 16 bits.
-  const bool edges = dtype == CPAB_F32 && C % 32 != 0 && T > kFewSamples && B * C >= 300 &&
-                     B * T * C > (1 << 23);
+  // many segments do not tell.  Forward and backward, us, 32 and 64 lanes:
+  //   by the rows beside each step   1 x 60,000 x 150 152 and 153   1 x 40,000 x 200 124 and 128
+  //     1 x 40,000 x 232 133 and 129   1 x 40,000 x 300 181 and 162   2 x 40,000 x 116 149 and 132
+  //   by the values                  64 x 200 x 300 77 and 85       64 x 300 x 300 98 and 86
+  //     128 x 100 x 500 94 and 79      16 x 1700 x 300 126 and 104    4 x 8000 x 1111 588 and 442
+  //   whole lines                    4 x 26,204 x 160 131 and 144
+  // A wave cannot have a lane to each of twice as many channels of 16 bits.
+  const bool edges = dtype == CPAB_F32 && C % 32 != 0 && T > kFewSamples && B * C > 216 &&
+                     B * T * C > (1 << 22);
   s.lanes = std::max(8, pow2_at_least((C + V - 1) / V, edges ? 64 : 32));
   // as many segments as the samples fill, up to the workgroup's lanes
   s.segs = pow2_at_least((T + L - 1) / L, kBlock / s.lanes);

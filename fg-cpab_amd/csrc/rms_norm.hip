@@ -431,7 +431,11 @@ struct Layout {
 //   backward,          float32    333: 346, 304, 304    4096: 284, 285, 292
 //                      bfloat16   333: 178, 227, 226    4096: 158, 157, 395
 // In the forward 32 values to a lane come before 1024 lanes, of which one workgroup alone
-// finds room (16384, 8 bits: 190 us in 32 bits, 245 with 16; bfloat16 129 and 173).
+// finds room (16384, 8 bits: 190 us in 32 bits, 245 with 16; bfloat16 129 and 173).  Where
+// 1024 lanes are not enough a lane takes up to four pieces in the backward too: in bfloat16
+// (16385 to 32768) they do not all fit its registers (12 to 83 words a lane in scratch), and
+// still take less than reading the row again (4096 rows of 17,000 145 us and 452, 24,600 332
+// and 677, 32,768 393 and 905; 64 rows of 24,600 36 to 47 and 28).
 Layout layout(int dtype, int64_t rows, int64_t C, bool backward) {
   Layout l;
   const bool f32 = dtype == CPAB_F32;
