@@ -493,8 +493,8 @@ void with_layout(const Layout& l, F f) {
 // Workgroups that take rounds of rows in turn, their weights in registers: `waves` to a
 // compute unit.  Forward 64, twice what runs at once (16384 x 8192 bfloat16 to 8 bits:
 // 186 us, 5.0 TB/s as a large copy; 218 with 32, 208 with a workgroup for each round);
-// backward 16 (32768 x 1024: 46.6 and 4.8 us for dw's parts, 51 and 4.0 with 12, 49 and
-// 8.2 with 32).
+// backward 16 (32768 x 1024 from one array: 46.6 and 4.8 us for dw's parts, 51 and 4.0 with
+// 12, 49 and 8.2 with 32; from x and the residual 67.7 and 4.2).
 int64_t workgroups(int64_t rounds, int block, int waves) {
   return std::max<int64_t>(1, std::min<int64_t>(rounds, (int64_t)compute_units() * waves * 64 / block));
 }
