@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import cpab
+from cpab.pytorch import _native
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +64,29 @@ def test_single_samples_at_any_stride(cuda, dtype):
         out = cpab.gated_recurrence(*near)
         for a, b in zip(grads, torch.autograd.grad(out, near, (torch.ones_like(out[0]), torch.ones_like(out[1])))):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,C", [(2, 8), (16, 100), (40, 64), (300, 64), (1100, 8)])
+@pytest.mark.parametrize("more", [0, 1])
+def test_as_far_apart_as_the_kernels_reach(cuda, dtype, T, C, more):
+    # samples over 2^31 bytes of a tile, read in place, and one value further, copied
+    kind = 0 if dtype == torch.float32 else 1
+    stride = _native.load_library().cpab_recurrence_max_stride(kind, 1, T, C) + more
+    near = [torch.randn(1, T, C, device=cuda).to(dtype) for _ in range(3)]
+    room = torch.empty((T - 1) * stride + C, device=cuda, dtype=dtype)
+    far = room.as_strided((1, T, C), (0, stride, 1))
+    far.copy_(near[0])
+    dy = torch.randn(1, T, C, device=cuda).to(dtype)
+
+    def run(x, f, g):
+        leaves = [t.detach().requires_grad_() for t in (x, f, g)]
+        y, h = cpab.gated_recurrence(*leaves)
+        return (y, h, *torch.autograd.grad((y, h), leaves, (dy, torch.ones_like(h))))
+
+    want = run(*near)
+    assert all(torch.equal(a, b) for a, b in zip(run(far, *near[1:]), want))
+    far.copy_(near[1])
+    assert all(torch.equal(a, b) for a, b in zip(run(near[0], far, near[2]), want))
+    far.copy_(near[2])
+    assert all(torch.equal(a, b) for a, b in zip(run(*near[:2], far), want))
