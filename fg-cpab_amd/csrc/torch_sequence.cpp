@@ -309,6 +309,13 @@ void adamw(const Tensors& params, const Tensors& grads, const Tensors& exp_avgs,
            std::to_string(k) + " is " + dtype_of(p) + " on " + p.device().str());
     if (!p.is_non_overlapping_and_dense())
       fail("adamw_step: parameter " + std::to_string(k) + " is not dense in memory");
+    // autograd counts its changes, which it refuses only after they were made
+    const auto changed = [&](const Tensor& t, const char* name) {
+      if (t.is_inference() && !c10::InferenceMode::is_enabled())
+        fail(std::string("adamw_step: ") + name + where() +
+             " is an inference tensor, which may not be changed outside inference mode");
+      return t.data_ptr();
+    };
     // a state in the parameter's own layout: its values lie in the same order
     const auto like_p = [&](const Tensor& t, at::ScalarType type, const char* name) {
       if (t.device() != p.device() || t.scalar_type() != type || t.sizes() != p.sizes() ||
@@ -316,7 +323,7 @@ void adamw(const Tensors& params, const Tensors& grads, const Tensors& exp_avgs,
         fail(std::string("adamw_step: ") + name + where() + " must be " +
              c10::getDtypeNames(type).first + " in the parameter's shape " + shape_of(p) +
              ", strides and device, got " + shape_of(t) + " " + dtype_of(t));
-      return t.data_ptr();
+      return changed(t, name);
     };
     const auto flat = [&](const Tensor& t, at::ScalarType type, int64_t count, const char* name) {
       if (t.device() != p.device() || t.scalar_type() != type || t.numel() != count ||
@@ -324,7 +331,7 @@ void adamw(const Tensors& params, const Tensors& grads, const Tensors& exp_avgs,
         fail(std::string("adamw_step: ") + name + where() + " must be contiguous " +
              c10::getDtypeNames(type).first + " of " + std::to_string(count) +
              " values on the parameter's device, got " + shape_of(t) + " " + dtype_of(t));
-      return t.data_ptr();
+      return changed(t, name);
     };
     Tensor g = grads[k];
     if (g.device() != p.device() || g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes() ||
@@ -339,7 +346,7 @@ void adamw(const Tensors& params, const Tensors& grads, const Tensors& exp_avgs,
     }
     const int64_t count = p.numel();
     cpab_adamw_tensor& t = tensors[k];
-    t.param = p.data_ptr();
+    t.param = changed(p, "the value");
     t.grad = g.data_ptr();
     t.n = count;
     t.master = masters ? static_cast<float*>(like_p((*masters)[k], at::kFloat, "the master")) : nullptr;
