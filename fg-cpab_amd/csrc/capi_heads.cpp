@@ -1,0 +1,126 @@
+// The operators over heads at the extern "C" boundary: argument checks before any HIP
+// call, then the launch.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+
+#include "capi_common.hpp"
+#include "heads_launch.hpp"
+
+namespace {
+
+using cpab::check_hip;
+using cpab::fail;
+
+hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
+
+#define CPAB_TRY(call) \
+  do { const int rc_ = (call); if (rc_ != CPAB_OK) return rc_; } while (0)
+
+constexpr int64_t kMaxValues = 1LL << 37, kMaxCount = (1LL << 31) - 1, kMaxHeads = 65535;
+
+int size_of(int dtype) { return dtype == CPAB_F32 ? 4 : 2; }
+
+int check_dtype(const char* what, int dtype) {
+  if (dtype != CPAB_F32 && dtype != CPAB_BF16)
+    return fail(CPAB_ERR_INVALID, "%s must be CPAB_F32 or CPAB_BF16, got %d", what, dtype);
+  return CPAB_OK;
+}
+
+int check_strides(const char* what, const int64_t* strides, int count) {
+  for (int k = 0; k < count; ++k)
+    if (strides[k] < 0) return fail(CPAB_ERR_INVALID, "strides of %s must not be negative", what);
+  return CPAB_OK;
+}
+
+int check_workspace(const void* workspace, int64_t have, int64_t need) {
+  if (need <= 0) return CPAB_OK;
+  CPAB_REQUIRE(workspace);
+  CPAB_ALIGNED(workspace, 16);
+  if (have < need)
+    return fail(CPAB_ERR_INVALID, "workspace too small: %lld bytes, %lld needed", (long long)have,
+                (long long)need);
+  return CPAB_OK;
+}
+
+int check_qk_sizes(const cpab_qk_norm* norm) {
+  CPAB_REQUIRE(norm);
+  const cpab_qk_norm& n = *norm;
+  CPAB_TRY(check_dtype("dtype", n.dtype));
+  CPAB_TRY(check_dtype("weight_dtype", n.weight_dtype));
+  if (n.B < 0 || n.T < 0 || n.heads < 0 || n.key_heads < 0 || n.width < 0)
+    return fail(CPAB_ERR_INVALID, "negative size (B=%lld, T=%lld, heads=%lld, key_heads=%lld, width=%lld)",
+                (long long)n.B, (long long)n.T, (long long)n.heads, (long long)n.key_heads,
+                (long long)n.width);
+  if (n.width < 1 || n.width > cpab::kQkMostWidth)
+    return fail(CPAB_ERR_INVALID, "width must be from 1 to %d, got %lld", cpab::kQkMostWidth,
+                (long long)n.width);
+  if (n.turned < 0 || n.turned > n.width || n.turned % 2 != 0)
+    return fail(CPAB_ERR_INVALID, "turned must be even and at most width, got %lld", (long long)n.turned);
+  if (n.heads > kMaxHeads || n.key_heads > kMaxHeads || n.B > kMaxCount || n.T > kMaxCount ||
+      (double)n.B * (double)n.T > (double)kMaxCount ||
+      (double)n.B * (double)n.T * (double)(n.heads + n.key_heads) * (double)n.width >= (double)kMaxValues)
+    return fail(CPAB_ERR_INVALID, "norms of %lld x %lld x (%lld + %lld) x %lld values are too large",
+                (long long)n.B, (long long)n.T, (long long)n.heads, (long long)n.key_heads,
+                (long long)n.width);
+  return CPAB_OK;
+}
+
+int check_qk(const cpab_qk_norm* norm) {
+  CPAB_TRY(check_qk_sizes(norm));
+  const cpab_qk_norm& n = *norm;
+  if (!(n.eps >= 0.0f)) return fail(CPAB_ERR_INVALID, "eps must not be negative, got %g", (double)n.eps);
+  const bool any = n.B > 0 && n.T > 0;
+  if (any && n.heads > 0) { CPAB_REQUIRE(n.q); CPAB_REQUIRE(n.q_weight); }
+  if (any && n.key_heads > 0) { CPAB_REQUIRE(n.k); CPAB_REQUIRE(n.k_weight); }
+  if (any && n.turned > 0) CPAB_REQUIRE(n.freqs);
+  CPAB_ALIGNED(n.q, size_of(n.dtype)); CPAB_ALIGNED(n.k, size_of(n.dtype));
+  CPAB_ALIGNED(n.q_weight, size_of(n.weight_dtype)); CPAB_ALIGNED(n.k_weight, size_of(n.weight_dtype));
+  CPAB_ALIGNED(n.freqs, 4);
+  if (n.position_type < CPAB_POSITION_I32 || n.position_type > CPAB_POSITION_F32)
+    return fail(CPAB_ERR_INVALID, "position_type must be one of CPAB_POSITION_*, got %d", n.position_type);
+  CPAB_ALIGNED(n.positions, n.position_type == CPAB_POSITION_I64 ? 8 : 4);
+  CPAB_TRY(check_strides("q", n.q_strides, 3));
+  CPAB_TRY(check_strides("k", n.k_strides, 3));
+  return check_strides("positions", n.position_strides, 2);
+}
+
+}  // namespace
+
+extern "C" {
+
+int cpab_qk_norm_forward(const cpab_qk_norm* norm, void* q_out, void* k_out, void* stream) {
+  CPAB_TRY(check_qk(norm));
+  if (norm->B == 0 || norm->T == 0) return CPAB_OK;
+  if (norm->heads > 0) CPAB_REQUIRE(q_out);
+  if (norm->key_heads > 0) CPAB_REQUIRE(k_out);
+  CPAB_ALIGNED(q_out, size_of(norm->dtype)); CPAB_ALIGNED(k_out, size_of(norm->dtype));
+  return check_hip(cpab::launch_qk_norm_forward(*norm, q_out, k_out, as_stream(stream)),
+                   "cpab_qk_norm_forward");
+}
+
+int64_t cpab_qk_norm_backward_workspace_size(const cpab_qk_norm* norm) {
+  if (check_qk_sizes(norm) != CPAB_OK) return 0;
+  return cpab::qk_norm_backward_workspace(*norm);
+}
+
+int cpab_qk_norm_backward(const cpab_qk_norm* norm, const void* const* grads,
+                          const int64_t* grad_strides, void* const* outs, void* const* weight_outs,
+                          void* workspace, int64_t workspace_bytes, void* stream) {
+  CPAB_TRY(check_qk(norm));
+  CPAB_REQUIRE(grads); CPAB_REQUIRE(grad_strides); CPAB_REQUIRE(outs); CPAB_REQUIRE(weight_outs);
+  const bool any = norm->B > 0 && norm->T > 0;
+  if (any && norm->heads > 0) CPAB_REQUIRE(grads[0]);
+  if (any && norm->key_heads > 0) CPAB_REQUIRE(grads[1]);
+  for (int k = 0; k < 2; ++k) {
+    CPAB_ALIGNED(grads[k], size_of(norm->dtype)); CPAB_ALIGNED(outs[k], size_of(norm->dtype));
+    CPAB_ALIGNED(weight_outs[k], size_of(norm->weight_dtype));
+  }
+  CPAB_TRY(check_strides("the gradients", grad_strides, 6));
+  CPAB_TRY(check_workspace(workspace, workspace_bytes, cpab::qk_norm_backward_workspace(*norm)));
+  return check_hip(cpab::launch_qk_norm_backward(*norm, grads, grad_strides, outs, weight_outs,
+                                                 workspace, as_stream(stream)),
+                   "cpab_qk_norm_backward");
+}
+
+}  // extern "C"

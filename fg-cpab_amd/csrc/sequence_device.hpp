@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace cpab {
 
 typedef __bf16 bf16;
@@ -47,5 +49,40 @@ __device__ __forceinline__ Gate unfolded(float half) {
 }
 template <typename T>
 __device__ __forceinline__ Gate sigmoids(float v) { return unfolded(folded<T>(v)); }
+
+// V neighbouring values at any alignment of theirs.
+template <int BYTES, int ALIGN>
+struct Piece {
+  typedef uint32_t Wide __attribute__((ext_vector_type(BYTES >= 4 ? BYTES / 4 : 1)));
+  typedef typename std::conditional<BYTES >= 4, Wide, typename std::conditional<BYTES == 2, uint16_t, uint8_t>::type>::type Bits;
+  typedef Bits __attribute__((aligned(ALIGN))) Unit;
+};
+template <int V, typename T>
+__device__ __forceinline__ void load(const T* p, float out[V]) {
+  constexpr int kAll = V * (int)sizeof(T), kBytes = kAll < 16 ? kAll : 16, kEach = kBytes / (int)sizeof(T);
+  typedef Piece<kBytes, sizeof(T)> P;
+#pragma unroll
+  for (int k = 0; k < V / kEach; ++k) {
+    struct { T v[kEach]; } raw;
+    const typename P::Bits bits = reinterpret_cast<const typename P::Unit*>(p)[k];
+    __builtin_memcpy(&raw, &bits, sizeof(raw));
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) out[k * kEach + e] = to_float(raw.v[e]);
+  }
+}
+template <int V, typename T>
+__device__ __forceinline__ void store(T* p, const float in[V]) {
+  constexpr int kAll = V * (int)sizeof(T), kBytes = kAll < 16 ? kAll : 16, kEach = kBytes / (int)sizeof(T);
+  typedef Piece<kBytes, sizeof(T)> P;
+#pragma unroll
+  for (int k = 0; k < V / kEach; ++k) {
+    struct { T v[kEach]; } raw;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) raw.v[e] = from_float<T>(in[k * kEach + e]);
+    typename P::Bits bits;
+    __builtin_memcpy(&bits, &raw, sizeof(raw));
+    reinterpret_cast<typename P::Unit*>(p)[k] = bits;
+  }
+}
 
 }  // namespace cpab

@@ -393,6 +393,7 @@ Tensor interp(int64_t ndim, const Tensor& data, const Tensor& grid, std::vector<
 }  // namespace
 
 void sequence_functions(py::module& m);   // torch_sequence.cpp
+void heads_functions(py::module& m);      // torch_heads.cpp
 
 PYBIND11_MODULE(_cpab_torch, m) {
   m.def("grid", &grid);
@@ -400,4 +401,5 @@ PYBIND11_MODULE(_cpab_torch, m) {
   m.def("image", &image);
   m.def("interp", &interp);
   sequence_functions(m);
+  heads_functions(m);
 }

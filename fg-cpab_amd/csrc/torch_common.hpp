@@ -7,8 +7,10 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <optional>
 #include <sstream>
 #include <stdexcept>
 #include <string>
@@ -70,5 +72,45 @@ inline variable_list once(variable_list grads, const Tensor& grad_out) {
 }
 
 inline Tensor plain(const Tensor& t) { return t.detach().contiguous(); }
+
+typedef std::optional<Tensor> Maybe;
+
+inline int type_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? CPAB_F32 : CPAB_BF16; }
+inline bool has_type(const Tensor& t) {
+  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16;
+}
+inline void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+inline Tensor of(const Maybe& t) { return t.has_value() ? *t : Tensor(); }
+
+// A gradient of type `type`, or none.
+inline Tensor grad_of(const Tensor& g, at::ScalarType type) {
+  return !g.defined() || g.scalar_type() == type ? g : g.to(type);
+}
+
+// Whether a gradient came at all: a function behind an output may have none to give.
+inline bool any_defined(const variable_list& grads) {
+  for (const Tensor& g : grads)
+    if (g.defined()) return true;
+  return false;
+}
+
+inline bool any_grad(std::initializer_list<Tensor> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor& t : ts)
+    if (t.defined() && t.requires_grad()) return true;
+  return false;
+}
+
+// The gradients, which cannot be differentiated again (create_graph): not through the
+// upstream gradient, and not through the inputs.
+inline variable_list once_any(variable_list out) {
+  if (!at::GradMode::is_enabled()) return out;
+  for (const Tensor& g : out)
+    if (g.defined()) {
+      Tensor asks = at::empty({0}, g.options()).set_requires_grad(true);
+      return once(std::move(out), asks);
+    }
+  return out;
+}
 
 }  // namespace cpab_torch

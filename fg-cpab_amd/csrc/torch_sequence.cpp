@@ -2,23 +2,11 @@
 // cpab/pytorch/sequence.py calls.
 #include "torch_common.hpp"
 
-#include <torch/csrc/autograd/function.h>
-
 #include <array>
-#include <optional>
 
 namespace {
 
 using namespace cpab_torch;
-typedef std::optional<Tensor> Maybe;
-
-int type_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? CPAB_F32 : CPAB_BF16; }
-bool has_type(const Tensor& t) {
-  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16;
-}
-void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-Tensor of(const Maybe& t) { return t.has_value() ? *t : Tensor(); }
-
 // [B, T, C] with its channels contiguous, detached; no copy where they are already and its
 // samples no further apart than the kernels reach.
 Tensor samples_of(const Tensor& t) {
@@ -27,37 +15,6 @@ Tensor samples_of(const Tensor& t) {
   return (C <= 1 || d.stride(2) == 1) &&
                  (T <= 1 || d.stride(1) <= cpab_recurrence_max_stride(type_of(d), B, T, C))
              ? d : d.contiguous();
-}
-
-// A gradient of type `type`, or none.
-Tensor grad_of(const Tensor& g, at::ScalarType type) {
-  return !g.defined() || g.scalar_type() == type ? g : g.to(type);
-}
-
-// Whether a gradient came at all: a function behind an output may have none to give.
-bool any_defined(const variable_list& grads) {
-  for (const Tensor& g : grads)
-    if (g.defined()) return true;
-  return false;
-}
-
-bool any_grad(std::initializer_list<Tensor> ts) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const Tensor& t : ts)
-    if (t.defined() && t.requires_grad()) return true;
-  return false;
-}
-
-// The gradients, which cannot be differentiated again (create_graph): not through the
-// upstream gradient, and not through the inputs.
-variable_list once_any(variable_list out) {
-  if (!at::GradMode::is_enabled()) return out;
-  for (const Tensor& g : out)
-    if (g.defined()) {
-      Tensor asks = at::empty({0}, g.options()).set_requires_grad(true);
-      return once(std::move(out), asks);
-    }
-  return out;
 }
 
 // ---- gated recurrence --------------------------------------------------------

@@ -50,7 +50,7 @@ const char* cpab_last_error_string(void);
  * workspace sizes and cpab_interp_backward_ws that go with it).  402:
  * cpab_transform_data_backward_data.  403: the operators around the transform
  * (cpab_recurrence_*, cpab_rms_norm_*, cpab_adamw_step).  404:
- * cpab_recurrence_max_stride. */
+ * cpab_recurrence_max_stride.  405: cpab_qk_norm_*. */
 int cpab_abi_version(void);
 
 /* A = B theta per theta: As[b, r] = sum_k vals[k] * theta[b, col_idx[k]] over
@@ -470,6 +470,44 @@ typedef struct {
 int cpab_adamw_step(int dtype, int state_bits, int64_t n_tensors, const cpab_adamw_tensor* tensors,
                     int64_t step, double lr, double beta1, double beta2, double eps,
                     double weight_decay, uint32_t seed, void* stream);
+
+/* Norms of queries and keys by head, rotated by the position.  For each of a token's
+ * heads x of `width` values: y = x / sqrt(mean(x^2) + eps) * weight, and the first
+ * `turned` of y, as turned / 2 pairs (a, b), turn by p = position freqs[pair]:
+ *   (a cos p - b sin p, b cos p + a sin p);
+ * a pair is two neighbours where `neighbours` is set, else values turned / 2 apart.  p is
+ * reduced in 64 bits.  q: [B, T, heads, width], k: [B, T, key_heads, width] at strides
+ * over B, T and the heads (elements), the width contiguous and at most 512; weights
+ * [width] of weight_dtype; freqs [turned / 2]; positions [B, T] of position_type at
+ * position_strides, or NULL: 0 to T - 1.  q_out, k_out: contiguous, of q's shape and k's.
+ * Backward, with the same inputs: grads {q's, k's} at grad_strides (three each; the width
+ * contiguous) give outs {grad_q, grad_k} and weight_outs (each may be NULL), the weights'
+ * summed in an order that depends on the sizes and the device alone.
+ * workspace: cpab_qk_norm_backward_workspace_size(...) bytes, 16-byte aligned.  The
+ * description lies in host memory and is read before the call returns. */
+#define CPAB_POSITION_I32 0
+#define CPAB_POSITION_I64 1
+#define CPAB_POSITION_F32 2
+typedef struct {
+  int dtype, weight_dtype, neighbours, position_type;
+  int64_t B, T, heads, key_heads, width, turned;
+  const void* q;
+  const void* k;
+  int64_t q_strides[3], k_strides[3];
+  const void* q_weight;
+  const void* k_weight;
+  const float* freqs;
+  const void* positions;
+  int64_t position_strides[2];
+  float eps;
+} cpab_qk_norm;
+
+int cpab_qk_norm_forward(const cpab_qk_norm* norm, void* q_out, void* k_out, void* stream);
+int64_t cpab_qk_norm_backward_workspace_size(const cpab_qk_norm* norm);
+int cpab_qk_norm_backward(const cpab_qk_norm* norm, const void* const* grads,
+                          const int64_t* grad_strides, void* const* outs,
+                          void* const* weight_outs, void* workspace, int64_t workspace_bytes,
+                          void* stream);
 
 #ifdef __cplusplus
 }
