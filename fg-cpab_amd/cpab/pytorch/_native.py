@@ -96,6 +96,11 @@ _SIGNATURES = {
     "cpab_qk_norm_forward": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp]),
     "cpab_qk_norm_backward_workspace_size": (_c_i64, [_c_vp]),
     "cpab_qk_norm_backward": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_vp]),
+    "cpab_delta_rule_kept": (_c_i64, [_c_vp]),
+    "cpab_delta_rule_workspace_size": (_c_i64, [_c_vp, _c_int, _c_int]),
+    "cpab_delta_rule_forward": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_vp]),
+    "cpab_delta_rule_backward": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp,
+                                          _c_vp, _c_vp, _c_vp, _c_i64, _c_vp]),
     "cpab_adamw_step": (_c_int, [_c_int, _c_int, _c_i64, _c_vp, _c_i64, _c_f64, _c_f64, _c_f64,
                                  _c_f64, _c_f64, ctypes.c_uint32, _c_vp]),
 }

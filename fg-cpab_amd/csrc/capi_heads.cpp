@@ -85,6 +85,53 @@ int check_qk(const cpab_qk_norm* norm) {
   return check_strides("positions", n.position_strides, 2);
 }
 
+int check_delta_sizes(const cpab_delta_rule* rule) {
+  CPAB_REQUIRE(rule);
+  const cpab_delta_rule& r = *rule;
+  CPAB_TRY(check_dtype("dtype", r.dtype));
+  CPAB_TRY(check_dtype("gate_dtype", r.gate_dtype));
+  if (r.B < 0 || r.T < 0 || r.heads < 0 || r.key_heads < 0 || r.dk < 0 || r.dv < 0)
+    return fail(CPAB_ERR_INVALID, "negative size (B=%lld, T=%lld, heads=%lld, key_heads=%lld, dk=%lld, dv=%lld)",
+                (long long)r.B, (long long)r.T, (long long)r.heads, (long long)r.key_heads,
+                (long long)r.dk, (long long)r.dv);
+  if (r.dk > CPAB_DELTA_MOST_KEY)
+    return fail(CPAB_ERR_INVALID, "dk must be at most %d, got %lld", CPAB_DELTA_MOST_KEY, (long long)r.dk);
+  if (r.heads > 0 && (r.key_heads < 1 || r.heads % r.key_heads != 0))
+    return fail(CPAB_ERR_INVALID, "heads must be a multiple of key_heads, got %lld and %lld",
+                (long long)r.heads, (long long)r.key_heads);
+  // a launch's workgroups: a chunk or 32 columns of a head each
+  const double heads = (double)r.B * (double)r.heads, blocks = (double)kMaxCount / 256;
+  if (r.heads > kMaxHeads || r.B > kMaxCount || r.T > kMaxCount - 64 || r.dv > kMaxCount / 64 ||
+      heads * ((double)r.T / 64 + 1) > blocks || heads * ((double)r.dv / 32 + 1) > blocks ||
+      heads * (double)(r.T + 64) * (double)(r.dv + r.dk) >= (double)kMaxValues ||
+      heads * ((double)r.T / 64 + 2) * (double)r.dk * (double)r.dv >= (double)kMaxValues)
+    return fail(CPAB_ERR_INVALID, "delta rule of %lld x %lld x %lld heads of %lld x %lld is too large",
+                (long long)r.B, (long long)r.T, (long long)r.heads, (long long)r.dk, (long long)r.dv);
+  return CPAB_OK;
+}
+
+// Whether there is anything to do.
+bool any_delta(const cpab_delta_rule& r) { return r.B > 0 && r.heads > 0; }
+
+int check_delta(const cpab_delta_rule* rule) {
+  CPAB_TRY(check_delta_sizes(rule));
+  const cpab_delta_rule& r = *rule;
+  if (!std::isfinite(r.scale)) return fail(CPAB_ERR_INVALID, "scale must be finite");
+  if (any_delta(r) && r.T > 0) {
+    if (r.dk > 0) { CPAB_REQUIRE(r.q); CPAB_REQUIRE(r.k); }
+    if (r.dv > 0) CPAB_REQUIRE(r.v);
+    CPAB_REQUIRE(r.decay); CPAB_REQUIRE(r.beta);
+  }
+  CPAB_ALIGNED(r.q, size_of(r.dtype)); CPAB_ALIGNED(r.k, size_of(r.dtype)); CPAB_ALIGNED(r.v, size_of(r.dtype));
+  CPAB_ALIGNED(r.decay, size_of(r.gate_dtype)); CPAB_ALIGNED(r.beta, size_of(r.gate_dtype));
+  CPAB_ALIGNED(r.h0, 4); CPAB_ALIGNED(r.lengths, r.lengths64 ? 8 : 4);
+  CPAB_TRY(check_strides("q", r.q_strides, 3));
+  CPAB_TRY(check_strides("k", r.k_strides, 3));
+  CPAB_TRY(check_strides("v", r.v_strides, 3));
+  CPAB_TRY(check_strides("decay", r.decay_strides, 3));
+  return check_strides("beta", r.beta_strides, 3);
+}
+
 }  // namespace
 
 extern "C" {
@@ -121,6 +168,48 @@ int cpab_qk_norm_backward(const cpab_qk_norm* norm, const void* const* grads,
   return check_hip(cpab::launch_qk_norm_backward(*norm, grads, grad_strides, outs, weight_outs,
                                                  workspace, as_stream(stream)),
                    "cpab_qk_norm_backward");
+}
+
+int64_t cpab_delta_rule_kept(const cpab_delta_rule* rule) {
+  if (check_delta_sizes(rule) != CPAB_OK || !any_delta(*rule)) return 0;
+  return cpab::delta_rule_kept(*rule);
+}
+
+int64_t cpab_delta_rule_workspace_size(const cpab_delta_rule* rule, int keep, int backward) {
+  if (check_delta_sizes(rule) != CPAB_OK || !any_delta(*rule)) return 0;
+  return cpab::delta_rule_workspace(*rule, keep != 0, backward != 0);
+}
+
+int cpab_delta_rule_forward(const cpab_delta_rule* rule, void* o, float* h, float* kept,
+                            void* workspace, int64_t workspace_bytes, void* stream) {
+  CPAB_TRY(check_delta(rule));
+  const cpab_delta_rule& r = *rule;
+  if (!any_delta(r) || r.dv == 0) return CPAB_OK;
+  if (r.T > 0) CPAB_REQUIRE(o);
+  if (r.dk > 0) CPAB_REQUIRE(h);
+  CPAB_ALIGNED(o, size_of(r.dtype)); CPAB_ALIGNED(h, 4); CPAB_ALIGNED(kept, 4);
+  CPAB_TRY(check_workspace(workspace, workspace_bytes, cpab::delta_rule_workspace(r, kept != nullptr, false)));
+  return check_hip(cpab::launch_delta_rule_forward(r, o, h, kept, workspace, as_stream(stream)),
+                   "cpab_delta_rule_forward");
+}
+
+int cpab_delta_rule_backward(const cpab_delta_rule* rule, const float* kept, const void* grad_o,
+                             const float* grad_h, void* grad_q, void* grad_k, void* grad_v,
+                             void* grad_decay, void* grad_beta, float* grad_h0, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  CPAB_TRY(check_delta(rule));
+  const cpab_delta_rule& r = *rule;
+  if (!any_delta(r)) return CPAB_OK;
+  if (r.T > 0 && r.dv > 0) CPAB_REQUIRE(kept);
+  CPAB_ALIGNED(kept, 4); CPAB_ALIGNED(grad_h, 4); CPAB_ALIGNED(grad_h0, 4);
+  CPAB_ALIGNED(grad_o, size_of(r.dtype)); CPAB_ALIGNED(grad_q, size_of(r.dtype));
+  CPAB_ALIGNED(grad_k, size_of(r.dtype)); CPAB_ALIGNED(grad_v, size_of(r.dtype));
+  CPAB_ALIGNED(grad_decay, size_of(r.gate_dtype)); CPAB_ALIGNED(grad_beta, size_of(r.gate_dtype));
+  CPAB_TRY(check_workspace(workspace, workspace_bytes, cpab::delta_rule_workspace(r, true, true)));
+  return check_hip(cpab::launch_delta_rule_backward(r, kept, grad_o, grad_h, grad_q, grad_k, grad_v,
+                                                    grad_decay, grad_beta, grad_h0, workspace,
+                                                    as_stream(stream)),
+                   "cpab_delta_rule_backward");
 }
 
 }  // extern "C"

@@ -18,4 +18,15 @@ hipError_t launch_qk_norm_backward(const cpab_qk_norm& n, const void* const grad
                                    const int64_t grad_strides[6], void* const outs[2],
                                    void* const weight_outs[2], void* workspace, hipStream_t s);
 
+
+// Floats that a forward keeps for its backward; bytes of workspace.
+int64_t delta_rule_kept(const cpab_delta_rule& r);
+int64_t delta_rule_workspace(const cpab_delta_rule& r, bool keep, bool backward);
+hipError_t launch_delta_rule_forward(const cpab_delta_rule& r, void* o, float* h, float* kept,
+                                     void* workspace, hipStream_t s);
+hipError_t launch_delta_rule_backward(const cpab_delta_rule& r, const float* kept, const void* grad_o,
+                                      const float* grad_h, void* grad_q, void* grad_k, void* grad_v,
+                                      void* grad_decay, void* grad_beta, float* grad_h0,
+                                      void* workspace, hipStream_t s);
+
 }  // namespace cpab

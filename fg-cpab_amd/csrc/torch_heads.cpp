@@ -2,6 +2,8 @@
 // cpab/pytorch/heads.py calls.
 #include "torch_common.hpp"
 
+#include <cmath>
+
 namespace {
 
 using namespace cpab_torch;
@@ -147,6 +149,124 @@ variable_list qk_norm(const Tensor& q, const Tensor& k, const Tensor& qw, const 
   return QkNorm::apply(q, k, qw, kw, freqs_, places, neighbours, eps, keep);
 }
 
+// ---- gated delta rule ------------------------------------------------------------
+
+struct DeltaRule : torch::autograd::Function<DeltaRule> {
+  static cpab_delta_rule describe(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& decay,
+                                  const Tensor& beta, const Tensor& h0, const Tensor& lengths,
+                                  double scale) {
+    cpab_delta_rule r{};
+    r.dtype = type_of(q);
+    r.gate_dtype = type_of(decay);
+    r.B = v.size(0), r.T = v.size(1), r.heads = v.size(2), r.key_heads = q.size(2);
+    r.dk = q.size(3), r.dv = v.size(3);
+    r.q = ptr(q), r.k = ptr(k), r.v = ptr(v), r.decay = ptr(decay), r.beta = ptr(beta);
+    strides_to(q, r.q_strides, 3);
+    strides_to(k, r.k_strides, 3);
+    strides_to(v, r.v_strides, 3);
+    strides_to(decay, r.decay_strides, 3);
+    strides_to(beta, r.beta_strides, 3);
+    r.h0 = in(h0);
+    r.lengths = ptr(lengths);
+    r.lengths64 = lengths.defined() && lengths.scalar_type() == at::kLong;
+    r.scale = (float)scale;
+    return r;
+  }
+
+  static variable_list forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_,
+                               const Tensor& decay_, const Tensor& beta_, const Maybe& maybe_h0,
+                               const Maybe& maybe_lengths, double scale, bool keep) {
+    const c10::OptionalDeviceGuard guard(v_.device());
+    const Tensor q = heads_of(q_), k = heads_of(k_), v = heads_of(v_), decay = decay_.detach(),
+                 beta = beta_.detach(), h0_ = of(maybe_h0), lengths = of(maybe_lengths);
+    const Tensor h0 = h0_.defined() ? plain(h0_) : Tensor();
+    const cpab_delta_rule r = describe(q, k, v, decay, beta, h0, lengths, scale);
+    Tensor o = at::empty(v.sizes(), v.options()), h = empty({r.B, r.heads, r.dk, r.dv}, v), kept;
+    if (keep) kept = empty({cpab_delta_rule_kept(&r)}, v);
+    const int64_t bytes = cpab_delta_rule_workspace_size(&r, keep, 0);
+    at::DataPtr ws;
+    if (bytes > 0) ws = scratch(bytes);
+    check(cpab_delta_rule_forward(&r, ptr(o), out(h), out(kept), ws.get(), bytes, stream_of(v)),
+          "cpab_delta_rule_forward");
+    ctx->set_materialize_grads(false);
+    if (keep) {
+      ctx->save_for_backward({q, k, v, decay, beta, h0, lengths, kept});
+      ctx->saved_data["scale"] = scale;
+    }
+    return {o, h};
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    if (!any_defined(grads)) return variable_list(9);
+    variable_list d(9);
+    {
+      const at::NoGradGuard no_grad;
+      const auto saved = ctx->get_saved_variables();
+      const Tensor &v = saved[2], &h0 = saved[5], &kept = saved[7];
+      const c10::OptionalDeviceGuard guard(v.device());
+      const cpab_delta_rule r = describe(saved[0], saved[1], v, saved[3], saved[4], h0, saved[6],
+                                         ctx->saved_data["scale"].toDouble());
+      Tensor go = grad_of(grads[0], v.scalar_type()), gh = grad_of(grads[1], at::kFloat);
+      if (go.defined()) go = go.contiguous();
+      if (gh.defined()) gh = gh.contiguous();
+      // h0, where it was given, is the sixth that may need a gradient
+      for (int k = 0; k < (h0.defined() ? 6 : 5); ++k)
+        if (ctx->needs_input_grad(k)) d[k] = at::empty(saved[k].sizes(), saved[k].options());
+      const int64_t bytes = cpab_delta_rule_workspace_size(&r, 1, 1);
+      at::DataPtr ws;
+      if (bytes > 0) ws = scratch(bytes);
+      check(cpab_delta_rule_backward(&r, in(kept), ptr(go), in(gh), ptr(d[0]), ptr(d[1]), ptr(d[2]),
+                                     ptr(d[3]), ptr(d[4]), out(d[5]), ws.get(), bytes, stream_of(v)),
+            "cpab_delta_rule_backward");
+    }
+    return once_any(std::move(d));
+  }
+};
+
+variable_list delta_rule(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& decay,
+                         const Tensor& beta, const Maybe& h0_, const Maybe& lengths_,
+                         const std::optional<double>& scale_) {
+  const Tensor h0 = of(h0_), lengths = of(lengths_);
+  if (!v.is_cuda()) fail("gated_delta_rule: only GPU tensors are supported");
+  if (!has_type(v)) fail("gated_delta_rule: expected float32 or bfloat16, got " + dtype_of(v));
+  if (v.dim() != 4) fail("gated_delta_rule: v must be [B, T, heads, dv], got " + shape_of(v));
+  const int64_t B = v.size(0), T = v.size(1), H = v.size(2);
+  const auto text = [](int64_t n) { return std::to_string(n); };
+  for (const auto& [t, name] : {std::make_pair(&q, "q"), std::make_pair(&k, "k")})
+    if (t->device() != v.device() || t->scalar_type() != v.scalar_type() || t->dim() != 4 ||
+        t->size(0) != B || t->size(1) != T || t->sizes() != q.sizes() ||
+        (H > 0 && (t->size(2) == 0 || H % t->size(2) != 0)))
+      fail(std::string("gated_delta_rule: ") + name + " must be [" + text(B) + ", " + text(T) +
+           ", heads, dk] (the heads of v, " + text(H) + ", a multiple of q's and k's) of v's type and " +
+           "device, got " + shape_of(*t) + " " + dtype_of(*t));
+  const int64_t dk = q.size(3), dv = v.size(3);
+  if (dk > CPAB_DELTA_MOST_KEY)
+    fail("gated_delta_rule: dk must be at most " + text(CPAB_DELTA_MOST_KEY) + ", got " + text(dk));
+  for (const auto& [t, name] : {std::make_pair(&decay, "decay"), std::make_pair(&beta, "beta")})
+    if (t->device() != v.device() || !has_type(*t) || t->scalar_type() != decay.scalar_type() ||
+        t->dim() != 3 || t->size(0) != B || t->size(1) != T || t->size(2) != H)
+      fail(std::string("gated_delta_rule: ") + name + " must be float32 or bfloat16 (decay and beta of " +
+           "one type) [" + text(B) + ", " + text(T) + ", " + text(H) + "] on v's device, got " +
+           shape_of(*t) + " " + dtype_of(*t));
+  if (h0.defined() && (h0.device() != v.device() || h0.scalar_type() != at::kFloat || h0.dim() != 4 ||
+                       h0.size(0) != B || h0.size(1) != H || h0.size(2) != dk || h0.size(3) != dv))
+    fail("gated_delta_rule: h0 must be float32 [" + text(B) + ", " + text(H) + ", " + text(dk) + ", " +
+         text(dv) + "] on v's device, got " + shape_of(h0) + " " + dtype_of(h0));
+  if (lengths.defined() &&
+      (lengths.device() != v.device() || lengths.dim() != 1 || lengths.size(0) != B ||
+       (lengths.scalar_type() != at::kInt && lengths.scalar_type() != at::kLong)))
+    fail("gated_delta_rule: lengths must be int32 or int64 [" + text(B) + "] on v's device, got " +
+         shape_of(lengths) + " " + dtype_of(lengths));
+  const double scale = scale_ ? *scale_ : dk > 0 ? 1.0 / std::sqrt((double)dk) : 1.0;
+  const bool keep = any_grad({q, k, v, decay, beta, h0});
+  py::gil_scoped_release nogil;
+  const Maybe dense = lengths.defined() ? Maybe(lengths.contiguous()) : Maybe();
+  return DeltaRule::apply(q, k, v, decay, beta, h0_, dense, scale, keep);
+}
+
 }  // namespace
 
-void heads_functions(py::module& m) { m.def("qk_norm", &qk_norm); }
+void heads_functions(py::module& m) {
+  m.def("qk_norm", &qk_norm);
+  m.def("delta_rule", &delta_rule);
+}

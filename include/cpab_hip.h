@@ -50,7 +50,8 @@ const char* cpab_last_error_string(void);
  * workspace sizes and cpab_interp_backward_ws that go with it).  402:
  * cpab_transform_data_backward_data.  403: the operators around the transform
  * (cpab_recurrence_*, cpab_rms_norm_*, cpab_adamw_step).  404:
- * cpab_recurrence_max_stride.  405: cpab_qk_norm_*. */
+ * cpab_recurrence_max_stride.  405: cpab_qk_norm_*.
+ * 406: cpab_delta_rule_*. */
 int cpab_abi_version(void);
 
 /* A = B theta per theta: As[b, r] = sum_k vals[k] * theta[b, col_idx[k]] over
@@ -508,6 +509,50 @@ int cpab_qk_norm_backward(const cpab_qk_norm* norm, const void* const* grads,
                           const int64_t* grad_strides, void* const* outs,
                           void* const* weight_outs, void* workspace, int64_t workspace_bytes,
                           void* stream);
+
+/* The gated delta rule over B rows of T samples of `heads` heads, each with a state S of
+ * [dk, dv], zeros or h0 before the first sample:
+ *   S' = exp(decay_t) S_{t-1},  S_t = S' + beta_t k_t (v_t - S'^T k_t)^T,
+ *   o_t = scale S_t^T q_t,
+ * for t < lengths[b] (T where lengths is NULL; clamped to [0, T]); behind a row's end o is
+ * 0, the state stays, and nothing of the inputs is used.  Each `heads / key_heads`
+ * neighbouring heads share a query and a key.  q, k: [B, T, key_heads, dk] and v
+ * [B, T, heads, dv] of dtype, at strides over B, T and the heads (elements), their last
+ * dimension contiguous; decay, beta: [B, T, heads] of gate_dtype at three strides; o
+ * [B, T, heads, dv] contiguous; h [B, heads, dk, dv] float32, the state after each row's
+ * last sample.  dk is at most CPAB_DELTA_MOST_KEY.  decay is the decay's logarithm, at most
+ * 0; below -128 it counts as -128, whose exponential is 0.
+ * kept: NULL, or cpab_delta_rule_kept(...) floats that the backward of the same sizes
+ * takes.  workspace: cpab_delta_rule_workspace_size(...) bytes, 16-byte aligned.  The
+ * description lies in host memory and is read before the call returns. */
+#define CPAB_DELTA_MOST_KEY 128
+typedef struct {
+  int dtype, gate_dtype, lengths64;
+  int64_t B, T, heads, key_heads, dk, dv;
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* decay;
+  const void* beta;
+  int64_t q_strides[3], k_strides[3], v_strides[3], decay_strides[3], beta_strides[3];
+  const float* h0;
+  const void* lengths;
+  float scale;
+} cpab_delta_rule;
+
+int64_t cpab_delta_rule_kept(const cpab_delta_rule* rule);
+int64_t cpab_delta_rule_workspace_size(const cpab_delta_rule* rule, int keep, int backward);
+int cpab_delta_rule_forward(const cpab_delta_rule* rule, void* o, float* h, float* kept,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Backward of cpab_delta_rule_forward with the same description and what it kept: grad_o
+ * [B, T, heads, dv] contiguous and grad_h [B, heads, dk, dv] (either may be NULL: zeros)
+ * give the gradients of q, k, v, decay and beta, contiguous and of their types, and of h0
+ * (each may be NULL).  Behind a row's end they are 0. */
+int cpab_delta_rule_backward(const cpab_delta_rule* rule, const float* kept, const void* grad_o,
+                             const float* grad_h, void* grad_q, void* grad_k, void* grad_v,
+                             void* grad_decay, void* grad_beta, float* grad_h0, void* workspace,
+                             int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
