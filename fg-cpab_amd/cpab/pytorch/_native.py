@@ -103,6 +103,9 @@ _SIGNATURES = {
                                           _c_vp, _c_vp, _c_vp, _c_i64, _c_vp]),
     "cpab_adamw_step": (_c_int, [_c_int, _c_int, _c_i64, _c_vp, _c_i64, _c_f64, _c_f64, _c_f64,
                                  _c_f64, _c_f64, ctypes.c_uint32, _c_vp]),
+    "cpab_muon_workspace_size": (_c_i64, [_c_i64, _c_vp]),
+    "cpab_muon_step": (_c_int, [_c_int, _c_i64, _c_vp, _c_vp, _c_f64, _c_f64, _c_f64, _c_int, _c_vp,
+                                _c_f64, _c_int, _c_vp, _c_i64, _c_vp]),
 }
 
 

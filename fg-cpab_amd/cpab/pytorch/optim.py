@@ -1,15 +1,18 @@
-"""AdamW over many tensors in few launches, its states in 32 bits or in 8.
+"""AdamW over many tensors in few launches, its states in 32 bits or in 8, and Muon over
+many matrices.
 
-``adamw_step`` is the step itself over lists of tensors; ``AdamW`` the optimiser that
-holds the states.  The step is a HIP kernel behind the C ABI
-(csrc/torch_sequence.cpp, csrc/adamw.hip); there is no torch or CPU fallback.  No
-counterpart in the reference, which trains with torch's optimisers.
+``adamw_step`` and ``muon_step`` are the steps themselves over lists of tensors; ``AdamW``
+and ``Muon`` the optimisers that hold the states.  The steps are HIP kernels behind the C
+ABI (csrc/torch_sequence.cpp, csrc/adamw.hip, csrc/muon.hip); there is no torch or CPU
+fallback.  No counterpart in the reference, which trains with torch's optimisers.
 """
+import math
+
 import torch
 
 from ._native import torch_binding
 
-__all__ = ["adamw_step", "AdamW"]
+__all__ = ["adamw_step", "AdamW", "muon_step", "Muon"]
 
 _E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 _GROUP = 32   # values that share a scale
@@ -47,7 +50,21 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
                           exp_avg_scales, exp_avg_sq_scales, masters, int(seed))
 
 
-class AdamW(torch.optim.Optimizer):
+class _Optimizer(torch.optim.Optimizer):
+    def load_state_dict(self, state_dict):
+        """As torch's, but the states keep their own types (torch casts them to the
+        parameter's)."""
+        super().load_state_dict(state_dict)
+        saved = state_dict["state"]
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        own = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(ids, own):
+            for name, value in saved.get(i, {}).items():
+                if isinstance(value, torch.Tensor):
+                    self.state[p][name] = value.to(p.device).clone(memory_format=torch.preserve_format)
+
+
+class AdamW(_Optimizer):
     """AdamW on ``adamw_step``.
 
     Arguments:
@@ -136,14 +153,110 @@ class AdamW(torch.optim.Optimizer):
                    [s["master"] for s in states] if master else None,
                    group["seed"] + 7919 * first)
 
-    def load_state_dict(self, state_dict):
-        """As torch's, but the states keep their own types (torch casts them to the
-        parameter's)."""
-        super().load_state_dict(state_dict)
-        saved = state_dict["state"]
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        own = [p for g in self.param_groups for p in g["params"]]
-        for i, p in zip(ids, own):
-            for name, value in saved.get(i, {}).items():
-                if isinstance(value, torch.Tensor):
-                    self.state[p][name] = value.to(p.device).clone(memory_format=torch.preserve_format)
+
+def _rate(lr, adjust_lr_fn, shape):
+    rows, cols = shape
+    if rows == 0 or cols == 0:
+        return 0.0
+    if adjust_lr_fn == "match_rms_adamw":
+        return lr * 0.2 * math.sqrt(max(rows, cols))
+    return lr * math.sqrt(max(1.0, rows / cols))
+
+
+def muon_step(params, grads, momenta, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True,
+              ns_coefficients=(3.4445, -4.775, 2.0315), eps=1e-7, ns_steps=5, adjust_lr_fn=None,
+              masters=None):
+    """One Muon step, in place, over lists of matrices:
+
+        m = momentum m + (1 - momentum) g
+        u = momentum m + (1 - momentum) g  (nesterov; else u = m)
+        X = u / max(|u|, eps),  ns_steps times  X = c0 X + (c1 A + c2 A^2) X,  A = X X^T
+        p = p (1 - lr weight_decay) - lr adjust X
+
+    Arguments:
+        params: contiguous matrices of one type (float32 or bfloat16) on one device
+        grads: their gradients, of the same type and shapes
+        momenta: m, contiguous float32 in the parameters' shapes
+        lr, weight_decay, momentum, eps: floats
+        ns_coefficients: c0, c1, c2; such that X's values stay below 60
+        ns_steps: int, 1 to 100
+        adjust_lr_fn: None or "original": adjust = sqrt(max(1, rows / cols));
+            "match_rms_adamw": 0.2 sqrt(max(rows, cols))
+        masters: contiguous float32 matrices in the parameters' shapes that the step moves
+            in the parameters' place; each parameter becomes its master's rounding
+
+    X and A are held to 22 bits whatever the parameters' type.  The matrices that it writes
+    do not overlap; one that comes twice is refused.  The rates are part of the launch: a
+    step captured in a graph keeps them.
+    """
+    assert adjust_lr_fn in (None, "original", "match_rms_adamw"), \
+        'adjust_lr_fn must be None, "original" or "match_rms_adamw"'
+    assert all(p.dim() == 2 for p in params), 'muon_step takes matrices'
+    rates = [_rate(float(lr), adjust_lr_fn, p.shape) for p in params]
+    torch_binding().muon(params, grads, momenta, rates, float(lr), float(weight_decay),
+                         float(momentum), bool(nesterov), tuple(map(float, ns_coefficients)),
+                         float(eps), int(ns_steps), masters)
+
+
+class Muon(_Optimizer):
+    """Muon on ``muon_step``, for the matrices of a network (the others take AdamW).
+
+    Arguments:
+        params: matrices or groups of them, contiguous, float32 or bfloat16 on the GPU
+        lr, weight_decay, momentum, nesterov, ns_coefficients, eps, ns_steps,
+            adjust_lr_fn: as ``muon_step``
+        master_weights: bool, keep 32-bit values of bfloat16 parameters, which otherwise
+            lose steps smaller than their rounding (taken from the parameters at the first
+            step; a parameter set by hand afterwards is not seen)
+    """
+
+    def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True,
+                 ns_coefficients=(3.4445, -4.775, 2.0315), eps=1e-7, ns_steps=5, adjust_lr_fn=None, *,
+                 master_weights=True):
+        assert lr >= 0 and eps >= 0 and weight_decay >= 0, \
+            'lr, eps and weight_decay must not be negative'
+        assert 0 <= momentum < 1, 'momentum must be in [0, 1)'
+        assert 1 <= ns_steps <= 100, 'ns_steps must be from 1 to 100'
+        assert adjust_lr_fn in (None, "original", "match_rms_adamw"), \
+            'adjust_lr_fn must be None, "original" or "match_rms_adamw"'
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum,
+                                      nesterov=nesterov, ns_coefficients=tuple(ns_coefficients),
+                                      eps=eps, ns_steps=ns_steps, adjust_lr_fn=adjust_lr_fn,
+                                      master_weights=master_weights))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() != 2:
+                self.param_groups.pop()
+                raise AssertionError('Muon takes matrices; give the other parameters to AdamW')
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """One step for every matrix that has a gradient."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            for p in group["params"]:
+                assert p.grad is None or not p.grad.is_sparse, 'Muon does not take sparse gradients'
+        for group in self.param_groups:
+            # one call for the matrices of one type and device
+            calls = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                state = self.state[p]
+                if not state:
+                    state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                    if p.dtype != torch.float32 and group["master_weights"]:
+                        state["master"] = p.detach().float()
+                calls.setdefault((p.dtype, p.device, "master" in state), []).append((p, state))
+            for (_, _, master), found in calls.items():
+                muon_step([p for p, _ in found], [p.grad for p, _ in found],
+                          [s["momentum_buffer"] for _, s in found], group["lr"], group["weight_decay"],
+                          group["momentum"], group["nesterov"], group["ns_coefficients"], group["eps"],
+                          group["ns_steps"], group["adjust_lr_fn"],
+                          [s["master"] for _, s in found] if master else None)
+        return loss

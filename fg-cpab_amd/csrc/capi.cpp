@@ -672,8 +672,8 @@ const char* cpab_last_error_string(void) { return g_last_error.c_str(); }
 // the uniform grid's per-axis coordinates instead of the meshgrid.  402:
 // cpab_transform_data_backward_data.  403: the operators around the transform.
 // 404: cpab_recurrence_max_stride.  405: cpab_qk_norm_*.
-// 406: cpab_delta_rule_*.
-int cpab_abi_version(void) { return 406; }
+// 406: cpab_delta_rule_*.  407: cpab_muon_*.
+int cpab_abi_version(void) { return 407; }
 
 int cpab_affine(int ndim, int64_t n_theta, int nC, int d, const float* theta,
                 const int32_t* row_ptr, const int32_t* col_idx, const float* vals, float* As,

@@ -30,6 +30,8 @@ int size_of(int dtype) { return dtype == CPAB_F32 ? 4 : 2; }
 
 // Values of one array below 2^37, rows and channels below 2^31.
 constexpr int64_t kMaxValues = 1LL << 37, kMaxCount = (1LL << 31) - 1;
+// Rows, columns and values of a matrix of a Muon step.
+constexpr int64_t kMuonMost = 1LL << 20, kMuonMostValues = 1LL << 30;
 
 int check_recurrence(int dtype, int64_t B, int64_t T, int64_t C) {
   CPAB_TRY(check_dtype("dtype", dtype));
@@ -148,6 +150,22 @@ int norm_forward(const char* who, int dtype, int residual_dtype, int weight_dtyp
   return check_hip(cpab::launch_rms_norm_forward(n, y, eight ? scale : nullptr, residual_out, rstd,
                                                  as_stream(stream)),
                    who);
+}
+
+int check_muon_sizes(int64_t n_matrices, const cpab_muon_matrix* matrices) {
+  if (n_matrices < 0) return fail(CPAB_ERR_INVALID, "negative number of matrices");
+  if (n_matrices > kMaxCount) return fail(CPAB_ERR_INVALID, "%lld matrices are too many", (long long)n_matrices);
+  if (n_matrices > 0) CPAB_REQUIRE(matrices);
+  for (int64_t k = 0; k < n_matrices; ++k) {
+    const int64_t rows = matrices[k].rows, cols = matrices[k].cols;
+    if (rows < 0 || cols < 0)
+      return fail(CPAB_ERR_INVALID, "matrix %lld has a negative size", (long long)k);
+    // a launch's workgroups and lanes are counted in 32 bits over all its matrices
+    if (rows > kMuonMost || cols > kMuonMost || rows * cols > kMuonMostValues)
+      return fail(CPAB_ERR_INVALID, "matrix %lld of %lld x %lld is too large", (long long)k, (long long)rows,
+                  (long long)cols);
+  }
+  return CPAB_OK;
 }
 
 }  // namespace
@@ -313,6 +331,60 @@ int cpab_adamw_step(int dtype, int state_bits, int64_t n_tensors, const cpab_ada
   a.key = cpab::adamw_mix(seed ^ ((uint32_t)step * 0x9E3779B1u));
   return check_hip(cpab::launch_adamw(dtype, state_bits, n_tensors, tensors, a, as_stream(stream)),
                    "cpab_adamw_step");
+}
+
+int64_t cpab_muon_workspace_size(int64_t n_matrices, const cpab_muon_matrix* matrices) {
+  if (check_muon_sizes(n_matrices, matrices) != CPAB_OK) return 0;
+  return cpab::muon_workspace(n_matrices, matrices);
+}
+
+int cpab_muon_step(int dtype, int64_t n_matrices, const cpab_muon_matrix* matrices,
+                   const double* rates, double lr, double weight_decay, double momentum, int nesterov,
+                   const double* coefficients, double eps, int ns_steps, void* workspace,
+                   int64_t workspace_bytes, void* stream) {
+  CPAB_TRY(check_dtype("dtype", dtype));
+  CPAB_TRY(check_muon_sizes(n_matrices, matrices));
+  if (!(momentum >= 0.0 && momentum < 1.0))
+    return fail(CPAB_ERR_INVALID, "momentum must be in [0, 1), got %g", momentum);
+  if (!(lr >= 0.0 && weight_decay >= 0.0 && eps >= 0.0))
+    return fail(CPAB_ERR_INVALID, "lr, weight_decay and eps must not be negative, got %g, %g and %g", lr,
+                weight_decay, eps);
+  if (ns_steps < 1 || ns_steps > 100)
+    return fail(CPAB_ERR_INVALID, "ns_steps must be from 1 to 100, got %d", ns_steps);
+  CPAB_REQUIRE(coefficients);
+  for (int k = 0; k < 3; ++k)
+    if (!std::isfinite(coefficients[k])) return fail(CPAB_ERR_INVALID, "coefficients must be finite");
+  bool any = false;
+  Once once(3 * n_matrices);
+  if (!once.room()) return fail(CPAB_ERR_INVALID, "no memory to look %lld matrices over", (long long)n_matrices);
+  for (int64_t k = 0; k < n_matrices; ++k) {
+    const cpab_muon_matrix& t = matrices[k];
+    if (t.rows == 0 || t.cols == 0) continue;
+    any = true;
+    CPAB_REQUIRE(t.param); CPAB_REQUIRE(t.grad); CPAB_REQUIRE(t.momentum);
+    CPAB_TYPED(t.param, dtype); CPAB_TYPED(t.grad, dtype);
+    CPAB_ALIGNED(t.momentum, 4); CPAB_ALIGNED(t.master, 4);
+    for (void* p : {t.param, (void*)t.momentum, (void*)t.master})
+      if (p && !once.add(p))
+        return fail(CPAB_ERR_INVALID, "an array of matrix %lld comes twice among those that the step writes",
+                    (long long)k);
+  }
+  if (!any) return CPAB_OK;
+  CPAB_REQUIRE(rates);
+  for (int64_t k = 0; k < n_matrices; ++k)
+    if (!std::isfinite(rates[k])) return fail(CPAB_ERR_INVALID, "rates must be finite");
+  CPAB_TRY(check_workspace(workspace, workspace_bytes, cpab::muon_workspace(n_matrices, matrices)));
+  CPAB_ALIGNED(workspace, 256);
+  cpab::Muon s;
+  s.momentum = (float)momentum;
+  s.rest = (float)(1.0 - momentum);
+  s.decay = (float)(1.0 - lr * weight_decay);
+  s.c0 = (float)coefficients[0], s.c1 = (float)coefficients[1], s.c2 = (float)coefficients[2];
+  s.eps = (float)eps;
+  s.steps = ns_steps;
+  s.nesterov = nesterov != 0;
+  return check_hip(cpab::launch_muon(dtype, n_matrices, matrices, rates, s, workspace, as_stream(stream)),
+                   "cpab_muon_step");
 }
 
 }  // extern "C"

@@ -1,0 +1,405 @@
+// A Muon step over many matrices: the momentum, the orthogonalisation of its update by
+// Newton-Schulz products, and the parameters' move.
+//
+// m = mu m + (1 - mu) g, u = mu m + (1 - mu) g (Nesterov) or m, X = u / max(|u|, eps),
+// then some times  A = X X^T,  B = c1 A + c2 A A,  X = c0 X + B X,  at last
+// p = p (1 - lr wd) - rate X.  X is taken with its shorter side first.
+//
+// Bound by the matrix unit.  Its 32-bit products run at a fourteenth of the 16-bit ones'
+// rate, so X, A and B are held as two 16-bit floats, the nearest to 2^10 times the value and
+// 2^11 times what is left, 22 bits together, and a product is three: hi hi in one sum and
+// hi lo + lo hi in another, 2^-11 of which joins it at the end; lo lo, 2^-22 of the whole,
+// is left out.  2^10: what is below 2^-24 of 1 falls under the normal 16-bit floats, what is
+// above 63 over them; X's values stay near 1 and the polynomial's near 5.
+// All products are of rows with rows, the summed index contiguous, since A and B are their
+// own transposes and X is kept both ways; of A and B the half above the diagonal is computed
+// and written twice.  Each step is one launch for all matrices together.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "sequence_device.hpp"
+#include "sequence_launch.hpp"
+
+namespace cpab {
+namespace {
+
+typedef _Float16 f16;
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kLanes = 256;
+constexpr int kMatrices = 40;      // of a launch
+constexpr int kSpan = kLanes * 16; // values of a workgroup of the momentum's kernel
+constexpr float kUp = 1024.0f, kDown = 1.0f / 1024.0f, kLow = 2048.0f, kJoin = 1.0f / 2048.0f;
+
+// A matrix and where its parts lie in the workspace (bytes).  X is [m, n], m <= n, of
+// padded sizes; planes of 16-bit floats: hi, then lo.
+struct Matrix {
+  void* param;
+  const void* grad;
+  float* momentum;
+  float* master;
+  int64_t at;
+  int rows, cols;
+  float rate;
+};
+struct Batch {
+  Matrix m[kMatrices];
+  uint32_t first[kMatrices + 1];   // workgroups before each matrix's
+};
+
+constexpr int kPad = 64;
+__host__ __device__ __forceinline__ int64_t padded(int64_t n) { return (n + kPad - 1) / kPad * kPad; }
+struct Places {
+  int64_t m, n;   // padded
+  int64_t sums, x0, x1, xt0, xt1, a, b, end;   // x: [m, n]; xt: [n, m]
+  __host__ __device__ int64_t x(int k) const { return k ? x1 : x0; }
+  __host__ __device__ int64_t xt(int k) const { return k ? xt1 : xt0; }
+};
+__host__ __device__ __forceinline__ Places places(int64_t rows, int64_t cols) {
+  Places p;
+  p.m = padded(rows < cols ? rows : cols);
+  p.n = padded(rows < cols ? cols : rows);
+  const int64_t spans = (rows * cols + kSpan - 1) / kSpan;
+  p.sums = 0;
+  p.x0 = (spans * 8 + 255) / 256 * 256;
+  const int64_t whole = 4 * p.m * p.n, square = 4 * p.m * p.m;
+  p.x1 = p.x0 + whole;
+  p.xt0 = p.x1 + whole;
+  p.xt1 = p.xt0 + whole;
+  p.a = p.xt1 + whole;
+  p.b = p.a + square;
+  p.end = p.b + square;
+  return p;
+}
+
+__device__ __forceinline__ int find(const Batch& batch, int count) {
+  int lo = 0, hi = count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (batch.first[mid] <= blockIdx.x) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+struct Momentum {
+  float mu, rest, eps;
+  bool nesterov;
+};
+__device__ __forceinline__ float update(const Momentum& s, float m, float g) {
+  return s.nesterov ? fmaf(s.mu, m, s.rest * g) : m;
+}
+
+// The momentum, and each span's sum of the update's squares (in 64 bits: squares of small
+// gradients leave the 32-bit range).
+template <typename T>
+__global__ __launch_bounds__(kLanes) void muon_momentum_kernel(Batch batch, int count, Momentum s, char* room) {
+  __shared__ double parts[kLanes / 64];
+  const int which = find(batch, count);
+  const Matrix& t = batch.m[which];
+  const int64_t n = (int64_t)t.rows * t.cols, span = blockIdx.x - batch.first[which];
+  double sum = 0.0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int64_t at = span * kSpan + 4 * (k * kLanes + (int64_t)threadIdx.x);
+    const int here = (int)min(n - at, (int64_t)4);
+    if (here <= 0) continue;
+    float m[4] = {}, g[4] = {};
+    const T* gp = static_cast<const T*>(t.grad) + at;
+    float* mp = t.momentum + at;
+    if (here == 4) {
+      load<4>(gp, g);
+      load<4>(mp, m);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < here) g[e] = to_float(gp[e]), m[e] = mp[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      m[e] = fmaf(s.mu, m[e], s.rest * g[e]);
+      const double u = e < here ? (double)update(s, m[e], g[e]) : 0.0;
+      sum = fma(u, u, sum);
+    }
+    if (here == 4) {
+      store<4>(mp, m);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < here) mp[e] = m[e];
+    }
+  }
+  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    reinterpret_cast<double*>(room + t.at)[span] = (parts[0] + parts[1]) + (parts[2] + parts[3]);
+}
+
+// 2^10 times a value in two 16-bit floats.
+struct Two {
+  f16 hi, lo;
+};
+__device__ __forceinline__ Two two_of(float x) {
+  const float v = x * kUp;
+  const f16 hi = (f16)v;
+  return Two{hi, (f16)((v - (float)hi) * kLow)};
+}
+
+// X and its transpose from the update, 64 x 64 values to a workgroup; zeros in the padding.
+template <typename T>
+__global__ __launch_bounds__(kLanes) void muon_start_kernel(Batch batch, int count, Momentum s, char* room) {
+  __shared__ f16 turn[2][64][66];
+  __shared__ double parts[kLanes / 64];
+  const int which = find(batch, count);
+  const Matrix& t = batch.m[which];
+  const Places p = places(t.rows, t.cols);
+  const double* sums = reinterpret_cast<const double*>(room + t.at);
+  const int64_t spans = ((int64_t)t.rows * t.cols + kSpan - 1) / kSpan;
+  double sum = 0.0;
+  for (int64_t k = threadIdx.x; k < spans; k += kLanes) sum += sums[k];
+  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  const double norm = sqrt((parts[0] + parts[1]) + (parts[2] + parts[3]));
+  const float by = (float)(1.0 / (norm < (double)s.eps ? (double)s.eps : norm));
+  // the parameter's own layout, [rows, cols], is X's or its transpose's
+  const bool wide = t.rows <= t.cols;
+  const int64_t prows = wide ? p.m : p.n, pcols = wide ? p.n : p.m;
+  f16* own = reinterpret_cast<f16*>(room + t.at + (wide ? p.x0 : p.xt0));
+  f16* other = reinterpret_cast<f16*>(room + t.at + (wide ? p.xt0 : p.x0));
+  const int64_t plane = p.m * p.n;
+  const int64_t tile = blockIdx.x - batch.first[which], across = pcols / 64;
+  const int64_t r0 = tile / across * 64, c0 = tile % across * 64;
+#pragma unroll 4
+  for (int k = 0; k < 16; ++k) {
+    const int r = k * 4 + (threadIdx.x >> 6), c = threadIdx.x & 63;
+    const int64_t row = r0 + r, col = c0 + c;
+    float x = 0.0f;
+    if (row < t.rows && col < t.cols) {
+      const int64_t at = row * t.cols + col;
+      x = update(s, t.momentum[at], to_float(static_cast<const T*>(t.grad)[at])) * by;
+    }
+    const Two v = two_of(x);
+    own[row * pcols + col] = v.hi;
+    own[plane + row * pcols + col] = v.lo;
+    turn[0][c][r] = v.hi;
+    turn[1][c][r] = v.lo;
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int k = 0; k < 16; ++k) {
+    const int c = k * 4 + (threadIdx.x >> 6), r = threadIdx.x & 63;
+    other[(c0 + c) * prows + r0 + r] = turn[0][c][r];
+    other[plane + (c0 + c) * prows + r0 + r] = turn[1][c][r];
+  }
+}
+
+enum Product { kGram, kPolynomial, kStep, kLast };
+struct Coefficients {
+  float c0, c1, c2, decay;
+  int from;   // which of the two X
+};
+
+// One tile of a product.  64 x 64: a wave has 32 x 32 of it, in two sums.
+template <Product WHAT, typename T>
+__global__ __launch_bounds__(kLanes) void muon_product_kernel(Batch batch, int count, Coefficients c, char* room) {
+  constexpr int kTile = 64, kStepK = 32, kPitch = kStepK + 8;
+  __shared__ f16 lds[2][4][kTile][kPitch];   // twice: rows' hi and lo, columns' hi and lo
+  const int which = find(batch, count);
+  const Matrix& t = batch.m[which];
+  const Places p = places(t.rows, t.cols);
+  char* const base = room + t.at;
+  const int64_t tile = blockIdx.x - batch.first[which];
+  int64_t ti, tj;
+  if (WHAT == kGram || WHAT == kPolynomial) {   // tj >= ti
+    tj = (int64_t)((sqrt(8.0 * (double)tile + 1.0) - 1.0) * 0.5);
+    while (tj * (tj + 1) / 2 > tile) --tj;
+    while ((tj + 1) * (tj + 2) / 2 <= tile) ++tj;
+    ti = tile - tj * (tj + 1) / 2;
+  } else {
+    const int64_t down = p.m / kTile;
+    ti = tile % down;
+    tj = tile / down;
+  }
+  const f16* x = reinterpret_cast<const f16*>(base + p.x(c.from));
+  const f16* xt = reinterpret_cast<const f16*>(base + p.xt(c.from));
+  f16* a = reinterpret_cast<f16*>(base + p.a);
+  f16* b = reinterpret_cast<f16*>(base + p.b);
+  const int64_t whole = p.m * p.n, square = p.m * p.m;
+  const int64_t K = WHAT == kGram ? p.n : p.m;
+  const f16* left = WHAT == kGram ? x : WHAT == kPolynomial ? a : b;
+  const f16* right = WHAT == kGram ? x : WHAT == kPolynomial ? a : xt;
+  const int64_t left_plane = WHAT == kGram ? whole : square;
+  const int64_t right_plane = WHAT == kPolynomial ? square : whole;
+  left += ti * kTile * K;
+  right += tj * kTile * K;
+  // a lane brings 16 bytes of each of the four arrays
+  const int row = threadIdx.x >> 2, part = (threadIdx.x & 3) * 8;
+  const f16* from[4] = {left + row * K + part, left + left_plane + row * K + part,
+                        right + row * K + part, right + right_plane + row * K + part};
+  u32x4 next[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) next[k] = *reinterpret_cast<const u32x4*>(from[k]);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 31, g = lane >> 5;
+  const int wr = (wave >> 1) * 32, wc = (wave & 1) * 32;
+  f32x16 acc = {}, low = {};
+  int buffer = 0;
+  for (int64_t k0 = 0; k0 < K; k0 += kStepK, buffer ^= 1) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) *reinterpret_cast<u32x4*>(&lds[buffer][k][row][part]) = next[k];
+    __syncthreads();
+    if (k0 + kStepK < K)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) next[k] = *reinterpret_cast<const u32x4*>(from[k] + k0 + kStepK);
+#pragma unroll
+    for (int k = 0; k < kStepK; k += 16) {
+      const f16x8 lh = *reinterpret_cast<const f16x8*>(&lds[buffer][0][wr + i][k + 8 * g]);
+      const f16x8 ll = *reinterpret_cast<const f16x8*>(&lds[buffer][1][wr + i][k + 8 * g]);
+      const f16x8 rh = *reinterpret_cast<const f16x8*>(&lds[buffer][2][wc + i][k + 8 * g]);
+      const f16x8 rl = *reinterpret_cast<const f16x8*>(&lds[buffer][3][wc + i][k + 8 * g]);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rh, acc, 0, 0, 0);
+      low = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rl, low, 0, 0, 0);
+      low = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll, rh, low, 0, 0, 0);
+    }
+  }
+  // a lane's column, and its 16 rows: four at a time, 8 apart
+  const int64_t col = tj * kTile + wc + i;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int64_t r0 = ti * kTile + wr + 8 * q + 4 * g;
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = fmaf(low[4 * q + e], kJoin, acc[4 * q + e]) * (kDown * kDown);
+    if (WHAT == kPolynomial) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float av = fmaf((float)a[square + (r0 + e) * p.m + col], kJoin, (float)a[(r0 + e) * p.m + col]) * kDown;
+        v[e] = fmaf(c.c2, v[e], c.c1 * av);
+      }
+    }
+    if (WHAT == kStep || WHAT == kLast) {
+      const f16x4 hi = *reinterpret_cast<const f16x4*>(xt + col * p.m + r0);
+      const f16x4 lo = *reinterpret_cast<const f16x4*>(xt + whole + col * p.m + r0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        v[e] = fmaf(c.c0, fmaf((float)lo[e], kJoin, (float)hi[e]) * kDown, v[e]);
+    }
+    if (WHAT == kLast) {
+      const bool wide = t.rows <= t.cols;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t pr = wide ? r0 + e : col, pc = wide ? col : r0 + e;
+        if (pr >= t.rows || pc >= t.cols) continue;
+        const int64_t at = pr * t.cols + pc;
+        T* to = static_cast<T*>(t.param) + at;
+        const float w = (t.master ? t.master[at] : to_float(*to)) * c.decay - t.rate * v[e];
+        *to = from_float<T>(w);
+        if (t.master) t.master[at] = w;
+      }
+      continue;
+    }
+    f16* out = WHAT == kGram ? a : WHAT == kPolynomial ? b : reinterpret_cast<f16*>(base + p.x(c.from ^ 1));
+    f16* turned = WHAT == kStep ? reinterpret_cast<f16*>(base + p.xt(c.from ^ 1)) : out;
+    const int64_t plane = WHAT == kStep ? whole : square, pitch = WHAT == kStep ? p.n : p.m;
+    f16x4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const Two w = two_of(v[e]);
+      hi[e] = w.hi, lo[e] = w.lo;
+      out[(r0 + e) * pitch + col] = w.hi;
+      out[plane + (r0 + e) * pitch + col] = w.lo;
+    }
+    if (WHAT == kStep || ti != tj) {
+      *reinterpret_cast<f16x4*>(turned + col * p.m + r0) = hi;
+      *reinterpret_cast<f16x4*>(turned + plane + col * p.m + r0) = lo;
+    }
+  }
+}
+
+// The matrices from k on that one launch takes, and their workspace.
+int64_t gather(int64_t n, const cpab_muon_matrix* matrices, const double* rates, int64_t* k, Batch* batch,
+               int* count) {
+  int64_t bytes = 0;
+  *count = 0;
+  for (; *k < n && *count < kMatrices; ++*k) {
+    const cpab_muon_matrix& t = matrices[*k];
+    if (t.rows == 0 || t.cols == 0) continue;
+    const int64_t need = (places(t.rows, t.cols).end + 255) / 256 * 256;
+    if (*count > 0 && bytes + need > (1LL << 32)) break;   // a few GB of workspace are enough
+    if (batch)
+      batch->m[*count] = Matrix{t.param, t.grad, t.momentum, t.master, bytes, (int)t.rows, (int)t.cols,
+                                (float)rates[*k]};
+    ++*count;
+    bytes += need;
+  }
+  return bytes;
+}
+
+}  // namespace
+
+int64_t muon_workspace(int64_t n, const cpab_muon_matrix* matrices) {
+  int64_t most = 0;
+  for (int64_t k = 0; k < n;) {
+    int count = 0;
+    most = std::max(most, gather(n, matrices, nullptr, &k, nullptr, &count));
+  }
+  return most;
+}
+
+hipError_t launch_muon(int dtype, int64_t n, const cpab_muon_matrix* matrices, const double* rates,
+                       const Muon& s, void* workspace, hipStream_t st) {
+  char* room = static_cast<char*>(workspace);
+  for (int64_t k = 0; k < n;) {
+    Batch batch;
+    int count = 0;
+    gather(n, matrices, rates, &k, &batch, &count);
+    if (count == 0) break;
+    // a launch of `each` workgroups for each matrix
+    const auto launch = [&](auto each, auto kernel) {
+      uint32_t total = 0;
+      for (int i = 0; i < count; ++i) {
+        batch.first[i] = total;
+        total += (uint32_t)each(batch.m[i], places(batch.m[i].rows, batch.m[i].cols));
+      }
+      kernel(total);
+      return hipGetLastError();
+    };
+    const auto typed = [&](auto t) {
+      typedef decltype(t) T;
+      const Momentum m{s.momentum, s.rest, s.eps, s.nesterov};
+      hipError_t e = launch(
+          [](const Matrix& a, const Places&) { return ((int64_t)a.rows * a.cols + kSpan - 1) / kSpan; },
+          [&](uint32_t blocks) { muon_momentum_kernel<T><<<blocks, kLanes, 0, st>>>(batch, count, m, room); });
+      if (e != hipSuccess) return e;
+      e = launch([](const Matrix&, const Places& p) { return p.m / 64 * (p.n / 64); },
+                 [&](uint32_t blocks) { muon_start_kernel<T><<<blocks, kLanes, 0, st>>>(batch, count, m, room); });
+      for (int i = 0; i < s.steps && e == hipSuccess; ++i) {
+        const Coefficients c{s.c0, s.c1, s.c2, s.decay, i & 1};
+        const auto half = [](const Matrix&, const Places& p) { return p.m / 64 * (p.m / 64 + 1) / 2; };
+        const auto whole = [](const Matrix&, const Places& p) { return p.m / 64 * (p.n / 64); };
+        e = launch(half, [&](uint32_t blocks) {
+          muon_product_kernel<kGram, T><<<blocks, kLanes, 0, st>>>(batch, count, c, room);
+          muon_product_kernel<kPolynomial, T><<<blocks, kLanes, 0, st>>>(batch, count, c, room);
+        });
+        if (e != hipSuccess) break;
+        e = launch(whole, [&](uint32_t blocks) {
+          if (i + 1 < s.steps)
+            muon_product_kernel<kStep, T><<<blocks, kLanes, 0, st>>>(batch, count, c, room);
+          else
+            muon_product_kernel<kLast, T><<<blocks, kLanes, 0, st>>>(batch, count, c, room);
+        });
+      }
+      return e;
+    };
+    const hipError_t e = dtype == CPAB_F32 ? typed(0.0f) : typed(bf16());
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace cpab

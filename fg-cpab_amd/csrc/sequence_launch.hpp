@@ -1,5 +1,5 @@
 // Launch interface of the operators around the transform (recurrence.hip,
-// rms_norm.hip, adamw.hip).  Arguments are validated by the caller
+// rms_norm.hip, adamw.hip, muon.hip).  Arguments are validated by the caller
 // (capi_sequence.cpp); a launcher only enqueues work on `s`.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -79,5 +79,16 @@ constexpr int64_t kAdamWMost = (1LL << 34) - 1024;   // values of one tensor
 hipError_t launch_adamw(int dtype, int state_bits, int64_t n_tensors,
                         const cpab_adamw_tensor* tensors, const AdamW& a, hipStream_t s);
 uint32_t adamw_mix(uint32_t z);
+
+struct Muon {
+  float momentum, rest;   // rest: 1 - momentum
+  float decay;            // 1 - lr weight_decay
+  float c0, c1, c2, eps;
+  int steps;
+  bool nesterov;
+};
+int64_t muon_workspace(int64_t n_matrices, const cpab_muon_matrix* matrices);
+hipError_t launch_muon(int dtype, int64_t n_matrices, const cpab_muon_matrix* matrices,
+                       const double* rates, const Muon& s, void* workspace, hipStream_t st);
 
 }  // namespace cpab

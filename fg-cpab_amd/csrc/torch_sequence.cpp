@@ -330,9 +330,73 @@ void adamw(const Tensors& params, const Tensors& grads, const Tensors& exp_avgs,
       for (const Tensor& t : **list) torch::autograd::impl::bump_version(t);
 }
 
+// ---- Muon ------------------------------------------------------------------------
+
+void muon(const Tensors& params, const Tensors& grads, const Tensors& momenta, const std::vector<double>& rates,
+          double lr, double weight_decay, double momentum, bool nesterov,
+          const std::array<double, 3>& coefficients, double eps, int64_t ns_steps,
+          const std::optional<Tensors>& masters) {
+  const size_t n = params.size();
+  if (grads.size() != n || momenta.size() != n || rates.size() != n || (masters && masters->size() != n))
+    fail("muon_step: the lists must have one entry for each of the " + std::to_string(n) + " parameters");
+  if (n == 0) return;
+  const Tensor& first = params[0];
+  if (!first.is_cuda()) fail("muon_step: only GPU tensors are supported");
+  if (!has_type(first)) fail("muon_step: expected float32 or bfloat16 parameters, got " + dtype_of(first));
+  const c10::OptionalDeviceGuard guard(first.device());
+  const at::NoGradGuard no_grad;
+  std::vector<cpab_muon_matrix> matrices(n);
+  Tensors copies;   // gradients in other layouts, until they are queued
+  for (size_t k = 0; k < n; ++k) {
+    const Tensor& p = params[k];
+    const auto where = [k] { return " of parameter " + std::to_string(k); };
+    const auto written = [&](const Tensor& t, at::ScalarType type, const char* name) {
+      if (t.device() != p.device() || t.scalar_type() != type || t.sizes() != p.sizes() || !t.is_contiguous())
+        fail(std::string("muon_step: ") + name + where() + " must be contiguous " + c10::getDtypeNames(type).first +
+             " in the parameter's shape " + shape_of(p) + " on its device, got " + shape_of(t) + " " + dtype_of(t));
+      if (t.is_inference() && !c10::InferenceMode::is_enabled())
+        fail(std::string("muon_step: ") + name + where() +
+             " is an inference tensor, which may not be changed outside inference mode");
+      return t.data_ptr();
+    };
+    if (p.device() != first.device() || p.scalar_type() != first.scalar_type())
+      fail("muon_step: the parameters must have one type and one device; parameter " + std::to_string(k) +
+           " is " + dtype_of(p) + " on " + p.device().str());
+    if (p.dim() != 2) fail("muon_step: parameter " + std::to_string(k) + " must be a matrix, got " + shape_of(p));
+    Tensor g = grads[k];
+    if (g.device() != p.device() || g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes() ||
+        g.layout() != at::kStrided)
+      fail("muon_step: the gradient" + where() + " must be dense in the parameter's shape " + shape_of(p) +
+           ", type and device, got " + shape_of(g) + " " + dtype_of(g));
+    if (!g.is_contiguous()) {
+      g = g.contiguous();
+      copies.push_back(g);
+    }
+    cpab_muon_matrix& t = matrices[k];
+    t.param = written(p, p.scalar_type(), "the value");
+    t.grad = g.data_ptr();
+    t.momentum = static_cast<float*>(written(momenta[k], at::kFloat, "the momentum"));
+    t.master = masters ? static_cast<float*>(written((*masters)[k], at::kFloat, "the master")) : nullptr;
+    t.rows = p.size(0), t.cols = p.size(1);
+  }
+  if (ns_steps < 1 || ns_steps > 100) fail("muon_step: ns_steps must be from 1 to 100");
+  const int64_t bytes = cpab_muon_workspace_size((int64_t)n, matrices.data());
+  at::DataPtr ws;
+  if (bytes > 0) ws = scratch(bytes);
+  check(cpab_muon_step(type_of(first), (int64_t)n, matrices.data(), rates.data(), lr, weight_decay, momentum,
+                       nesterov, coefficients.data(), eps, (int)ns_steps, ws.get(), bytes, stream_of(first)),
+        "cpab_muon_step");
+  // autograd sees the tensors as changed in place
+  for (const Tensors* list : {&params, &momenta})
+    for (const Tensor& t : *list) torch::autograd::impl::bump_version(t);
+  if (masters)
+    for (const Tensor& t : *masters) torch::autograd::impl::bump_version(t);
+}
+
 }  // namespace
 
 void sequence_functions(py::module& m) {
+  m.def("muon", &muon);
   m.def("recurrence", &recurrence);
   m.def("rms_norm", &rms_norm);
   m.def("adamw", &adamw);

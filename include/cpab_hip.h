@@ -51,7 +51,7 @@ const char* cpab_last_error_string(void);
  * cpab_transform_data_backward_data.  403: the operators around the transform
  * (cpab_recurrence_*, cpab_rms_norm_*, cpab_adamw_step).  404:
  * cpab_recurrence_max_stride.  405: cpab_qk_norm_*.
- * 406: cpab_delta_rule_*. */
+ * 406: cpab_delta_rule_*.  407: cpab_muon_*. */
 int cpab_abi_version(void);
 
 /* A = B theta per theta: As[b, r] = sum_k vals[k] * theta[b, col_idx[k]] over
@@ -553,6 +553,32 @@ int cpab_delta_rule_backward(const cpab_delta_rule* rule, const float* kept, con
                              const float* grad_h, void* grad_q, void* grad_k, void* grad_v,
                              void* grad_decay, void* grad_beta, float* grad_h0, void* workspace,
                              int64_t workspace_bytes, void* stream);
+
+/* One matrix of a Muon step: rows x cols values, contiguous, of the parameter and its
+ * gradient (of the step's dtype) and of the momentum (float32); master as for AdamW.  The
+ * arrays that a step writes do not overlap; one that comes twice is refused. */
+typedef struct {
+  void* param;
+  const void* grad;
+  float* momentum;
+  float* master;
+  int64_t rows, cols;
+} cpab_muon_matrix;
+
+/* A Muon step over n matrices (an array in host memory, read before the call returns):
+ *   m = momentum m + (1 - momentum) g,  u = momentum m + (1 - momentum) g (nesterov; else m),
+ *   X = u / max(|u|, eps) (Frobenius; transposed where rows > cols),
+ *   ns_steps times: A = X X^T, X = c0 X + (c1 A + c2 A^2) X,
+ *   p = p (1 - lr weight_decay) - rates[i] X,
+ * rates: one for each matrix.  X and A are held to 22 bits and multiplied in three 16-bit
+ * products, which are added in 32; coefficients that bring a value of X or of the
+ * polynomial's factor past 60 give what is not finite.  workspace:
+ * cpab_muon_workspace_size(...) bytes, 256-byte aligned. */
+int64_t cpab_muon_workspace_size(int64_t n_matrices, const cpab_muon_matrix* matrices);
+int cpab_muon_step(int dtype, int64_t n_matrices, const cpab_muon_matrix* matrices,
+                   const double* rates, double lr, double weight_decay, double momentum,
+                   int nesterov, const double* coefficients, double eps, int ns_steps,
+                   void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
