@@ -32,7 +32,10 @@ namespace cpab {
 constexpr int kChunk = 64;    // samples
 constexpr int kDeltaBlock = 256;
 constexpr int kSquare = kChunk * kChunk;
+constexpr int kRow = kChunk + 8;   // pitch of 64 16-bit values in LDS: rows begin 4 banks apart
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 // A call as the kernels take it.
 struct Delta {
@@ -53,93 +56,104 @@ __device__ __forceinline__ float gate_at(const Delta& d, const void* p, int64_t 
 }
 __device__ __forceinline__ float clamped(float decay) { return decay < -128.0f ? -128.0f : decay; }
 
-// The gates of a chunk.  The logarithms are added in 64 bits: their differences are what
-// counts, and a sample that clears the state (-128) would leave 32 bits 2^-17 of it.
-struct Gates {
-  double G[kChunk];
-  float since[kChunk];   // exp(G_i)
-  float until[kChunk];   // exp(G_63 - G_i)
-  float beta[kChunk];
+// ---- products ------------------------------------------------------------------
+
+// The matrix unit's 32-bit products run at a sixteenth of the bfloat16 ones' rate, so that
+// values of 32 bits go as sums of bfloat16 parts, each the nearest to what the ones before
+// leave: two with 16-bit inputs, 17 bits, far beyond what a 16-bit result shows and enough
+// for the states and gates' gradients in 32; three with 32-bit inputs, 24 bits.  A 16-bit
+// input is its own first part.  Of the products of parts those are taken that are not below
+// the last part's rounding.
+template <typename T>
+struct Parts {
+  static constexpr int kInput = 1, kValue = 2;
 };
-// By the first wave; the caller synchronises.
-__device__ __forceinline__ void load_gates(Gates& s, const Delta& d, int64_t b, int h, int64_t t0, int live) {
-  if (threadIdx.x >= 64) return;
-  const int t = threadIdx.x;
-  double g = 0.0;
-  float beta = 0.0f;
-  if (t < live) {
-    g = (double)clamped(gate_at(d, d.r.decay, b * d.r.decay_strides[0] + (t0 + t) * d.r.decay_strides[1] +
-                                                  h * d.r.decay_strides[2]));
-    beta = gate_at(d, d.r.beta, b * d.r.beta_strides[0] + (t0 + t) * d.r.beta_strides[1] +
-                                    h * d.r.beta_strides[2]);
+template <>
+struct Parts<float> {
+  static constexpr int kInput = 3, kValue = 3;
+};
+template <int N>
+struct Frag {   // 8 neighbours of the summed index
+  bf16x8 p[N];
+};
+template <int N>
+__device__ __forceinline__ void split(float v, bf16 (&p)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    p[k] = (bf16)v;
+    v -= (float)p[k];
   }
-  for (int k = 1; k < 64; k *= 2) {
-    const double before = __shfl_up(g, k);
-    if (t >= k) g += before;
+}
+template <int N>
+__device__ __forceinline__ Frag<N> frag_of(const float v[8]) {
+  Frag<N> f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    bf16 p[N];
+    split<N>(v[e], p);
+#pragma unroll
+    for (int k = 0; k < N; ++k) f.p[k][e] = p[k];
   }
-  s.G[t] = g;
-  s.beta[t] = beta;
-  s.since[t] = expf((float)g);
-  s.until[t] = expf((float)(__shfl(g, 63) - g));
+  return f;
+}
+// acc += A B^T: 16 x 16, over 32 of the summed index.
+template <int NA, int NB>
+__device__ __forceinline__ void mma(f32x4& acc, const Frag<NA>& a, const Frag<NB>& b) {
+  constexpr int kLast = (NA > NB ? NA : NB) - 1;
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      if (i + j <= kLast) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[j], acc, 0, 0, 0);
 }
 
-// [64, D] of a chunk as 32-bit floats in LDS, zeros beyond `live` and D (up to DP).
-template <int DP, typename T>
-__device__ __forceinline__ void load_rows(float* to, int pitch, const T* from, int64_t stride, int live, int D) {
-  constexpr int kQuads = DP / 4;
-#pragma unroll 4
-  for (int k = threadIdx.x; k < kChunk * kQuads; k += kDeltaBlock) {
-    const int row = k / kQuads, col = k % kQuads * 4;
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (row < live) {
-      const T* p = from + row * stride + col;
-      if (col + 4 <= D) {
-        load<4>(p, v);
-      } else {
+// 8 neighbours of a row of an input, zeros where it has fewer (`left`).
+__device__ __forceinline__ Frag<1> input_frag(const bf16* p, int left) {
+  typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+  typedef U4 __attribute__((aligned(2))) Unit;
+  Frag<1> f;
+  if (left >= 8) {
+    f.p[0] = __builtin_bit_cast(bf16x8, (U4)*reinterpret_cast<const Unit*>(p));
+  } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (col + e < D) v[e] = to_float(p[e]);
-      }
-    }
-    *reinterpret_cast<f32x4*>(to + row * pitch + col) = f32x4{v[0], v[1], v[2], v[3]};
+    for (int e = 0; e < 8; ++e) f.p[0][e] = e < left ? p[e] : (bf16)0.0f;
   }
+  return f;
+}
+__device__ __forceinline__ Frag<3> input_frag(const float* p, int left) {
+  float v[8];
+  if (left >= 8) {
+    load<8>(p, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < left ? p[e] : 0.0f;
+  }
+  return frag_of<3>(v);
 }
 
-// acc += A B^T of 16 x 16 tiles by the matrix unit: A [16 MT, n], B [16 NT, n] in LDS, the
-// summed index contiguous, or with AT / BT the other one; `scale`: of the summed index (or
-// NULL).  A lane takes four neighbours of the summed index at once, the same of A and B, so
-// that one wide read feeds four products.
-template <bool ACROSS>
-__device__ __forceinline__ f32x4 operand(const float* p, int pitch, int row, int k) {
-  if (!ACROSS) return *reinterpret_cast<const f32x4*>(p + row * pitch + k);
-  return f32x4{p[k * pitch + row], p[(k + 1) * pitch + row], p[(k + 2) * pitch + row], p[(k + 3) * pitch + row]};
+// Operands in planes of 16-bit parts, in LDS or the workspace: 8 neighbours to a lane.
+template <int N>
+__device__ __forceinline__ Frag<N> plane_frag(const bf16* at, int plane) {
+  Frag<N> f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) f.p[k] = *reinterpret_cast<const bf16x8*>(at + k * plane);
+  return f;
 }
-template <bool AT, bool BT, int MT, int NT>
-__device__ __forceinline__ void multiply(f32x4 (&acc)[MT][NT], const float* A, int lda, const float* B,
-                                         int ldb, int n, const float* scale = nullptr) {
-  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-#pragma unroll 2
-  for (int k0 = 0; k0 < n; k0 += 16) {
-    const int k = k0 + 4 * g;
-    f32x4 a[MT], b[NT];
+// Four neighbours of the summed index, as the sums of a product lie in a lane.
+template <int N>
+__device__ __forceinline__ void put4(bf16* at, int plane, const f32x4& v) {
+  bf16x4 out[N];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) a[m] = operand<AT>(A, lda, 16 * m + i, k);
+  for (int e = 0; e < 4; ++e) {
+    bf16 p[N];
+    split<N>(v[e], p);
 #pragma unroll
-    for (int c = 0; c < NT; ++c) b[c] = operand<BT>(B, ldb, 16 * c + i, k);
-    if (scale) {
-      const f32x4 s = *reinterpret_cast<const f32x4*>(scale + k);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) a[m] *= s;
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int c = 0; c < NT; ++c)
-          acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[m][e], b[c][e], acc[m][c], 0, 0, 0);
+    for (int k = 0; k < N; ++k) out[k][e] = p[k];
   }
+#pragma unroll
+  for (int k = 0; k < N; ++k) *reinterpret_cast<bf16x4*>(at + k * plane) = out[k];
 }
+
 template <int MT, int NT>
 __device__ __forceinline__ void clear(f32x4 (&acc)[MT][NT]) {
 #pragma unroll
@@ -148,12 +162,34 @@ __device__ __forceinline__ void clear(f32x4 (&acc)[MT][NT]) {
     for (int c = 0; c < NT; ++c) acc[m][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 }
 
-// How four waves share a state's block of [DP, E]: WD of them over DP.
+// How the waves of a workgroup share a state's block of [DP, E]: WD of them over DP.
 template <int DP, int E>
 struct Shares {
-  static constexpr int WD = DP / 16 < 4 ? DP / 16 : 4, WE = 4 / WD;
+  static constexpr int W = E / 8, WD = DP / 16 < 4 ? DP / 16 : 4, WE = W / WD;
   static constexpr int MT = DP / 16 / WD, NT = E / 16 / WE;
 };
+
+// ---- workspace -----------------------------------------------------------------
+
+// What the first kernel leaves of a chunk of a head: exp(G_i), exp(G_63 - G_i) and beta;
+// M and P (their transposes for the backward) in planes.
+struct Gates {
+  float since[kChunk], until[kChunk], beta[kChunk];
+};
+template <typename T>
+struct Squares {
+  Gates gates;
+  bf16 m[Parts<T>::kValue][kChunk][kChunk];
+  bf16 p[Parts<T>::kValue][kChunk][kChunk];
+};
+inline int64_t squares_bytes(int dtype) {
+  return dtype == CPAB_F32 ? (int64_t)sizeof(Squares<float>) : (int64_t)sizeof(Squares<bf16>);
+}
+// And of a chunk of a key's head: k transposed, and for the backward q too: [DP, 64].
+inline int key_rows(const cpab_delta_rule& r) { return r.dk <= 32 ? 32 : r.dk <= 64 ? 64 : 128; }
+inline int64_t turned_bytes(const cpab_delta_rule& r) {
+  return (int64_t)key_rows(r) * kChunk * (r.dtype == CPAB_F32 ? 4 : 2);
+}
 
 // f(T(), DP) as types and constants.
 template <typename F>
@@ -170,9 +206,35 @@ inline Delta delta_of(const cpab_delta_rule& r) {
   return Delta{r, (int)((r.T + kChunk - 1) / kChunk), (int)(r.heads / r.key_heads)};
 }
 
-// Workspace of a chunk of a head: M, P, A.
-constexpr int64_t kSquares = 3 * kSquare;
+// How a call is cut: a head's chunks in `segs` segments of `each`.
+struct Cut {
+  int segs, each;
+};
+Cut cut_of(const Delta& d);
 
-hipError_t launch_delta_squares(const Delta& d, float* squares, hipStream_t s);
+// Which part of a head a workgroup has.  The column blocks of one segment lie on one XCD,
+// whose cache they share: workgroup n runs on XCD n mod 8.
+struct Where {
+  int64_t bh;
+  int seg, block;
+  bool in;
+};
+__device__ __forceinline__ Where where(int64_t heads, int segs, int blocks) {
+  const int64_t slot = blockIdx.x / 8, group = slot / blocks * 8 + blockIdx.x % 8;
+  return Where{group % heads, (int)(group / heads), (int)(slot % blocks), group < heads * segs};
+}
+
+// What a forward keeps, in floats: the states before each chunk, X, and the segments' ends.
+struct Kept {
+  int64_t states, xs, ends, all;
+};
+Kept kept_of(const Delta& d, const Cut& cut);
+
+// squares: of each chunk of each head; kt, qt: of each of each key's head, qt NULL in the
+// forward.
+hipError_t launch_delta_squares(const Delta& d, void* squares, void* kt, void* qt, hipStream_t s);
+hipError_t launch_delta_join(const Delta& d, const Cut& cut, bool forward, const float* ends, const float* adds,
+                             const float* given, float* to, hipStream_t s);
+int64_t delta_backward_workspace(const Delta& d);   // bytes
 
 }  // namespace cpab

@@ -11,99 +11,188 @@ namespace {
 
 // ---- a chunk's matrices ------------------------------------------------------
 
-// M, P and A of each chunk of each head.  M by rows: M_i = A_i - sum over j < i of
-// A_ij beta_j M_j; a column is four lanes', each with a quarter of the rows.
-template <typename T, int DP>
-__global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, float* squares) {
-  constexpr int kPitch = DP + 4, kRow = kChunk + 4;
+// 64 x 64 values from LDS to planes in the workspace, or their transpose.
+template <int N, bool TURNED>
+__device__ __forceinline__ void put_square(const float* from, int pitch, bf16 (&to)[N][kChunk][kChunk]) {
+  const int row = threadIdx.x >> 2, col = (threadIdx.x & 3) * 16;
+#pragma unroll
+  for (int half = 0; half < 16; half += 8) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      v[e] = TURNED ? from[(col + half + e) * pitch + row] : from[row * pitch + col + half + e];
+    const Frag<N> f = frag_of<N>(v);
+#pragma unroll
+    for (int k = 0; k < N; ++k) *reinterpret_cast<bf16x8*>(&to[k][row][col + half]) = f.p[k];
+  }
+}
+
+// A chunk's [64, D] of an input, transposed, to the workspace: [DP, 64], zeros beyond `live`
+// and D.  Called by the whole workgroup; `room` holds DP rows of kRow values.
+template <int DP, typename T>
+__device__ __forceinline__ void put_turned(T* room, const T* from, int64_t stride, int live, int D, T* to) {
+  for (int k = threadIdx.x; k < kChunk * DP / 4; k += kDeltaBlock) {
+    const int row = k / (DP / 4), col = k % (DP / 4) * 4;
+    const T* p = from + row * stride + col;
+    const int left = row < live ? D - col : 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) room[(col + e) * kRow + row] = e < left ? p[e] : (T)0.0f;
+  }
+  __syncthreads();
+  constexpr int kEach = 16 / sizeof(T);
+  typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+  for (int k = threadIdx.x; k < DP * kChunk / kEach; k += kDeltaBlock) {
+    const int row = k / (kChunk / kEach), col = k % (kChunk / kEach) * kEach;
+    *reinterpret_cast<U4*>(to + row * kChunk + col) = *reinterpret_cast<const U4*>(room + row * kRow + col);
+  }
+  __syncthreads();
+}
+
+// The gates, M and P of each chunk of each head, and the transposes of its keys and queries.
+// The decays' logarithms are added in 64 bits: their differences are what counts, and a
+// sample that clears the state (-128) would leave 32 bits 2^-17 of it.  M by rows:
+// M_i = A_i - sum over j < i of A_ij beta_j M_j; a column is four lanes', each with a quarter
+// of the rows.
+template <typename T, int DP, bool BACKWARD>
+__global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, Squares<T>* squares, T* kt, T* qt) {
+  constexpr int kPitch = kChunk + 4, NV = Parts<T>::kValue, NI = Parts<T>::kInput;
   extern __shared__ float room[];
-  __shared__ Gates gates;
-  float* K = room;
-  float* Q = K + kChunk * kPitch;
+  __shared__ double G[kChunk];
+  __shared__ float betas[kChunk];
   const int c = blockIdx.x % d.chunks;
   const int64_t bh = blockIdx.x / d.chunks, b = bh / d.r.heads;
-  const int h = (int)(bh - b * d.r.heads), kh = h / d.group;
+  const int h = (int)(bh - b * d.r.heads), kh = h / d.group, dk = (int)d.r.dk;
   const int64_t t0 = (int64_t)c * kChunk;
   const int live = (int)min(max(live_of(d, b) - t0, (int64_t)0), (int64_t)kChunk);
   if (live == 0) return;
-  load_gates(gates, d, b, h, t0, live);
-  load_rows<DP>(K, kPitch, static_cast<const T*>(d.r.k) + b * d.r.k_strides[0] + t0 * d.r.k_strides[1] + kh * d.r.k_strides[2],
-                d.r.k_strides[1], live, (int)d.r.dk);
-  load_rows<DP>(Q, kPitch, static_cast<const T*>(d.r.q) + b * d.r.q_strides[0] + t0 * d.r.q_strides[1] + kh * d.r.q_strides[2],
-                d.r.q_strides[1], live, (int)d.r.dk);
-  __syncthreads();
+  Squares<T>& out = squares[bh * d.chunks + c];
+  if (threadIdx.x < kChunk) {
+    const int t = threadIdx.x;
+    double g = 0.0;
+    float beta = 0.0f;
+    if (t < live) {
+      g = (double)clamped(gate_at(d, d.r.decay, b * d.r.decay_strides[0] + (t0 + t) * d.r.decay_strides[1] +
+                                                    h * d.r.decay_strides[2]));
+      beta = gate_at(d, d.r.beta, b * d.r.beta_strides[0] + (t0 + t) * d.r.beta_strides[1] +
+                                      h * d.r.beta_strides[2]);
+    }
+    for (int k = 1; k < 64; k *= 2) {
+      const double before = __shfl_up(g, k);
+      if (t >= k) g += before;
+    }
+    G[t] = g;
+    betas[t] = beta;
+    out.gates.since[t] = expf((float)g);
+    out.gates.until[t] = expf((float)(__shfl(g, 63) - g));
+    out.gates.beta[t] = beta;
+  }
+  const T* k = static_cast<const T*>(d.r.k) + b * d.r.k_strides[0] + t0 * d.r.k_strides[1] + kh * d.r.k_strides[2];
+  const T* q = static_cast<const T*>(d.r.q) + b * d.r.q_strides[0] + t0 * d.r.q_strides[1] + kh * d.r.q_strides[2];
+  const int64_t ks = d.r.k_strides[1], qs = d.r.q_strides[1];
+  if (h % d.group == 0) {
+    const int64_t at = ((b * d.r.key_heads + kh) * d.chunks + c) * DP * kChunk;
+    put_turned<DP>(reinterpret_cast<T*>(room), k, ks, live, dk, kt + at);
+    if (BACKWARD) put_turned<DP>(reinterpret_cast<T*>(room), q, qs, live, dk, qt + at);
+  }
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   f32x4 kk[1][4], qk[1][4];
   clear(kk);
   clear(qk);
-  multiply<false, false>(kk, K + 16 * wave * kPitch, kPitch, K, kPitch, DP);
-  multiply<false, false>(qk, Q + 16 * wave * kPitch, kPitch, K, kPitch, DP);
+#pragma unroll
+  for (int col = 8 * g; col < DP; col += 32) {
+    const int row = 16 * wave + i, left = row < live ? dk - col : 0;
+    const Frag<NI> ak = input_frag(k + row * ks + col, left), aq = input_frag(q + row * qs + col, left);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int other = 16 * n + i;
+      const Frag<NI> bk = input_frag(k + other * ks + col, other < live ? dk - col : 0);
+      mma(kk[0][n], ak, bk);
+      mma(qk[0][n], aq, bk);
+    }
+  }
   __syncthreads();
-  float* Ab = room;                  // A beta, in K's place; its columns 4 q + p at 16 p + q
-  float* A = room + kChunk * kRow;
-  float* out = squares + (bh * d.chunks + c) * kSquares;
+  float* Ab = room;                  // A beta; its columns 4 q + p at 16 p + q
+  float* A = room + kChunk * kPitch;
 #pragma unroll
   for (int n = 0; n < 4; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int row = 16 * wave + 4 * g + e, col = 16 * n + i;
-      const float decay = col <= row ? expf((float)(gates.G[row] - gates.G[col])) : 0.0f;
+      const float decay = col <= row ? expf((float)(G[row] - G[col])) : 0.0f;
       const float a = col < row ? decay * kk[0][n][e] : 0.0f;
-      out[kSquare + row * kChunk + col] = d.r.scale * decay * qk[0][n][e];
-      out[2 * kSquare + row * kChunk + col] = a;
-      Ab[row * kRow + (col & 3) * 16 + (col >> 2)] = a * gates.beta[col];
-      A[row * kRow + col] = a;
+      qk[0][n][e] *= d.r.scale * decay;
+      Ab[row * kPitch + (col & 3) * 16 + (col >> 2)] = a * betas[col];
+      A[row * kPitch + col] = a;
     }
   __syncthreads();
   const int col = threadIdx.x >> 2, p = threadIdx.x & 3;
   float m[16];
 #pragma unroll
-  for (int q = 0; q < 16; ++q) m[q] = 0.0f;
+  for (int r = 0; r < 16; ++r) m[r] = 0.0f;
 #pragma unroll
-  for (int q = 0; q < 16; ++q)
+  for (int r = 0; r < 16; ++r)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int row = 4 * q + e;
+      const int row = 4 * r + e;
       float sum = 0.0f;
 #pragma unroll
-      for (int k = 0; k <= q; ++k) sum = fmaf(Ab[row * kRow + 16 * p + k], m[k], sum);
+      for (int n = 0; n <= r; ++n) sum = fmaf(Ab[row * kPitch + 16 * p + n], m[n], sum);
       sum += __shfl_xor(sum, 1);
       sum += __shfl_xor(sum, 2);
-      const float v = A[row * kRow + col] - sum;
-      if (p == e) m[q] = v;
+      const float v = A[row * kPitch + col] - sum;
+      if (p == e) m[r] = v;
     }
 #pragma unroll
-  for (int q = 0; q < 16; ++q) out[(4 * q + p) * kChunk + col] = m[q];
+  for (int r = 0; r < 16; ++r) A[(4 * r + p) * kPitch + col] = m[r];   // a column's own lanes read it
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) Ab[(16 * wave + 4 * g + e) * kPitch + 16 * n + i] = qk[0][n][e];
+  put_square<NV, BACKWARD>(A, kPitch, out.m);
+  __syncthreads();
+  put_square<NV, BACKWARD>(Ab, kPitch, out.p);
 }
 
 // ---- the chain of chunks -----------------------------------------------------
 
-// One workgroup goes through a head's chunks with E columns of its state in registers, the
-// sums of the matrix unit; a copy in LDS feeds the next chunk's products.
-template <typename T, int DP, int E>
-__global__ __launch_bounds__(kDeltaBlock) void delta_chain_kernel(Delta d, const float* squares, T* o,
-                                                                float* h_out, float* states, float* xs) {
+// One workgroup goes through the chunks of a segment with E columns of a head's state in
+// registers, the sums of the matrix unit; LDS holds its parts for the next chunk's products.
+// Keys, queries, M and P go from memory to the lanes as the matrix unit takes them.
+// ENDS: no outputs but the state after the segment, from zeros, and, in columns of their
+// own, from the unit matrix without values: what the segment adds and what it makes of the
+// state before it.
+template <typename T, int DP, int E, bool ENDS>
+__global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squares<T>* squares, const T* kt,
+                                                          const float* starts, Cut cut, T* o, float* h_out,
+                                                          float* states, float* xs, float* ends, int segs) {
   typedef Shares<DP, E> Sh;
-  constexpr int kPitch = DP + 4, kRow = kChunk + 4, NT = E / 16;
-  extern __shared__ float room[];
-  __shared__ Gates gates;
-  float* K = room;
-  float* Q = K + kChunk * kPitch;
-  float* St = Q + kChunk * kPitch;   // [E][DP]
-  float* Rt = St + E * kPitch;       // [E][64]
-  float* M = Rt + E * kRow;
-  float* P = M + kChunk * kRow;
-  const int64_t heads = d.r.B * d.r.heads, bh = blockIdx.x % heads, b = bh / d.r.heads;
-  const int h = (int)(bh - b * d.r.heads), kh = h / d.group, e0 = (int)(blockIdx.x / heads) * E;
-  const int dk = (int)d.r.dk, dv = (int)d.r.dv;
+  constexpr int kPitch = DP + 8, NV = Parts<T>::kValue, NI = Parts<T>::kInput, kSteps = DP / 32;
+  constexpr int kState = E * kPitch, kSamples = E * kRow;   // planes
+  extern __shared__ __align__(16) bf16 lds[];
+  bf16* St = lds;                  // [E][DP]
+  bf16* Rt = St + NV * kState;     // beta R, [E][64]
+  bf16* Ut = Rt + NV * kSamples;
+  bf16* Ht = Ut + NV * kSamples;   // U until the chunk's end
+  const int dk = (int)d.r.dk, dv = (int)d.r.dv, blocks_v = (dv + E - 1) / E;
+  const int64_t heads = d.r.B * d.r.heads;
+  const Where at = where(heads, segs, blocks_v + (ENDS ? (dk + E - 1) / E : 0));
+  if (!at.in) return;
+  const int64_t bh = at.bh, b = bh / d.r.heads;
+  const int h = (int)(bh - b * d.r.heads), kh = h / d.group;
+  const bool unit = ENDS && at.block >= blocks_v;
+  const int e0 = (unit ? at.block - blocks_v : at.block) * E, width = unit ? dk : dv;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int64_t length = live_of(d, b);
   const T* q = static_cast<const T*>(d.r.q) + b * d.r.q_strides[0] + kh * d.r.q_strides[2];
   const T* k = static_cast<const T*>(d.r.k) + b * d.r.k_strides[0] + kh * d.r.k_strides[2];
   const T* v = static_cast<const T*>(d.r.v) + b * d.r.v_strides[0] + h * d.r.v_strides[2];
+  const int64_t ks = d.r.k_strides[1], qs = d.r.q_strides[1], vs = d.r.v_strides[1];
   const int d0 = wave % Sh::WD * Sh::MT * 16, s0 = wave / Sh::WD * Sh::NT * 16;   // this wave's part of the state
+  const int w0 = 16 * (wave & 3), c0 = wave / 4 * 32;                             // and of a chunk's samples
   f32x4 S[Sh::MT][Sh::NT];
-  const float* h0 = d.r.h0 ? d.r.h0 + bh * dk * dv : nullptr;
+  const float* start = ENDS ? nullptr : at.seg > 0 ? starts + (bh * cut.segs + at.seg) * dk * dv
+                                      : d.r.h0     ? d.r.h0 + bh * dk * dv : nullptr;
 #pragma unroll
   for (int m = 0; m < Sh::MT; ++m)
 #pragma unroll
@@ -111,9 +200,10 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_chain_kernel(Delta d, const
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int row = d0 + 16 * m + 4 * g + e, col = e0 + s0 + 16 * n + i;
-        S[m][n][e] = h0 && row < dk && col < dv ? h0[(int64_t)row * dv + col] : 0.0f;
+        S[m][n][e] = unit ? (row == col ? 1.0f : 0.0f)
+                          : start && row < dk && col < dv ? start[(int64_t)row * dv + col] : 0.0f;
       }
-  const auto put_state = [&](float* to) {   // [dk, dv]
+  const auto put_state = [&](float* to, int64_t pitch) {
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
 #pragma unroll
@@ -121,84 +211,205 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_chain_kernel(Delta d, const
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int row = d0 + 16 * m + 4 * g + e, col = e0 + s0 + 16 * n + i;
-          if (row < dk && col < dv) to[(int64_t)row * dv + col] = S[m][n][e];
+          if (row < dk && col < width) to[row * pitch + col] = S[m][n][e];
         }
   };
   const int chunks = (int)((length + kChunk - 1) / kChunk);
-  for (int c = 0; c < chunks; ++c) {
+  const int first = at.seg * cut.each, last = min(first + cut.each, chunks);
+  Frag<NI> kf[kSteps], qf[kSteps];
+  float vf[2][4];
+  const auto fetch = [&](int c) {   // what the chunk's first products take
+    const int64_t t0 = (int64_t)c * kChunk;
+    const int live = (int)min(length - t0, (int64_t)kChunk), row = w0 + i;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int col = 32 * s + 8 * g, left = row < live ? dk - col : 0;
+      kf[s] = input_frag(k + (t0 + row) * ks + col, left);
+      if (!ENDS) qf[s] = input_frag(q + (t0 + row) * qs + col, left);
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int t = w0 + 4 * g + e, col = e0 + c0 + 16 * n + i;
+        vf[n][e] = !unit && t < live && col < dv ? to_float(v[(t0 + t) * vs + col]) : 0.0f;
+      }
+  };
+  if (first < last) fetch(first);
+  for (int c = first; c < last; ++c) {
     const int64_t t0 = (int64_t)c * kChunk;
     const int live = (int)min(length - t0, (int64_t)kChunk);
-    if (states) put_state(states + (bh * d.chunks + c) * dk * dv);
-    load_gates(gates, d, b, h, t0, live);
-    load_rows<DP>(K, kPitch, k + t0 * d.r.k_strides[1], d.r.k_strides[1], live, dk);
-    load_rows<DP>(Q, kPitch, q + t0 * d.r.q_strides[1], d.r.q_strides[1], live, dk);
-    const float* sq = squares + (bh * d.chunks + c) * kSquares;
-    load_rows<kChunk>(M, kRow, sq, (int64_t)kChunk, kChunk, kChunk);
-    load_rows<kChunk>(P, kRow, sq + kSquare, (int64_t)kChunk, kChunk, kChunk);
+    const Squares<T>& sq = squares[bh * d.chunks + c];
+    const T* ktc = kt + ((b * d.r.key_heads + kh) * d.chunks + c) * DP * kChunk;
+    Frag<NV> mf[2], pf[2];
+    Frag<NI> ktf[Sh::MT][2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      mf[s] = plane_frag<NV>(&sq.m[0][w0 + i][32 * s + 8 * g], kSquare);
+      if (!ENDS) pf[s] = plane_frag<NV>(&sq.p[0][w0 + i][32 * s + 8 * g], kSquare);
+#pragma unroll
+      for (int m = 0; m < Sh::MT; ++m)
+        ktf[m][s] = input_frag(ktc + (d0 + 16 * m + i) * kChunk + 32 * s + 8 * g, 8);
+    }
+    const f32x4 since = *reinterpret_cast<const f32x4*>(sq.gates.since + w0 + 4 * g);
+    const f32x4 until = *reinterpret_cast<const f32x4*>(sq.gates.until + w0 + 4 * g);
+    const f32x4 beta = *reinterpret_cast<const f32x4*>(sq.gates.beta + w0 + 4 * g);
+    const float total = sq.gates.since[kChunk - 1];
+    if (!ENDS && states) put_state(states + (bh * d.chunks + c) * dk * dv, dv);
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
 #pragma unroll
       for (int n = 0; n < Sh::NT; ++n)
-        *reinterpret_cast<f32x4*>(St + (s0 + 16 * n + i) * kPitch + d0 + 16 * m + 4 * g) = S[m][n];
+        put4<NV>(St + (s0 + 16 * n + i) * kPitch + d0 + 16 * m + 4 * g, kState, S[m][n]);
     __syncthreads();
-    // this wave's 16 samples from here on
-    const int w0 = 16 * wave + 4 * g;
-    f32x4 R[1][NT], O[1][NT], X[1][NT];
+    f32x4 R[1][2], O[1][2], X[1][2];
     clear(R);
     clear(O);
-    multiply<false, false>(R, K + 16 * wave * kPitch, kPitch, St, kPitch, DP);
-    multiply<false, false>(O, Q + 16 * wave * kPitch, kPitch, St, kPitch, DP);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      f32x4 br;
+    for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int t = w0 + e, col = e0 + 16 * n + i;
-        const float val = t < live && col < dv ? to_float(v[(t0 + t) * d.r.v_strides[1] + col]) : 0.0f;
-        R[0][n][e] = fmaf(-gates.since[t], R[0][n][e], val);
-        O[0][n][e] *= d.r.scale * gates.since[t];
-        br[e] = gates.beta[t] * R[0][n][e];
+      for (int n = 0; n < 2; ++n) {
+        const Frag<NV> st = plane_frag<NV>(St + (c0 + 16 * n + i) * kPitch + 32 * s + 8 * g, kState);
+        mma(R[0][n], kf[s], st);
+        if (!ENDS) mma(O[0][n], qf[s], st);
       }
-      *reinterpret_cast<f32x4*>(Rt + (16 * n + i) * kRow + w0) = br;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) R[0][n][e] = fmaf(-since[e], R[0][n][e], vf[n][e]);
+      O[0][n] *= d.r.scale * since;
+      put4<NV>(Rt + (c0 + 16 * n + i) * kRow + w0 + 4 * g, kSamples, beta * R[0][n]);
     }
+    if (c + 1 < last) fetch(c + 1);
     __syncthreads();
     clear(X);
-    multiply<false, false>(X, M + 16 * wave * kRow, kRow, Rt, kRow, kChunk);
-    __syncthreads();
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      f32x4 u;
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int t = w0 + e, col = e0 + 16 * n + i;
-        const float x = R[0][n][e] - X[0][n][e];
-        u[e] = gates.beta[t] * x;
-        if (xs && t < live && col < dv) xs[((b * d.r.T + t0 + t) * d.r.heads + h) * dv + col] = x;
-      }
-      *reinterpret_cast<f32x4*>(Rt + (16 * n + i) * kRow + w0) = u;
+      for (int n = 0; n < 2; ++n)
+        mma(X[0][n], mf[s], plane_frag<NV>(Rt + (c0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples));
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const f32x4 x = R[0][n] - X[0][n], u = beta * x;
+      const int to = (c0 + 16 * n + i) * kRow + w0 + 4 * g;
+      if (!ENDS) put4<NV>(Ut + to, kSamples, u);
+      put4<NV>(Ht + to, kSamples, until * u);
+      if (!ENDS && xs)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int t = w0 + 4 * g + e, col = e0 + c0 + 16 * n + i;
+          if (t < live && col < dv) xs[((b * d.r.T + t0 + t) * d.r.heads + h) * dv + col] = x[e];
+        }
     }
     __syncthreads();
-    multiply<false, false>(O, P + 16 * wave * kRow, kRow, Rt, kRow, kChunk);
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int t = w0 + e, col = e0 + 16 * n + i;
-        if (t < live && col < dv) o[((b * d.r.T + t0 + t) * d.r.heads + h) * dv + col] = from_float<T>(O[0][n][e]);
-      }
-    const float total = gates.since[kChunk - 1];
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
 #pragma unroll
       for (int n = 0; n < Sh::NT; ++n) S[m][n] *= total;
-    multiply<true, false>(S, K + d0, kPitch, Rt + s0 * kRow, kRow, kChunk, gates.until);
-    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int n = 0; n < Sh::NT; ++n) {
+        const Frag<NV> u = plane_frag<NV>(Ht + (s0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples);
+#pragma unroll
+        for (int m = 0; m < Sh::MT; ++m) mma(S[m][n], ktf[m][s], u);
+      }
+    if (ENDS) continue;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+        mma(O[0][n], pf[s], plane_frag<NV>(Ut + (c0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples));
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int t = w0 + 4 * g + e, col = e0 + c0 + 16 * n + i;
+        if (t < live && col < dv) o[((b * d.r.T + t0 + t) * d.r.heads + h) * dv + col] = from_float<T>(O[0][n][e]);
+      }
   }
-  put_state(h_out + bh * dk * dv);
-  for (int64_t at = length * E + threadIdx.x; at < d.r.T * E; at += kDeltaBlock) {
-    const int64_t t = at / E;
-    const int col = e0 + (int)(at % E);
+  if (ENDS) {
+    put_state(ends + (bh * cut.segs + at.seg) * dk * (dv + dk) + (unit ? dv : 0), dv + dk);
+    return;
+  }
+  if (at.seg == (chunks > 0 ? (chunks - 1) / cut.each : 0)) put_state(h_out + bh * dk * dv, dv);
+  const int64_t rest = max(length, (int64_t)first * kChunk), stop = min((int64_t)(first + cut.each) * kChunk, d.r.T);
+  for (int64_t n = rest * E + threadIdx.x; n < stop * E; n += 8 * E) {
+    const int64_t t = n / E;
+    const int col = e0 + (int)(n % E);
     if (col < dv) o[((b * d.r.T + t) * d.r.heads + h) * dv + col] = from_float<T>(0.0f);
+  }
+}
+
+// The states that the segments begin with, one after another: 16 columns to a workgroup.
+// FORWARD: starts[s + 1] = what segment s makes of starts[s] and what it adds.  Else the
+// gradients that they end with: from[s - 1] = the transposed of from[s] and what s adds.
+template <int DP, bool FORWARD>
+__global__ __launch_bounds__(kDeltaBlock) void delta_join_kernel(Delta d, Cut cut, const float* ends,
+                                                               const float* adds, const float* given, float* to) {
+  constexpr int kPitch = DP + 8, kPlane = 16 * kPitch, kSteps = DP / 32, kTiles = (DP / 16 + 3) / 4;
+  __shared__ __align__(16) bf16 St[3 * kPlane];
+  const int dk = (int)d.r.dk, dv = (int)d.r.dv, wide = dv + dk;
+  const int64_t heads = d.r.B * d.r.heads, bh = blockIdx.x % heads, b = bh / d.r.heads;
+  const int col = (int)(blockIdx.x / heads) * 16 + (threadIdx.x & 15);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int chunks = (int)((live_of(d, b) + kChunk - 1) / kChunk);
+  const int live = min((chunks + cut.each - 1) / cut.each, cut.segs);   // segments with samples
+  f32x4 S[kTiles];
+#pragma unroll
+  for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int row = 16 * (wave + 4 * m) + 4 * g + e;
+      S[m][e] = given && row < dk && col < dv ? given[(bh * dk + row) * dv + col] : 0.0f;
+    }
+  for (int n = 0; n + 1 < live; ++n) {
+    const int s = FORWARD ? n : live - 1 - n;
+    const float* end = ends + (bh * cut.segs + s) * dk * wide;
+    const float* add = FORWARD ? end : adds + (bh * cut.segs + s) * dk * dv;
+    const int64_t pitch = FORWARD ? wide : dv;
+    Frag<3> a[kTiles][kSteps];
+    f32x4 acc[kTiles];
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) {
+      const int tile = 16 * (wave + 4 * m);
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int row = FORWARD ? tile + i : 32 * k + 8 * g + e, c = FORWARD ? 32 * k + 8 * g + e : tile + i;
+          v[e] = row < dk && c < dk ? end[row * (int64_t)wide + dv + c] : 0.0f;
+        }
+        a[m][k] = frag_of<3>(v);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = tile + 4 * g + e;
+        acc[m][e] = row < dk && col < dv ? add[row * pitch + col] : 0.0f;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m)
+      if (16 * (wave + 4 * m) < DP) put4<3>(St + i * kPitch + 16 * (wave + 4 * m) + 4 * g, kPlane, S[m]);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      const Frag<3> st = plane_frag<3>(St + i * kPitch + 32 * k + 8 * g, kPlane);
+#pragma unroll
+      for (int m = 0; m < kTiles; ++m) mma(acc[m], a[m][k], st);
+    }
+    float* out = to + (bh * cut.segs + (FORWARD ? s + 1 : s - 1)) * dk * dv;
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) {
+      S[m] = acc[m];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = 16 * (wave + 4 * m) + 4 * g + e;
+        if (row < dk && col < dv) out[(int64_t)row * dv + col] = acc[m][e];
+      }
+    }
   }
 }
 
@@ -326,32 +537,80 @@ bool steps(const cpab_delta_rule& r, bool keep) { return r.T <= (keep ? 0 : 16);
 
 }  // namespace
 
-hipError_t launch_delta_squares(const Delta& d, float* squares, hipStream_t st) {
-  hipError_t e = hipSuccess;
+hipError_t launch_delta_squares(const Delta& d, void* squares, void* kt, void* qt, hipStream_t st) {
   with_key(d, [&](auto t, auto dp) {
     typedef decltype(t) T;
     constexpr int DP = decltype(dp)::value;
-    constexpr int kRoom = 4 * 2 * std::max(kChunk * (DP + 4), kChunk * (kChunk + 4));
-    static LdsAllowed allowed;
-    e = allow_lds(reinterpret_cast<const void*>(delta_squares_kernel<T, DP>), kRoom, allowed);
-    if (e != hipSuccess) return;
-    delta_squares_kernel<T, DP><<<(unsigned)(d.r.B * d.r.heads * d.chunks), kDeltaBlock, kRoom, st>>>(d, squares);
-    e = hipGetLastError();
+    constexpr int kRoom = std::max<int>(4 * 2 * kChunk * (kChunk + 4), DP * kRow * (int)sizeof(T));
+    const unsigned blocks = (unsigned)(d.r.B * d.r.heads * d.chunks);
+    if (qt)
+      delta_squares_kernel<T, DP, true><<<blocks, kDeltaBlock, kRoom, st>>>(d, (Squares<T>*)squares, (T*)kt, (T*)qt);
+    else
+      delta_squares_kernel<T, DP, false><<<blocks, kDeltaBlock, kRoom, st>>>(d, (Squares<T>*)squares, (T*)kt, nullptr);
   });
-  return e;
+  return hipGetLastError();
 }
 
+hipError_t launch_delta_join(const Delta& d, const Cut& cut, bool forward, const float* ends, const float* adds,
+                             const float* given, float* to, hipStream_t st) {
+  with_key(d, [&](auto, auto dp) {
+    constexpr int DP = decltype(dp)::value;
+    const unsigned blocks = (unsigned)(d.r.B * d.r.heads * ((d.r.dv + 15) / 16));
+    if (forward)
+      delta_join_kernel<DP, true><<<blocks, kDeltaBlock, 0, st>>>(d, cut, ends, adds, given, to);
+    else
+      delta_join_kernel<DP, false><<<blocks, kDeltaBlock, 0, st>>>(d, cut, ends, adds, given, to);
+  });
+  return hipGetLastError();
+}
+
+Cut cut_of(const Delta& d) {
+  const int64_t columns = d.r.B * d.r.heads * ((d.r.dv + 31) / 32);
+  const int64_t want = columns > 0 ? 2 * compute_units() / columns : 1;
+  const int segs = (int)std::min<int64_t>(want, d.chunks / 4);
+  if (segs < 4) return Cut{1, std::max(d.chunks, 1)};
+  const int each = (d.chunks + segs - 1) / segs;
+  return Cut{(d.chunks + each - 1) / each, each};
+}
+
+Kept kept_of(const Delta& d, const Cut& cut) {
+  const int64_t heads = d.r.B * d.r.heads;
+  Kept k;
+  k.states = 0;
+  k.xs = heads * d.chunks * d.r.dk * d.r.dv;
+  k.ends = k.xs + heads * d.r.T * d.r.dv;
+  k.all = k.ends + (cut.segs > 1 ? heads * cut.segs * d.r.dk * (d.r.dv + d.r.dk) : 0);
+  return k;
+}
 int64_t delta_rule_kept(const cpab_delta_rule& r) {
   const Delta d = delta_of(r);
-  return r.B * r.heads * (d.chunks * r.dk + r.T) * r.dv;
+  return kept_of(d, cut_of(d)).all;
 }
+
+namespace {
+
+// The forward's workspace (bytes).
+struct Room {
+  int64_t squares, kt, starts, ends, all;
+};
+Room room_of(const Delta& d, const Cut& cut, bool keep) {
+  const int64_t heads = d.r.B * d.r.heads;
+  const auto next = [](int64_t n) { return (n + 255) / 256 * 256; };
+  Room w;
+  w.squares = 0;
+  w.kt = next(heads * d.chunks * squares_bytes(d.r.dtype));
+  w.starts = w.kt + next(d.r.B * d.r.key_heads * d.chunks * turned_bytes(d.r));
+  w.ends = w.starts + (cut.segs > 1 ? next(heads * cut.segs * d.r.dk * d.r.dv * 4) : 0);
+  w.all = w.ends + (cut.segs > 1 && !keep ? next(heads * cut.segs * d.r.dk * (d.r.dv + d.r.dk) * 4) : 0);
+  return w;
+}
+
+}  // namespace
 
 int64_t delta_rule_workspace(const cpab_delta_rule& r, bool keep, bool backward) {
   const Delta d = delta_of(r);
-  if (!backward && steps(r, keep)) return 0;
-  int64_t n = r.B * r.heads * d.chunks * kSquares;
-  if (backward) n += r.B * r.heads * (d.chunks * r.dk + r.T) * r.dv;
-  return 4 * n;
+  if (backward) return delta_backward_workspace(d);
+  return steps(r, keep) ? 0 : room_of(d, cut_of(d), keep).all;
 }
 
 hipError_t launch_delta_rule_forward(const cpab_delta_rule& r, void* o, float* h, float* kept,
@@ -366,24 +625,45 @@ hipError_t launch_delta_rule_forward(const cpab_delta_rule& r, void* o, float* h
       delta_steps_kernel<bf16><<<blocks, kDeltaBlock, 0, st>>>(d, (bf16*)o, h);
     return hipGetLastError();
   }
-  float* squares = static_cast<float*>(workspace);
-  hipError_t e = launch_delta_squares(d, squares, st);
+  const Cut cut = cut_of(d);
+  const Room w = room_of(d, cut, kept != nullptr);
+  const Kept k = kept_of(d, cut);
+  char* room = static_cast<char*>(workspace);
+  float* starts = reinterpret_cast<float*>(room + w.starts);
+  float* ends = kept ? kept + k.ends : reinterpret_cast<float*>(room + w.ends);
+  hipError_t e = launch_delta_squares(d, room + w.squares, room + w.kt, nullptr, st);
   if (e != hipSuccess) return e;
-  float* xs = kept ? kept + heads * d.chunks * r.dk * r.dv : nullptr;
   with_key(d, [&](auto t, auto dp) {
     typedef decltype(t) T;
-    constexpr int DP = decltype(dp)::value;
-    const auto run = [&](auto width) {
+    constexpr int DP = decltype(dp)::value, NV = Parts<T>::kValue;
+    const Squares<T>* squares = reinterpret_cast<const Squares<T>*>(room + w.squares);
+    const T* kt = reinterpret_cast<const T*>(room + w.kt);
+    const auto run = [&](auto width, auto only_ends, int segs) {
       constexpr int E = decltype(width)::value;
-      constexpr int kRoom = 4 * ((2 * kChunk + E) * (DP + 4) + (E + 2 * kChunk) * (kChunk + 4));
+      constexpr bool ENDS = decltype(only_ends)::value;
+      constexpr int kRoom = 2 * NV * E * (DP + 8 + 3 * kRow);
       static LdsAllowed allowed;
-      e = allow_lds(reinterpret_cast<const void*>(delta_chain_kernel<T, DP, E>), kRoom, allowed);
+      e = allow_lds(reinterpret_cast<const void*>(delta_chain_kernel<T, DP, E, ENDS>), kRoom, allowed);
       if (e != hipSuccess) return;
-      delta_chain_kernel<T, DP, E><<<(unsigned)(heads * ((r.dv + E - 1) / E)), kDeltaBlock, kRoom, st>>>(
-          d, squares, (T*)o, h, kept, xs);
+      const int64_t blocks = (r.dv + E - 1) / E + (ENDS ? (r.dk + E - 1) / E : 0);
+      delta_chain_kernel<T, DP, E, ENDS><<<(unsigned)((heads * segs + 7) / 8 * 8 * blocks), 8 * E, kRoom, st>>>(
+          d, squares, kt, starts, cut, (T*)o, h, kept, kept ? kept + k.xs : nullptr, ends, segs);
       e = hipGetLastError();
     };
-    r.dv <= 32 ? run(std::integral_constant<int, 32>()) : run(std::integral_constant<int, 64>());
+    typedef std::integral_constant<int, 32> Narrow;
+    typedef std::integral_constant<int, 64> Wide;
+    const auto both = [&](auto only_ends, int segs) {
+      if constexpr (sizeof(T) == 2)
+        if (r.dv > 32) return run(Wide(), only_ends, segs);
+      run(Narrow(), only_ends, segs);
+    };
+    if (cut.segs > 1) {
+      // the backward takes what the last segment makes of the state too
+      both(std::true_type(), kept ? cut.segs : cut.segs - 1);
+      if (e == hipSuccess) e = launch_delta_join(d, cut, true, ends, nullptr, r.h0, starts, st);
+      if (e != hipSuccess) return;
+    }
+    both(std::false_type(), cut.segs);
   });
   return e;
 }

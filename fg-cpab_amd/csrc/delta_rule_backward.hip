@@ -9,35 +9,44 @@
 namespace cpab {
 namespace {
 
-constexpr int kRow = kChunk + 4;
-constexpr int kWide = 32, kWidePitch = kWide + 4;   // columns of values at once
+// ---- the chain of chunks, backwards --------------------------------------------
 
-// One workgroup goes back through a head's chunks with 32 columns of the state's gradient
-// in registers.  Keeps the gradient after each chunk and E, and writes grad_v and grad_h0.
-template <typename T, int DP>
-__global__ __launch_bounds__(kDeltaBlock) void delta_back_chain_kernel(
-    Delta d, const float* squares, const T* grad_o, const float* grad_h, T* grad_v, float* grad_h0,
-    float* dstates, float* es) {
-  typedef Shares<DP, kWide> Sh;
-  constexpr int kPitch = DP + 4, NT = kWide / 16;
-  extern __shared__ float room[];
-  __shared__ Gates gates;
-  __shared__ float scaled[kChunk];   // scale exp(G_i)
-  float* K = room;
-  float* Q = K + kChunk * kPitch;
-  float* St = Q + kChunk * kPitch;   // the gradient [32][DP]
-  float* Ot = St + kWide * kPitch;   // dO [32][64]
-  float* Zt = Ot + kWide * kRow;
-  float* M = Zt + kWide * kRow;
-  float* P = M + kChunk * kRow;
-  const int64_t heads = d.r.B * d.r.heads, bh = blockIdx.x % heads, b = bh / d.r.heads;
-  const int h = (int)(bh - b * d.r.heads), kh = h / d.group, e0 = (int)(blockIdx.x / heads) * kWide;
+// As the forward's chain: E columns of the state's gradient in registers, back through a
+// segment's chunks.  Keeps the gradient after each chunk and E, and writes grad_v and
+// grad_h0.  M and P lie transposed.  ENDS: only what the segment adds to the gradient before
+// it.
+template <typename T, int DP, int E, bool ENDS>
+__global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
+    Delta d, const Squares<T>* squares, const T* kt, const T* qt, Cut cut, const T* grad_o,
+    const float* grad_h, const float* starts, T* grad_v, float* grad_h0, float* dstates, float* es,
+    float* adds) {
+  typedef Shares<DP, E> Sh;
+  constexpr int kPitch = DP + 8, NV = Parts<T>::kValue, NI = Parts<T>::kInput, kSteps = DP / 32;
+  constexpr int kState = E * kPitch, kSamples = E * kRow;   // planes
+  extern __shared__ __align__(16) bf16 lds[];
+  bf16* St = lds;                       // the gradient, [E][DP]
+  bf16* Bt = St + NV * kState;          // beta dU, [E][64]
+  bf16* Zt = Bt + NV * kSamples;        // - exp(G) Z
+  bf16* Ot = Zt + NV * kSamples;        // dO, as the input that it is
+  bf16* Gt = Ot + NI * kSamples;        // scale exp(G) dO, of this chunk and the next in turn
   const int dk = (int)d.r.dk, dv = (int)d.r.dv;
+  const int64_t heads = d.r.B * d.r.heads;
+  const Where at = where(heads, cut.segs, (dv + E - 1) / E);
+  if (!at.in) return;
+  const int64_t bh = at.bh, b = bh / d.r.heads;
+  const int h = (int)(bh - b * d.r.heads), kh = h / d.group, e0 = at.block * E;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int64_t length = live_of(d, b);
-  const T* q = static_cast<const T*>(d.r.q) + b * d.r.q_strides[0] + kh * d.r.q_strides[2];
   const T* k = static_cast<const T*>(d.r.k) + b * d.r.k_strides[0] + kh * d.r.k_strides[2];
+  const int64_t ks = d.r.k_strides[1];
   const int d0 = wave % Sh::WD * Sh::MT * 16, s0 = wave / Sh::WD * Sh::NT * 16;
+  const int w0 = 16 * (wave & 3), c0 = wave / 4 * 32;
+  const int chunks = (int)((length + kChunk - 1) / kChunk);
+  const int first = at.seg * cut.each, last = min(first + cut.each, chunks);
+  // what comes from behind: the state's own gradient, or that of the segment behind
+  const bool end = last == chunks;
+  const float* start = ENDS ? nullptr : end ? (grad_h ? grad_h + bh * dk * dv : nullptr)
+                                            : starts + (bh * cut.segs + at.seg) * dk * dv;
   f32x4 S[Sh::MT][Sh::NT];
 #pragma unroll
   for (int m = 0; m < Sh::MT; ++m)
@@ -46,7 +55,7 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_back_chain_kernel(
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int row = d0 + 16 * m + 4 * g + e, col = e0 + s0 + 16 * n + i;
-        S[m][n][e] = grad_h && row < dk && col < dv ? grad_h[(bh * dk + row) * dv + col] : 0.0f;
+        S[m][n][e] = start && row < dk && col < dv ? start[(int64_t)row * dv + col] : 0.0f;
       }
   const auto put_state = [&](float* to) {
 #pragma unroll
@@ -59,83 +68,136 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_back_chain_kernel(
           if (row < dk && col < dv) to[(int64_t)row * dv + col] = S[m][n][e];
         }
   };
-  const int chunks = (int)((length + kChunk - 1) / kChunk);
-  for (int c = chunks - 1; c >= 0; --c) {
+  Frag<NI> kf[kSteps];
+  f32x4 of[2];
+  const auto fetch = [&](int c) {
+    const int64_t t0 = (int64_t)c * kChunk;
+    const int live = (int)min(length - t0, (int64_t)kChunk), row = w0 + i;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int col = 32 * s + 8 * g;
+      kf[s] = input_frag(k + (t0 + row) * ks + col, row < live ? dk - col : 0);
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int t = w0 + 4 * g + e, col = e0 + c0 + 16 * n + i;
+        of[n][e] = grad_o && t < live && col < dv
+                       ? to_float(grad_o[((b * d.r.T + t0 + t) * d.r.heads + h) * dv + col]) : 0.0f;
+      }
+  };
+  if (first < last) fetch(last - 1);
+  for (int c = last - 1; c >= first; --c) {
     const int64_t t0 = (int64_t)c * kChunk;
     const int live = (int)min(length - t0, (int64_t)kChunk);
-    put_state(dstates + (bh * d.chunks + c) * dk * dv);
-    load_gates(gates, d, b, h, t0, live);
-    load_rows<DP>(K, kPitch, k + t0 * d.r.k_strides[1], d.r.k_strides[1], live, dk);
-    load_rows<DP>(Q, kPitch, q + t0 * d.r.q_strides[1], d.r.q_strides[1], live, dk);
-    const float* sq = squares + (bh * d.chunks + c) * kSquares;
-    load_rows<kChunk>(M, kRow, sq, (int64_t)kChunk, kChunk, kChunk);
-    load_rows<kChunk>(P, kRow, sq + kSquare, (int64_t)kChunk, kChunk, kChunk);
-    for (int at = threadIdx.x; at < kChunk * kWide; at += kDeltaBlock) {
-      const int t = at / kWide, col = at % kWide;
-      Ot[col * kRow + t] = grad_o && t < live && e0 + col < dv
-                               ? to_float(grad_o[((b * d.r.T + t0 + t) * d.r.heads + h) * dv + e0 + col]) : 0.0f;
+    const Squares<T>& sq = squares[bh * d.chunks + c];
+    const int64_t turned = ((b * d.r.key_heads + kh) * d.chunks + c) * DP * kChunk;
+    Frag<NV> mf[2], pf[2];
+    Frag<NI> ktf[Sh::MT][2], qtf[Sh::MT][2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      mf[s] = plane_frag<NV>(&sq.m[0][w0 + i][32 * s + 8 * g], kSquare);
+      pf[s] = plane_frag<NV>(&sq.p[0][w0 + i][32 * s + 8 * g], kSquare);
+#pragma unroll
+      for (int m = 0; m < Sh::MT; ++m) {
+        const int from = (d0 + 16 * m + i) * kChunk + 32 * s + 8 * g;
+        ktf[m][s] = input_frag(kt + turned + from, 8);
+        qtf[m][s] = input_frag(qt + turned + from, 8);
+      }
     }
+    const f32x4 since = *reinterpret_cast<const f32x4*>(sq.gates.since + w0 + 4 * g);
+    const f32x4 until = *reinterpret_cast<const f32x4*>(sq.gates.until + w0 + 4 * g);
+    const f32x4 beta = *reinterpret_cast<const f32x4*>(sq.gates.beta + w0 + 4 * g);
+    const float total = sq.gates.since[kChunk - 1];
+    bf16* gt = Gt + (c & 1) * NV * kSamples;
+    if (!ENDS) put_state(dstates + (bh * d.chunks + c) * dk * dv);
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
 #pragma unroll
       for (int n = 0; n < Sh::NT; ++n)
-        *reinterpret_cast<f32x4*>(St + (s0 + 16 * n + i) * kPitch + d0 + 16 * m + 4 * g) = S[m][n];
+        put4<NV>(St + (s0 + 16 * n + i) * kPitch + d0 + 16 * m + 4 * g, kState, S[m][n]);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int to = (c0 + 16 * n + i) * kRow + w0 + 4 * g;
+      put4<NI>(Ot + to, kSamples, of[n]);
+      put4<NV>(gt + to, kSamples, d.r.scale * since * of[n]);
+    }
     __syncthreads();
-    if (threadIdx.x < kChunk) scaled[threadIdx.x] = d.r.scale * gates.since[threadIdx.x];
-    const int w0 = 16 * wave + 4 * g;
-    f32x4 U[1][NT], V[1][NT];
+    f32x4 U[1][2], V[1][2];
     clear(U);
     clear(V);
-    multiply<false, false>(U, K + 16 * wave * kPitch, kPitch, St, kPitch, DP);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) U[0][n][e] *= gates.until[w0 + e];
-    multiply<true, false>(U, P + 16 * wave, kRow, Ot, kRow, kChunk);
+      for (int n = 0; n < 2; ++n)
+        mma(U[0][n], kf[s], plane_frag<NV>(St + (c0 + 16 * n + i) * kPitch + 32 * s + 8 * g, kState));
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      f32x4 bu;
+    for (int n = 0; n < 2; ++n) U[0][n] *= until;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) bu[e] = gates.beta[w0 + e] * U[0][n][e];
-      *reinterpret_cast<f32x4*>(Zt + (16 * n + i) * kRow + w0) = bu;
-    }
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+        mma(U[0][n], pf[s], plane_frag<NI>(Ot + (c0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples));
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+      put4<NV>(Bt + (c0 + 16 * n + i) * kRow + w0 + 4 * g, kSamples, beta * U[0][n]);
+    if (c > first) fetch(c - 1);
     __syncthreads();
-    multiply<true, false>(V, M + 16 * wave, kRow, Zt, kRow, kChunk);
-    __syncthreads();
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      f32x4 gz;
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+        mma(V[0][n], mf[s], plane_frag<NV>(Bt + (c0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples));
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const f32x4 ev = U[0][n] - V[0][n], z = beta * ev;
+      put4<NV>(Zt + (c0 + 16 * n + i) * kRow + w0 + 4 * g, kSamples, -since * z);
+      if (ENDS) continue;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int t = w0 + e, col = e0 + 16 * n + i;
-        const float ev = U[0][n][e] - V[0][n][e], z = gates.beta[t] * ev;
-        gz[e] = -gates.since[t] * z;
+        const int t = w0 + 4 * g + e, col = e0 + c0 + 16 * n + i;
         if (t < live && col < dv) {
-          const int64_t at = ((b * d.r.T + t0 + t) * d.r.heads + h) * dv + col;
-          es[at] = ev;
-          if (grad_v) grad_v[at] = from_float<T>(z);
+          const int64_t to = ((b * d.r.T + t0 + t) * d.r.heads + h) * dv + col;
+          es[to] = ev[e];
+          if (grad_v) grad_v[to] = from_float<T>(z[e]);
         }
       }
-      *reinterpret_cast<f32x4*>(Zt + (16 * n + i) * kRow + w0) = gz;
     }
     __syncthreads();
-    const float total = gates.since[kChunk - 1];
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
 #pragma unroll
       for (int n = 0; n < Sh::NT; ++n) S[m][n] *= total;
-    multiply<true, false>(S, Q + d0, kPitch, Ot + s0 * kRow, kRow, kChunk, scaled);
-    multiply<true, false>(S, K + d0, kPitch, Zt + s0 * kRow, kRow, kChunk);
-    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int n = 0; n < Sh::NT; ++n) {
+        const int from = (s0 + 16 * n + i) * kRow + 32 * s + 8 * g;
+        const Frag<NV> go = plane_frag<NV>(gt + from, kSamples), z = plane_frag<NV>(Zt + from, kSamples);
+#pragma unroll
+        for (int m = 0; m < Sh::MT; ++m) {
+          mma(S[m][n], qtf[m][s], go);
+          mma(S[m][n], ktf[m][s], z);
+        }
+      }
   }
-  if (grad_h0) put_state(grad_h0 + bh * dk * dv);
-  if (grad_v)
-    for (int64_t at = length * kWide + threadIdx.x; at < d.r.T * kWide; at += kDeltaBlock) {
-      const int64_t t = at / kWide;
-      const int col = e0 + (int)(at % kWide);
+  if (ENDS) {
+    put_state(adds + (bh * cut.segs + at.seg) * dk * dv);
+    return;
+  }
+  if (grad_h0 && at.seg == 0) put_state(grad_h0 + bh * dk * dv);
+  if (grad_v) {
+    const int64_t rest = max(length, (int64_t)first * kChunk), stop = min((int64_t)(first + cut.each) * kChunk, d.r.T);
+    for (int64_t n = rest * E + threadIdx.x; n < stop * E; n += 8 * E) {
+      const int64_t t = n / E;
+      const int col = e0 + (int)(n % E);
       if (col < dv) grad_v[((b * d.r.T + t) * d.r.heads + h) * dv + col] = from_float<T>(0.0f);
     }
+  }
 }
+
+// ---- everything else, by chunks ------------------------------------------------
 
 __device__ __forceinline__ void put_gate(const Delta& d, void* p, int64_t at, float v) {
   if (d.r.gate_dtype == CPAB_F32)
@@ -144,55 +206,68 @@ __device__ __forceinline__ void put_gate(const Delta& d, void* p, int64_t at, fl
     static_cast<bf16*>(p)[at] = from_float<bf16>(v);
 }
 
-// [rows, 32] columns of a 32-bit array in LDS, zeros beyond `live` rows and `cols` columns.
-__device__ __forceinline__ f32x4 quad(const float* row, bool in, int left) {
+// Four neighbours of a row, zeros beyond `left`.
+template <typename T>
+__device__ __forceinline__ f32x4 quad(const T* p, int left) {
   f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (!in) return v;
   if (left >= 4) {
     float w[4];
-    load<4>(row, w);
+    load<4>(p, w);
     return f32x4{w[0], w[1], w[2], w[3]};
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (e < left) v[e] = row[e];
+    if (e < left) v[e] = to_float(p[e]);
   return v;
 }
 
-// A chunk of a key's head: the gradients of its queries and keys, added up over the heads
-// that share them, and of those heads' gates.
+constexpr int kPartsBlock = 512;
+constexpr int kWide = 32, kWidePitch = kWide + 8;   // columns of values at once
+
 template <typename T, int DP>
-__global__ __launch_bounds__(kDeltaBlock) void delta_parts_kernel(
-    Delta d, const float* squares, const float* states, const float* xs, const float* dstates,
-    const float* es, const T* grad_o, T* grad_q, T* grad_k, void* grad_decay, void* grad_beta) {
-  constexpr int kPitch = DP + 4, NT = DP / 16;
-  extern __shared__ float room[];
-  __shared__ Gates gates;
-  __shared__ float dbeta[kChunk], before[kChunk], after[kChunk], whole[4];
-  float* K = room;
-  float* Q = K + kChunk * kPitch;
-  float* S = Q + kChunk * kPitch;      // [DP][32]
-  float* L = S + DP * kWidePitch;      // the gradient's, [DP][32]
-  float* O = L + DP * kWidePitch;      // dO [64][32]
-  float* U = O + kChunk * kWidePitch;
-  float* Z = U + kChunk * kWidePitch;
-  float* W1 = S;                       // the chunk's squares, in the same place afterwards
-  float* W2 = W1 + kChunk * kRow;
-  float* H = W2 + kChunk * kRow;       // [64][65]
+struct PartsRoom {
+  static constexpr int NV = Parts<T>::kValue;
+  static constexpr int kState = DP * kWidePitch, kSamples = kChunk * kWidePitch, kFlat = kChunk * kRow;
+  // S, its gradient and U, then in their place W, its transpose and the other square
+  static constexpr int kLoop = NV * (2 * kState + kSamples), kAfter = 3 * NV * kFlat;
+  static constexpr int kParts = kLoop > kAfter ? kLoop : kAfter;   // 16-bit values
+  static constexpr int kBytes = 2 * kParts + 4 * kChunk * (kChunk + 1);
+};
+
+// A chunk of a key's head: the gradients of its queries and keys, added up over the heads
+// that share them, and of those heads' gates.  Of the eight waves four share the samples and
+// two the columns.
+template <typename T, int DP>
+__global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
+    Delta d, const Squares<T>* squares, const T* kt, const T* qt, const float* states, const float* xs,
+    const float* dstates, const float* es, const T* grad_o, T* grad_q, T* grad_k, void* grad_decay,
+    void* grad_beta) {
+  typedef PartsRoom<T, DP> Room;
+  constexpr int NV = Parts<T>::kValue, NI = Parts<T>::kInput, kSteps = DP / 32, NT = DP / 32;
+  extern __shared__ __align__(16) bf16 lds[];
+  __shared__ double G[kChunk];
+  __shared__ float betas[kChunk], dbeta[kChunk], before[2][kChunk], after[2][kChunk], whole[8], sums[8][kChunk];
+  bf16* S = lds;                              // [DP][32]
+  bf16* L = S + NV * Room::kState;            // the gradient, [DP][32]
+  bf16* U = L + NV * Room::kState;            // [64][32]
+  bf16* W = lds;                              // scale D dP, [64][64]
+  bf16* Wt = W + NV * Room::kFlat;
+  bf16* Y = Wt + NV * Room::kFlat;            // D dA + (D dA)^T
+  float* H = reinterpret_cast<float*>(lds + Room::kParts);   // dP P + dA A, [64][65]
   const int c = blockIdx.x % d.chunks;
   const int64_t rest = blockIdx.x / d.chunks, b = rest / d.r.key_heads;
   const int kh = (int)(rest - b * d.r.key_heads);
   const int dk = (int)d.r.dk, dv = (int)d.r.dv;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int w0 = 16 * (wave & 3), half = wave >> 2;   // samples; columns of DP and of 64
+  const int d0 = half * (DP / 2), j0 = half * 32;
   const int64_t t0 = (int64_t)c * kChunk;
   const int live = (int)min(max(live_of(d, b) - t0, (int64_t)0), (int64_t)kChunk);
   const int rows = (int)min(d.r.T - t0, (int64_t)kChunk);   // that there are
-  if (live > 0) {
-    load_rows<DP>(K, kPitch, static_cast<const T*>(d.r.k) + b * d.r.k_strides[0] + t0 * d.r.k_strides[1] + kh * d.r.k_strides[2],
-                  d.r.k_strides[1], live, dk);
-    load_rows<DP>(Q, kPitch, static_cast<const T*>(d.r.q) + b * d.r.q_strides[0] + t0 * d.r.q_strides[1] + kh * d.r.q_strides[2],
-                  d.r.q_strides[1], live, dk);
-  }
+  const T* k = static_cast<const T*>(d.r.k) + b * d.r.k_strides[0] + t0 * d.r.k_strides[1] + kh * d.r.k_strides[2];
+  const T* q = static_cast<const T*>(d.r.q) + b * d.r.q_strides[0] + t0 * d.r.q_strides[1] + kh * d.r.q_strides[2];
+  const int64_t ks = d.r.k_strides[1], qs_ = d.r.q_strides[1];
+  const int64_t turned = ((b * d.r.key_heads + kh) * d.chunks + c) * DP * kChunk;
   f32x4 dQ[1][NT], dK[1][NT];
   clear(dQ);
   clear(dK);
@@ -207,11 +282,24 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_parts_kernel(
       }
       continue;
     }
-    load_gates(gates, d, b, h, t0, live);
-    if (threadIdx.x < kChunk) dbeta[threadIdx.x] = 0.0f;
+    const Squares<T>& sq = squares[bh * d.chunks + c];
+    if (threadIdx.x < kChunk) {
+      const int t = threadIdx.x;
+      double sum = 0.0;
+      if (t < live)
+        sum = (double)clamped(gate_at(d, d.r.decay, b * d.r.decay_strides[0] + (t0 + t) * d.r.decay_strides[1] +
+                                                        h * d.r.decay_strides[2]));
+      for (int n = 1; n < 64; n *= 2) {
+        const double prior = __shfl_up(sum, n);
+        if (t >= n) sum += prior;
+      }
+      G[t] = sum;
+      betas[t] = sq.gates.beta[t];
+      dbeta[t] = 0.0f;
+    }
     const float* state = states + (bh * d.chunks + c) * dk * dv;
     const float* dstate = dstates + (bh * d.chunks + c) * dk * dv;
-    f32x4 qs[1][NT], k1[1][NT], k2[1][NT], P[1][4], ZU[1][4];
+    f32x4 qs[1][NT], k1[1][NT], k2[1][NT], P[1][2], ZU[1][2];
     clear(qs);
     clear(k1);
     clear(k2);
@@ -220,28 +308,24 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_parts_kernel(
     float dot = 0.0f;
     __syncthreads();
     for (int e0 = 0; e0 < dv; e0 += kWide) {
-      for (int at = threadIdx.x; at < DP * (kWide / 4); at += kDeltaBlock) {
+#pragma unroll 2
+      for (int at = threadIdx.x; at < DP * (kWide / 4); at += kPartsBlock) {
         const int row = at / (kWide / 4), col = at % (kWide / 4) * 4;
+        const int left = row < dk ? dv - e0 - col : 0;
         const int64_t from = (int64_t)row * dv + e0 + col;
-        const f32x4 s = quad(state + from, row < dk, dv - e0 - col), l = quad(dstate + from, row < dk, dv - e0 - col);
-        *reinterpret_cast<f32x4*>(S + row * kWidePitch + col) = s;
-        *reinterpret_cast<f32x4*>(L + row * kWidePitch + col) = l;
+        const f32x4 s = quad(state + from, left), l = quad(dstate + from, left);
+        put4<NV>(S + row * kWidePitch + col, Room::kState, s);
+        put4<NV>(L + row * kWidePitch + col, Room::kState, l);
 #pragma unroll
         for (int e = 0; e < 4; ++e) dot = fmaf(s[e], l[e], dot);
       }
-      for (int at = threadIdx.x; at < kChunk * (kWide / 4); at += kDeltaBlock) {
-        const int t = at / (kWide / 4), col = at % (kWide / 4) * 4;
+      static_assert(kChunk * (kWide / 4) == kPartsBlock, "a quad of X to a lane");
+      {
+        const int t = threadIdx.x / (kWide / 4), col = threadIdx.x % (kWide / 4) * 4;
+        const int left = t < live ? dv - e0 - col : 0;
         const int64_t from = ((b * d.r.T + t0 + t) * d.r.heads + h) * dv + e0 + col;
-        const f32x4 x = quad(xs + from, t < live, dv - e0 - col), ev = quad(es + from, t < live, dv - e0 - col);
-        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (grad_o && t < live)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (e0 + col + e < dv) o[e] = to_float(grad_o[from + e]);
-        const float beta = gates.beta[t];
-        *reinterpret_cast<f32x4*>(O + t * kWidePitch + col) = o;
-        *reinterpret_cast<f32x4*>(U + t * kWidePitch + col) = beta * x;
-        *reinterpret_cast<f32x4*>(Z + t * kWidePitch + col) = beta * ev;
+        const f32x4 x = quad(xs + from, left), ev = quad(es + from, left);
+        put4<NV>(U + t * kWidePitch + col, Room::kSamples, betas[t] * x);
         float part = x[0] * ev[0];
 #pragma unroll
         for (int e = 1; e < 4; ++e) part = fmaf(x[e], ev[e], part);
@@ -250,24 +334,60 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_parts_kernel(
         part += __shfl_xor(part, 4);
         if (col == 0) dbeta[t] += part;
       }
+      // this wave's own samples of dO and Z
+      const int row = w0 + i, col = 8 * g, left = row < live ? dv - e0 - col : 0;
+      const int64_t from = ((b * d.r.T + t0 + row) * d.r.heads + h) * dv + e0 + col;
+      const Frag<NI> of = input_frag(grad_o + from, grad_o ? left : 0);
+      float z[8];
+      const f32x4 z0 = quad(es + from, left), z1 = quad(es + from + 4, left - 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[e] = betas[row] * z0[e], z[4 + e] = betas[row] * z1[e];
+      const Frag<NV> zf = frag_of<NV>(z);
       __syncthreads();
-      const int w = 16 * wave * kWidePitch;
-      multiply<false, false>(qs, O + w, kWidePitch, S, kWidePitch, kWide);
-      multiply<false, false>(k1, U + w, kWidePitch, L, kWidePitch, kWide);
-      multiply<false, false>(k2, Z + w, kWidePitch, S, kWidePitch, kWide);
-      multiply<false, false>(P, O + w, kWidePitch, U, kWidePitch, kWide);
-      multiply<false, false>(ZU, Z + w, kWidePitch, U, kWidePitch, kWide);
+      const Frag<NV> uf = plane_frag<NV>(U + row * kWidePitch + col, Room::kSamples);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int at = (d0 + 16 * n + i) * kWidePitch + col;
+        const Frag<NV> s = plane_frag<NV>(S + at, Room::kState), l = plane_frag<NV>(L + at, Room::kState);
+        mma(qs[0][n], of, s);
+        mma(k2[0][n], zf, s);
+        mma(k1[0][n], uf, l);
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const Frag<NV> u = plane_frag<NV>(U + (j0 + 16 * n + i) * kWidePitch + col, Room::kSamples);
+        mma(P[0][n], of, u);
+        mma(ZU[0][n], zf, u);
+      }
       __syncthreads();
+    }
+    // the products that M and P were made of
+    f32x4 kk[1][2], qk[1][2];
+    clear(kk);
+    clear(qk);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int col = 32 * s + 8 * g, row = w0 + i, left = row < live ? dk - col : 0;
+      const Frag<NI> ak = input_frag(k + row * ks + col, left), aq = input_frag(q + row * qs_ + col, left);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int other = j0 + 16 * n + i;
+        const Frag<NI> bk = input_frag(k + other * ks + col, other < live ? dk - col : 0);
+        mma(kk[0][n], ak, bk);
+        mma(qk[0][n], aq, bk);
+      }
     }
     // what passes a sample's decay from the state before the chunk, and to the one after
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int row = 16 * wave + 4 * g + e;
-      const float since = gates.since[row], until = gates.until[row], ss = d.r.scale * since;
+      const int row = w0 + 4 * g + e;
+      const float since = sq.gates.since[row], until = sq.gates.until[row], ss = d.r.scale * since;
       float from = 0.0f, to = 0.0f;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const float qv = Q[row * kPitch + 16 * n + i], kv = K[row * kPitch + 16 * n + i];
+        const int col = d0 + 16 * n + i;
+        const bool in = row < live && col < dk;
+        const float qv = in ? to_float(q[row * qs_ + col]) : 0.0f, kv = in ? to_float(k[row * ks + col]) : 0.0f;
         const float a = ss * qs[0][n][e], z = since * k2[0][n][e], u = until * k1[0][n][e];
         from = fmaf(qv, a, from);
         from = fmaf(-kv, z, from);
@@ -276,47 +396,85 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_parts_kernel(
         dK[0][n][e] += u - z;
       }
 #pragma unroll
-      for (int k = 1; k < 16; k *= 2) {
-        from += __shfl_xor(from, k);
-        to += __shfl_xor(to, k);
+      for (int n = 1; n < 16; n *= 2) {
+        from += __shfl_xor(from, n);
+        to += __shfl_xor(to, n);
       }
-      if (i == 0) before[row] = from, after[row] = to;
+      if (i == 0) before[half][row] = from, after[half][row] = to;
     }
 #pragma unroll
-    for (int k = 1; k < 64; k *= 2) dot += __shfl_xor(dot, k);
+    for (int n = 1; n < 64; n *= 2) dot += __shfl_xor(dot, n);
     if (lane == 0) whole[wave] = dot;
-    const float* sq = squares + (bh * d.chunks + c) * kSquares;
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
+    for (int n = 0; n < 2; ++n) {
+      const int col = j0 + 16 * n + i;
+      f32x4 w, y;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int row = 16 * wave + 4 * g + e, col = 16 * n + i;
-        const float decay = col <= row ? expf((float)(gates.G[row] - gates.G[col])) : 0.0f;
-        W1[row * kRow + col] = d.r.scale * decay * P[0][n][e];
-        W2[row * kRow + col] = col < row ? -decay * ZU[0][n][e] : 0.0f;
-        H[row * (kChunk + 1) + col] = P[0][n][e] * sq[kSquare + row * kChunk + col] -
-                                      ZU[0][n][e] * sq[2 * kSquare + row * kChunk + col];
+        const int row = w0 + 4 * g + e;
+        const float decay = col <= row ? expf((float)(G[row] - G[col])) : 0.0f;
+        w[e] = d.r.scale * decay * P[0][n][e];
+        y[e] = col < row ? -decay * ZU[0][n][e] : 0.0f;
+        H[row * (kChunk + 1) + col] = w[e] * qk[0][n][e] + y[e] * kk[0][n][e];
       }
+      put4<NV>(Wt + col * kRow + w0 + 4 * g, Room::kFlat, w);
+      // both halves of Y: above the diagonal its mirror image
+      const int top = w0 + 4 * g;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = top + e;
+        bf16 p[NV], r[NV];
+        split<NV>(w[e], p);
+        split<NV>(y[e], r);
+#pragma unroll
+        for (int n2 = 0; n2 < NV; ++n2) {
+          W[n2 * Room::kFlat + row * kRow + col] = p[n2];
+          if (col <= row) Y[n2 * Room::kFlat + row * kRow + col] = r[n2];
+          if (col < row) Y[n2 * Room::kFlat + col * kRow + row] = r[n2];
+        }
+      }
+    }
     __syncthreads();
-    multiply<false, true>(dQ, W1 + 16 * wave * kRow, kRow, K, kPitch, kChunk);
-    multiply<true, true>(dK, W1 + 16 * wave, kRow, Q, kPitch, kChunk);
-    multiply<false, true>(dK, W2 + 16 * wave * kRow, kRow, K, kPitch, kChunk);
-    multiply<true, true>(dK, W2 + 16 * wave, kRow, K, kPitch, kChunk);
-    if (threadIdx.x < kChunk) {   // H: each row's sum of the columns before
-      float sum = 0.0f;
-      for (int k = 0; k < kChunk; ++k) {
-        float& v = H[threadIdx.x * (kChunk + 1) + k];
-        const float now = v;
-        v = sum;
-        sum += now;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int from = (w0 + i) * kRow + 32 * s + 8 * g;
+      const Frag<NV> wf = plane_frag<NV>(W + from, Room::kFlat), wt = plane_frag<NV>(Wt + from, Room::kFlat),
+                     yf = plane_frag<NV>(Y + from, Room::kFlat);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int64_t at = turned + (d0 + 16 * n + i) * kChunk + 32 * s + 8 * g;
+        const Frag<NI> kf = input_frag(kt + at, 8), qf = input_frag(qt + at, 8);
+        mma(dQ[0][n], wf, kf);
+        mma(dK[0][n], wt, qf);
+        mma(dK[0][n], yf, kf);
       }
+    }
+    // the decays: a wave has 8 of the rows, a lane a sample; what crosses it from the columns
+    // before, for each row from it on
+    {
+      float sum = 0.0f;
+      for (int n = 0; n < 8; ++n) {
+        const int row = 8 * wave + n;
+        float v = H[row * (kChunk + 1) + lane];
+#pragma unroll
+        for (int m = 1; m < 64; m *= 2) {
+          const float prior = __shfl_up(v, m);
+          if (lane >= m) v += prior;
+        }
+        v = __shfl_up(v, 1);   // of the columns before
+        if (lane == 0) v = 0.0f;
+        if (row >= lane) sum += v + (before[0][row] + before[1][row]);
+        else sum += after[0][row] + after[1][row];
+      }
+      sums[wave][lane] = sum;
     }
     __syncthreads();
     if (threadIdx.x < kChunk) {
       const int t = threadIdx.x;
-      float sum = gates.since[kChunk - 1] * ((whole[0] + whole[1]) + (whole[2] + whole[3]));
-      for (int k = 0; k < t; ++k) sum += after[k];
-      for (int k = t; k < kChunk; ++k) sum += before[k] + H[k * (kChunk + 1) + t];
+      float dots = 0.0f, sum = 0.0f;
+#pragma unroll
+      for (int n = 0; n < 8; ++n) dots += whole[n], sum += sums[n][t];
+      sum = fmaf(sq.gates.since[kChunk - 1], dots, sum);
       if (t < rows) {
         const int64_t at = (b * d.r.T + t0 + t) * d.r.heads + h;
         if (grad_decay) put_gate(d, grad_decay, at, t < live ? sum : 0.0f);
@@ -329,7 +487,7 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_parts_kernel(
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int t = 16 * wave + 4 * g + e, col = 16 * n + i;
+      const int t = w0 + 4 * g + e, col = d0 + 16 * n + i;
       if (t >= rows || col >= dk) continue;
       const int64_t at = ((b * d.r.T + t0 + t) * d.r.key_heads + kh) * dk + col;
       if (grad_q) grad_q[at] = from_float<T>(dQ[0][n][e]);
@@ -337,40 +495,83 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_parts_kernel(
     }
 }
 
+// The backward's workspace (bytes).
+struct Space {
+  int64_t squares, kt, qt, dstates, es, adds, starts, all;
+};
+Space space_of(const Delta& d, const Cut& cut) {
+  const int64_t heads = d.r.B * d.r.heads, turned = d.r.B * d.r.key_heads * d.chunks * turned_bytes(d.r);
+  const auto next = [](int64_t n) { return (n + 255) / 256 * 256; };
+  Space w;
+  w.squares = 0;
+  w.kt = next(heads * d.chunks * squares_bytes(d.r.dtype));
+  w.qt = w.kt + next(turned);
+  w.dstates = w.qt + next(turned);
+  w.es = w.dstates + next(heads * d.chunks * d.r.dk * d.r.dv * 4);
+  w.adds = w.es + next(heads * d.r.T * d.r.dv * 4);
+  const int64_t segments = cut.segs > 1 ? next(heads * cut.segs * d.r.dk * d.r.dv * 4) : 0;
+  w.starts = w.adds + segments;
+  w.all = w.starts + segments;
+  return w;
+}
+
 }  // namespace
+
+int64_t delta_backward_workspace(const Delta& d) { return space_of(d, cut_of(d)).all; }
 
 hipError_t launch_delta_rule_backward(const cpab_delta_rule& r, const float* kept, const void* grad_o,
                                       const float* grad_h, void* grad_q, void* grad_k, void* grad_v,
                                       void* grad_decay, void* grad_beta, float* grad_h0,
                                       void* workspace, hipStream_t st) {
   const Delta d = delta_of(r);
-  const int64_t heads = r.B * r.heads, states = heads * d.chunks * r.dk * r.dv;
-  float* squares = static_cast<float*>(workspace);
-  float* dstates = squares + heads * d.chunks * kSquares;
-  float* es = dstates + states;
+  const Cut cut = cut_of(d);
+  const Space w = space_of(d, cut);
+  const Kept k = kept_of(d, cut);
+  const int64_t heads = r.B * r.heads;
+  char* room = static_cast<char*>(workspace);
+  float* dstates = reinterpret_cast<float*>(room + w.dstates);
+  float* es = reinterpret_cast<float*>(room + w.es);
+  float* adds = reinterpret_cast<float*>(room + w.adds);
+  float* starts = reinterpret_cast<float*>(room + w.starts);
   hipError_t e = hipSuccess;
-  if (d.chunks > 0) e = launch_delta_squares(d, squares, st);
+  if (d.chunks > 0) e = launch_delta_squares(d, room + w.squares, room + w.kt, room + w.qt, st);
   if (e != hipSuccess) return e;
   with_key(d, [&](auto t, auto dp) {
     typedef decltype(t) T;
-    constexpr int DP = decltype(dp)::value;
-    constexpr int kChain = 4 * ((2 * kChunk + kWide) * (DP + 4) + (2 * kWide + 2 * kChunk) * kRow);
-    static LdsAllowed chain, parts;
-    if (r.dv > 0) {
-      e = allow_lds(reinterpret_cast<const void*>(delta_back_chain_kernel<T, DP>), kChain, chain);
+    constexpr int DP = decltype(dp)::value, NV = Parts<T>::kValue, NI = Parts<T>::kInput;
+    const Squares<T>* squares = reinterpret_cast<const Squares<T>*>(room + w.squares);
+    const T *kt = reinterpret_cast<const T*>(room + w.kt), *qt = reinterpret_cast<const T*>(room + w.qt);
+    const auto run = [&](auto width, auto only_ends) {
+      constexpr int E = decltype(width)::value;
+      constexpr bool ENDS = decltype(only_ends)::value;
+      constexpr int kRoom = 2 * E * (NV * (DP + 8) + (4 * NV + NI) * kRow);
+      static LdsAllowed allowed;
+      e = allow_lds(reinterpret_cast<const void*>(delta_back_chain_kernel<T, DP, E, ENDS>), kRoom, allowed);
       if (e != hipSuccess) return;
-      delta_back_chain_kernel<T, DP><<<(unsigned)(heads * ((r.dv + kWide - 1) / kWide)), kDeltaBlock, kChain, st>>>(
-          d, squares, (const T*)grad_o, grad_h, (T*)grad_v, grad_h0, dstates, es);
+      delta_back_chain_kernel<T, DP, E, ENDS>
+          <<<(unsigned)((heads * cut.segs + 7) / 8 * 8 * ((r.dv + E - 1) / E)), 8 * E, kRoom, st>>>(
+              d, squares, kt, qt, cut, (const T*)grad_o, grad_h, starts, (T*)grad_v, grad_h0, dstates, es, adds);
       e = hipGetLastError();
+    };
+    const auto both = [&](auto only_ends) {
+      if constexpr (sizeof(T) == 2)
+        if (r.dv > 32) return run(std::integral_constant<int, 64>(), only_ends);
+      run(std::integral_constant<int, 32>(), only_ends);
+    };
+    if (r.dv > 0 && cut.segs > 1) {
+      both(std::true_type());
+      if (e == hipSuccess) e = launch_delta_join(d, cut, false, kept + k.ends, adds, grad_h, starts, st);
+      if (e != hipSuccess) return;
     }
+    if (r.dv > 0) both(std::false_type());
     if (e != hipSuccess || d.chunks == 0 || !(grad_q || grad_k || grad_decay || grad_beta)) return;
-    constexpr int kAfter = 3 * kChunk * kRow, kLoop = (2 * DP + 3 * kChunk) * kWidePitch;
-    constexpr int kParts = 4 * (2 * kChunk * (DP + 4) + std::max(kAfter, kLoop));
-    e = allow_lds(reinterpret_cast<const void*>(delta_parts_kernel<T, DP>), kParts, parts);
+    constexpr int kRoom = PartsRoom<T, DP>::kBytes;
+    static LdsAllowed allowed;
+    e = allow_lds(reinterpret_cast<const void*>(delta_parts_kernel<T, DP>), kRoom, allowed);
     if (e != hipSuccess) return;
-    delta_parts_kernel<T, DP><<<(unsigned)(r.B * r.key_heads * d.chunks), kDeltaBlock, kParts, st>>>(
-        d, squares, kept, kept + states, dstates, es, (const T*)grad_o, (T*)grad_q, (T*)grad_k,
-        grad_decay, grad_beta);
+    delta_parts_kernel<T, DP><<<(unsigned)(r.B * r.key_heads * d.chunks), kPartsBlock, kRoom, st>>>(
+        d, squares, kt, qt, kept + k.states, kept + k.xs, dstates, es, (const T*)grad_o, (T*)grad_q,
+        (T*)grad_k, grad_decay, grad_beta);
     e = hipGetLastError();
   });
   return e;
