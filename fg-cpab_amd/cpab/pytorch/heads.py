@@ -21,7 +21,7 @@ def gated_delta_rule(q, k, v, decay, beta, h0=None, lengths=None, scale=None):
     The state is held in 32 bits, and so is what passes between samples.
 
     Arguments:
-        q, k: [B, T, key heads, dk] of v's type, dk at most 128.  Keys longer than 1 can
+        q, k: [B, T, key heads, dk] of v's type, dk from 1 to 128.  Keys longer than 1 can
             make the state grow without bound, as they do in the formula
         v: [B, T, heads, dv] float32 or bfloat16; heads is a multiple of the key heads,
             neighbouring ones share a query and a key.  Slices of one projection's output

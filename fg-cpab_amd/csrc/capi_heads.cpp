@@ -94,8 +94,8 @@ int check_delta_sizes(const cpab_delta_rule* rule) {
     return fail(CPAB_ERR_INVALID, "negative size (B=%lld, T=%lld, heads=%lld, key_heads=%lld, dk=%lld, dv=%lld)",
                 (long long)r.B, (long long)r.T, (long long)r.heads, (long long)r.key_heads,
                 (long long)r.dk, (long long)r.dv);
-  if (r.dk > CPAB_DELTA_MOST_KEY)
-    return fail(CPAB_ERR_INVALID, "dk must be at most %d, got %lld", CPAB_DELTA_MOST_KEY, (long long)r.dk);
+  if (r.dk < 1 || r.dk > CPAB_DELTA_MOST_KEY)
+    return fail(CPAB_ERR_INVALID, "dk must be from 1 to %d, got %lld", CPAB_DELTA_MOST_KEY, (long long)r.dk);
   if (r.heads > 0 && (r.key_heads < 1 || r.heads % r.key_heads != 0))
     return fail(CPAB_ERR_INVALID, "heads must be a multiple of key_heads, got %lld and %lld",
                 (long long)r.heads, (long long)r.key_heads);
@@ -118,7 +118,7 @@ int check_delta(const cpab_delta_rule* rule) {
   const cpab_delta_rule& r = *rule;
   if (!std::isfinite(r.scale)) return fail(CPAB_ERR_INVALID, "scale must be finite");
   if (any_delta(r) && r.T > 0) {
-    if (r.dk > 0) { CPAB_REQUIRE(r.q); CPAB_REQUIRE(r.k); }
+    CPAB_REQUIRE(r.q); CPAB_REQUIRE(r.k);
     if (r.dv > 0) CPAB_REQUIRE(r.v);
     CPAB_REQUIRE(r.decay); CPAB_REQUIRE(r.beta);
   }
@@ -186,7 +186,7 @@ int cpab_delta_rule_forward(const cpab_delta_rule* rule, void* o, float* h, floa
   const cpab_delta_rule& r = *rule;
   if (!any_delta(r) || r.dv == 0) return CPAB_OK;
   if (r.T > 0) CPAB_REQUIRE(o);
-  if (r.dk > 0) CPAB_REQUIRE(h);
+  CPAB_REQUIRE(h);
   CPAB_ALIGNED(o, size_of(r.dtype)); CPAB_ALIGNED(h, 4); CPAB_ALIGNED(kept, 4);
   CPAB_TRY(check_workspace(workspace, workspace_bytes, cpab::delta_rule_workspace(r, kept != nullptr, false)));
   return check_hip(cpab::launch_delta_rule_forward(r, o, h, kept, workspace, as_stream(stream)),

@@ -37,10 +37,11 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// A call as the kernels take it.
+// A call as the kernels take it.  q and k are read in eights: rows of `read`, a multiple of
+// 8, are dk wide or a copy that is padded with zeros.
 struct Delta {
   cpab_delta_rule r;
-  int chunks, group;
+  int chunks, group, read;
 };
 
 __device__ __forceinline__ int64_t live_of(const Delta& d, int64_t b) {
@@ -59,18 +60,18 @@ __device__ __forceinline__ float clamped(float decay) { return decay < -128.0f ?
 // ---- products ------------------------------------------------------------------
 
 // The matrix unit's 32-bit products run at a sixteenth of the bfloat16 ones' rate, so that
-// values of 32 bits go as sums of bfloat16 parts, each the nearest to what the ones before
-// leave: two with 16-bit inputs, 17 bits, far beyond what a 16-bit result shows and enough
-// for the states and gates' gradients in 32; three with 32-bit inputs, 24 bits.  A 16-bit
-// input is its own first part.  Of the products of parts those are taken that are not below
-// the last part's rounding.
+// values of 32 bits go as sums of three bfloat16 parts, each the nearest to what the ones
+// before leave: 24 bits.  A 16-bit input is its own first part, a 32-bit one has three.  Of
+// the products of parts those are taken that are not below the last part's rounding: three
+// with an input of 16 bits, six of two values.  Outputs of 16 bits are made of two parts, 17
+// bits (two throughout left the 32-bit states behind 16-bit inputs 3e-6 to 1e-5 off).
 template <typename T>
 struct Parts {
-  static constexpr int kInput = 1, kValue = 2;
+  static constexpr int kInput = 1, kValue = 3, kOut = 2;
 };
 template <>
 struct Parts<float> {
-  static constexpr int kInput = 3, kValue = 3;
+  static constexpr int kInput = 3, kValue = 3, kOut = 3;
 };
 template <int N>
 struct Frag {   // 8 neighbours of the summed index
@@ -107,28 +108,72 @@ __device__ __forceinline__ void mma(f32x4& acc, const Frag<NA>& a, const Frag<NB
       if (i + j <= kLast) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[j], acc, 0, 0, 0);
 }
 
-// 8 neighbours of a row of an input, zeros where it has fewer (`left`).
-__device__ __forceinline__ Frag<1> input_frag(const bf16* p, int left) {
+// The first parts of an operand.
+template <int N, int M>
+__device__ __forceinline__ Frag<N> first_of(const Frag<M>& f) {
+  Frag<N> r;
+#pragma unroll
+  for (int k = 0; k < N; ++k) r.p[k] = f.p[k];
+  return r;
+}
+
+// 8 neighbours of an input's row, as they lie in memory.
+__device__ __forceinline__ Frag<1> eight(const bf16* p) {
   typedef uint32_t U4 __attribute__((ext_vector_type(4)));
   typedef U4 __attribute__((aligned(2))) Unit;
-  Frag<1> f;
-  if (left >= 8) {
-    f.p[0] = __builtin_bit_cast(bf16x8, (U4)*reinterpret_cast<const Unit*>(p));
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f.p[0][e] = e < left ? p[e] : (bf16)0.0f;
-  }
-  return f;
+  return Frag<1>{{__builtin_bit_cast(bf16x8, (U4)*reinterpret_cast<const Unit*>(p))}};
 }
-__device__ __forceinline__ Frag<3> input_frag(const float* p, int left) {
+__device__ __forceinline__ Frag<3> eight(const float* p) {
   float v[8];
-  if (left >= 8) {
-    load<8>(p, v);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < left ? p[e] : 0.0f;
-  }
+  load<8>(p, v);
   return frag_of<3>(v);
+}
+
+// Rows of an input: `live` of them, `width` values each, a multiple of 8, zeros beyond.
+// Where there is nothing to read the first row is: without a branch between the lanes loads
+// are not waited for one by one.  FULL: every row and column is there.
+template <typename T>
+struct Rows {
+  const T* p;
+  int64_t stride;
+  int live, width;
+  template <bool FULL>
+  __device__ __forceinline__ Frag<Parts<T>::kInput> at(int row, int col) const {
+    if (FULL) return eight(p + row * stride + col);
+    const bool in = row < live && col < width;
+    Frag<Parts<T>::kInput> f = eight(p + (in ? row * stride + col : 0));
+#pragma unroll
+    for (int k = 0; k < Parts<T>::kInput; ++k) {
+      typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+      U4 v = __builtin_bit_cast(U4, f.p[k]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = in ? v[e] : 0u;
+      f.p[k] = __builtin_bit_cast(bf16x8, v);
+    }
+    return f;
+  }
+  template <bool FULL>
+  __device__ __forceinline__ float one(int row, int col) const {
+    if (FULL) return to_float(p[row * stride + col]);
+    const bool in = row < live && col < width;
+    const float v = to_float(p[in ? row * stride + col : 0]);
+    return in ? v : 0.0f;
+  }
+  // Four neighbours; the width a multiple of 4.
+  __device__ __forceinline__ f32x4 four(int row, int col) const {
+    const bool in = row < live && col < width;
+    float w[4];
+    load<4>(p + (in ? row * stride + col : 0), w);
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = in ? w[e] : 0.0f;
+    return v;
+  }
+};
+// f(FULL) as a constant.
+template <typename F>
+__device__ __forceinline__ void either(bool full, F f) {
+  full ? f(std::true_type()) : f(std::false_type());
 }
 
 // Operands in planes of 16-bit parts, in LDS or the workspace: 8 neighbours to a lane.
@@ -203,8 +248,21 @@ void with_key(const Delta& d, F f) {
 }
 
 inline Delta delta_of(const cpab_delta_rule& r) {
-  return Delta{r, (int)((r.T + kChunk - 1) / kChunk), (int)(r.heads / r.key_heads)};
+  return Delta{r, (int)((r.T + kChunk - 1) / kChunk), (int)(r.heads / r.key_heads), (int)(r.dk + 7) / 8 * 8};
 }
+// Widths that the library's own arrays of values have: rows of whole eights.
+inline int64_t wide_of(const cpab_delta_rule& r) { return (r.dv + 7) / 8 * 8; }
+
+// Rows of `width` values (three strides before them) to contiguous rows of whole eights,
+// padded with zeros.
+hipError_t launch_delta_pad(int dtype, const void* from, const int64_t strides[3], int64_t B, int64_t T,
+                            int64_t heads, int64_t width, void* to, hipStream_t s);
+// Padded copies of q and k where their width is not whole eights: bytes of both, and the
+// call on them.
+inline int64_t padded_keys(const cpab_delta_rule& r) {
+  return r.dk % 8 == 0 ? 0 : 2 * r.B * r.T * r.key_heads * ((r.dk + 7) / 8 * 8) * (r.dtype == CPAB_F32 ? 4 : 2);
+}
+hipError_t pad_keys(Delta* d, void* room, hipStream_t s);
 
 // How a call is cut: a head's chunks in `segs` segments of `each`.
 struct Cut {

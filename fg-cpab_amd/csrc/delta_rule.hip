@@ -12,8 +12,8 @@ namespace {
 // ---- a chunk's matrices ------------------------------------------------------
 
 // 64 x 64 values from LDS to planes in the workspace, or their transpose.
-template <int N, bool TURNED>
-__device__ __forceinline__ void put_square(const float* from, int pitch, bf16 (&to)[N][kChunk][kChunk]) {
+template <int N, bool TURNED, int M>
+__device__ __forceinline__ void put_square(const float* from, int pitch, bf16 (&to)[M][kChunk][kChunk]) {
   const int row = threadIdx.x >> 2, col = (threadIdx.x & 3) * 16;
 #pragma unroll
   for (int half = 0; half < 16; half += 8) {
@@ -27,16 +27,20 @@ __device__ __forceinline__ void put_square(const float* from, int pitch, bf16 (&
   }
 }
 
-// A chunk's [64, D] of an input, transposed, to the workspace: [DP, 64], zeros beyond `live`
-// and D.  Called by the whole workgroup; `room` holds DP rows of kRow values.
+// A chunk of an input, transposed, to the workspace: [DP, 64], zeros beyond its rows and
+// columns.  Four samples of four columns to a lane.  Called by the whole workgroup; `room`
+// holds DP rows of kRow values.
 template <int DP, typename T>
-__device__ __forceinline__ void put_turned(T* room, const T* from, int64_t stride, int live, int D, T* to) {
-  for (int k = threadIdx.x; k < kChunk * DP / 4; k += kDeltaBlock) {
-    const int row = k / (DP / 4), col = k % (DP / 4) * 4;
-    const T* p = from + row * stride + col;
-    const int left = row < live ? D - col : 0;
+__device__ __forceinline__ void put_turned(T* room, const Rows<T>& from, T* to) {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  for (int k = threadIdx.x; k < 16 * (DP / 4); k += kDeltaBlock) {
+    const int row = k % 16 * 4, col = k / 16 * 4;
+    f32x4 v[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) room[(col + e) * kRow + row] = e < left ? p[e] : (T)0.0f;
+    for (int e = 0; e < 4; ++e) v[e] = from.four(row + e, col);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      *reinterpret_cast<T4*>(room + (col + e) * kRow + row) = T4{(T)v[0][e], (T)v[1][e], (T)v[2][e], (T)v[3][e]};
   }
   __syncthreads();
   constexpr int kEach = 16 / sizeof(T);
@@ -48,11 +52,21 @@ __device__ __forceinline__ void put_turned(T* room, const T* from, int64_t strid
   __syncthreads();
 }
 
+// [16 x 16] += A B with 32-bit products, B as a product's sums lie in a lane: column i, rows
+// 4 g to 4 g + 3, which are the summed index, in the order in which A is read.
+__device__ __forceinline__ void multiply16(f32x4& acc, const float* A, int pitch, const f32x4& B) {
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const f32x4 a = *reinterpret_cast<const f32x4*>(A + i * pitch + 4 * g);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], B[e], acc, 0, 0, 0);
+}
+
 // The gates, M and P of each chunk of each head, and the transposes of its keys and queries.
 // The decays' logarithms are added in 64 bits: their differences are what counts, and a
-// sample that clears the state (-128) would leave 32 bits 2^-17 of it.  M by rows:
-// M_i = A_i - sum over j < i of A_ij beta_j M_j; a column is four lanes', each with a quarter
-// of the rows.
+// sample that clears the state (-128) would leave 32 bits 2^-17 of it.
+// M by blocks of 16 rows, all in 32 bits: with T_b = (I + A_bb beta_b)^-1 of the blocks on the
+// diagonal, by rows, a wave each, M_b = T_b (A_b - sum over c < b of A_bc beta_c M_c); a wave
+// has 16 columns.
 template <typename T, int DP, bool BACKWARD>
 __global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, Squares<T>* squares, T* kt, T* qt) {
   constexpr int kPitch = kChunk + 4, NV = Parts<T>::kValue, NI = Parts<T>::kInput;
@@ -61,7 +75,7 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, Squ
   __shared__ float betas[kChunk];
   const int c = blockIdx.x % d.chunks;
   const int64_t bh = blockIdx.x / d.chunks, b = bh / d.r.heads;
-  const int h = (int)(bh - b * d.r.heads), kh = h / d.group, dk = (int)d.r.dk;
+  const int h = (int)(bh - b * d.r.heads), kh = h / d.group;
   const int64_t t0 = (int64_t)c * kChunk;
   const int live = (int)min(max(live_of(d, b) - t0, (int64_t)0), (int64_t)kChunk);
   if (live == 0) return;
@@ -86,33 +100,37 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, Squ
     out.gates.until[t] = expf((float)(__shfl(g, 63) - g));
     out.gates.beta[t] = beta;
   }
-  const T* k = static_cast<const T*>(d.r.k) + b * d.r.k_strides[0] + t0 * d.r.k_strides[1] + kh * d.r.k_strides[2];
-  const T* q = static_cast<const T*>(d.r.q) + b * d.r.q_strides[0] + t0 * d.r.q_strides[1] + kh * d.r.q_strides[2];
-  const int64_t ks = d.r.k_strides[1], qs = d.r.q_strides[1];
+  const Rows<T> krows{static_cast<const T*>(d.r.k) + b * d.r.k_strides[0] + t0 * d.r.k_strides[1] + kh * d.r.k_strides[2],
+                      d.r.k_strides[1], live, d.read};
+  const Rows<T> qrows{static_cast<const T*>(d.r.q) + b * d.r.q_strides[0] + t0 * d.r.q_strides[1] + kh * d.r.q_strides[2],
+                      d.r.q_strides[1], live, d.read};
   if (h % d.group == 0) {
     const int64_t at = ((b * d.r.key_heads + kh) * d.chunks + c) * DP * kChunk;
-    put_turned<DP>(reinterpret_cast<T*>(room), k, ks, live, dk, kt + at);
-    if (BACKWARD) put_turned<DP>(reinterpret_cast<T*>(room), q, qs, live, dk, qt + at);
+    put_turned<DP>(reinterpret_cast<T*>(room), krows, kt + at);
+    if (BACKWARD) put_turned<DP>(reinterpret_cast<T*>(room), qrows, qt + at);
   }
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   f32x4 kk[1][4], qk[1][4];
   clear(kk);
   clear(qk);
+  either(live == kChunk && d.read == DP, [&](auto full) {
+    constexpr bool F = decltype(full)::value;
 #pragma unroll
-  for (int col = 8 * g; col < DP; col += 32) {
-    const int row = 16 * wave + i, left = row < live ? dk - col : 0;
-    const Frag<NI> ak = input_frag(k + row * ks + col, left), aq = input_frag(q + row * qs + col, left);
+    for (int s = 0; s < DP / 32; ++s) {
+      const int col = 32 * s + 8 * g;
+      const Frag<NI> ak = krows.template at<F>(16 * wave + i, col), aq = qrows.template at<F>(16 * wave + i, col);
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int other = 16 * n + i;
-      const Frag<NI> bk = input_frag(k + other * ks + col, other < live ? dk - col : 0);
-      mma(kk[0][n], ak, bk);
-      mma(qk[0][n], aq, bk);
+      for (int n = 0; n < 4; ++n) {
+        const Frag<NI> bk = krows.template at<F>(16 * n + i, col);
+        mma(kk[0][n], ak, bk);
+        mma(qk[0][n], aq, bk);
+      }
     }
-  }
+  });
   __syncthreads();
-  float* Ab = room;                  // A beta; its columns 4 q + p at 16 p + q
-  float* A = room + kChunk * kPitch;
+  float* Ab = room;                   // A beta
+  float* A = Ab + kChunk * kPitch;
+  float* Ti = A + kChunk * kPitch;    // the four T
 #pragma unroll
   for (int n = 0; n < 4; ++n)
 #pragma unroll
@@ -121,37 +139,53 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, Squ
       const float decay = col <= row ? expf((float)(G[row] - G[col])) : 0.0f;
       const float a = col < row ? decay * kk[0][n][e] : 0.0f;
       qk[0][n][e] *= d.r.scale * decay;
-      Ab[row * kPitch + (col & 3) * 16 + (col >> 2)] = a * betas[col];
+      Ab[row * kPitch + col] = a * betas[col];
       A[row * kPitch + col] = a;
     }
   __syncthreads();
-  const int col = threadIdx.x >> 2, p = threadIdx.x & 3;
-  float m[16];
+  {
+    // column i of T, rows 4 g to 4 g + 3 of it: T_r = e_r - sum over j < r of (A beta)_rj T_j
+    const float* block = Ab + 16 * wave * kPitch + 16 * wave;
+    f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int r = 0; r < 16; ++r) m[r] = 0.0f;
+    for (int r = 0; r < 16; ++r) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(block + r * kPitch + 4 * g);
+      float sum = a[0] * t[0];   // rows that are not there yet are 0
 #pragma unroll
-  for (int r = 0; r < 16; ++r)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int row = 4 * r + e;
-      float sum = 0.0f;
-#pragma unroll
-      for (int n = 0; n <= r; ++n) sum = fmaf(Ab[row * kPitch + 16 * p + n], m[n], sum);
-      sum += __shfl_xor(sum, 1);
-      sum += __shfl_xor(sum, 2);
-      const float v = A[row * kPitch + col] - sum;
-      if (p == e) m[r] = v;
+      for (int e = 1; e < 4; ++e) sum = fmaf(a[e], t[e], sum);
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      const float v = (i == r ? 1.0f : 0.0f) - sum;
+      t[r & 3] = g == r >> 2 ? v : t[r & 3];
     }
 #pragma unroll
-  for (int r = 0; r < 16; ++r) A[(4 * r + p) * kPitch + col] = m[r];   // a column's own lanes read it
+    for (int e = 0; e < 4; ++e) Ti[(16 * wave + 4 * g + e) * 20 + i] = t[e];
+  }
+  __syncthreads();
+  f32x4 m[4];
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {   // the block row; what lies above this wave's diagonal block is 0
+    m[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (n < wave) continue;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f}, y;
+#pragma unroll
+    for (int c2 = 0; c2 < n; ++c2)
+      if (c2 >= wave) multiply16(sum, Ab + 16 * n * kPitch + 16 * c2, kPitch, m[c2]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = A[(16 * n + 4 * g + e) * kPitch + 16 * wave + i] - sum[e];
+    multiply16(m[n], Ti + 16 * n * 20, 20, y);
+  }
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < 4; ++n)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) Ab[(16 * wave + 4 * g + e) * kPitch + 16 * n + i] = qk[0][n][e];
-  put_square<NV, BACKWARD>(A, kPitch, out.m);
+    for (int e = 0; e < 4; ++e) {
+      A[(16 * n + 4 * g + e) * kPitch + 16 * wave + i] = m[n][e];
+      Ab[(16 * wave + 4 * g + e) * kPitch + 16 * n + i] = qk[0][n][e];
+    }
   __syncthreads();
-  put_square<NV, BACKWARD>(Ab, kPitch, out.p);
+  put_square<NV, BACKWARD>(A, kPitch, out.m);
+  put_square<BACKWARD ? NV : Parts<T>::kOut, BACKWARD>(Ab, kPitch, out.p);
 }
 
 // ---- the chain of chunks -----------------------------------------------------
@@ -167,14 +201,14 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
                                                           const float* starts, Cut cut, T* o, float* h_out,
                                                           float* states, float* xs, float* ends, int segs) {
   typedef Shares<DP, E> Sh;
-  constexpr int kPitch = DP + 8, NV = Parts<T>::kValue, NI = Parts<T>::kInput, kSteps = DP / 32;
+  constexpr int kPitch = DP + 8, NV = Parts<T>::kValue, NI = Parts<T>::kInput, NO = Parts<T>::kOut, kSteps = DP / 32;
   constexpr int kState = E * kPitch, kSamples = E * kRow;   // planes
   extern __shared__ __align__(16) bf16 lds[];
   bf16* St = lds;                  // [E][DP]
   bf16* Rt = St + NV * kState;     // beta R, [E][64]
   bf16* Ut = Rt + NV * kSamples;
-  bf16* Ht = Ut + NV * kSamples;   // U until the chunk's end
-  const int dk = (int)d.r.dk, dv = (int)d.r.dv, blocks_v = (dv + E - 1) / E;
+  bf16* Ht = Ut + NO * kSamples;   // U until the chunk's end
+  const int dk = (int)d.r.dk, dv = (int)d.r.dv, blocks_v = (dv + E - 1) / E, wide = (dv + 7) / 8 * 8;
   const int64_t heads = d.r.B * d.r.heads;
   const Where at = where(heads, segs, blocks_v + (ENDS ? (dk + E - 1) / E : 0));
   if (!at.in) return;
@@ -182,7 +216,7 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
   const int h = (int)(bh - b * d.r.heads), kh = h / d.group;
   const bool unit = ENDS && at.block >= blocks_v;
   const int e0 = (unit ? at.block - blocks_v : at.block) * E, width = unit ? dk : dv;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int64_t length = live_of(d, b);
   const T* q = static_cast<const T*>(d.r.q) + b * d.r.q_strides[0] + kh * d.r.q_strides[2];
   const T* k = static_cast<const T*>(d.r.k) + b * d.r.k_strides[0] + kh * d.r.k_strides[2];
@@ -216,46 +250,59 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
   };
   const int chunks = (int)((length + kChunk - 1) / kChunk);
   const int first = at.seg * cut.each, last = min(first + cut.each, chunks);
-  Frag<NI> kf[kSteps], qf[kSteps];
+  // What a chunk's products take is fetched as soon as the chunk before is done with the
+  // registers: memory has most of a chunk's time to answer.
+  Frag<NI> kf[kSteps], qf[kSteps], ktf[Sh::MT][2];
+  Frag<NV> mf[2];
+  Frag<NO> pf[2];
   float vf[2][4];
-  const auto fetch = [&](int c) {   // what the chunk's first products take
-    const int64_t t0 = (int64_t)c * kChunk;
-    const int live = (int)min(length - t0, (int64_t)kChunk), row = w0 + i;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int col = 32 * s + 8 * g, left = row < live ? dk - col : 0;
-      kf[s] = input_frag(k + (t0 + row) * ks + col, left);
-      if (!ENDS) qf[s] = input_frag(q + (t0 + row) * qs + col, left);
-    }
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int t = w0 + 4 * g + e, col = e0 + c0 + 16 * n + i;
-        vf[n][e] = !unit && t < live && col < dv ? to_float(v[(t0 + t) * vs + col]) : 0.0f;
-      }
-  };
-  if (first < last) fetch(first);
-  for (int c = first; c < last; ++c) {
+  f32x4 since, until, beta;
+  float total;
+  const auto fetch_rows = [&](int c) {
     const int64_t t0 = (int64_t)c * kChunk;
     const int live = (int)min(length - t0, (int64_t)kChunk);
-    const Squares<T>& sq = squares[bh * d.chunks + c];
+    const Rows<T> krows{k + t0 * ks, ks, live, d.read}, qrows{q + t0 * qs, qs, live, d.read};
+    const Rows<T> vrows{v + t0 * vs, vs, live, unit ? 0 : dv};
+    either(live == kChunk && d.read == DP && e0 + E <= dv && !unit, [&](auto full) {
+      constexpr bool F = decltype(full)::value;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        kf[s] = krows.template at<F>(w0 + i, 32 * s + 8 * g);
+        if (!ENDS) qf[s] = qrows.template at<F>(w0 + i, 32 * s + 8 * g);
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) vf[n][e] = vrows.template one<F>(w0 + 4 * g + e, e0 + c0 + 16 * n + i);
+    });
+  };
+  const auto fetch_m = [&](const Squares<T>& sq) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) mf[s] = plane_frag<NV>(&sq.m[0][w0 + i][32 * s + 8 * g], kSquare);
+    since = *reinterpret_cast<const f32x4*>(sq.gates.since + w0 + 4 * g);
+    until = *reinterpret_cast<const f32x4*>(sq.gates.until + w0 + 4 * g);
+    beta = *reinterpret_cast<const f32x4*>(sq.gates.beta + w0 + 4 * g);
+  };
+  const auto fetch_rest = [&](const Squares<T>& sq, int c) {
     const T* ktc = kt + ((b * d.r.key_heads + kh) * d.chunks + c) * DP * kChunk;
-    Frag<NV> mf[2], pf[2];
-    Frag<NI> ktf[Sh::MT][2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      mf[s] = plane_frag<NV>(&sq.m[0][w0 + i][32 * s + 8 * g], kSquare);
-      if (!ENDS) pf[s] = plane_frag<NV>(&sq.p[0][w0 + i][32 * s + 8 * g], kSquare);
+      if (!ENDS) pf[s] = plane_frag<NO>(&sq.p[0][w0 + i][32 * s + 8 * g], kSquare);
 #pragma unroll
-      for (int m = 0; m < Sh::MT; ++m)
-        ktf[m][s] = input_frag(ktc + (d0 + 16 * m + i) * kChunk + 32 * s + 8 * g, 8);
+      for (int m = 0; m < Sh::MT; ++m) ktf[m][s] = eight(ktc + (d0 + 16 * m + i) * kChunk + 32 * s + 8 * g);
     }
-    const f32x4 since = *reinterpret_cast<const f32x4*>(sq.gates.since + w0 + 4 * g);
-    const f32x4 until = *reinterpret_cast<const f32x4*>(sq.gates.until + w0 + 4 * g);
-    const f32x4 beta = *reinterpret_cast<const f32x4*>(sq.gates.beta + w0 + 4 * g);
-    const float total = sq.gates.since[kChunk - 1];
-    if (!ENDS && states) put_state(states + (bh * d.chunks + c) * dk * dv, dv);
+    total = sq.gates.since[kChunk - 1];
+  };
+  const Squares<T>* sqs = squares + bh * d.chunks;
+  if (first < last) {
+    fetch_rows(first);
+    fetch_m(sqs[first]);
+    fetch_rest(sqs[first], first);
+  }
+  for (int c = first; c < last; ++c) {
+    const int64_t t0 = (int64_t)c * kChunk;
+    const int live = (int)min(length - t0, (int64_t)kChunk), next = min(c + 1, last - 1);
+    if (!ENDS && states) put_state(states + (bh * d.chunks + c) * dk * wide, wide);
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
 #pragma unroll
@@ -271,7 +318,7 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
       for (int n = 0; n < 2; ++n) {
         const Frag<NV> st = plane_frag<NV>(St + (c0 + 16 * n + i) * kPitch + 32 * s + 8 * g, kState);
         mma(R[0][n], kf[s], st);
-        if (!ENDS) mma(O[0][n], qf[s], st);
+        if (!ENDS) mma(O[0][n], qf[s], first_of<NO>(st));
       }
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
@@ -280,7 +327,7 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
       O[0][n] *= d.r.scale * since;
       put4<NV>(Rt + (c0 + 16 * n + i) * kRow + w0 + 4 * g, kSamples, beta * R[0][n]);
     }
-    if (c + 1 < last) fetch(c + 1);
+    fetch_rows(next);
     __syncthreads();
     clear(X);
 #pragma unroll
@@ -292,15 +339,16 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
     for (int n = 0; n < 2; ++n) {
       const f32x4 x = R[0][n] - X[0][n], u = beta * x;
       const int to = (c0 + 16 * n + i) * kRow + w0 + 4 * g;
-      if (!ENDS) put4<NV>(Ut + to, kSamples, u);
+      if (!ENDS) put4<NO>(Ut + to, kSamples, u);
       put4<NV>(Ht + to, kSamples, until * u);
       if (!ENDS && xs)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int t = w0 + 4 * g + e, col = e0 + c0 + 16 * n + i;
-          if (t < live && col < dv) xs[((b * d.r.T + t0 + t) * d.r.heads + h) * dv + col] = x[e];
+          if (t < live && col < dv) xs[((b * d.r.T + t0 + t) * d.r.heads + h) * wide + col] = x[e];
         }
     }
+    fetch_m(sqs[next]);
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
@@ -314,12 +362,15 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
 #pragma unroll
         for (int m = 0; m < Sh::MT; ++m) mma(S[m][n], ktf[m][s], u);
       }
+    if (!ENDS) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+          mma(O[0][n], pf[s], plane_frag<NO>(Ut + (c0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples));
+    }
+    fetch_rest(sqs[next], next);
     if (ENDS) continue;
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-        mma(O[0][n], pf[s], plane_frag<NV>(Ut + (c0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples));
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -352,7 +403,7 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_join_kernel(Delta d, Cut cu
   const int dk = (int)d.r.dk, dv = (int)d.r.dv, wide = dv + dk;
   const int64_t heads = d.r.B * d.r.heads, bh = blockIdx.x % heads, b = bh / d.r.heads;
   const int col = (int)(blockIdx.x / heads) * 16 + (threadIdx.x & 15);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int chunks = (int)((live_of(d, b) + kChunk - 1) / kChunk);
   const int live = min((chunks + cut.each - 1) / cut.each, cut.segs);   // segments with samples
   f32x4 S[kTiles];
@@ -532,16 +583,57 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_steps_kernel(Delta d, T* o,
         if (e < here) o[((b * d.r.T + t) * d.r.heads + h) * dv + col + e] = from_float<T>(0.0f);
 }
 
+template <typename T>
+__global__ __launch_bounds__(kDeltaBlock) void delta_pad_kernel(const T* from, int64_t s0, int64_t s1, int64_t s2,
+                                                              int64_t T_, int64_t heads, int width, int wide,
+                                                              int64_t n, T* to) {
+  for (int64_t at = (int64_t)blockIdx.x * kDeltaBlock + threadIdx.x; at < n; at += (int64_t)gridDim.x * kDeltaBlock) {
+    const int64_t row = at / wide, token = row / heads, b = token / T_;
+    const int col = (int)(at - row * wide);
+    to[at] = col < width ? from[b * s0 + (token - b * T_) * s1 + (row - token * heads) * s2 + col] : (T)0.0f;
+  }
+}
+
 // Sample by sample where there are so few of them.
 bool steps(const cpab_delta_rule& r, bool keep) { return r.T <= (keep ? 0 : 16); }
 
 }  // namespace
 
+hipError_t launch_delta_pad(int dtype, const void* from, const int64_t strides[3], int64_t B, int64_t T,
+                            int64_t heads, int64_t width, void* to, hipStream_t st) {
+  const int wide = (int)((width + 7) / 8 * 8);
+  const int64_t n = B * T * heads * wide;
+  if (n == 0) return hipSuccess;
+  const unsigned blocks = (unsigned)std::min<int64_t>((n + kDeltaBlock - 1) / kDeltaBlock, 1 << 16);
+  const auto run = [&](auto t) {
+    typedef decltype(t) V;
+    delta_pad_kernel<V><<<blocks, kDeltaBlock, 0, st>>>((const V*)from, strides[0], strides[1], strides[2], T, heads,
+                                                        (int)width, wide, n, (V*)to);
+  };
+  dtype == CPAB_F32 ? run(0.0f) : run(bf16());
+  return hipGetLastError();
+}
+
+hipError_t pad_keys(Delta* d, void* room, hipStream_t st) {
+  cpab_delta_rule& r = d->r;
+  if (r.dk % 8 == 0) return hipSuccess;
+  char* second = static_cast<char*>(room) + padded_keys(r) / 2;
+  hipError_t e = launch_delta_pad(r.dtype, r.q, r.q_strides, r.B, r.T, r.key_heads, r.dk, room, st);
+  if (e == hipSuccess) e = launch_delta_pad(r.dtype, r.k, r.k_strides, r.B, r.T, r.key_heads, r.dk, second, st);
+  r.q = room, r.k = second;
+  for (int64_t* s : {r.q_strides, r.k_strides}) {
+    s[2] = d->read;
+    s[1] = r.key_heads * d->read;
+    s[0] = r.T * s[1];
+  }
+  return e;
+}
+
 hipError_t launch_delta_squares(const Delta& d, void* squares, void* kt, void* qt, hipStream_t st) {
   with_key(d, [&](auto t, auto dp) {
     typedef decltype(t) T;
     constexpr int DP = decltype(dp)::value;
-    constexpr int kRoom = std::max<int>(4 * 2 * kChunk * (kChunk + 4), DP * kRow * (int)sizeof(T));
+    constexpr int kRoom = std::max<int>(4 * kChunk * (2 * (kChunk + 4) + 20), DP * kRow * (int)sizeof(T));
     const unsigned blocks = (unsigned)(d.r.B * d.r.heads * d.chunks);
     if (qt)
       delta_squares_kernel<T, DP, true><<<blocks, kDeltaBlock, kRoom, st>>>(d, (Squares<T>*)squares, (T*)kt, (T*)qt);
@@ -577,8 +669,8 @@ Kept kept_of(const Delta& d, const Cut& cut) {
   const int64_t heads = d.r.B * d.r.heads;
   Kept k;
   k.states = 0;
-  k.xs = heads * d.chunks * d.r.dk * d.r.dv;
-  k.ends = k.xs + heads * d.r.T * d.r.dv;
+  k.xs = heads * d.chunks * d.r.dk * wide_of(d.r);
+  k.ends = k.xs + heads * d.r.T * wide_of(d.r);
   k.all = k.ends + (cut.segs > 1 ? heads * cut.segs * d.r.dk * (d.r.dv + d.r.dk) : 0);
   return k;
 }
@@ -591,7 +683,7 @@ namespace {
 
 // The forward's workspace (bytes).
 struct Room {
-  int64_t squares, kt, starts, ends, all;
+  int64_t squares, kt, starts, ends, keys, all;
 };
 Room room_of(const Delta& d, const Cut& cut, bool keep) {
   const int64_t heads = d.r.B * d.r.heads;
@@ -601,7 +693,8 @@ Room room_of(const Delta& d, const Cut& cut, bool keep) {
   w.kt = next(heads * d.chunks * squares_bytes(d.r.dtype));
   w.starts = w.kt + next(d.r.B * d.r.key_heads * d.chunks * turned_bytes(d.r));
   w.ends = w.starts + (cut.segs > 1 ? next(heads * cut.segs * d.r.dk * d.r.dv * 4) : 0);
-  w.all = w.ends + (cut.segs > 1 && !keep ? next(heads * cut.segs * d.r.dk * (d.r.dv + d.r.dk) * 4) : 0);
+  w.keys = w.ends + (cut.segs > 1 && !keep ? next(heads * cut.segs * d.r.dk * (d.r.dv + d.r.dk) * 4) : 0);
+  w.all = w.keys + padded_keys(d.r);
   return w;
 }
 
@@ -615,7 +708,7 @@ int64_t delta_rule_workspace(const cpab_delta_rule& r, bool keep, bool backward)
 
 hipError_t launch_delta_rule_forward(const cpab_delta_rule& r, void* o, float* h, float* kept,
                                      void* workspace, hipStream_t st) {
-  const Delta d = delta_of(r);
+  Delta d = delta_of(r);
   const int64_t heads = r.B * r.heads;
   if (steps(r, kept != nullptr)) {
     const unsigned blocks = (unsigned)(heads * ((r.dv + 63) / 64));
@@ -631,17 +724,18 @@ hipError_t launch_delta_rule_forward(const cpab_delta_rule& r, void* o, float* h
   char* room = static_cast<char*>(workspace);
   float* starts = reinterpret_cast<float*>(room + w.starts);
   float* ends = kept ? kept + k.ends : reinterpret_cast<float*>(room + w.ends);
-  hipError_t e = launch_delta_squares(d, room + w.squares, room + w.kt, nullptr, st);
+  hipError_t e = pad_keys(&d, room + w.keys, st);
+  if (e == hipSuccess) e = launch_delta_squares(d, room + w.squares, room + w.kt, nullptr, st);
   if (e != hipSuccess) return e;
   with_key(d, [&](auto t, auto dp) {
     typedef decltype(t) T;
-    constexpr int DP = decltype(dp)::value, NV = Parts<T>::kValue;
+    constexpr int DP = decltype(dp)::value, NV = Parts<T>::kValue, NO = Parts<T>::kOut;
     const Squares<T>* squares = reinterpret_cast<const Squares<T>*>(room + w.squares);
     const T* kt = reinterpret_cast<const T*>(room + w.kt);
     const auto run = [&](auto width, auto only_ends, int segs) {
       constexpr int E = decltype(width)::value;
       constexpr bool ENDS = decltype(only_ends)::value;
-      constexpr int kRoom = 2 * NV * E * (DP + 8 + 3 * kRow);
+      constexpr int kRoom = 2 * E * (NV * (DP + 8) + (2 * NV + NO) * kRow);
       static LdsAllowed allowed;
       e = allow_lds(reinterpret_cast<const void*>(delta_chain_kernel<T, DP, E, ENDS>), kRoom, allowed);
       if (e != hipSuccess) return;

@@ -28,14 +28,14 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
   bf16* Bt = St + NV * kState;          // beta dU, [E][64]
   bf16* Zt = Bt + NV * kSamples;        // - exp(G) Z
   bf16* Ot = Zt + NV * kSamples;        // dO, as the input that it is
-  bf16* Gt = Ot + NI * kSamples;        // scale exp(G) dO, of this chunk and the next in turn
-  const int dk = (int)d.r.dk, dv = (int)d.r.dv;
+  bf16* Gt = Ot + NI * kSamples;        // scale exp(G) dO
+  const int dk = (int)d.r.dk, dv = (int)d.r.dv, wide = (dv + 7) / 8 * 8;
   const int64_t heads = d.r.B * d.r.heads;
   const Where at = where(heads, cut.segs, (dv + E - 1) / E);
   if (!at.in) return;
   const int64_t bh = at.bh, b = bh / d.r.heads;
   const int h = (int)(bh - b * d.r.heads), kh = h / d.group, e0 = at.block * E;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int64_t length = live_of(d, b);
   const T* k = static_cast<const T*>(d.r.k) + b * d.r.k_strides[0] + kh * d.r.k_strides[2];
   const int64_t ks = d.r.k_strides[1];
@@ -57,7 +57,7 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
         const int row = d0 + 16 * m + 4 * g + e, col = e0 + s0 + 16 * n + i;
         S[m][n][e] = start && row < dk && col < dv ? start[(int64_t)row * dv + col] : 0.0f;
       }
-  const auto put_state = [&](float* to) {
+  const auto put_state = [&](float* to, int pitch) {
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
 #pragma unroll
@@ -65,53 +65,72 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int row = d0 + 16 * m + 4 * g + e, col = e0 + s0 + 16 * n + i;
-          if (row < dk && col < dv) to[(int64_t)row * dv + col] = S[m][n][e];
+          if (row < dk && col < dv) to[row * pitch + col] = S[m][n][e];
         }
   };
-  Frag<NI> kf[kSteps];
-  f32x4 of[2];
-  const auto fetch = [&](int c) {
-    const int64_t t0 = (int64_t)c * kChunk;
-    const int live = (int)min(length - t0, (int64_t)kChunk), row = w0 + i;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int col = 32 * s + 8 * g;
-      kf[s] = input_frag(k + (t0 + row) * ks + col, row < live ? dk - col : 0);
-    }
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int t = w0 + 4 * g + e, col = e0 + c0 + 16 * n + i;
-        of[n][e] = grad_o && t < live && col < dv
-                       ? to_float(grad_o[((b * d.r.T + t0 + t) * d.r.heads + h) * dv + col]) : 0.0f;
-      }
-  };
-  if (first < last) fetch(last - 1);
-  for (int c = last - 1; c >= first; --c) {
+  // Fetched as in the forward's chain.
+  Frag<NI> kf[kSteps], ktf[Sh::MT][2], qtf[Sh::MT][2];
+  Frag<NV> mf[2], pf[2];
+  f32x4 of[2] = {}, since, until, beta;
+  float total;
+  const auto fetch_k = [&](int c) {
     const int64_t t0 = (int64_t)c * kChunk;
     const int live = (int)min(length - t0, (int64_t)kChunk);
-    const Squares<T>& sq = squares[bh * d.chunks + c];
-    const int64_t turned = ((b * d.r.key_heads + kh) * d.chunks + c) * DP * kChunk;
-    Frag<NV> mf[2], pf[2];
-    Frag<NI> ktf[Sh::MT][2], qtf[Sh::MT][2];
+    const Rows<T> krows{k + t0 * ks, ks, live, d.read};
+    either(live == kChunk && d.read == DP, [&](auto full) {
+      constexpr bool F = decltype(full)::value;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      mf[s] = plane_frag<NV>(&sq.m[0][w0 + i][32 * s + 8 * g], kSquare);
-      pf[s] = plane_frag<NV>(&sq.p[0][w0 + i][32 * s + 8 * g], kSquare);
+      for (int s = 0; s < kSteps; ++s) kf[s] = krows.template at<F>(w0 + i, 32 * s + 8 * g);
+    });
+  };
+  const auto fetch_o = [&](int c) {
+    if (!grad_o) return;
+    const int64_t t0 = (int64_t)c * kChunk;
+    const int live = (int)min(length - t0, (int64_t)kChunk);
+    const Rows<T> orows{grad_o + ((b * d.r.T + t0) * d.r.heads + h) * wide, d.r.heads * wide, live, dv};
+    either(live == kChunk && e0 + E <= dv, [&](auto full) {
+      constexpr bool F = decltype(full)::value;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) of[n][e] = orows.template one<F>(w0 + 4 * g + e, e0 + c0 + 16 * n + i);
+    });
+  };
+  const auto fetch_p = [&](const Squares<T>& sq) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) pf[s] = plane_frag<NV>(&sq.p[0][w0 + i][32 * s + 8 * g], kSquare);
+    until = *reinterpret_cast<const f32x4*>(sq.gates.until + w0 + 4 * g);
+  };
+  const auto fetch_m = [&](const Squares<T>& sq) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) mf[s] = plane_frag<NV>(&sq.m[0][w0 + i][32 * s + 8 * g], kSquare);
+    since = *reinterpret_cast<const f32x4*>(sq.gates.since + w0 + 4 * g);
+    beta = *reinterpret_cast<const f32x4*>(sq.gates.beta + w0 + 4 * g);
+  };
+  const auto fetch_turned = [&](const Squares<T>& sq, int c) {
+    const int64_t turned = ((b * d.r.key_heads + kh) * d.chunks + c) * DP * kChunk;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int m = 0; m < Sh::MT; ++m) {
         const int from = (d0 + 16 * m + i) * kChunk + 32 * s + 8 * g;
-        ktf[m][s] = input_frag(kt + turned + from, 8);
-        qtf[m][s] = input_frag(qt + turned + from, 8);
+        ktf[m][s] = eight(kt + turned + from);
+        qtf[m][s] = eight(qt + turned + from);
       }
-    }
-    const f32x4 since = *reinterpret_cast<const f32x4*>(sq.gates.since + w0 + 4 * g);
-    const f32x4 until = *reinterpret_cast<const f32x4*>(sq.gates.until + w0 + 4 * g);
-    const f32x4 beta = *reinterpret_cast<const f32x4*>(sq.gates.beta + w0 + 4 * g);
-    const float total = sq.gates.since[kChunk - 1];
-    bf16* gt = Gt + (c & 1) * NV * kSamples;
-    if (!ENDS) put_state(dstates + (bh * d.chunks + c) * dk * dv);
+    total = sq.gates.since[kChunk - 1];
+  };
+  const Squares<T>* sqs = squares + bh * d.chunks;
+  if (first < last) {
+    fetch_o(last - 1);
+    fetch_k(last - 1);
+    fetch_p(sqs[last - 1]);
+    fetch_m(sqs[last - 1]);
+    fetch_turned(sqs[last - 1], last - 1);
+  }
+  for (int c = last - 1; c >= first; --c) {
+    const int64_t t0 = (int64_t)c * kChunk;
+    const int live = (int)min(length - t0, (int64_t)kChunk), next = max(c - 1, first);
+    if (!ENDS) put_state(dstates + (bh * d.chunks + c) * dk * wide, wide);
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
 #pragma unroll
@@ -119,9 +138,7 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
         put4<NV>(St + (s0 + 16 * n + i) * kPitch + d0 + 16 * m + 4 * g, kState, S[m][n]);
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      const int to = (c0 + 16 * n + i) * kRow + w0 + 4 * g;
-      put4<NI>(Ot + to, kSamples, of[n]);
-      put4<NV>(gt + to, kSamples, d.r.scale * since * of[n]);
+      put4<NI>(Ot + (c0 + 16 * n + i) * kRow + w0 + 4 * g, kSamples, of[n]);
     }
     __syncthreads();
     f32x4 U[1][2], V[1][2];
@@ -142,7 +159,8 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
 #pragma unroll
     for (int n = 0; n < 2; ++n)
       put4<NV>(Bt + (c0 + 16 * n + i) * kRow + w0 + 4 * g, kSamples, beta * U[0][n]);
-    if (c > first) fetch(c - 1);
+    fetch_k(next);
+    fetch_p(sqs[next]);
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < 2; ++s)
@@ -152,18 +170,22 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       const f32x4 ev = U[0][n] - V[0][n], z = beta * ev;
-      put4<NV>(Zt + (c0 + 16 * n + i) * kRow + w0 + 4 * g, kSamples, -since * z);
+      const int at = (c0 + 16 * n + i) * kRow + w0 + 4 * g;
+      put4<NV>(Zt + at, kSamples, -since * z);
+      put4<NV>(Gt + at, kSamples, d.r.scale * since * of[n]);
       if (ENDS) continue;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int t = w0 + 4 * g + e, col = e0 + c0 + 16 * n + i;
         if (t < live && col < dv) {
-          const int64_t to = ((b * d.r.T + t0 + t) * d.r.heads + h) * dv + col;
-          es[to] = ev[e];
-          if (grad_v) grad_v[to] = from_float<T>(z[e]);
+          const int64_t to = (b * d.r.T + t0 + t) * d.r.heads + h;
+          es[to * wide + col] = ev[e];
+          if (grad_v) grad_v[to * dv + col] = from_float<T>(z[e]);
         }
       }
     }
+    fetch_m(sqs[next]);
+    fetch_o(next);
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
@@ -174,19 +196,20 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
 #pragma unroll
       for (int n = 0; n < Sh::NT; ++n) {
         const int from = (s0 + 16 * n + i) * kRow + 32 * s + 8 * g;
-        const Frag<NV> go = plane_frag<NV>(gt + from, kSamples), z = plane_frag<NV>(Zt + from, kSamples);
+        const Frag<NV> go = plane_frag<NV>(Gt + from, kSamples), z = plane_frag<NV>(Zt + from, kSamples);
 #pragma unroll
         for (int m = 0; m < Sh::MT; ++m) {
           mma(S[m][n], qtf[m][s], go);
           mma(S[m][n], ktf[m][s], z);
         }
       }
+    fetch_turned(sqs[next], next);
   }
   if (ENDS) {
-    put_state(adds + (bh * cut.segs + at.seg) * dk * dv);
+    put_state(adds + (bh * cut.segs + at.seg) * dk * dv, dv);
     return;
   }
-  if (grad_h0 && at.seg == 0) put_state(grad_h0 + bh * dk * dv);
+  if (grad_h0 && at.seg == 0) put_state(grad_h0 + bh * dk * dv, dv);
   if (grad_v) {
     const int64_t rest = max(length, (int64_t)first * kChunk), stop = min((int64_t)(first + cut.each) * kChunk, d.r.T);
     for (int64_t n = rest * E + threadIdx.x; n < stop * E; n += 8 * E) {
@@ -206,18 +229,10 @@ __device__ __forceinline__ void put_gate(const Delta& d, void* p, int64_t at, fl
     static_cast<bf16*>(p)[at] = from_float<bf16>(v);
 }
 
-// Four neighbours of a row, zeros beyond `left`.
-template <typename T>
-__device__ __forceinline__ f32x4 quad(const T* p, int left) {
-  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (left >= 4) {
-    float w[4];
-    load<4>(p, w);
-    return f32x4{w[0], w[1], w[2], w[3]};
-  }
+// The first `left` of four values, zeros behind them.
+__device__ __forceinline__ f32x4 edge(f32x4 v, int left) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (e < left) v[e] = to_float(p[e]);
+  for (int e = 0; e < 4; ++e) v[e] = e < left ? v[e] : 0.0f;
   return v;
 }
 
@@ -257,8 +272,8 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
   const int c = blockIdx.x % d.chunks;
   const int64_t rest = blockIdx.x / d.chunks, b = rest / d.r.key_heads;
   const int kh = (int)(rest - b * d.r.key_heads);
-  const int dk = (int)d.r.dk, dv = (int)d.r.dv;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int dk = (int)d.r.dk, dv = (int)d.r.dv, wide = (dv + 7) / 8 * 8;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int w0 = 16 * (wave & 3), half = wave >> 2;   // samples; columns of DP and of 64
   const int d0 = half * (DP / 2), j0 = half * 32;
   const int64_t t0 = (int64_t)c * kChunk;
@@ -266,7 +281,7 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
   const int rows = (int)min(d.r.T - t0, (int64_t)kChunk);   // that there are
   const T* k = static_cast<const T*>(d.r.k) + b * d.r.k_strides[0] + t0 * d.r.k_strides[1] + kh * d.r.k_strides[2];
   const T* q = static_cast<const T*>(d.r.q) + b * d.r.q_strides[0] + t0 * d.r.q_strides[1] + kh * d.r.q_strides[2];
-  const int64_t ks = d.r.k_strides[1], qs_ = d.r.q_strides[1];
+  const Rows<T> krows{k, d.r.k_strides[1], live, d.read}, qrows{q, d.r.q_strides[1], live, d.read};
   const int64_t turned = ((b * d.r.key_heads + kh) * d.chunks + c) * DP * kChunk;
   f32x4 dQ[1][NT], dK[1][NT];
   clear(dQ);
@@ -297,8 +312,8 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
       betas[t] = sq.gates.beta[t];
       dbeta[t] = 0.0f;
     }
-    const float* state = states + (bh * d.chunks + c) * dk * dv;
-    const float* dstate = dstates + (bh * d.chunks + c) * dk * dv;
+    const float* state = states + (bh * d.chunks + c) * dk * wide;
+    const float* dstate = dstates + (bh * d.chunks + c) * dk * wide;
     f32x4 qs[1][NT], k1[1][NT], k2[1][NT], P[1][2], ZU[1][2];
     clear(qs);
     clear(k1);
@@ -306,14 +321,18 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
     clear(P);
     clear(ZU);
     float dot = 0.0f;
+    const int64_t token = (b * d.r.T + t0) * d.r.heads + h, across = d.r.heads * wide;
+    const Rows<T> orows{grad_o + token * wide, across, live, wide};
+    // what the library wrote itself has no value beyond dv in rows of whole eights
+    const Rows<float> srows{state, wide, dk, dv}, lrows{dstate, wide, dk, dv};
+    const Rows<float> xrows{xs + token * wide, across, live, dv}, erows{es + token * wide, across, live, dv};
     __syncthreads();
+#pragma unroll 1
     for (int e0 = 0; e0 < dv; e0 += kWide) {
 #pragma unroll 2
       for (int at = threadIdx.x; at < DP * (kWide / 4); at += kPartsBlock) {
         const int row = at / (kWide / 4), col = at % (kWide / 4) * 4;
-        const int left = row < dk ? dv - e0 - col : 0;
-        const int64_t from = (int64_t)row * dv + e0 + col;
-        const f32x4 s = quad(state + from, left), l = quad(dstate + from, left);
+        const f32x4 s = edge(srows.four(row, e0 + col), dv - e0 - col), l = edge(lrows.four(row, e0 + col), dv - e0 - col);
         put4<NV>(S + row * kWidePitch + col, Room::kState, s);
         put4<NV>(L + row * kWidePitch + col, Room::kState, l);
 #pragma unroll
@@ -322,9 +341,7 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
       static_assert(kChunk * (kWide / 4) == kPartsBlock, "a quad of X to a lane");
       {
         const int t = threadIdx.x / (kWide / 4), col = threadIdx.x % (kWide / 4) * 4;
-        const int left = t < live ? dv - e0 - col : 0;
-        const int64_t from = ((b * d.r.T + t0 + t) * d.r.heads + h) * dv + e0 + col;
-        const f32x4 x = quad(xs + from, left), ev = quad(es + from, left);
+        const f32x4 x = edge(xrows.four(t, e0 + col), dv - e0 - col), ev = edge(erows.four(t, e0 + col), dv - e0 - col);
         put4<NV>(U + t * kWidePitch + col, Room::kSamples, betas[t] * x);
         float part = x[0] * ev[0];
 #pragma unroll
@@ -335,11 +352,12 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
         if (col == 0) dbeta[t] += part;
       }
       // this wave's own samples of dO and Z
-      const int row = w0 + i, col = 8 * g, left = row < live ? dv - e0 - col : 0;
-      const int64_t from = ((b * d.r.T + t0 + row) * d.r.heads + h) * dv + e0 + col;
-      const Frag<NI> of = input_frag(grad_o + from, grad_o ? left : 0);
+      const int row = w0 + i, col = 8 * g;
+      Frag<NI> of = {};
+      if (grad_o) of = orows.template at<false>(row, e0 + col);
       float z[8];
-      const f32x4 z0 = quad(es + from, left), z1 = quad(es + from + 4, left - 4);
+      const f32x4 z0 = edge(erows.four(row, e0 + col), dv - e0 - col);
+      const f32x4 z1 = edge(erows.four(row, e0 + col + 4), dv - e0 - col - 4);
 #pragma unroll
       for (int e = 0; e < 4; ++e) z[e] = betas[row] * z0[e], z[4 + e] = betas[row] * z1[e];
       const Frag<NV> zf = frag_of<NV>(z);
@@ -367,12 +385,11 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
     clear(qk);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      const int col = 32 * s + 8 * g, row = w0 + i, left = row < live ? dk - col : 0;
-      const Frag<NI> ak = input_frag(k + row * ks + col, left), aq = input_frag(q + row * qs_ + col, left);
+      const int col = 32 * s + 8 * g;
+      const Frag<NI> ak = krows.template at<false>(w0 + i, col), aq = qrows.template at<false>(w0 + i, col);
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const int other = j0 + 16 * n + i;
-        const Frag<NI> bk = input_frag(k + other * ks + col, other < live ? dk - col : 0);
+        const Frag<NI> bk = krows.template at<false>(j0 + 16 * n + i, col);
         mma(kk[0][n], ak, bk);
         mma(qk[0][n], aq, bk);
       }
@@ -386,8 +403,7 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int col = d0 + 16 * n + i;
-        const bool in = row < live && col < dk;
-        const float qv = in ? to_float(q[row * qs_ + col]) : 0.0f, kv = in ? to_float(k[row * ks + col]) : 0.0f;
+        const float qv = qrows.template one<false>(row, col), kv = krows.template one<false>(row, col);
         const float a = ss * qs[0][n][e], z = since * k2[0][n][e], u = until * k1[0][n][e];
         from = fmaf(qv, a, from);
         from = fmaf(-kv, z, from);
@@ -443,7 +459,7 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int64_t at = turned + (d0 + 16 * n + i) * kChunk + 32 * s + 8 * g;
-        const Frag<NI> kf = input_frag(kt + at, 8), qf = input_frag(qt + at, 8);
+        const Frag<NI> kf = eight(kt + at), qf = eight(qt + at);
         mma(dQ[0][n], wf, kf);
         mma(dK[0][n], wt, qf);
         mma(dK[0][n], yf, kf);
@@ -497,7 +513,7 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
 
 // The backward's workspace (bytes).
 struct Space {
-  int64_t squares, kt, qt, dstates, es, adds, starts, all;
+  int64_t squares, kt, qt, dstates, es, adds, starts, keys, grads, all;
 };
 Space space_of(const Delta& d, const Cut& cut) {
   const int64_t heads = d.r.B * d.r.heads, turned = d.r.B * d.r.key_heads * d.chunks * turned_bytes(d.r);
@@ -507,11 +523,13 @@ Space space_of(const Delta& d, const Cut& cut) {
   w.kt = next(heads * d.chunks * squares_bytes(d.r.dtype));
   w.qt = w.kt + next(turned);
   w.dstates = w.qt + next(turned);
-  w.es = w.dstates + next(heads * d.chunks * d.r.dk * d.r.dv * 4);
-  w.adds = w.es + next(heads * d.r.T * d.r.dv * 4);
+  w.es = w.dstates + next(heads * d.chunks * d.r.dk * wide_of(d.r) * 4);
+  w.adds = w.es + next(heads * d.r.T * wide_of(d.r) * 4);
   const int64_t segments = cut.segs > 1 ? next(heads * cut.segs * d.r.dk * d.r.dv * 4) : 0;
   w.starts = w.adds + segments;
-  w.all = w.starts + segments;
+  w.keys = w.starts + segments;
+  w.grads = w.keys + next(padded_keys(d.r));
+  w.all = w.grads + (d.r.dv % 8 ? heads * d.r.T * wide_of(d.r) * (d.r.dtype == CPAB_F32 ? 4 : 2) : 0);
   return w;
 }
 
@@ -523,7 +541,7 @@ hipError_t launch_delta_rule_backward(const cpab_delta_rule& r, const float* kep
                                       const float* grad_h, void* grad_q, void* grad_k, void* grad_v,
                                       void* grad_decay, void* grad_beta, float* grad_h0,
                                       void* workspace, hipStream_t st) {
-  const Delta d = delta_of(r);
+  Delta d = delta_of(r);
   const Cut cut = cut_of(d);
   const Space w = space_of(d, cut);
   const Kept k = kept_of(d, cut);
@@ -534,7 +552,13 @@ hipError_t launch_delta_rule_backward(const cpab_delta_rule& r, const float* kep
   float* adds = reinterpret_cast<float*>(room + w.adds);
   float* starts = reinterpret_cast<float*>(room + w.starts);
   hipError_t e = hipSuccess;
-  if (d.chunks > 0) e = launch_delta_squares(d, room + w.squares, room + w.kt, room + w.qt, st);
+  if (r.dv % 8 != 0 && grad_o) {
+    const int64_t strides[3] = {r.T * r.heads * r.dv, r.heads * r.dv, r.dv};
+    e = launch_delta_pad(r.dtype, grad_o, strides, r.B, r.T, r.heads, r.dv, room + w.grads, st);
+    grad_o = room + w.grads;
+  }
+  if (e == hipSuccess && d.chunks > 0) e = pad_keys(&d, room + w.keys, st);
+  if (e == hipSuccess && d.chunks > 0) e = launch_delta_squares(d, room + w.squares, room + w.kt, room + w.qt, st);
   if (e != hipSuccess) return e;
   with_key(d, [&](auto t, auto dp) {
     typedef decltype(t) T;
@@ -544,7 +568,7 @@ hipError_t launch_delta_rule_backward(const cpab_delta_rule& r, const float* kep
     const auto run = [&](auto width, auto only_ends) {
       constexpr int E = decltype(width)::value;
       constexpr bool ENDS = decltype(only_ends)::value;
-      constexpr int kRoom = 2 * E * (NV * (DP + 8) + (4 * NV + NI) * kRow);
+      constexpr int kRoom = 2 * E * (NV * (DP + 8) + (3 * NV + NI) * kRow);
       static LdsAllowed allowed;
       e = allow_lds(reinterpret_cast<const void*>(delta_back_chain_kernel<T, DP, E, ENDS>), kRoom, allowed);
       if (e != hipSuccess) return;

@@ -240,8 +240,8 @@ variable_list delta_rule(const Tensor& q, const Tensor& k, const Tensor& v, cons
            ", heads, dk] (the heads of v, " + text(H) + ", a multiple of q's and k's) of v's type and " +
            "device, got " + shape_of(*t) + " " + dtype_of(*t));
   const int64_t dk = q.size(3), dv = v.size(3);
-  if (dk > CPAB_DELTA_MOST_KEY)
-    fail("gated_delta_rule: dk must be at most " + text(CPAB_DELTA_MOST_KEY) + ", got " + text(dk));
+  if (dk < 1 || dk > CPAB_DELTA_MOST_KEY)
+    fail("gated_delta_rule: dk must be from 1 to " + text(CPAB_DELTA_MOST_KEY) + ", got " + text(dk));
   for (const auto& [t, name] : {std::make_pair(&decay, "decay"), std::make_pair(&beta, "beta")})
     if (t->device() != v.device() || !has_type(*t) || t->scalar_type() != decay.scalar_type() ||
         t->dim() != 3 || t->size(0) != B || t->size(1) != T || t->size(2) != H)
@@ -257,7 +257,7 @@ variable_list delta_rule(const Tensor& q, const Tensor& k, const Tensor& v, cons
        (lengths.scalar_type() != at::kInt && lengths.scalar_type() != at::kLong)))
     fail("gated_delta_rule: lengths must be int32 or int64 [" + text(B) + "] on v's device, got " +
          shape_of(lengths) + " " + dtype_of(lengths));
-  const double scale = scale_ ? *scale_ : dk > 0 ? 1.0 / std::sqrt((double)dk) : 1.0;
+  const double scale = scale_ ? *scale_ : 1.0 / std::sqrt((double)dk);
   const bool keep = any_grad({q, k, v, decay, beta, h0});
   py::gil_scoped_release nogil;
   const Maybe dense = lengths.defined() ? Maybe(lengths.contiguous()) : Maybe();
