@@ -101,7 +101,8 @@ int check_delta_sizes(const cpab_delta_rule* rule) {
                 (long long)r.heads, (long long)r.key_heads);
   // a launch's workgroups: a chunk or 32 columns of a head each
   const double heads = (double)r.B * (double)r.heads, blocks = (double)kMaxCount / 256;
-  if (r.heads > kMaxHeads || r.B > kMaxCount || r.T > kMaxCount - 64 || r.dv > kMaxCount / 64 ||
+  if (r.heads * (r.dv + 8) > CPAB_DELTA_MOST_STRIDE || r.key_heads * (r.dk + 8) > CPAB_DELTA_MOST_STRIDE ||
+      r.heads > kMaxHeads || r.B > kMaxCount || r.T > kMaxCount - 64 || r.dv > kMaxCount / 64 ||
       heads * ((double)r.T / 64 + 1) > blocks || heads * ((double)r.dv / 32 + 1) > blocks ||
       heads * (double)(r.T + 64) * (double)(r.dv + r.dk) >= (double)kMaxValues ||
       heads * ((double)r.T / 64 + 2) * (double)r.dk * (double)r.dv >= (double)kMaxValues)
@@ -128,6 +129,12 @@ int check_delta(const cpab_delta_rule* rule) {
   CPAB_TRY(check_strides("q", r.q_strides, 3));
   CPAB_TRY(check_strides("k", r.k_strides, 3));
   CPAB_TRY(check_strides("v", r.v_strides, 3));
+  // a chunk's offsets have 32 bits
+  if (r.T > 1)
+    for (const int64_t* strides : {r.q_strides, r.k_strides, r.v_strides})
+      if (strides[1] > CPAB_DELTA_MOST_STRIDE)
+        return fail(CPAB_ERR_INVALID, "samples %lld values apart are too far, at most %d", (long long)strides[1],
+                    CPAB_DELTA_MOST_STRIDE);
   CPAB_TRY(check_strides("decay", r.decay_strides, 3));
   return check_strides("beta", r.beta_strides, 3);
 }

@@ -129,52 +129,71 @@ __device__ __forceinline__ Frag<3> eight(const float* p) {
   return frag_of<3>(v);
 }
 
-// Rows of an input: `live` of them, `width` values each, a multiple of 8, zeros beyond.
-// Where there is nothing to read the first row is: without a branch between the lanes loads
-// are not waited for one by one.  FULL: every row and column is there.
+// 8 neighbours of a row as they come from memory, and what they are as an operand.  What is
+// fetched ahead stays as it came: anything done with it would wait for it.
+template <typename T>
+struct Raw {
+  typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+  static constexpr int kWords = sizeof(T) / 2;   // of 16 bytes
+  U4 v[kWords];
+  __device__ __forceinline__ void fetch(const T* p) {
+    typedef U4 __attribute__((aligned(2))) Unit;
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) v[k] = reinterpret_cast<const Unit*>(p)[k];
+  }
+  __device__ __forceinline__ void keep(bool in) {
+#pragma unroll
+    for (int k = 0; k < kWords; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[k][e] = in ? v[k][e] : 0u;
+  }
+  __device__ __forceinline__ Frag<Parts<T>::kInput> frag() const {
+    if constexpr (sizeof(T) == 2) {
+      return Frag<1>{{__builtin_bit_cast(bf16x8, v[0])}};
+    } else {
+      float f[8];
+      __builtin_memcpy(f, v, 32);
+      return frag_of<3>(f);
+    }
+  }
+};
+
+// Rows of an input: `live` of them, `width` values each, zeros beyond.  The last row or
+// column is read again where there is nothing to read: without a branch between the lanes
+// loads are not waited for one by one.  Offsets within a chunk have 32 bits
+// (CPAB_DELTA_MOST_STRIDE), beside a base that is the whole wave's.
 template <typename T>
 struct Rows {
   const T* p;
-  int64_t stride;
-  int live, width;
-  template <bool FULL>
+  int stride, live, width;
+  template <int N>
+  __device__ __forceinline__ const T* place(int row, int col) const {   // of N neighbours; the width a multiple of N
+    const uint32_t at = (uint32_t)(min(row, live - 1) * stride + min(col, width - N)) * (uint32_t)sizeof(T);
+    return reinterpret_cast<const T*>(reinterpret_cast<const char*>(p) + at);
+  }
+  __device__ __forceinline__ bool in(int row, int col) const { return row < live && col < width; }
   __device__ __forceinline__ Frag<Parts<T>::kInput> at(int row, int col) const {
-    if (FULL) return eight(p + row * stride + col);
-    const bool in = row < live && col < width;
-    Frag<Parts<T>::kInput> f = eight(p + (in ? row * stride + col : 0));
-#pragma unroll
-    for (int k = 0; k < Parts<T>::kInput; ++k) {
-      typedef uint32_t U4 __attribute__((ext_vector_type(4)));
-      U4 v = __builtin_bit_cast(U4, f.p[k]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = in ? v[e] : 0u;
-      f.p[k] = __builtin_bit_cast(bf16x8, v);
-    }
-    return f;
+    Raw<T> r;
+    r.fetch(place<8>(row, col));
+    r.keep(in(row, col));
+    return r.frag();
   }
-  template <bool FULL>
   __device__ __forceinline__ float one(int row, int col) const {
-    if (FULL) return to_float(p[row * stride + col]);
-    const bool in = row < live && col < width;
-    const float v = to_float(p[in ? row * stride + col : 0]);
-    return in ? v : 0.0f;
+    const float v = to_float(*place<1>(row, col));
+    return in(row, col) ? v : 0.0f;
   }
-  // Four neighbours; the width a multiple of 4.
   __device__ __forceinline__ f32x4 four(int row, int col) const {
-    const bool in = row < live && col < width;
     float w[4];
-    load<4>(p + (in ? row * stride + col : 0), w);
+    load<4>(place<4>(row, col), w);
     f32x4 v;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = in ? w[e] : 0.0f;
+    for (int e = 0; e < 4; ++e) v[e] = in(row, col) ? w[e] : 0.0f;
     return v;
   }
 };
-// f(FULL) as a constant.
-template <typename F>
-__device__ __forceinline__ void either(bool full, F f) {
-  full ? f(std::true_type()) : f(std::false_type());
-}
+// Makes a lane's number new to the compiler, which else computes every address that a loop
+// takes from it once, before the loop, and has no registers for them.
+__device__ __forceinline__ void renew(int& a, int& b) { asm volatile("" : "+v"(a), "+v"(b)); }
 
 // Operands in planes of 16-bit parts, in LDS or the workspace: 8 neighbours to a lane.
 template <int N>

@@ -101,9 +101,9 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, Squ
     out.gates.beta[t] = beta;
   }
   const Rows<T> krows{static_cast<const T*>(d.r.k) + b * d.r.k_strides[0] + t0 * d.r.k_strides[1] + kh * d.r.k_strides[2],
-                      d.r.k_strides[1], live, d.read};
+                      (int)d.r.k_strides[1], live, d.read};
   const Rows<T> qrows{static_cast<const T*>(d.r.q) + b * d.r.q_strides[0] + t0 * d.r.q_strides[1] + kh * d.r.q_strides[2],
-                      d.r.q_strides[1], live, d.read};
+                      (int)d.r.q_strides[1], live, d.read};
   if (h % d.group == 0) {
     const int64_t at = ((b * d.r.key_heads + kh) * d.chunks + c) * DP * kChunk;
     put_turned<DP>(reinterpret_cast<T*>(room), krows, kt + at);
@@ -113,20 +113,17 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, Squ
   f32x4 kk[1][4], qk[1][4];
   clear(kk);
   clear(qk);
-  either(live == kChunk && d.read == DP, [&](auto full) {
-    constexpr bool F = decltype(full)::value;
 #pragma unroll
-    for (int s = 0; s < DP / 32; ++s) {
-      const int col = 32 * s + 8 * g;
-      const Frag<NI> ak = krows.template at<F>(16 * wave + i, col), aq = qrows.template at<F>(16 * wave + i, col);
+  for (int s = 0; s < DP / 32; ++s) {
+    const int col = 32 * s + 8 * g;
+    const Frag<NI> ak = krows.at(16 * wave + i, col), aq = qrows.at(16 * wave + i, col);
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const Frag<NI> bk = krows.template at<F>(16 * n + i, col);
-        mma(kk[0][n], ak, bk);
-        mma(qk[0][n], aq, bk);
-      }
+    for (int n = 0; n < 4; ++n) {
+      const Frag<NI> bk = krows.at(16 * n + i, col);
+      mma(kk[0][n], ak, bk);
+      mma(qk[0][n], aq, bk);
     }
-  });
+  }
   __syncthreads();
   float* Ab = room;                   // A beta
   float* A = Ab + kChunk * kPitch;
@@ -216,12 +213,13 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
   const int h = (int)(bh - b * d.r.heads), kh = h / d.group;
   const bool unit = ENDS && at.block >= blocks_v;
   const int e0 = (unit ? at.block - blocks_v : at.block) * E, width = unit ? dk : dv;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  int i = lane & 15, g = lane >> 4;
   const int64_t length = live_of(d, b);
   const T* q = static_cast<const T*>(d.r.q) + b * d.r.q_strides[0] + kh * d.r.q_strides[2];
   const T* k = static_cast<const T*>(d.r.k) + b * d.r.k_strides[0] + kh * d.r.k_strides[2];
   const T* v = static_cast<const T*>(d.r.v) + b * d.r.v_strides[0] + h * d.r.v_strides[2];
-  const int64_t ks = d.r.k_strides[1], qs = d.r.q_strides[1], vs = d.r.v_strides[1];
+  const int ks = (int)d.r.k_strides[1], qs = (int)d.r.q_strides[1], vs = (int)d.r.v_strides[1];
   const int d0 = wave % Sh::WD * Sh::MT * 16, s0 = wave / Sh::WD * Sh::NT * 16;   // this wave's part of the state
   const int w0 = 16 * (wave & 3), c0 = wave / 4 * 32;                             // and of a chunk's samples
   f32x4 S[Sh::MT][Sh::NT];
@@ -237,7 +235,7 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
         S[m][n][e] = unit ? (row == col ? 1.0f : 0.0f)
                           : start && row < dk && col < dv ? start[(int64_t)row * dv + col] : 0.0f;
       }
-  const auto put_state = [&](float* to, int64_t pitch) {
+  const auto put_state = [&](float* to, int pitch) {
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
 #pragma unroll
@@ -252,28 +250,44 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
   const int first = at.seg * cut.each, last = min(first + cut.each, chunks);
   // What a chunk's products take is fetched as soon as the chunk before is done with the
   // registers: memory has most of a chunk's time to answer.
-  Frag<NI> kf[kSteps], qf[kSteps], ktf[Sh::MT][2];
+  Raw<T> kf[kSteps], qf[kSteps], ktf[Sh::MT][2];
   Frag<NV> mf[2];
   Frag<NO> pf[2];
-  float vf[2][4];
+  T vf[2][4];
   f32x4 since, until, beta;
   float total;
-  const auto fetch_rows = [&](int c) {
+  const auto rows_of = [&](int c, auto f) {
     const int64_t t0 = (int64_t)c * kChunk;
     const int live = (int)min(length - t0, (int64_t)kChunk);
-    const Rows<T> krows{k + t0 * ks, ks, live, d.read}, qrows{q + t0 * qs, qs, live, d.read};
-    const Rows<T> vrows{v + t0 * vs, vs, live, unit ? 0 : dv};
-    either(live == kChunk && d.read == DP && e0 + E <= dv && !unit, [&](auto full) {
-      constexpr bool F = decltype(full)::value;
+    f(Rows<T>{k + t0 * ks, ks, live, d.read}, Rows<T>{q + t0 * qs, qs, live, d.read},
+      Rows<T>{v + t0 * vs, vs, live, dv});
+  };
+  const auto fetch_rows = [&](int c) {
+    rows_of(c, [&](const Rows<T>& krows, const Rows<T>& qrows, const Rows<T>& vrows) {
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        kf[s] = krows.template at<F>(w0 + i, 32 * s + 8 * g);
-        if (!ENDS) qf[s] = qrows.template at<F>(w0 + i, 32 * s + 8 * g);
+        kf[s].fetch(krows.template place<8>(w0 + i, 32 * s + 8 * g));
+        if (!ENDS) qf[s].fetch(qrows.template place<8>(w0 + i, 32 * s + 8 * g));
       }
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) vf[n][e] = vrows.template one<F>(w0 + 4 * g + e, e0 + c0 + 16 * n + i);
+        for (int e = 0; e < 4; ++e) vf[n][e] = *vrows.template place<1>(w0 + 4 * g + e, e0 + c0 + 16 * n + i);
+    });
+  };
+  const auto mask_rows = [&](int c) {   // zeros where there was nothing to fetch
+    rows_of(c, [&](const Rows<T>& krows, const Rows<T>& qrows, const Rows<T>& vrows) {
+      if (krows.live == kChunk && d.read == DP && e0 + E <= dv && !unit) return;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        kf[s].keep(krows.in(w0 + i, 32 * s + 8 * g));
+        if (!ENDS) qf[s].keep(qrows.in(w0 + i, 32 * s + 8 * g));
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          vf[n][e] = !unit && vrows.in(w0 + 4 * g + e, e0 + c0 + 16 * n + i) ? vf[n][e] : (T)0.0f;
     });
   };
   const auto fetch_m = [&](const Squares<T>& sq) {
@@ -289,7 +303,7 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
     for (int s = 0; s < 2; ++s) {
       if (!ENDS) pf[s] = plane_frag<NO>(&sq.p[0][w0 + i][32 * s + 8 * g], kSquare);
 #pragma unroll
-      for (int m = 0; m < Sh::MT; ++m) ktf[m][s] = eight(ktc + (d0 + 16 * m + i) * kChunk + 32 * s + 8 * g);
+      for (int m = 0; m < Sh::MT; ++m) ktf[m][s].fetch(ktc + (d0 + 16 * m + i) * kChunk + 32 * s + 8 * g);
     }
     total = sq.gates.since[kChunk - 1];
   };
@@ -302,39 +316,63 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
   for (int c = first; c < last; ++c) {
     const int64_t t0 = (int64_t)c * kChunk;
     const int live = (int)min(length - t0, (int64_t)kChunk), next = min(c + 1, last - 1);
+    float* xc = xs ? xs + ((b * d.r.T + t0) * d.r.heads + h) * wide : nullptr;
+    T* oc = o + ((b * d.r.T + t0) * d.r.heads + h) * dv;
+    renew(i, g);
     if (!ENDS && states) put_state(states + (bh * d.chunks + c) * dk * wide, wide);
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
 #pragma unroll
       for (int n = 0; n < Sh::NT; ++n)
         put4<NV>(St + (s0 + 16 * n + i) * kPitch + d0 + 16 * m + 4 * g, kState, S[m][n]);
+    mask_rows(c);
     __syncthreads();
     f32x4 R[1][2], O[1][2], X[1][2];
     clear(R);
     clear(O);
+    {
+      Frag<NV> st[2][2];   // this step's and the next's: LDS answers while the matrix unit works
+      const auto read = [&](int s) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
+        for (int n = 0; n < 2; ++n)
+          st[s & 1][n] = plane_frag<NV>(St + (c0 + 16 * n + i) * kPitch + 32 * s + 8 * g, kState);
+      };
+      read(0);
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const Frag<NV> st = plane_frag<NV>(St + (c0 + 16 * n + i) * kPitch + 32 * s + 8 * g, kState);
-        mma(R[0][n], kf[s], st);
-        if (!ENDS) mma(O[0][n], qf[s], first_of<NO>(st));
+      for (int s = 0; s < kSteps; ++s) {
+        if (s + 1 < kSteps) read(s + 1);
+        const Frag<NI> kv = kf[s].frag();
+#pragma unroll
+        for (int n = 0; n < 2; ++n) mma(R[0][n], kv, st[s & 1][n]);
+        if (!ENDS) {
+          const Frag<NI> qv = qf[s].frag();
+#pragma unroll
+          for (int n = 0; n < 2; ++n) mma(O[0][n], qv, first_of<NO>(st[s & 1][n]));
+        }
       }
+    }
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) R[0][n][e] = fmaf(-since[e], R[0][n][e], vf[n][e]);
+      for (int e = 0; e < 4; ++e) R[0][n][e] = fmaf(-since[e], R[0][n][e], to_float(vf[n][e]));
       O[0][n] *= d.r.scale * since;
       put4<NV>(Rt + (c0 + 16 * n + i) * kRow + w0 + 4 * g, kSamples, beta * R[0][n]);
     }
     fetch_rows(next);
     __syncthreads();
     clear(X);
+    {
+      Frag<NV> rt[2][2];
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-        mma(X[0][n], mf[s], plane_frag<NV>(Rt + (c0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples));
+        for (int n = 0; n < 2; ++n)
+          rt[s][n] = plane_frag<NV>(Rt + (c0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) mma(X[0][n], mf[s], rt[s][n]);
+    }
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       const f32x4 x = R[0][n] - X[0][n], u = beta * x;
@@ -345,7 +383,7 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int t = w0 + 4 * g + e, col = e0 + c0 + 16 * n + i;
-          if (t < live && col < dv) xs[((b * d.r.T + t0 + t) * d.r.heads + h) * wide + col] = x[e];
+          if (t < live && col < dv) xc[t * (int)d.r.heads * wide + col] = x[e];
         }
     }
     fetch_m(sqs[next]);
@@ -360,7 +398,7 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
       for (int n = 0; n < Sh::NT; ++n) {
         const Frag<NV> u = plane_frag<NV>(Ht + (s0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples);
 #pragma unroll
-        for (int m = 0; m < Sh::MT; ++m) mma(S[m][n], ktf[m][s], u);
+        for (int m = 0; m < Sh::MT; ++m) mma(S[m][n], ktf[m][s].frag(), u);
       }
     if (!ENDS) {
 #pragma unroll
@@ -376,7 +414,7 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int t = w0 + 4 * g + e, col = e0 + c0 + 16 * n + i;
-        if (t < live && col < dv) o[((b * d.r.T + t0 + t) * d.r.heads + h) * dv + col] = from_float<T>(O[0][n][e]);
+        if (t < live && col < dv) oc[t * (int)d.r.heads * dv + col] = from_float<T>(O[0][n][e]);
       }
   }
   if (ENDS) {

@@ -35,10 +35,11 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
   if (!at.in) return;
   const int64_t bh = at.bh, b = bh / d.r.heads;
   const int h = (int)(bh - b * d.r.heads), kh = h / d.group, e0 = at.block * E;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  int i = lane & 15, g = lane >> 4;
   const int64_t length = live_of(d, b);
   const T* k = static_cast<const T*>(d.r.k) + b * d.r.k_strides[0] + kh * d.r.k_strides[2];
-  const int64_t ks = d.r.k_strides[1];
+  const int ks = (int)d.r.k_strides[1];
   const int d0 = wave % Sh::WD * Sh::MT * 16, s0 = wave / Sh::WD * Sh::NT * 16;
   const int w0 = 16 * (wave & 3), c0 = wave / 4 * 32;
   const int chunks = (int)((length + kChunk - 1) / kChunk);
@@ -69,32 +70,43 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
         }
   };
   // Fetched as in the forward's chain.
-  Frag<NI> kf[kSteps], ktf[Sh::MT][2], qtf[Sh::MT][2];
+  Raw<T> kf[kSteps], ktf[Sh::MT][2], qtf[Sh::MT][2];
   Frag<NV> mf[2], pf[2];
-  f32x4 of[2] = {}, since, until, beta;
+  T of[2][4] = {};
+  f32x4 since, until, beta;
   float total;
-  const auto fetch_k = [&](int c) {
+  const auto krows_of = [&](int c) {
     const int64_t t0 = (int64_t)c * kChunk;
-    const int live = (int)min(length - t0, (int64_t)kChunk);
-    const Rows<T> krows{k + t0 * ks, ks, live, d.read};
-    either(live == kChunk && d.read == DP, [&](auto full) {
-      constexpr bool F = decltype(full)::value;
+    return Rows<T>{k + t0 * ks, ks, (int)min(length - t0, (int64_t)kChunk), d.read};
+  };
+  const auto orows_of = [&](int c) {
+    const int64_t t0 = (int64_t)c * kChunk;
+    return Rows<T>{grad_o + ((b * d.r.T + t0) * d.r.heads + h) * wide, (int)d.r.heads * wide,
+                   (int)min(length - t0, (int64_t)kChunk), dv};
+  };
+  const auto fetch_k = [&](int c) {
+    const Rows<T> krows = krows_of(c);
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) kf[s] = krows.template at<F>(w0 + i, 32 * s + 8 * g);
-    });
+    for (int s = 0; s < kSteps; ++s) kf[s].fetch(krows.template place<8>(w0 + i, 32 * s + 8 * g));
   };
   const auto fetch_o = [&](int c) {
     if (!grad_o) return;
-    const int64_t t0 = (int64_t)c * kChunk;
-    const int live = (int)min(length - t0, (int64_t)kChunk);
-    const Rows<T> orows{grad_o + ((b * d.r.T + t0) * d.r.heads + h) * wide, d.r.heads * wide, live, dv};
-    either(live == kChunk && e0 + E <= dv, [&](auto full) {
-      constexpr bool F = decltype(full)::value;
+    const Rows<T> orows = orows_of(c);
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) of[n][e] = orows.template one<F>(w0 + 4 * g + e, e0 + c0 + 16 * n + i);
-    });
+      for (int e = 0; e < 4; ++e) of[n][e] = *orows.template place<1>(w0 + 4 * g + e, e0 + c0 + 16 * n + i);
+  };
+  const auto mask_rows = [&](int c) {   // zeros where there was nothing to fetch
+    const Rows<T> krows = krows_of(c), orows = orows_of(c);
+    if (krows.live == kChunk && d.read == DP && e0 + E <= dv) return;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) kf[s].keep(krows.in(w0 + i, 32 * s + 8 * g));
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        of[n][e] = orows.in(w0 + 4 * g + e, e0 + c0 + 16 * n + i) ? of[n][e] : (T)0.0f;
   };
   const auto fetch_p = [&](const Squares<T>& sq) {
 #pragma unroll
@@ -114,8 +126,8 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
 #pragma unroll
       for (int m = 0; m < Sh::MT; ++m) {
         const int from = (d0 + 16 * m + i) * kChunk + 32 * s + 8 * g;
-        ktf[m][s] = eight(kt + turned + from);
-        qtf[m][s] = eight(qt + turned + from);
+        ktf[m][s].fetch(kt + turned + from);
+        qtf[m][s].fetch(qt + turned + from);
       }
     total = sq.gates.since[kChunk - 1];
   };
@@ -130,62 +142,94 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
   for (int c = last - 1; c >= first; --c) {
     const int64_t t0 = (int64_t)c * kChunk;
     const int live = (int)min(length - t0, (int64_t)kChunk), next = max(c - 1, first);
+    float* ec = es + ((b * d.r.T + t0) * d.r.heads + h) * wide;
+    T* vc = grad_v ? grad_v + ((b * d.r.T + t0) * d.r.heads + h) * dv : nullptr;
+    renew(i, g);
     if (!ENDS) put_state(dstates + (bh * d.chunks + c) * dk * wide, wide);
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
 #pragma unroll
       for (int n = 0; n < Sh::NT; ++n)
         put4<NV>(St + (s0 + 16 * n + i) * kPitch + d0 + 16 * m + 4 * g, kState, S[m][n]);
+    mask_rows(c);
+    f32x4 ov[2];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      put4<NI>(Ot + (c0 + 16 * n + i) * kRow + w0 + 4 * g, kSamples, of[n]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ov[n][e] = to_float(of[n][e]);
+      put4<NI>(Ot + (c0 + 16 * n + i) * kRow + w0 + 4 * g, kSamples, ov[n]);
     }
+    fetch_o(next);
     __syncthreads();
     f32x4 U[1][2], V[1][2];
     clear(U);
     clear(V);
+    {
+      Frag<NV> st[2][2];
+      const auto read = [&](int s) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
+        for (int n = 0; n < 2; ++n)
+          st[s & 1][n] = plane_frag<NV>(St + (c0 + 16 * n + i) * kPitch + 32 * s + 8 * g, kState);
+      };
+      read(0);
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-        mma(U[0][n], kf[s], plane_frag<NV>(St + (c0 + 16 * n + i) * kPitch + 32 * s + 8 * g, kState));
+      for (int s = 0; s < kSteps; ++s) {
+        if (s + 1 < kSteps) read(s + 1);
+        const Frag<NI> kv = kf[s].frag();
 #pragma unroll
-    for (int n = 0; n < 2; ++n) U[0][n] *= until;
+        for (int n = 0; n < 2; ++n) mma(U[0][n], kv, st[s & 1][n]);
+      }
+    }
+    {
+      Frag<NI> ot[2][2];
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-        mma(U[0][n], pf[s], plane_frag<NI>(Ot + (c0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples));
+        for (int n = 0; n < 2; ++n)
+          ot[s][n] = plane_frag<NI>(Ot + (c0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) U[0][n] *= until;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) mma(U[0][n], pf[s], ot[s][n]);
+    }
 #pragma unroll
     for (int n = 0; n < 2; ++n)
       put4<NV>(Bt + (c0 + 16 * n + i) * kRow + w0 + 4 * g, kSamples, beta * U[0][n]);
     fetch_k(next);
     fetch_p(sqs[next]);
     __syncthreads();
+    {
+      Frag<NV> bt[2][2];
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-        mma(V[0][n], mf[s], plane_frag<NV>(Bt + (c0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples));
+        for (int n = 0; n < 2; ++n)
+          bt[s][n] = plane_frag<NV>(Bt + (c0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) mma(V[0][n], mf[s], bt[s][n]);
+    }
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       const f32x4 ev = U[0][n] - V[0][n], z = beta * ev;
       const int at = (c0 + 16 * n + i) * kRow + w0 + 4 * g;
       put4<NV>(Zt + at, kSamples, -since * z);
-      put4<NV>(Gt + at, kSamples, d.r.scale * since * of[n]);
+      put4<NV>(Gt + at, kSamples, d.r.scale * since * ov[n]);
       if (ENDS) continue;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int t = w0 + 4 * g + e, col = e0 + c0 + 16 * n + i;
         if (t < live && col < dv) {
-          const int64_t to = (b * d.r.T + t0 + t) * d.r.heads + h;
-          es[to * wide + col] = ev[e];
-          if (grad_v) grad_v[to * dv + col] = from_float<T>(z[e]);
+          const int to = t * (int)d.r.heads;
+          ec[to * wide + col] = ev[e];
+          if (vc) vc[to * dv + col] = from_float<T>(z[e]);
         }
       }
     }
     fetch_m(sqs[next]);
-    fetch_o(next);
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
@@ -199,8 +243,8 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
         const Frag<NV> go = plane_frag<NV>(Gt + from, kSamples), z = plane_frag<NV>(Zt + from, kSamples);
 #pragma unroll
         for (int m = 0; m < Sh::MT; ++m) {
-          mma(S[m][n], qtf[m][s], go);
-          mma(S[m][n], ktf[m][s], z);
+          mma(S[m][n], qtf[m][s].frag(), go);
+          mma(S[m][n], ktf[m][s].frag(), z);
         }
       }
     fetch_turned(sqs[next], next);
@@ -273,7 +317,8 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
   const int64_t rest = blockIdx.x / d.chunks, b = rest / d.r.key_heads;
   const int kh = (int)(rest - b * d.r.key_heads);
   const int dk = (int)d.r.dk, dv = (int)d.r.dv, wide = (dv + 7) / 8 * 8;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  int i = lane & 15, g = lane >> 4;
   const int w0 = 16 * (wave & 3), half = wave >> 2;   // samples; columns of DP and of 64
   const int d0 = half * (DP / 2), j0 = half * 32;
   const int64_t t0 = (int64_t)c * kChunk;
@@ -281,7 +326,7 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
   const int rows = (int)min(d.r.T - t0, (int64_t)kChunk);   // that there are
   const T* k = static_cast<const T*>(d.r.k) + b * d.r.k_strides[0] + t0 * d.r.k_strides[1] + kh * d.r.k_strides[2];
   const T* q = static_cast<const T*>(d.r.q) + b * d.r.q_strides[0] + t0 * d.r.q_strides[1] + kh * d.r.q_strides[2];
-  const Rows<T> krows{k, d.r.k_strides[1], live, d.read}, qrows{q, d.r.q_strides[1], live, d.read};
+  const Rows<T> krows{k, (int)d.r.k_strides[1], live, d.read}, qrows{q, (int)d.r.q_strides[1], live, d.read};
   const int64_t turned = ((b * d.r.key_heads + kh) * d.chunks + c) * DP * kChunk;
   f32x4 dQ[1][NT], dK[1][NT];
   clear(dQ);
@@ -321,11 +366,12 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
     clear(P);
     clear(ZU);
     float dot = 0.0f;
-    const int64_t token = (b * d.r.T + t0) * d.r.heads + h, across = d.r.heads * wide;
+    const int64_t token = (b * d.r.T + t0) * d.r.heads + h;
+    const int across = (int)d.r.heads * wide;
     const Rows<T> orows{grad_o + token * wide, across, live, wide};
-    // what the library wrote itself has no value beyond dv in rows of whole eights
-    const Rows<float> srows{state, wide, dk, dv}, lrows{dstate, wide, dk, dv};
-    const Rows<float> xrows{xs + token * wide, across, live, dv}, erows{es + token * wide, across, live, dv};
+    // rows of whole eights, in which the library itself wrote nothing beyond dv
+    const Rows<float> srows{state, wide, dk, wide}, lrows{dstate, wide, dk, wide};
+    const Rows<float> xrows{xs + token * wide, across, live, wide}, erows{es + token * wide, across, live, wide};
     __syncthreads();
 #pragma unroll 1
     for (int e0 = 0; e0 < dv; e0 += kWide) {
@@ -351,10 +397,11 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
         part += __shfl_xor(part, 4);
         if (col == 0) dbeta[t] += part;
       }
+      renew(i, g);
       // this wave's own samples of dO and Z
       const int row = w0 + i, col = 8 * g;
       Frag<NI> of = {};
-      if (grad_o) of = orows.template at<false>(row, e0 + col);
+      if (grad_o) of = orows.at(row, e0 + col);
       float z[8];
       const f32x4 z0 = edge(erows.four(row, e0 + col), dv - e0 - col);
       const f32x4 z1 = edge(erows.four(row, e0 + col + 4), dv - e0 - col - 4);
@@ -379,6 +426,7 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
       }
       __syncthreads();
     }
+    renew(i, g);
     // the products that M and P were made of
     f32x4 kk[1][2], qk[1][2];
     clear(kk);
@@ -386,14 +434,15 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const int col = 32 * s + 8 * g;
-      const Frag<NI> ak = krows.template at<false>(w0 + i, col), aq = qrows.template at<false>(w0 + i, col);
+      const Frag<NI> ak = krows.at(w0 + i, col), aq = qrows.at(w0 + i, col);
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const Frag<NI> bk = krows.template at<false>(j0 + 16 * n + i, col);
+        const Frag<NI> bk = krows.at(j0 + 16 * n + i, col);
         mma(kk[0][n], ak, bk);
         mma(qk[0][n], aq, bk);
       }
     }
+    renew(i, g);
     // what passes a sample's decay from the state before the chunk, and to the one after
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -403,7 +452,7 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int col = d0 + 16 * n + i;
-        const float qv = qrows.template one<false>(row, col), kv = krows.template one<false>(row, col);
+        const float qv = qrows.one(row, col), kv = krows.one(row, col);
         const float a = ss * qs[0][n][e], z = since * k2[0][n][e], u = until * k1[0][n][e];
         from = fmaf(qv, a, from);
         from = fmaf(-kv, z, from);

@@ -177,7 +177,11 @@ struct DeltaRule : torch::autograd::Function<DeltaRule> {
                                const Tensor& decay_, const Tensor& beta_, const Maybe& maybe_h0,
                                const Maybe& maybe_lengths, double scale, bool keep) {
     const c10::OptionalDeviceGuard guard(v_.device());
-    const Tensor q = heads_of(q_), k = heads_of(k_), v = heads_of(v_), decay = decay_.detach(),
+    const auto near = [](const Tensor& t) {   // samples no further apart than the kernels reach
+      const Tensor n = heads_of(t);
+      return n.size(1) <= 1 || n.stride(1) <= CPAB_DELTA_MOST_STRIDE ? n : n.contiguous();
+    };
+    const Tensor q = near(q_), k = near(k_), v = near(v_), decay = decay_.detach(),
                  beta = beta_.detach(), h0_ = of(maybe_h0), lengths = of(maybe_lengths);
     const Tensor h0 = h0_.defined() ? plain(h0_) : Tensor();
     const cpab_delta_rule r = describe(q, k, v, decay, beta, h0, lengths, scale);

@@ -517,8 +517,8 @@ int cpab_qk_norm_backward(const cpab_qk_norm* norm, const void* const* grads,
  * for t < lengths[b] (T where lengths is NULL; clamped to [0, T]); behind a row's end o is
  * 0, the state stays, and nothing of the inputs is used.  Each `heads / key_heads`
  * neighbouring heads share a query and a key.  q, k: [B, T, key_heads, dk] and v
- * [B, T, heads, dv] of dtype, at strides over B, T and the heads (elements), their last
- * dimension contiguous; decay, beta: [B, T, heads] of gate_dtype at three strides; o
+ * [B, T, heads, dv] of dtype, at strides over B, T and the heads (elements), that over T at
+ * most CPAB_DELTA_MOST_STRIDE, their last dimension contiguous; decay, beta: [B, T, heads] of gate_dtype at three strides; o
  * [B, T, heads, dv] contiguous; h [B, heads, dk, dv] float32, the state after each row's
  * last sample.  dk is from 1 to CPAB_DELTA_MOST_KEY.  decay is the decay's logarithm, at most
  * 0; below -128 it counts as -128, whose exponential is 0.
@@ -526,6 +526,7 @@ int cpab_qk_norm_backward(const cpab_qk_norm* norm, const void* const* grads,
  * takes.  workspace: cpab_delta_rule_workspace_size(...) bytes, 16-byte aligned.  The
  * description lies in host memory and is read before the call returns. */
 #define CPAB_DELTA_MOST_KEY 128
+#define CPAB_DELTA_MOST_STRIDE 4194304
 typedef struct {
   int dtype, gate_dtype, lengths64;
   int64_t B, T, heads, key_heads, dk, dv;
