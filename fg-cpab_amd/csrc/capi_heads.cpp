@@ -96,6 +96,7 @@ int check_delta_sizes(const cpab_delta_rule* rule) {
                 (long long)r.dk, (long long)r.dv);
   if (r.dk < 1 || r.dk > CPAB_DELTA_MOST_KEY)
     return fail(CPAB_ERR_INVALID, "dk must be from 1 to %d, got %lld", CPAB_DELTA_MOST_KEY, (long long)r.dk);
+  if (r.dv < 1) return fail(CPAB_ERR_INVALID, "dv must be at least 1, got %lld", (long long)r.dv);
   if (r.heads > 0 && (r.key_heads < 1 || r.heads % r.key_heads != 0))
     return fail(CPAB_ERR_INVALID, "heads must be a multiple of key_heads, got %lld and %lld",
                 (long long)r.heads, (long long)r.key_heads);
@@ -120,7 +121,7 @@ int check_delta(const cpab_delta_rule* rule) {
   if (!std::isfinite(r.scale)) return fail(CPAB_ERR_INVALID, "scale must be finite");
   if (any_delta(r) && r.T > 0) {
     CPAB_REQUIRE(r.q); CPAB_REQUIRE(r.k);
-    if (r.dv > 0) CPAB_REQUIRE(r.v);
+    CPAB_REQUIRE(r.v);
     CPAB_REQUIRE(r.decay); CPAB_REQUIRE(r.beta);
   }
   CPAB_ALIGNED(r.q, size_of(r.dtype)); CPAB_ALIGNED(r.k, size_of(r.dtype)); CPAB_ALIGNED(r.v, size_of(r.dtype));
@@ -191,7 +192,7 @@ int cpab_delta_rule_forward(const cpab_delta_rule* rule, void* o, float* h, floa
                             void* workspace, int64_t workspace_bytes, void* stream) {
   CPAB_TRY(check_delta(rule));
   const cpab_delta_rule& r = *rule;
-  if (!any_delta(r) || r.dv == 0) return CPAB_OK;
+  if (!any_delta(r)) return CPAB_OK;
   if (r.T > 0) CPAB_REQUIRE(o);
   CPAB_REQUIRE(h);
   CPAB_ALIGNED(o, size_of(r.dtype)); CPAB_ALIGNED(h, 4); CPAB_ALIGNED(kept, 4);
@@ -207,7 +208,7 @@ int cpab_delta_rule_backward(const cpab_delta_rule* rule, const float* kept, con
   CPAB_TRY(check_delta(rule));
   const cpab_delta_rule& r = *rule;
   if (!any_delta(r)) return CPAB_OK;
-  if (r.T > 0 && r.dv > 0) CPAB_REQUIRE(kept);
+  if (r.T > 0) CPAB_REQUIRE(kept);
   CPAB_ALIGNED(kept, 4); CPAB_ALIGNED(grad_h, 4); CPAB_ALIGNED(grad_h0, 4);
   CPAB_ALIGNED(grad_o, size_of(r.dtype)); CPAB_ALIGNED(grad_q, size_of(r.dtype));
   CPAB_ALIGNED(grad_k, size_of(r.dtype)); CPAB_ALIGNED(grad_v, size_of(r.dtype));

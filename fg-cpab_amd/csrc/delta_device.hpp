@@ -158,6 +158,20 @@ struct Raw {
   }
 };
 
+// One value, likewise.
+template <typename T>
+struct RawOne {
+  uint32_t v;
+  __device__ __forceinline__ void fetch(const T* p) {
+    if constexpr (sizeof(T) == 2)
+      v = *reinterpret_cast<const uint16_t*>(p);
+    else
+      v = *reinterpret_cast<const uint32_t*>(p);
+  }
+  __device__ __forceinline__ void keep(bool in) { v = in ? v : 0u; }
+  __device__ __forceinline__ float value() const { return __uint_as_float(sizeof(T) == 2 ? v << 16 : v); }
+};
+
 // Rows of an input: `live` of them, `width` values each, zeros beyond.  The last row or
 // column is read again where there is nothing to read: without a branch between the lanes
 // loads are not waited for one by one.  Offsets within a chunk have 32 bits
@@ -194,6 +208,11 @@ struct Rows {
 // Makes a lane's number new to the compiler, which else computes every address that a loop
 // takes from it once, before the loop, and has no registers for them.
 __device__ __forceinline__ void renew(int& a, int& b) { asm volatile("" : "+v"(a), "+v"(b)); }
+
+// Waits for what has been loaded.  Before a loop whose registers begin with loads: the
+// compiler, which does not tell its first round from the others, would wait in each of them,
+// for everything that is fetched ahead.
+__device__ __forceinline__ void loaded() { __builtin_amdgcn_s_waitcnt(0x0f70); }   // vmcnt(0) alone
 
 // Operands in planes of 16-bit parts, in LDS or the workspace: 8 neighbours to a lane.
 template <int N>

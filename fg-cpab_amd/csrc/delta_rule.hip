@@ -253,7 +253,7 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
   Raw<T> kf[kSteps], qf[kSteps], ktf[Sh::MT][2];
   Frag<NV> mf[2];
   Frag<NO> pf[2];
-  T vf[2][4];
+  RawOne<T> vf[2][4];
   f32x4 since, until, beta;
   float total;
   const auto rows_of = [&](int c, auto f) {
@@ -272,7 +272,7 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) vf[n][e] = *vrows.template place<1>(w0 + 4 * g + e, e0 + c0 + 16 * n + i);
+        for (int e = 0; e < 4; ++e) vf[n][e].fetch(vrows.template place<1>(w0 + 4 * g + e, e0 + c0 + 16 * n + i));
     });
   };
   const auto mask_rows = [&](int c) {   // zeros where there was nothing to fetch
@@ -287,7 +287,7 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          vf[n][e] = !unit && vrows.in(w0 + 4 * g + e, e0 + c0 + 16 * n + i) ? vf[n][e] : (T)0.0f;
+          vf[n][e].keep(!unit && vrows.in(w0 + 4 * g + e, e0 + c0 + 16 * n + i));
     });
   };
   const auto fetch_m = [&](const Squares<T>& sq) {
@@ -308,6 +308,7 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
     total = sq.gates.since[kChunk - 1];
   };
   const Squares<T>* sqs = squares + bh * d.chunks;
+  loaded();
   if (first < last) {
     fetch_rows(first);
     fetch_m(sqs[first]);
@@ -354,7 +355,7 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) R[0][n][e] = fmaf(-since[e], R[0][n][e], to_float(vf[n][e]));
+      for (int e = 0; e < 4; ++e) R[0][n][e] = fmaf(-since[e], R[0][n][e], vf[n][e].value());
       O[0][n] *= d.r.scale * since;
       put4<NV>(Rt + (c0 + 16 * n + i) * kRow + w0 + 4 * g, kSamples, beta * R[0][n]);
     }

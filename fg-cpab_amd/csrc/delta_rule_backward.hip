@@ -69,10 +69,11 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
           if (row < dk && col < dv) to[row * pitch + col] = S[m][n][e];
         }
   };
-  // Fetched as in the forward's chain.
+  // Fetched as in the forward's chain.  Without grad_o as many bytes of E's place, as zeros.
+  const T* go = grad_o ? grad_o : reinterpret_cast<const T*>(es);
   Raw<T> kf[kSteps], ktf[Sh::MT][2], qtf[Sh::MT][2];
   Frag<NV> mf[2], pf[2];
-  T of[2][4] = {};
+  RawOne<T> of[2][4];
   f32x4 since, until, beta;
   float total;
   const auto krows_of = [&](int c) {
@@ -81,7 +82,7 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
   };
   const auto orows_of = [&](int c) {
     const int64_t t0 = (int64_t)c * kChunk;
-    return Rows<T>{grad_o + ((b * d.r.T + t0) * d.r.heads + h) * wide, (int)d.r.heads * wide,
+    return Rows<T>{go + ((b * d.r.T + t0) * d.r.heads + h) * wide, (int)d.r.heads * wide,
                    (int)min(length - t0, (int64_t)kChunk), dv};
   };
   const auto fetch_k = [&](int c) {
@@ -90,23 +91,22 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
     for (int s = 0; s < kSteps; ++s) kf[s].fetch(krows.template place<8>(w0 + i, 32 * s + 8 * g));
   };
   const auto fetch_o = [&](int c) {
-    if (!grad_o) return;
     const Rows<T> orows = orows_of(c);
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) of[n][e] = *orows.template place<1>(w0 + 4 * g + e, e0 + c0 + 16 * n + i);
+      for (int e = 0; e < 4; ++e) of[n][e].fetch(orows.template place<1>(w0 + 4 * g + e, e0 + c0 + 16 * n + i));
   };
   const auto mask_rows = [&](int c) {   // zeros where there was nothing to fetch
     const Rows<T> krows = krows_of(c), orows = orows_of(c);
-    if (krows.live == kChunk && d.read == DP && e0 + E <= dv) return;
+    if (krows.live == kChunk && d.read == DP && e0 + E <= dv && grad_o) return;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) kf[s].keep(krows.in(w0 + i, 32 * s + 8 * g));
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        of[n][e] = orows.in(w0 + 4 * g + e, e0 + c0 + 16 * n + i) ? of[n][e] : (T)0.0f;
+        of[n][e].keep(grad_o && orows.in(w0 + 4 * g + e, e0 + c0 + 16 * n + i));
   };
   const auto fetch_p = [&](const Squares<T>& sq) {
 #pragma unroll
@@ -132,6 +132,7 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
     total = sq.gates.since[kChunk - 1];
   };
   const Squares<T>* sqs = squares + bh * d.chunks;
+  loaded();
   if (first < last) {
     fetch_o(last - 1);
     fetch_k(last - 1);
@@ -156,7 +157,7 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) ov[n][e] = to_float(of[n][e]);
+      for (int e = 0; e < 4; ++e) ov[n][e] = of[n][e].value();
       put4<NI>(Ot + (c0 + 16 * n + i) * kRow + w0 + 4 * g, kSamples, ov[n]);
     }
     fetch_o(next);
@@ -368,26 +369,57 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
     float dot = 0.0f;
     const int64_t token = (b * d.r.T + t0) * d.r.heads + h;
     const int across = (int)d.r.heads * wide;
-    const Rows<T> orows{grad_o + token * wide, across, live, wide};
+    const Rows<T> orows{(grad_o ? grad_o : reinterpret_cast<const T*>(es)) + token * wide, across, live, wide};
     // rows of whole eights, in which the library itself wrote nothing beyond dv
     const Rows<float> srows{state, wide, dk, wide}, lrows{dstate, wide, dk, wide};
     const Rows<float> xrows{xs + token * wide, across, live, wide}, erows{es + token * wide, across, live, wide};
+    // A block of columns is fetched while the matrix unit has the one before.
+    constexpr int kQuads = (DP * (kWide / 4) + kPartsBlock - 1) / kPartsBlock;
+    static_assert(kChunk * (kWide / 4) == kPartsBlock, "a quad of X to a lane");
+    int tid = threadIdx.x, unused = 0;
+    f32x4 sq4[kQuads], lq4[kQuads], xq, eq, zq[2];
+    Raw<T> oraw;
+    const auto load4 = [](const Rows<float>& r, int row, int col) {
+      float w[4];
+      load<4>(r.template place<4>(row, col), w);
+      return f32x4{w[0], w[1], w[2], w[3]};
+    };
+    const auto fetch = [&](int e0) {
+#pragma unroll
+      for (int n = 0; n < kQuads; ++n) {
+        const int at = tid + n * kPartsBlock, row = at / (kWide / 4), col = at % (kWide / 4) * 4;
+        sq4[n] = load4(srows, row, e0 + col);
+        lq4[n] = load4(lrows, row, e0 + col);
+      }
+      const int t = tid / (kWide / 4), col = tid % (kWide / 4) * 4;
+      xq = load4(xrows, t, e0 + col);
+      eq = load4(erows, t, e0 + col);
+      // this wave's own samples of dO and Z
+      oraw.fetch(orows.template place<8>(w0 + i, e0 + 8 * g));
+      zq[0] = load4(erows, w0 + i, e0 + 8 * g);
+      zq[1] = load4(erows, w0 + i, e0 + 8 * g + 4);
+    };
     __syncthreads();
+    fetch(0);
 #pragma unroll 1
     for (int e0 = 0; e0 < dv; e0 += kWide) {
-#pragma unroll 2
-      for (int at = threadIdx.x; at < DP * (kWide / 4); at += kPartsBlock) {
-        const int row = at / (kWide / 4), col = at % (kWide / 4) * 4;
-        const f32x4 s = edge(srows.four(row, e0 + col), dv - e0 - col), l = edge(lrows.four(row, e0 + col), dv - e0 - col);
-        put4<NV>(S + row * kWidePitch + col, Room::kState, s);
-        put4<NV>(L + row * kWidePitch + col, Room::kState, l);
+      renew(i, g);
+      renew(tid, unused);
+#pragma unroll
+      for (int n = 0; n < kQuads; ++n) {
+        const int at = tid + n * kPartsBlock, row = at / (kWide / 4), col = at % (kWide / 4) * 4;
+        const int left = row < dk ? dv - e0 - col : 0;
+        const f32x4 s = edge(sq4[n], left), l = edge(lq4[n], left);
+        if (DP * (kWide / 4) % kPartsBlock == 0 || at < DP * (kWide / 4)) {
+          put4<NV>(S + row * kWidePitch + col, Room::kState, s);
+          put4<NV>(L + row * kWidePitch + col, Room::kState, l);
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) dot = fmaf(s[e], l[e], dot);
       }
-      static_assert(kChunk * (kWide / 4) == kPartsBlock, "a quad of X to a lane");
       {
-        const int t = threadIdx.x / (kWide / 4), col = threadIdx.x % (kWide / 4) * 4;
-        const f32x4 x = edge(xrows.four(t, e0 + col), dv - e0 - col), ev = edge(erows.four(t, e0 + col), dv - e0 - col);
+        const int t = tid / (kWide / 4), col = tid % (kWide / 4) * 4, left = t < live ? dv - e0 - col : 0;
+        const f32x4 x = edge(xq, left), ev = edge(eq, left);
         put4<NV>(U + t * kWidePitch + col, Room::kSamples, betas[t] * x);
         float part = x[0] * ev[0];
 #pragma unroll
@@ -397,17 +429,15 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
         part += __shfl_xor(part, 4);
         if (col == 0) dbeta[t] += part;
       }
-      renew(i, g);
-      // this wave's own samples of dO and Z
-      const int row = w0 + i, col = 8 * g;
-      Frag<NI> of = {};
-      if (grad_o) of = orows.at(row, e0 + col);
+      const int row = w0 + i, col = 8 * g, left = row < live ? dv - e0 - col : 0;
+      oraw.keep(grad_o && left > 0);
+      const Frag<NI> of = oraw.frag();
       float z[8];
-      const f32x4 z0 = edge(erows.four(row, e0 + col), dv - e0 - col);
-      const f32x4 z1 = edge(erows.four(row, e0 + col + 4), dv - e0 - col - 4);
+      const f32x4 z0 = edge(zq[0], left), z1 = edge(zq[1], left - 4);
 #pragma unroll
       for (int e = 0; e < 4; ++e) z[e] = betas[row] * z0[e], z[4 + e] = betas[row] * z1[e];
       const Frag<NV> zf = frag_of<NV>(z);
+      fetch(min(e0 + kWide, (dv - 1) / kWide * kWide));
       __syncthreads();
       const Frag<NV> uf = plane_frag<NV>(U + row * kWidePitch + col, Room::kSamples);
 #pragma unroll
@@ -631,12 +661,12 @@ hipError_t launch_delta_rule_backward(const cpab_delta_rule& r, const float* kep
         if (r.dv > 32) return run(std::integral_constant<int, 64>(), only_ends);
       run(std::integral_constant<int, 32>(), only_ends);
     };
-    if (r.dv > 0 && cut.segs > 1) {
+    if (cut.segs > 1) {
       both(std::true_type());
       if (e == hipSuccess) e = launch_delta_join(d, cut, false, kept + k.ends, adds, grad_h, starts, st);
       if (e != hipSuccess) return;
     }
-    if (r.dv > 0) both(std::false_type());
+    both(std::false_type());
     if (e != hipSuccess || d.chunks == 0 || !(grad_q || grad_k || grad_decay || grad_beta)) return;
     constexpr int kRoom = PartsRoom<T, DP>::kBytes;
     static LdsAllowed allowed;

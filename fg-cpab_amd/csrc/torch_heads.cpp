@@ -246,6 +246,7 @@ variable_list delta_rule(const Tensor& q, const Tensor& k, const Tensor& v, cons
   const int64_t dk = q.size(3), dv = v.size(3);
   if (dk < 1 || dk > CPAB_DELTA_MOST_KEY)
     fail("gated_delta_rule: dk must be from 1 to " + text(CPAB_DELTA_MOST_KEY) + ", got " + text(dk));
+  if (dv < 1) fail("gated_delta_rule: v has heads of no values");
   for (const auto& [t, name] : {std::make_pair(&decay, "decay"), std::make_pair(&beta, "beta")})
     if (t->device() != v.device() || !has_type(*t) || t->scalar_type() != decay.scalar_type() ||
         t->dim() != 3 || t->size(0) != B || t->size(1) != T || t->size(2) != H)

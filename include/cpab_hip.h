@@ -520,7 +520,7 @@ int cpab_qk_norm_backward(const cpab_qk_norm* norm, const void* const* grads,
  * [B, T, heads, dv] of dtype, at strides over B, T and the heads (elements), that over T at
  * most CPAB_DELTA_MOST_STRIDE, their last dimension contiguous; decay, beta: [B, T, heads] of gate_dtype at three strides; o
  * [B, T, heads, dv] contiguous; h [B, heads, dk, dv] float32, the state after each row's
- * last sample.  dk is from 1 to CPAB_DELTA_MOST_KEY.  decay is the decay's logarithm, at most
+ * last sample.  dk is from 1 to CPAB_DELTA_MOST_KEY, dv at least 1.  decay is the decay's logarithm, at most
  * 0; below -128 it counts as -128, whose exponential is 0.
  * kept: NULL, or cpab_delta_rule_kept(...) floats that the backward of the same sizes
  * takes.  workspace: cpab_delta_rule_workspace_size(...) bytes, 16-byte aligned.  The
