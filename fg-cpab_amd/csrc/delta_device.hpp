@@ -77,23 +77,29 @@ template <int N>
 struct Frag {   // 8 neighbours of the summed index
   bf16x8 p[N];
 };
+// Two values at once, as the conversion takes them.
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 template <int N>
-__device__ __forceinline__ void split(float v, bf16 (&p)[N]) {
+__device__ __forceinline__ void split(float v0, float v1, bf16x2 (&p)[N]) {
 #pragma unroll
   for (int k = 0; k < N; ++k) {
-    p[k] = (bf16)v;
-    v -= (float)p[k];
+    p[k] = __builtin_convertvector(f32x2{v0, v1}, bf16x2);
+    if (k + 1 == N) break;
+    const uint32_t both = __builtin_bit_cast(uint32_t, p[k]);
+    v0 -= __uint_as_float(both << 16);
+    v1 -= __uint_as_float(both & 0xffff0000u);
   }
 }
 template <int N>
 __device__ __forceinline__ Frag<N> frag_of(const float v[8]) {
   Frag<N> f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    bf16 p[N];
-    split<N>(v[e], p);
+  for (int e = 0; e < 8; e += 2) {
+    bf16x2 p[N];
+    split<N>(v[e], v[e + 1], p);
 #pragma unroll
-    for (int k = 0; k < N; ++k) f.p[k][e] = p[k];
+    for (int k = 0; k < N; ++k) f.p[k][e] = p[k][0], f.p[k][e + 1] = p[k][1];
   }
   return f;
 }
@@ -117,18 +123,6 @@ __device__ __forceinline__ Frag<N> first_of(const Frag<M>& f) {
   return r;
 }
 
-// 8 neighbours of an input's row, as they lie in memory.
-__device__ __forceinline__ Frag<1> eight(const bf16* p) {
-  typedef uint32_t U4 __attribute__((ext_vector_type(4)));
-  typedef U4 __attribute__((aligned(2))) Unit;
-  return Frag<1>{{__builtin_bit_cast(bf16x8, (U4)*reinterpret_cast<const Unit*>(p))}};
-}
-__device__ __forceinline__ Frag<3> eight(const float* p) {
-  float v[8];
-  load<8>(p, v);
-  return frag_of<3>(v);
-}
-
 // 8 neighbours of a row as they come from memory, and what they are as an operand.  What is
 // fetched ahead stays as it came: anything done with it would wait for it.
 template <typename T>
@@ -140,6 +134,10 @@ struct Raw {
     typedef U4 __attribute__((aligned(2))) Unit;
 #pragma unroll
     for (int k = 0; k < kWords; ++k) v[k] = reinterpret_cast<const Unit*>(p)[k];
+  }
+  __device__ __forceinline__ void put(T* p) const {   // 16-byte aligned
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) reinterpret_cast<U4*>(p)[k] = v[k];
   }
   __device__ __forceinline__ void keep(bool in) {
 #pragma unroll
@@ -158,20 +156,6 @@ struct Raw {
   }
 };
 
-// One value, likewise.
-template <typename T>
-struct RawOne {
-  uint32_t v;
-  __device__ __forceinline__ void fetch(const T* p) {
-    if constexpr (sizeof(T) == 2)
-      v = *reinterpret_cast<const uint16_t*>(p);
-    else
-      v = *reinterpret_cast<const uint32_t*>(p);
-  }
-  __device__ __forceinline__ void keep(bool in) { v = in ? v : 0u; }
-  __device__ __forceinline__ float value() const { return __uint_as_float(sizeof(T) == 2 ? v << 16 : v); }
-};
-
 // Rows of an input: `live` of them, `width` values each, zeros beyond.  The last row or
 // column is read again where there is nothing to read: without a branch between the lanes
 // loads are not waited for one by one.  Offsets within a chunk have 32 bits
@@ -186,15 +170,14 @@ struct Rows {
     return reinterpret_cast<const T*>(reinterpret_cast<const char*>(p) + at);
   }
   __device__ __forceinline__ bool in(int row, int col) const { return row < live && col < width; }
-  __device__ __forceinline__ Frag<Parts<T>::kInput> at(int row, int col) const {
-    Raw<T> r;
+  __device__ __forceinline__ void fetch(Raw<T>& r, int row, int col) const {
     r.fetch(place<8>(row, col));
     r.keep(in(row, col));
-    return r.frag();
   }
-  __device__ __forceinline__ float one(int row, int col) const {
-    const float v = to_float(*place<1>(row, col));
-    return in(row, col) ? v : 0.0f;
+  __device__ __forceinline__ Frag<Parts<T>::kInput> at(int row, int col) const {
+    Raw<T> r;
+    fetch(r, row, col);
+    return r.frag();
   }
   __device__ __forceinline__ f32x4 four(int row, int col) const {
     float w[4];
@@ -207,7 +190,7 @@ struct Rows {
 };
 // Makes a lane's number new to the compiler, which else computes every address that a loop
 // takes from it once, before the loop, and has no registers for them.
-__device__ __forceinline__ void renew(int& a, int& b) { asm volatile("" : "+v"(a), "+v"(b)); }
+__device__ __forceinline__ void renew(int& a) { asm volatile("" : "+v"(a)); }
 
 // Waits for what has been loaded.  Before a loop whose registers begin with loads: the
 // compiler, which does not tell its first round from the others, would wait in each of them,
@@ -225,16 +208,12 @@ __device__ __forceinline__ Frag<N> plane_frag(const bf16* at, int plane) {
 // Four neighbours of the summed index, as the sums of a product lie in a lane.
 template <int N>
 __device__ __forceinline__ void put4(bf16* at, int plane, const f32x4& v) {
-  bf16x4 out[N];
+  bf16x2 lo[N], hi[N];
+  split<N>(v[0], v[1], lo);
+  split<N>(v[2], v[3], hi);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    bf16 p[N];
-    split<N>(v[e], p);
-#pragma unroll
-    for (int k = 0; k < N; ++k) out[k][e] = p[k];
-  }
-#pragma unroll
-  for (int k = 0; k < N; ++k) *reinterpret_cast<bf16x4*>(at + k * plane) = out[k];
+  for (int k = 0; k < N; ++k)
+    *reinterpret_cast<bf16x4*>(at + k * plane) = bf16x4{lo[k][0], lo[k][1], hi[k][0], hi[k][1]};
 }
 
 template <int MT, int NT>
@@ -245,33 +224,96 @@ __device__ __forceinline__ void clear(f32x4 (&acc)[MT][NT]) {
     for (int c = 0; c < NT; ++c) acc[m][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 }
 
-// How the waves of a workgroup share a state's block of [DP, E]: WD of them over DP.
-template <int DP, int E>
+// A chain's workgroup has 32 columns of a state; its four waves share its [DP, 32], WD of
+// them over DP.
+constexpr int kWide = 32;
+template <int DP>
 struct Shares {
-  static constexpr int W = E / 8, WD = DP / 16 < 4 ? DP / 16 : 4, WE = W / WD;
-  static constexpr int MT = DP / 16 / WD, NT = E / 16 / WE;
+  static constexpr int WD = DP / 16 < 4 ? DP / 16 : 4, WE = 4 / WD;
+  static constexpr int MT = DP / 16 / WD, NT = kWide / 16 / WE;
 };
+
+// The unit matrix, 16 of its columns from 16 n on: A times it is A, as a product's sums lie.
+// One wide load of a row and a product so bring an input to the sums' layout.
+__device__ __forceinline__ Frag<1> unit_frag(int n) {
+  const int at = 16 * n + (threadIdx.x & 15) - 8 * ((threadIdx.x >> 4) & 3);
+  Frag<1> f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f.p[0][e] = (bf16)(e == at ? 1.0f : 0.0f);
+  return f;
+}
+
+// A product's sums, four rows of a column to a lane, as four columns of a row: lane i of 16
+// then has row i mod 4 and columns from i - i mod 4 on.  One wide store in place of four.
+__device__ __forceinline__ float exchanged(float v, bool two) {
+  const int i = __float_as_int(v);
+  return __int_as_float(two ? __builtin_amdgcn_update_dpp(i, i, 0x4e, 0xf, 0xf, true)
+                            : __builtin_amdgcn_update_dpp(i, i, 0xb1, 0xf, 0xf, true));
+}
+__device__ __forceinline__ f32x4 across(f32x4 v) {
+  const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
+#pragma unroll
+  for (int k = 0; k < 4; k += 2) {
+    const float got = exchanged(odd ? v[k] : v[k + 1], false);
+    v[k] = odd ? got : v[k];
+    v[k + 1] = odd ? v[k + 1] : got;
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float got = exchanged(high ? v[k] : v[k + 2], true);
+    v[k] = high ? got : v[k];
+    v[k + 2] = high ? v[k + 2] : got;
+  }
+  return v;
+}
+__device__ __forceinline__ void store4(float* p, const f32x4& v) {
+  const float w[4] = {v[0], v[1], v[2], v[3]};
+  store<4>(p, w);
+}
+// Four neighbours of a row of an output; `left` of them are there.
+template <typename T>
+__device__ __forceinline__ void store_some(T* p, const f32x4& v, int left) {
+  if (left >= 4) {
+    const float w[4] = {v[0], v[1], v[2], v[3]};
+    store<4>(p, w);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) p[e] = from_float<T>(v[e]);
+  }
+}
 
 // ---- workspace -----------------------------------------------------------------
 
-// What the first kernel leaves of a chunk of a head: exp(G_i), exp(G_63 - G_i) and beta;
-// M and P (their transposes for the backward) in planes.
+// What the first kernel leaves lies as the matrix unit's operands do, 8 values to a lane:
+// [tile of 16 rows][32 of the summed index][64 lanes][8], so that a wave reads whole lines
+// (rows of 64 bytes, 16 of them, took the vector memory unit three times as long).  Of a
+// chunk of a head: exp(G_i), exp(G_63 - G_i) and beta; M and P (their transposes for the
+// backward) in planes.
 struct Gates {
   float since[kChunk], until[kChunk], beta[kChunk];
 };
 template <typename T>
 struct Squares {
   Gates gates;
-  bf16 m[Parts<T>::kValue][kChunk][kChunk];
-  bf16 p[Parts<T>::kValue][kChunk][kChunk];
+  bf16 m[Parts<T>::kValue][4][2][64][8];
+  bf16 p[Parts<T>::kValue][4][2][64][8];
 };
 inline int64_t squares_bytes(int dtype) {
   return dtype == CPAB_F32 ? (int64_t)sizeof(Squares<float>) : (int64_t)sizeof(Squares<bf16>);
 }
-// And of a chunk of a key's head: k transposed, and for the backward q too: [DP, 64].
+// And of a chunk of a key's head, zeros beyond its rows and columns: k and q [64, DP], and
+// their transposes [DP, 64].
 inline int key_rows(const cpab_delta_rule& r) { return r.dk <= 32 ? 32 : r.dk <= 64 ? 64 : 128; }
-inline int64_t turned_bytes(const cpab_delta_rule& r) {
-  return (int64_t)key_rows(r) * kChunk * (r.dtype == CPAB_F32 ? 4 : 2);
+template <typename T, int DP>
+struct Keys {
+  typedef T Own[4][DP / 32][64][8];
+  typedef T Turned[DP / 16][2][64][8];
+  Own k, q;
+  Turned kt, qt;   // qt for the backward
+};
+inline int64_t keys_bytes(const cpab_delta_rule& r) {
+  return 4 * (int64_t)key_rows(r) * kChunk * (r.dtype == CPAB_F32 ? 4 : 2);
 }
 
 // f(T(), DP) as types and constants.
@@ -296,11 +338,14 @@ inline int64_t wide_of(const cpab_delta_rule& r) { return (r.dv + 7) / 8 * 8; }
 hipError_t launch_delta_pad(int dtype, const void* from, const int64_t strides[3], int64_t B, int64_t T,
                             int64_t heads, int64_t width, void* to, hipStream_t s);
 // Padded copies of q and k where their width is not whole eights: bytes of both, and the
-// call on them.
+// call on them; of v likewise.
 inline int64_t padded_keys(const cpab_delta_rule& r) {
   return r.dk % 8 == 0 ? 0 : 2 * r.B * r.T * r.key_heads * ((r.dk + 7) / 8 * 8) * (r.dtype == CPAB_F32 ? 4 : 2);
 }
 hipError_t pad_keys(Delta* d, void* room, hipStream_t s);
+inline int64_t padded_values(const cpab_delta_rule& r) {
+  return r.dv % 8 == 0 ? 0 : r.B * r.T * r.heads * wide_of(r) * (r.dtype == CPAB_F32 ? 4 : 2);
+}
 
 // How a call is cut: a head's chunks in `segs` segments of `each`.
 struct Cut {
@@ -326,9 +371,8 @@ struct Kept {
 };
 Kept kept_of(const Delta& d, const Cut& cut);
 
-// squares: of each chunk of each head; kt, qt: of each of each key's head, qt NULL in the
-// forward.
-hipError_t launch_delta_squares(const Delta& d, void* squares, void* kt, void* qt, hipStream_t s);
+// squares: of each chunk of each head; keys: of each of each key's head.
+hipError_t launch_delta_squares(const Delta& d, void* squares, void* keys, bool backward, hipStream_t s);
 hipError_t launch_delta_join(const Delta& d, const Cut& cut, bool forward, const float* ends, const float* adds,
                              const float* given, float* to, hipStream_t s);
 int64_t delta_backward_workspace(const Delta& d);   // bytes

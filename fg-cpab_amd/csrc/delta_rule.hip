@@ -11,27 +11,26 @@ namespace {
 
 // ---- a chunk's matrices ------------------------------------------------------
 
-// 64 x 64 values from LDS to planes in the workspace, or their transpose.
+// 64 x 64 values from LDS to planes of operands in the workspace, or their transpose.
 template <int N, bool TURNED, int M>
-__device__ __forceinline__ void put_square(const float* from, int pitch, bf16 (&to)[M][kChunk][kChunk]) {
-  const int row = threadIdx.x >> 2, col = (threadIdx.x & 3) * 16;
-#pragma unroll
-  for (int half = 0; half < 16; half += 8) {
+__device__ __forceinline__ void put_square(const float* from, int pitch, bf16 (&to)[M][4][2][64][8]) {
+  for (int n = threadIdx.x; n < 512; n += kDeltaBlock) {
+    const int lane = n & 63, step = n >> 6 & 1, tile = n >> 7;
+    const int row = 16 * tile + (lane & 15), col = 32 * step + 8 * (lane >> 4);
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      v[e] = TURNED ? from[(col + half + e) * pitch + row] : from[row * pitch + col + half + e];
+    for (int e = 0; e < 8; ++e) v[e] = TURNED ? from[(col + e) * pitch + row] : from[row * pitch + col + e];
     const Frag<N> f = frag_of<N>(v);
 #pragma unroll
-    for (int k = 0; k < N; ++k) *reinterpret_cast<bf16x8*>(&to[k][row][col + half]) = f.p[k];
+    for (int k = 0; k < N; ++k) *reinterpret_cast<bf16x8*>(to[k][tile][step][lane]) = f.p[k];
   }
 }
 
-// A chunk of an input, transposed, to the workspace: [DP, 64], zeros beyond its rows and
-// columns.  Four samples of four columns to a lane.  Called by the whole workgroup; `room`
-// holds DP rows of kRow values.
+// A chunk of an input, transposed, to the workspace: zeros beyond its rows and columns.
+// Four samples of four columns to a lane.  Called by the whole workgroup; `room` holds DP
+// rows of kRow values.
 template <int DP, typename T>
-__device__ __forceinline__ void put_turned(T* room, const Rows<T>& from, T* to) {
+__device__ __forceinline__ void put_turned(T* room, const Rows<T>& from, T (&to)[DP / 16][2][64][8]) {
   typedef T T4 __attribute__((ext_vector_type(4)));
   for (int k = threadIdx.x; k < 16 * (DP / 4); k += kDeltaBlock) {
     const int row = k % 16 * 4, col = k / 16 * 4;
@@ -43,11 +42,11 @@ __device__ __forceinline__ void put_turned(T* room, const Rows<T>& from, T* to) 
       *reinterpret_cast<T4*>(room + (col + e) * kRow + row) = T4{(T)v[0][e], (T)v[1][e], (T)v[2][e], (T)v[3][e]};
   }
   __syncthreads();
-  constexpr int kEach = 16 / sizeof(T);
-  typedef uint32_t U4 __attribute__((ext_vector_type(4)));
-  for (int k = threadIdx.x; k < DP * kChunk / kEach; k += kDeltaBlock) {
-    const int row = k / (kChunk / kEach), col = k % (kChunk / kEach) * kEach;
-    *reinterpret_cast<U4*>(to + row * kChunk + col) = *reinterpret_cast<const U4*>(room + row * kRow + col);
+  for (int n = threadIdx.x; n < DP * 8; n += kDeltaBlock) {
+    const int lane = n & 63, step = n >> 6 & 1, tile = n >> 7;
+    Raw<T> r;
+    r.fetch(room + (16 * tile + (lane & 15)) * kRow + 32 * step + 8 * (lane >> 4));
+    r.put(to[tile][step][lane]);
   }
   __syncthreads();
 }
@@ -68,7 +67,7 @@ __device__ __forceinline__ void multiply16(f32x4& acc, const float* A, int pitch
 // diagonal, by rows, a wave each, M_b = T_b (A_b - sum over c < b of A_bc beta_c M_c); a wave
 // has 16 columns.
 template <typename T, int DP, bool BACKWARD>
-__global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, Squares<T>* squares, T* kt, T* qt) {
+__global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, Squares<T>* squares, Keys<T, DP>* keys) {
   constexpr int kPitch = kChunk + 4, NV = Parts<T>::kValue, NI = Parts<T>::kInput;
   extern __shared__ float room[];
   __shared__ double G[kChunk];
@@ -104,10 +103,11 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, Squ
                       (int)d.r.k_strides[1], live, d.read};
   const Rows<T> qrows{static_cast<const T*>(d.r.q) + b * d.r.q_strides[0] + t0 * d.r.q_strides[1] + kh * d.r.q_strides[2],
                       (int)d.r.q_strides[1], live, d.read};
-  if (h % d.group == 0) {
-    const int64_t at = ((b * d.r.key_heads + kh) * d.chunks + c) * DP * kChunk;
-    put_turned<DP>(reinterpret_cast<T*>(room), krows, kt + at);
-    if (BACKWARD) put_turned<DP>(reinterpret_cast<T*>(room), qrows, qt + at);
+  const bool first = h % d.group == 0;   // of those that share a key
+  Keys<T, DP>& own = keys[(b * d.r.key_heads + kh) * d.chunks + c];
+  if (first) {
+    put_turned<DP>(reinterpret_cast<T*>(room), krows, own.kt);
+    if (BACKWARD) put_turned<DP>(reinterpret_cast<T*>(room), qrows, own.qt);
   }
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   f32x4 kk[1][4], qk[1][4];
@@ -116,7 +116,14 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, Squ
 #pragma unroll
   for (int s = 0; s < DP / 32; ++s) {
     const int col = 32 * s + 8 * g;
-    const Frag<NI> ak = krows.at(16 * wave + i, col), aq = qrows.at(16 * wave + i, col);
+    Raw<T> rk, rq;
+    krows.fetch(rk, 16 * wave + i, col);
+    qrows.fetch(rq, 16 * wave + i, col);
+    if (first) {
+      rk.put(own.k[wave][s][lane]);
+      rq.put(own.q[wave][s][lane]);
+    }
+    const Frag<NI> ak = rk.frag(), aq = rq.frag();
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       const Frag<NI> bk = krows.at(16 * n + i, col);
@@ -187,22 +194,23 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, Squ
 
 // ---- the chain of chunks -----------------------------------------------------
 
-// One workgroup goes through the chunks of a segment with E columns of a head's state in
+// One workgroup goes through the chunks of a segment with 32 columns of a head's state in
 // registers, the sums of the matrix unit; LDS holds its parts for the next chunk's products.
 // Keys, queries, M and P go from memory to the lanes as the matrix unit takes them.
 // ENDS: no outputs but the state after the segment, from zeros, and, in columns of their
 // own, from the unit matrix without values: what the segment adds and what it makes of the
 // state before it.
-template <typename T, int DP, int E, bool ENDS>
-__global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squares<T>* squares, const T* kt,
-                                                          const float* starts, Cut cut, T* o, float* h_out,
-                                                          float* states, float* xs, float* ends, int segs) {
-  typedef Shares<DP, E> Sh;
-  constexpr int kPitch = DP + 8, NV = Parts<T>::kValue, NI = Parts<T>::kInput, NO = Parts<T>::kOut, kSteps = DP / 32;
+template <typename T, int DP, bool ENDS>
+__global__ __launch_bounds__(kDeltaBlock, 2) void delta_chain_kernel(
+    Delta d, const Squares<T>* squares, const Keys<T, DP>* keys, const float* starts, Cut cut, T* o,
+    float* h_out, float* states, float* xs, float* ends, int segs) {
+  typedef Shares<DP> Sh;
+  constexpr int E = kWide, kPitch = DP + 8, kSteps = DP / 32;
+  constexpr int NV = Parts<T>::kValue, NI = Parts<T>::kInput, NO = Parts<T>::kOut;
   constexpr int kState = E * kPitch, kSamples = E * kRow;   // planes
   extern __shared__ __align__(16) bf16 lds[];
-  bf16* St = lds;                  // [E][DP]
-  bf16* Rt = St + NV * kState;     // beta R, [E][64]
+  bf16* St = lds;                  // [32][DP]
+  bf16* Rt = St + NV * kState;     // beta R, [32][64]
   bf16* Ut = Rt + NV * kSamples;
   bf16* Ht = Ut + NO * kSamples;   // U until the chunk's end
   const int dk = (int)d.r.dk, dv = (int)d.r.dv, blocks_v = (dv + E - 1) / E, wide = (dv + 7) / 8 * 8;
@@ -213,15 +221,13 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
   const int h = (int)(bh - b * d.r.heads), kh = h / d.group;
   const bool unit = ENDS && at.block >= blocks_v;
   const int e0 = (unit ? at.block - blocks_v : at.block) * E, width = unit ? dk : dv;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  int i = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int64_t length = live_of(d, b);
-  const T* q = static_cast<const T*>(d.r.q) + b * d.r.q_strides[0] + kh * d.r.q_strides[2];
-  const T* k = static_cast<const T*>(d.r.k) + b * d.r.k_strides[0] + kh * d.r.k_strides[2];
   const T* v = static_cast<const T*>(d.r.v) + b * d.r.v_strides[0] + h * d.r.v_strides[2];
-  const int ks = (int)d.r.k_strides[1], qs = (int)d.r.q_strides[1], vs = (int)d.r.v_strides[1];
+  const int vs = (int)d.r.v_strides[1], hs = (int)d.r.heads;
   const int d0 = wave % Sh::WD * Sh::MT * 16, s0 = wave / Sh::WD * Sh::NT * 16;   // this wave's part of the state
-  const int w0 = 16 * (wave & 3), c0 = wave / 4 * 32;                             // and of a chunk's samples
+  const int w0 = 16 * wave;                                                       // and of a chunk's samples
   f32x4 S[Sh::MT][Sh::NT];
   const float* start = ENDS ? nullptr : at.seg > 0 ? starts + (bh * cut.segs + at.seg) * dk * dv
                                       : d.r.h0     ? d.r.h0 + bh * dk * dv : nullptr;
@@ -248,95 +254,85 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
   };
   const int chunks = (int)((length + kChunk - 1) / kChunk);
   const int first = at.seg * cut.each, last = min(first + cut.each, chunks);
+  const Frag<1> eye[2] = {unit_frag(0), unit_frag(1)};
   // What a chunk's products take is fetched as soon as the chunk before is done with the
   // registers: memory has most of a chunk's time to answer.
-  Raw<T> kf[kSteps], qf[kSteps], ktf[Sh::MT][2];
+  Raw<T> kf[kSteps], qf[kSteps], ktf[Sh::MT][2], vf;
   Frag<NV> mf[2];
   Frag<NO> pf[2];
-  RawOne<T> vf[2][4];
   f32x4 since, until, beta;
-  float total;
-  const auto rows_of = [&](int c, auto f) {
+  float mine, total;   // exp(G) of this lane's sample, and of the chunk's last
+  const Squares<T>* sqs = squares + bh * d.chunks;
+  const Keys<T, DP>* kys = keys + (b * d.r.key_heads + kh) * d.chunks;
+  const auto vrows = [&](int c) {
     const int64_t t0 = (int64_t)c * kChunk;
-    const int live = (int)min(length - t0, (int64_t)kChunk);
-    f(Rows<T>{k + t0 * ks, ks, live, d.read}, Rows<T>{q + t0 * qs, qs, live, d.read},
-      Rows<T>{v + t0 * vs, vs, live, dv});
+    return Rows<T>{v + t0 * vs, vs, (int)min(length - t0, (int64_t)kChunk), wide};
   };
   const auto fetch_rows = [&](int c) {
-    rows_of(c, [&](const Rows<T>& krows, const Rows<T>& qrows, const Rows<T>& vrows) {
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        kf[s].fetch(krows.template place<8>(w0 + i, 32 * s + 8 * g));
-        if (!ENDS) qf[s].fetch(qrows.template place<8>(w0 + i, 32 * s + 8 * g));
-      }
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) vf[n][e].fetch(vrows.template place<1>(w0 + 4 * g + e, e0 + c0 + 16 * n + i));
-    });
+    for (int s = 0; s < kSteps; ++s) {
+      kf[s].fetch(kys[c].k[wave][s][lane]);
+      if (!ENDS) qf[s].fetch(kys[c].q[wave][s][lane]);
+    }
+    if (!unit) vf.fetch(vrows(c).template place<8>(w0 + i, e0 + 8 * g));
   };
-  const auto mask_rows = [&](int c) {   // zeros where there was nothing to fetch
-    rows_of(c, [&](const Rows<T>& krows, const Rows<T>& qrows, const Rows<T>& vrows) {
-      if (krows.live == kChunk && d.read == DP && e0 + E <= dv && !unit) return;
+  const auto fetch_m = [&](int c) {
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        kf[s].keep(krows.in(w0 + i, 32 * s + 8 * g));
-        if (!ENDS) qf[s].keep(qrows.in(w0 + i, 32 * s + 8 * g));
-      }
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          vf[n][e].keep(!unit && vrows.in(w0 + 4 * g + e, e0 + c0 + 16 * n + i));
-    });
+    for (int s = 0; s < 2; ++s) mf[s] = plane_frag<NV>(sqs[c].m[0][wave][s][lane], kSquare);
+    since = *reinterpret_cast<const f32x4*>(sqs[c].gates.since + w0 + 4 * g);
+    until = *reinterpret_cast<const f32x4*>(sqs[c].gates.until + w0 + 4 * g);
+    beta = *reinterpret_cast<const f32x4*>(sqs[c].gates.beta + w0 + 4 * g);
+    if (!ENDS) mine = sqs[c].gates.since[w0 + i];
   };
-  const auto fetch_m = [&](const Squares<T>& sq) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) mf[s] = plane_frag<NV>(&sq.m[0][w0 + i][32 * s + 8 * g], kSquare);
-    since = *reinterpret_cast<const f32x4*>(sq.gates.since + w0 + 4 * g);
-    until = *reinterpret_cast<const f32x4*>(sq.gates.until + w0 + 4 * g);
-    beta = *reinterpret_cast<const f32x4*>(sq.gates.beta + w0 + 4 * g);
-  };
-  const auto fetch_rest = [&](const Squares<T>& sq, int c) {
-    const T* ktc = kt + ((b * d.r.key_heads + kh) * d.chunks + c) * DP * kChunk;
+  const auto fetch_rest = [&](int c) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      if (!ENDS) pf[s] = plane_frag<NO>(&sq.p[0][w0 + i][32 * s + 8 * g], kSquare);
+      if (!ENDS) pf[s] = plane_frag<NO>(sqs[c].p[0][wave][s][lane], kSquare);
 #pragma unroll
-      for (int m = 0; m < Sh::MT; ++m) ktf[m][s].fetch(ktc + (d0 + 16 * m + i) * kChunk + 32 * s + 8 * g);
+      for (int m = 0; m < Sh::MT; ++m) ktf[m][s].fetch(kys[c].kt[d0 / 16 + m][s][lane]);
     }
-    total = sq.gates.since[kChunk - 1];
+    total = sqs[c].gates.since[kChunk - 1];
   };
-  const Squares<T>* sqs = squares + bh * d.chunks;
   loaded();
   if (first < last) {
     fetch_rows(first);
-    fetch_m(sqs[first]);
-    fetch_rest(sqs[first], first);
+    fetch_m(first);
+    fetch_rest(first);
   }
   for (int c = first; c < last; ++c) {
-    const int64_t t0 = (int64_t)c * kChunk;
+    const int64_t t0 = (int64_t)c * kChunk, row0 = (b * d.r.T + t0) * d.r.heads + h;
     const int live = (int)min(length - t0, (int64_t)kChunk), next = min(c + 1, last - 1);
-    float* xc = xs ? xs + ((b * d.r.T + t0) * d.r.heads + h) * wide : nullptr;
-    T* oc = o + ((b * d.r.T + t0) * d.r.heads + h) * dv;
-    renew(i, g);
-    if (!ENDS && states) put_state(states + (bh * d.chunks + c) * dk * wide, wide);
+    renew(lane);
+    i = lane & 15, g = lane >> 4;
+    if (!ENDS && states) {
+      float* to = states + (bh * d.chunks + c) * dk * wide;
+#pragma unroll
+      for (int m = 0; m < Sh::MT; ++m)
+#pragma unroll
+        for (int n = 0; n < Sh::NT; ++n) {
+          const int row = d0 + 16 * m + 4 * g + (i & 3), col = e0 + s0 + 16 * n + (i & 12);
+          const f32x4 x = across(S[m][n]);
+          if (row < dk && col < wide) store4(to + row * wide + col, x);
+        }
+    }
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
 #pragma unroll
       for (int n = 0; n < Sh::NT; ++n)
         put4<NV>(St + (s0 + 16 * n + i) * kPitch + d0 + 16 * m + 4 * g, kState, S[m][n]);
-    mask_rows(c);
+    if (!unit) {
+      const Rows<T> rows = vrows(c);
+      if (live < kChunk || e0 + E > wide) vf.keep(rows.in(w0 + i, e0 + 8 * g));
+    }
     __syncthreads();
-    f32x4 R[1][2], O[1][2], X[1][2];
+    f32x4 R[1][2], O[2][1], X[1][2];   // O: rows are columns of values, columns are samples
     clear(R);
     clear(O);
     {
       Frag<NV> st[2][2];   // this step's and the next's: LDS answers while the matrix unit works
       const auto read = [&](int s) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-          st[s & 1][n] = plane_frag<NV>(St + (c0 + 16 * n + i) * kPitch + 32 * s + 8 * g, kState);
+        for (int n = 0; n < 2; ++n) st[s & 1][n] = plane_frag<NV>(St + (16 * n + i) * kPitch + 32 * s + 8 * g, kState);
       };
       read(0);
 #pragma unroll
@@ -348,16 +344,17 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
         if (!ENDS) {
           const Frag<NI> qv = qf[s].frag();
 #pragma unroll
-          for (int n = 0; n < 2; ++n) mma(O[0][n], qv, first_of<NO>(st[s & 1][n]));
+          for (int n = 0; n < 2; ++n) mma(O[n][0], first_of<NO>(st[s & 1][n]), qv);
         }
       }
     }
+    const Frag<NI> vv = vf.frag();
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) R[0][n][e] = fmaf(-since[e], R[0][n][e], vf[n][e].value());
-      O[0][n] *= d.r.scale * since;
-      put4<NV>(Rt + (c0 + 16 * n + i) * kRow + w0 + 4 * g, kSamples, beta * R[0][n]);
+      R[0][n] *= -since;
+      if (!unit) mma(R[0][n], vv, eye[n]);
+      if (!ENDS) O[n][0] *= d.r.scale * mine;
+      put4<NV>(Rt + (16 * n + i) * kRow + w0 + 4 * g, kSamples, beta * R[0][n]);
     }
     fetch_rows(next);
     __syncthreads();
@@ -367,8 +364,7 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-          rt[s][n] = plane_frag<NV>(Rt + (c0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples);
+        for (int n = 0; n < 2; ++n) rt[s][n] = plane_frag<NV>(Rt + (16 * n + i) * kRow + 32 * s + 8 * g, kSamples);
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -377,46 +373,51 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       const f32x4 x = R[0][n] - X[0][n], u = beta * x;
-      const int to = (c0 + 16 * n + i) * kRow + w0 + 4 * g;
+      const int to = (16 * n + i) * kRow + w0 + 4 * g;
       if (!ENDS) put4<NO>(Ut + to, kSamples, u);
       put4<NV>(Ht + to, kSamples, until * u);
-      if (!ENDS && xs)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int t = w0 + 4 * g + e, col = e0 + c0 + 16 * n + i;
-          if (t < live && col < dv) xc[t * (int)d.r.heads * wide + col] = x[e];
-        }
+      if (!ENDS && xs) {
+        const int t = w0 + 4 * g + (i & 3), col = e0 + 16 * n + (i & 12);
+        const f32x4 row = across(x);
+        if (t < live && col < wide) store4(xs + row0 * wide + t * hs * wide + col, row);
+      }
     }
-    fetch_m(sqs[next]);
+    fetch_m(next);
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
 #pragma unroll
       for (int n = 0; n < Sh::NT; ++n) S[m][n] *= total;
+    {
+      Frag<NV> ht[2][Sh::NT];
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int n = 0; n < Sh::NT; ++n) {
-        const Frag<NV> u = plane_frag<NV>(Ht + (s0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples);
+        for (int n = 0; n < Sh::NT; ++n)
+          ht[s][n] = plane_frag<NV>(Ht + (s0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples);
 #pragma unroll
-        for (int m = 0; m < Sh::MT; ++m) mma(S[m][n], ktf[m][s].frag(), u);
-      }
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int m = 0; m < Sh::MT; ++m) {
+          const Frag<NI> kv = ktf[m][s].frag();
+#pragma unroll
+          for (int n = 0; n < Sh::NT; ++n) mma(S[m][n], kv, ht[s][n]);
+        }
+    }
     if (!ENDS) {
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int n = 0; n < 2; ++n)
-          mma(O[0][n], pf[s], plane_frag<NO>(Ut + (c0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples));
+          mma(O[n][0], plane_frag<NO>(Ut + (16 * n + i) * kRow + 32 * s + 8 * g, kSamples), pf[s]);
     }
-    fetch_rest(sqs[next], next);
+    fetch_rest(next);
     if (ENDS) continue;
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int t = w0 + 4 * g + e, col = e0 + c0 + 16 * n + i;
-        if (t < live && col < dv) oc[t * (int)d.r.heads * dv + col] = from_float<T>(O[0][n][e]);
-      }
+    for (int n = 0; n < 2; ++n) {
+      const int t = w0 + i, col = e0 + 16 * n + 4 * g;
+      if (t < live && col < dv) store_some(o + row0 * dv + t * hs * dv + col, O[n][0], dv - col);
+    }
   }
   if (ENDS) {
     put_state(ends + (bh * cut.segs + at.seg) * dk * (dv + dk) + (unit ? dv : 0), dv + dk);
@@ -424,7 +425,7 @@ __global__ __launch_bounds__(8 * E) void delta_chain_kernel(Delta d, const Squar
   }
   if (at.seg == (chunks > 0 ? (chunks - 1) / cut.each : 0)) put_state(h_out + bh * dk * dv, dv);
   const int64_t rest = max(length, (int64_t)first * kChunk), stop = min((int64_t)(first + cut.each) * kChunk, d.r.T);
-  for (int64_t n = rest * E + threadIdx.x; n < stop * E; n += 8 * E) {
+  for (int64_t n = rest * E + threadIdx.x; n < stop * E; n += kDeltaBlock) {
     const int64_t t = n / E;
     const int col = e0 + (int)(n % E);
     if (col < dv) o[((b * d.r.T + t) * d.r.heads + h) * dv + col] = from_float<T>(0.0f);
@@ -668,16 +669,16 @@ hipError_t pad_keys(Delta* d, void* room, hipStream_t st) {
   return e;
 }
 
-hipError_t launch_delta_squares(const Delta& d, void* squares, void* kt, void* qt, hipStream_t st) {
+hipError_t launch_delta_squares(const Delta& d, void* squares, void* keys, bool backward, hipStream_t st) {
   with_key(d, [&](auto t, auto dp) {
     typedef decltype(t) T;
     constexpr int DP = decltype(dp)::value;
     constexpr int kRoom = std::max<int>(4 * kChunk * (2 * (kChunk + 4) + 20), DP * kRow * (int)sizeof(T));
     const unsigned blocks = (unsigned)(d.r.B * d.r.heads * d.chunks);
-    if (qt)
-      delta_squares_kernel<T, DP, true><<<blocks, kDeltaBlock, kRoom, st>>>(d, (Squares<T>*)squares, (T*)kt, (T*)qt);
+    if (backward)
+      delta_squares_kernel<T, DP, true><<<blocks, kDeltaBlock, kRoom, st>>>(d, (Squares<T>*)squares, (Keys<T, DP>*)keys);
     else
-      delta_squares_kernel<T, DP, false><<<blocks, kDeltaBlock, kRoom, st>>>(d, (Squares<T>*)squares, (T*)kt, nullptr);
+      delta_squares_kernel<T, DP, false><<<blocks, kDeltaBlock, kRoom, st>>>(d, (Squares<T>*)squares, (Keys<T, DP>*)keys);
   });
   return hipGetLastError();
 }
@@ -722,18 +723,19 @@ namespace {
 
 // The forward's workspace (bytes).
 struct Room {
-  int64_t squares, kt, starts, ends, keys, all;
+  int64_t squares, keys, starts, ends, padded, values, all;
 };
 Room room_of(const Delta& d, const Cut& cut, bool keep) {
   const int64_t heads = d.r.B * d.r.heads;
   const auto next = [](int64_t n) { return (n + 255) / 256 * 256; };
   Room w;
   w.squares = 0;
-  w.kt = next(heads * d.chunks * squares_bytes(d.r.dtype));
-  w.starts = w.kt + next(d.r.B * d.r.key_heads * d.chunks * turned_bytes(d.r));
+  w.keys = next(heads * d.chunks * squares_bytes(d.r.dtype));
+  w.starts = w.keys + next(d.r.B * d.r.key_heads * d.chunks * keys_bytes(d.r));
   w.ends = w.starts + (cut.segs > 1 ? next(heads * cut.segs * d.r.dk * d.r.dv * 4) : 0);
-  w.keys = w.ends + (cut.segs > 1 && !keep ? next(heads * cut.segs * d.r.dk * (d.r.dv + d.r.dk) * 4) : 0);
-  w.all = w.keys + padded_keys(d.r);
+  w.padded = w.ends + (cut.segs > 1 && !keep ? next(heads * cut.segs * d.r.dk * (d.r.dv + d.r.dk) * 4) : 0);
+  w.values = w.padded + next(padded_keys(d.r));
+  w.all = w.values + padded_values(d.r);
   return w;
 }
 
@@ -763,40 +765,39 @@ hipError_t launch_delta_rule_forward(const cpab_delta_rule& r, void* o, float* h
   char* room = static_cast<char*>(workspace);
   float* starts = reinterpret_cast<float*>(room + w.starts);
   float* ends = kept ? kept + k.ends : reinterpret_cast<float*>(room + w.ends);
-  hipError_t e = pad_keys(&d, room + w.keys, st);
-  if (e == hipSuccess) e = launch_delta_squares(d, room + w.squares, room + w.kt, nullptr, st);
+  hipError_t e = pad_keys(&d, room + w.padded, st);
+  if (e == hipSuccess && r.dv % 8 != 0) {
+    e = launch_delta_pad(r.dtype, r.v, r.v_strides, r.B, r.T, r.heads, r.dv, room + w.values, st);
+    d.r.v = room + w.values;
+    d.r.v_strides[2] = wide_of(r);
+    d.r.v_strides[1] = r.heads * wide_of(r);
+    d.r.v_strides[0] = r.T * r.heads * wide_of(r);
+  }
+  if (e == hipSuccess) e = launch_delta_squares(d, room + w.squares, room + w.keys, false, st);
   if (e != hipSuccess) return e;
   with_key(d, [&](auto t, auto dp) {
     typedef decltype(t) T;
     constexpr int DP = decltype(dp)::value, NV = Parts<T>::kValue, NO = Parts<T>::kOut;
     const Squares<T>* squares = reinterpret_cast<const Squares<T>*>(room + w.squares);
-    const T* kt = reinterpret_cast<const T*>(room + w.kt);
-    const auto run = [&](auto width, auto only_ends, int segs) {
-      constexpr int E = decltype(width)::value;
+    const Keys<T, DP>* keys = reinterpret_cast<const Keys<T, DP>*>(room + w.keys);
+    const auto run = [&](auto only_ends, int segs) {
       constexpr bool ENDS = decltype(only_ends)::value;
-      constexpr int kRoom = 2 * E * (NV * (DP + 8) + (2 * NV + NO) * kRow);
+      constexpr int kRoom = 2 * kWide * (NV * (DP + 8) + (2 * NV + NO) * kRow);
       static LdsAllowed allowed;
-      e = allow_lds(reinterpret_cast<const void*>(delta_chain_kernel<T, DP, E, ENDS>), kRoom, allowed);
+      e = allow_lds(reinterpret_cast<const void*>(delta_chain_kernel<T, DP, ENDS>), kRoom, allowed);
       if (e != hipSuccess) return;
-      const int64_t blocks = (r.dv + E - 1) / E + (ENDS ? (r.dk + E - 1) / E : 0);
-      delta_chain_kernel<T, DP, E, ENDS><<<(unsigned)((heads * segs + 7) / 8 * 8 * blocks), 8 * E, kRoom, st>>>(
-          d, squares, kt, starts, cut, (T*)o, h, kept, kept ? kept + k.xs : nullptr, ends, segs);
+      const int64_t blocks = (r.dv + kWide - 1) / kWide + (ENDS ? (r.dk + kWide - 1) / kWide : 0);
+      delta_chain_kernel<T, DP, ENDS><<<(unsigned)((heads * segs + 7) / 8 * 8 * blocks), kDeltaBlock, kRoom, st>>>(
+          d, squares, keys, starts, cut, (T*)o, h, kept, kept ? kept + k.xs : nullptr, ends, segs);
       e = hipGetLastError();
-    };
-    typedef std::integral_constant<int, 32> Narrow;
-    typedef std::integral_constant<int, 64> Wide;
-    const auto both = [&](auto only_ends, int segs) {
-      if constexpr (sizeof(T) == 2)
-        if (r.dv > 32) return run(Wide(), only_ends, segs);
-      run(Narrow(), only_ends, segs);
     };
     if (cut.segs > 1) {
       // the backward takes what the last segment makes of the state too
-      both(std::true_type(), kept ? cut.segs : cut.segs - 1);
+      run(std::true_type(), kept ? cut.segs : cut.segs - 1);
       if (e == hipSuccess) e = launch_delta_join(d, cut, true, ends, nullptr, r.h0, starts, st);
       if (e != hipSuccess) return;
     }
-    both(std::false_type(), cut.segs);
+    run(std::false_type(), cut.segs);
   });
   return e;
 }

@@ -11,21 +11,21 @@ namespace {
 
 // ---- the chain of chunks, backwards --------------------------------------------
 
-// As the forward's chain: E columns of the state's gradient in registers, back through a
+// As the forward's chain: 32 columns of the state's gradient in registers, back through a
 // segment's chunks.  Keeps the gradient after each chunk and E, and writes grad_v and
 // grad_h0.  M and P lie transposed.  ENDS: only what the segment adds to the gradient before
 // it.
-template <typename T, int DP, int E, bool ENDS>
-__global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
-    Delta d, const Squares<T>* squares, const T* kt, const T* qt, Cut cut, const T* grad_o,
+template <typename T, int DP, bool ENDS>
+__global__ __launch_bounds__(kDeltaBlock, 2) void delta_back_chain_kernel(
+    Delta d, const Squares<T>* squares, const Keys<T, DP>* keys, Cut cut, const T* grad_o,
     const float* grad_h, const float* starts, T* grad_v, float* grad_h0, float* dstates, float* es,
     float* adds) {
-  typedef Shares<DP, E> Sh;
-  constexpr int kPitch = DP + 8, NV = Parts<T>::kValue, NI = Parts<T>::kInput, kSteps = DP / 32;
+  typedef Shares<DP> Sh;
+  constexpr int E = kWide, kPitch = DP + 8, NV = Parts<T>::kValue, NI = Parts<T>::kInput, kSteps = DP / 32;
   constexpr int kState = E * kPitch, kSamples = E * kRow;   // planes
   extern __shared__ __align__(16) bf16 lds[];
-  bf16* St = lds;                       // the gradient, [E][DP]
-  bf16* Bt = St + NV * kState;          // beta dU, [E][64]
+  bf16* St = lds;                       // the gradient, [32][DP]
+  bf16* Bt = St + NV * kState;          // beta dU, [32][64]
   bf16* Zt = Bt + NV * kSamples;        // - exp(G) Z
   bf16* Ot = Zt + NV * kSamples;        // dO, as the input that it is
   bf16* Gt = Ot + NI * kSamples;        // scale exp(G) dO
@@ -34,14 +34,12 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
   const Where at = where(heads, cut.segs, (dv + E - 1) / E);
   if (!at.in) return;
   const int64_t bh = at.bh, b = bh / d.r.heads;
-  const int h = (int)(bh - b * d.r.heads), kh = h / d.group, e0 = at.block * E;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  int i = lane & 15, g = lane >> 4;
+  const int h = (int)(bh - b * d.r.heads), kh = h / d.group, e0 = at.block * E, hs = (int)d.r.heads;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int64_t length = live_of(d, b);
-  const T* k = static_cast<const T*>(d.r.k) + b * d.r.k_strides[0] + kh * d.r.k_strides[2];
-  const int ks = (int)d.r.k_strides[1];
   const int d0 = wave % Sh::WD * Sh::MT * 16, s0 = wave / Sh::WD * Sh::NT * 16;
-  const int w0 = 16 * (wave & 3), c0 = wave / 4 * 32;
+  const int w0 = 16 * wave;
   const int chunks = (int)((length + kChunk - 1) / kChunk);
   const int first = at.seg * cut.each, last = min(first + cut.each, chunks);
   // what comes from behind: the state's own gradient, or that of the segment behind
@@ -58,7 +56,7 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
         const int row = d0 + 16 * m + 4 * g + e, col = e0 + s0 + 16 * n + i;
         S[m][n][e] = start && row < dk && col < dv ? start[(int64_t)row * dv + col] : 0.0f;
       }
-  const auto put_state = [&](float* to, int pitch) {
+  const auto put_state = [&](float* to) {
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
 #pragma unroll
@@ -66,99 +64,84 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int row = d0 + 16 * m + 4 * g + e, col = e0 + s0 + 16 * n + i;
-          if (row < dk && col < dv) to[row * pitch + col] = S[m][n][e];
+          if (row < dk && col < dv) to[row * dv + col] = S[m][n][e];
         }
   };
+  const Frag<1> eye[2] = {unit_frag(0), unit_frag(1)};
   // Fetched as in the forward's chain.  Without grad_o as many bytes of E's place, as zeros.
   const T* go = grad_o ? grad_o : reinterpret_cast<const T*>(es);
-  Raw<T> kf[kSteps], ktf[Sh::MT][2], qtf[Sh::MT][2];
+  Raw<T> kf[kSteps], ktf[Sh::MT][2], qtf[Sh::MT][2], of;
   Frag<NV> mf[2], pf[2];
-  RawOne<T> of[2][4];
   f32x4 since, until, beta;
   float total;
-  const auto krows_of = [&](int c) {
+  const Squares<T>* sqs = squares + bh * d.chunks;
+  const Keys<T, DP>* kys = keys + (b * d.r.key_heads + kh) * d.chunks;
+  const auto orows = [&](int c) {
     const int64_t t0 = (int64_t)c * kChunk;
-    return Rows<T>{k + t0 * ks, ks, (int)min(length - t0, (int64_t)kChunk), d.read};
+    return Rows<T>{go + ((b * d.r.T + t0) * d.r.heads + h) * wide, hs * wide, (int)min(length - t0, (int64_t)kChunk), wide};
   };
-  const auto orows_of = [&](int c) {
-    const int64_t t0 = (int64_t)c * kChunk;
-    return Rows<T>{go + ((b * d.r.T + t0) * d.r.heads + h) * wide, (int)d.r.heads * wide,
-                   (int)min(length - t0, (int64_t)kChunk), dv};
-  };
+  const auto fetch_o = [&](int c) { of.fetch(orows(c).template place<8>(w0 + i, e0 + 8 * g)); };
   const auto fetch_k = [&](int c) {
-    const Rows<T> krows = krows_of(c);
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) kf[s].fetch(krows.template place<8>(w0 + i, 32 * s + 8 * g));
+    for (int s = 0; s < kSteps; ++s) kf[s].fetch(kys[c].k[wave][s][lane]);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) pf[s] = plane_frag<NV>(sqs[c].p[0][wave][s][lane], kSquare);
+    until = *reinterpret_cast<const f32x4*>(sqs[c].gates.until + w0 + 4 * g);
   };
-  const auto fetch_o = [&](int c) {
-    const Rows<T> orows = orows_of(c);
+  const auto fetch_m = [&](int c) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) of[n][e].fetch(orows.template place<1>(w0 + 4 * g + e, e0 + c0 + 16 * n + i));
+    for (int s = 0; s < 2; ++s) mf[s] = plane_frag<NV>(sqs[c].m[0][wave][s][lane], kSquare);
+    since = *reinterpret_cast<const f32x4*>(sqs[c].gates.since + w0 + 4 * g);
+    beta = *reinterpret_cast<const f32x4*>(sqs[c].gates.beta + w0 + 4 * g);
   };
-  const auto mask_rows = [&](int c) {   // zeros where there was nothing to fetch
-    const Rows<T> krows = krows_of(c), orows = orows_of(c);
-    if (krows.live == kChunk && d.read == DP && e0 + E <= dv && grad_o) return;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) kf[s].keep(krows.in(w0 + i, 32 * s + 8 * g));
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        of[n][e].keep(grad_o && orows.in(w0 + 4 * g + e, e0 + c0 + 16 * n + i));
-  };
-  const auto fetch_p = [&](const Squares<T>& sq) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) pf[s] = plane_frag<NV>(&sq.p[0][w0 + i][32 * s + 8 * g], kSquare);
-    until = *reinterpret_cast<const f32x4*>(sq.gates.until + w0 + 4 * g);
-  };
-  const auto fetch_m = [&](const Squares<T>& sq) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) mf[s] = plane_frag<NV>(&sq.m[0][w0 + i][32 * s + 8 * g], kSquare);
-    since = *reinterpret_cast<const f32x4*>(sq.gates.since + w0 + 4 * g);
-    beta = *reinterpret_cast<const f32x4*>(sq.gates.beta + w0 + 4 * g);
-  };
-  const auto fetch_turned = [&](const Squares<T>& sq, int c) {
-    const int64_t turned = ((b * d.r.key_heads + kh) * d.chunks + c) * DP * kChunk;
+  const auto fetch_turned = [&](int c) {
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int m = 0; m < Sh::MT; ++m) {
-        const int from = (d0 + 16 * m + i) * kChunk + 32 * s + 8 * g;
-        ktf[m][s].fetch(kt + turned + from);
-        qtf[m][s].fetch(qt + turned + from);
+        ktf[m][s].fetch(kys[c].kt[d0 / 16 + m][s][lane]);
+        qtf[m][s].fetch(kys[c].qt[d0 / 16 + m][s][lane]);
       }
-    total = sq.gates.since[kChunk - 1];
+    total = sqs[c].gates.since[kChunk - 1];
   };
-  const Squares<T>* sqs = squares + bh * d.chunks;
   loaded();
   if (first < last) {
     fetch_o(last - 1);
     fetch_k(last - 1);
-    fetch_p(sqs[last - 1]);
-    fetch_m(sqs[last - 1]);
-    fetch_turned(sqs[last - 1], last - 1);
+    fetch_m(last - 1);
+    fetch_turned(last - 1);
   }
   for (int c = last - 1; c >= first; --c) {
-    const int64_t t0 = (int64_t)c * kChunk;
+    const int64_t t0 = (int64_t)c * kChunk, row0 = (b * d.r.T + t0) * d.r.heads + h;
     const int live = (int)min(length - t0, (int64_t)kChunk), next = max(c - 1, first);
-    float* ec = es + ((b * d.r.T + t0) * d.r.heads + h) * wide;
-    T* vc = grad_v ? grad_v + ((b * d.r.T + t0) * d.r.heads + h) * dv : nullptr;
-    renew(i, g);
-    if (!ENDS) put_state(dstates + (bh * d.chunks + c) * dk * wide, wide);
+    renew(lane);
+    i = lane & 15, g = lane >> 4;
+    if (!ENDS) {
+      float* to = dstates + (bh * d.chunks + c) * dk * wide;
+#pragma unroll
+      for (int m = 0; m < Sh::MT; ++m)
+#pragma unroll
+        for (int n = 0; n < Sh::NT; ++n) {
+          const int row = d0 + 16 * m + 4 * g + (i & 3), col = e0 + s0 + 16 * n + (i & 12);
+          const f32x4 x = across(S[m][n]);
+          if (row < dk && col < wide) store4(to + row * wide + col, x);
+        }
+    }
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
 #pragma unroll
       for (int n = 0; n < Sh::NT; ++n)
         put4<NV>(St + (s0 + 16 * n + i) * kPitch + d0 + 16 * m + 4 * g, kState, S[m][n]);
-    mask_rows(c);
-    f32x4 ov[2];
+    if (live < kChunk || e0 + E > wide || !grad_o) of.keep(grad_o && orows(c).in(w0 + i, e0 + 8 * g));
+    f32x4 O[1][2];   // dO as the sums lie
+    clear(O);
+    {
+      const Frag<NI> ov = of.frag();
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) ov[n][e] = of[n][e].value();
-      put4<NI>(Ot + (c0 + 16 * n + i) * kRow + w0 + 4 * g, kSamples, ov[n]);
+      for (int n = 0; n < 2; ++n) {
+        mma(O[0][n], ov, eye[n]);
+        put4<NI>(Ot + (16 * n + i) * kRow + w0 + 4 * g, kSamples, O[0][n]);
+      }
     }
     fetch_o(next);
     __syncthreads();
@@ -169,8 +152,7 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
       Frag<NV> st[2][2];
       const auto read = [&](int s) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-          st[s & 1][n] = plane_frag<NV>(St + (c0 + 16 * n + i) * kPitch + 32 * s + 8 * g, kState);
+        for (int n = 0; n < 2; ++n) st[s & 1][n] = plane_frag<NV>(St + (16 * n + i) * kPitch + 32 * s + 8 * g, kState);
       };
       read(0);
 #pragma unroll
@@ -186,8 +168,7 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-          ot[s][n] = plane_frag<NI>(Ot + (c0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples);
+        for (int n = 0; n < 2; ++n) ot[s][n] = plane_frag<NI>(Ot + (16 * n + i) * kRow + 32 * s + 8 * g, kSamples);
 #pragma unroll
       for (int n = 0; n < 2; ++n) U[0][n] *= until;
 #pragma unroll
@@ -196,18 +177,15 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
         for (int n = 0; n < 2; ++n) mma(U[0][n], pf[s], ot[s][n]);
     }
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
-      put4<NV>(Bt + (c0 + 16 * n + i) * kRow + w0 + 4 * g, kSamples, beta * U[0][n]);
+    for (int n = 0; n < 2; ++n) put4<NV>(Bt + (16 * n + i) * kRow + w0 + 4 * g, kSamples, beta * U[0][n]);
     fetch_k(next);
-    fetch_p(sqs[next]);
     __syncthreads();
     {
       Frag<NV> bt[2][2];
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-          bt[s][n] = plane_frag<NV>(Bt + (c0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples);
+        for (int n = 0; n < 2; ++n) bt[s][n] = plane_frag<NV>(Bt + (16 * n + i) * kRow + 32 * s + 8 * g, kSamples);
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -216,48 +194,52 @@ __global__ __launch_bounds__(8 * E) void delta_back_chain_kernel(
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       const f32x4 ev = U[0][n] - V[0][n], z = beta * ev;
-      const int at = (c0 + 16 * n + i) * kRow + w0 + 4 * g;
-      put4<NV>(Zt + at, kSamples, -since * z);
-      put4<NV>(Gt + at, kSamples, d.r.scale * since * ov[n]);
+      const int to = (16 * n + i) * kRow + w0 + 4 * g;
+      put4<NV>(Zt + to, kSamples, -since * z);
+      put4<NV>(Gt + to, kSamples, d.r.scale * since * O[0][n]);
       if (ENDS) continue;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int t = w0 + 4 * g + e, col = e0 + c0 + 16 * n + i;
-        if (t < live && col < dv) {
-          const int to = t * (int)d.r.heads;
-          ec[to * wide + col] = ev[e];
-          if (vc) vc[to * dv + col] = from_float<T>(z[e]);
-        }
+      const int t = w0 + 4 * g + (i & 3), col = e0 + 16 * n + (i & 12);
+      const f32x4 er = across(ev), zr = across(z);
+      if (t < live && col < wide) {
+        store4(es + row0 * wide + t * hs * wide + col, er);
+        if (grad_v && col < dv) store_some(grad_v + row0 * dv + t * hs * dv + col, zr, dv - col);
       }
     }
-    fetch_m(sqs[next]);
+    fetch_m(next);
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < Sh::MT; ++m)
 #pragma unroll
       for (int n = 0; n < Sh::NT; ++n) S[m][n] *= total;
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int s = 0; s < 2; ++s) {
+      Frag<NV> gt[Sh::NT], zt[Sh::NT];
 #pragma unroll
       for (int n = 0; n < Sh::NT; ++n) {
         const int from = (s0 + 16 * n + i) * kRow + 32 * s + 8 * g;
-        const Frag<NV> go = plane_frag<NV>(Gt + from, kSamples), z = plane_frag<NV>(Zt + from, kSamples);
+        gt[n] = plane_frag<NV>(Gt + from, kSamples);
+        zt[n] = plane_frag<NV>(Zt + from, kSamples);
+      }
 #pragma unroll
-        for (int m = 0; m < Sh::MT; ++m) {
-          mma(S[m][n], qtf[m][s].frag(), go);
-          mma(S[m][n], ktf[m][s].frag(), z);
+      for (int m = 0; m < Sh::MT; ++m) {
+        const Frag<NI> qv = qtf[m][s].frag(), kv = ktf[m][s].frag();
+#pragma unroll
+        for (int n = 0; n < Sh::NT; ++n) {
+          mma(S[m][n], qv, gt[n]);
+          mma(S[m][n], kv, zt[n]);
         }
       }
-    fetch_turned(sqs[next], next);
+    }
+    fetch_turned(next);
   }
   if (ENDS) {
-    put_state(adds + (bh * cut.segs + at.seg) * dk * dv, dv);
+    put_state(adds + (bh * cut.segs + at.seg) * dk * dv);
     return;
   }
-  if (grad_h0 && at.seg == 0) put_state(grad_h0 + bh * dk * dv, dv);
+  if (grad_h0 && at.seg == 0) put_state(grad_h0 + bh * dk * dv);
   if (grad_v) {
     const int64_t rest = max(length, (int64_t)first * kChunk), stop = min((int64_t)(first + cut.each) * kChunk, d.r.T);
-    for (int64_t n = rest * E + threadIdx.x; n < stop * E; n += 8 * E) {
+    for (int64_t n = rest * E + threadIdx.x; n < stop * E; n += kDeltaBlock) {
       const int64_t t = n / E;
       const int col = e0 + (int)(n % E);
       if (col < dv) grad_v[((b * d.r.T + t) * d.r.heads + h) * dv + col] = from_float<T>(0.0f);
@@ -274,15 +256,14 @@ __device__ __forceinline__ void put_gate(const Delta& d, void* p, int64_t at, fl
     static_cast<bf16*>(p)[at] = from_float<bf16>(v);
 }
 
-// The first `left` of four values, zeros behind them.
-__device__ __forceinline__ f32x4 edge(f32x4 v, int left) {
+__device__ __forceinline__ f32x4 masked(f32x4 v, bool in) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = e < left ? v[e] : 0.0f;
+  for (int e = 0; e < 4; ++e) v[e] = in ? v[e] : 0.0f;
   return v;
 }
 
 constexpr int kPartsBlock = 512;
-constexpr int kWide = 32, kWidePitch = kWide + 8;   // columns of values at once
+constexpr int kWidePitch = kWide + 8;
 
 template <typename T, int DP>
 struct PartsRoom {
@@ -299,7 +280,7 @@ struct PartsRoom {
 // two the columns.
 template <typename T, int DP>
 __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
-    Delta d, const Squares<T>* squares, const T* kt, const T* qt, const float* states, const float* xs,
+    Delta d, const Squares<T>* squares, const Keys<T, DP>* keys, const float* states, const float* xs,
     const float* dstates, const float* es, const T* grad_o, T* grad_q, T* grad_k, void* grad_decay,
     void* grad_beta) {
   typedef PartsRoom<T, DP> Room;
@@ -325,10 +306,13 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
   const int64_t t0 = (int64_t)c * kChunk;
   const int live = (int)min(max(live_of(d, b) - t0, (int64_t)0), (int64_t)kChunk);
   const int rows = (int)min(d.r.T - t0, (int64_t)kChunk);   // that there are
-  const T* k = static_cast<const T*>(d.r.k) + b * d.r.k_strides[0] + t0 * d.r.k_strides[1] + kh * d.r.k_strides[2];
-  const T* q = static_cast<const T*>(d.r.q) + b * d.r.q_strides[0] + t0 * d.r.q_strides[1] + kh * d.r.q_strides[2];
-  const Rows<T> krows{k, (int)d.r.k_strides[1], live, d.read}, qrows{q, (int)d.r.q_strides[1], live, d.read};
-  const int64_t turned = ((b * d.r.key_heads + kh) * d.chunks + c) * DP * kChunk;
+  const Keys<T, DP>& own = keys[(b * d.r.key_heads + kh) * d.chunks + c];
+  const Frag<1> eye[2] = {unit_frag(0), unit_frag(1)};
+  const auto own_frag = [&](const auto& of, int tile, int step) {
+    Raw<T> r;
+    r.fetch(of[tile][step][threadIdx.x & 63]);
+    return r.frag();
+  };
   f32x4 dQ[1][NT], dK[1][NT];
   clear(dQ);
   clear(dK);
@@ -370,13 +354,13 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
     const int64_t token = (b * d.r.T + t0) * d.r.heads + h;
     const int across = (int)d.r.heads * wide;
     const Rows<T> orows{(grad_o ? grad_o : reinterpret_cast<const T*>(es)) + token * wide, across, live, wide};
-    // rows of whole eights, in which the library itself wrote nothing beyond dv
+    // the library's own: rows of whole eights, zeros beyond dv
     const Rows<float> srows{state, wide, dk, wide}, lrows{dstate, wide, dk, wide};
     const Rows<float> xrows{xs + token * wide, across, live, wide}, erows{es + token * wide, across, live, wide};
     // A block of columns is fetched while the matrix unit has the one before.
     constexpr int kQuads = (DP * (kWide / 4) + kPartsBlock - 1) / kPartsBlock;
     static_assert(kChunk * (kWide / 4) == kPartsBlock, "a quad of X to a lane");
-    int tid = threadIdx.x, unused = 0;
+    int tid = threadIdx.x;
     f32x4 sq4[kQuads], lq4[kQuads], xq, eq, zq[2];
     Raw<T> oraw;
     const auto load4 = [](const Rows<float>& r, int row, int col) {
@@ -403,13 +387,13 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
     fetch(0);
 #pragma unroll 1
     for (int e0 = 0; e0 < dv; e0 += kWide) {
-      renew(i, g);
-      renew(tid, unused);
+      renew(tid);
+      i = tid & 15, g = tid >> 4 & 3;
 #pragma unroll
       for (int n = 0; n < kQuads; ++n) {
         const int at = tid + n * kPartsBlock, row = at / (kWide / 4), col = at % (kWide / 4) * 4;
-        const int left = row < dk ? dv - e0 - col : 0;
-        const f32x4 s = edge(sq4[n], left), l = edge(lq4[n], left);
+        const bool in = row < dk && e0 + col < wide;
+        const f32x4 s = masked(sq4[n], in), l = masked(lq4[n], in);
         if (DP * (kWide / 4) % kPartsBlock == 0 || at < DP * (kWide / 4)) {
           put4<NV>(S + row * kWidePitch + col, Room::kState, s);
           put4<NV>(L + row * kWidePitch + col, Room::kState, l);
@@ -418,8 +402,9 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
         for (int e = 0; e < 4; ++e) dot = fmaf(s[e], l[e], dot);
       }
       {
-        const int t = tid / (kWide / 4), col = tid % (kWide / 4) * 4, left = t < live ? dv - e0 - col : 0;
-        const f32x4 x = edge(xq, left), ev = edge(eq, left);
+        const int t = tid / (kWide / 4), col = tid % (kWide / 4) * 4;
+        const bool in = t < live && e0 + col < wide;
+        const f32x4 x = masked(xq, in), ev = masked(eq, in);
         put4<NV>(U + t * kWidePitch + col, Room::kSamples, betas[t] * x);
         float part = x[0] * ev[0];
 #pragma unroll
@@ -429,11 +414,12 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
         part += __shfl_xor(part, 4);
         if (col == 0) dbeta[t] += part;
       }
-      const int row = w0 + i, col = 8 * g, left = row < live ? dv - e0 - col : 0;
-      oraw.keep(grad_o && left > 0);
+      const int row = w0 + i, col = 8 * g;
+      const bool in = row < live && e0 + col < wide;
+      oraw.keep(grad_o && in);
       const Frag<NI> of = oraw.frag();
       float z[8];
-      const f32x4 z0 = edge(zq[0], left), z1 = edge(zq[1], left - 4);
+      const f32x4 z0 = masked(zq[0], in), z1 = masked(zq[1], in);
 #pragma unroll
       for (int e = 0; e < 4; ++e) z[e] = betas[row] * z0[e], z[4 + e] = betas[row] * z1[e];
       const Frag<NV> zf = frag_of<NV>(z);
@@ -456,23 +442,31 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
       }
       __syncthreads();
     }
-    renew(i, g);
     // the products that M and P were made of
     f32x4 kk[1][2], qk[1][2];
     clear(kk);
     clear(qk);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      const int col = 32 * s + 8 * g;
-      const Frag<NI> ak = krows.at(w0 + i, col), aq = qrows.at(w0 + i, col);
+      const Frag<NI> ak = own_frag(own.k, wave & 3, s), aq = own_frag(own.q, wave & 3, s);
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const Frag<NI> bk = krows.at(j0 + 16 * n + i, col);
+        const Frag<NI> bk = own_frag(own.k, 2 * half + n, s);
         mma(kk[0][n], ak, bk);
         mma(qk[0][n], aq, bk);
       }
     }
-    renew(i, g);
+    // keys and queries as the sums lie
+    f32x4 qv[1][NT], kv[1][NT];
+    clear(qv);
+    clear(kv);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int step = (d0 + 16 * n) / 32;
+      const Frag<1> one = NT == 1 && half ? eye[1] : eye[n & 1];   // tiles of both halves of a step
+      mma(qv[0][n], own_frag(own.q, wave & 3, step), one);
+      mma(kv[0][n], own_frag(own.k, wave & 3, step), one);
+    }
     // what passes a sample's decay from the state before the chunk, and to the one after
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -481,12 +475,10 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
       float from = 0.0f, to = 0.0f;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const int col = d0 + 16 * n + i;
-        const float qv = qrows.one(row, col), kv = krows.one(row, col);
         const float a = ss * qs[0][n][e], z = since * k2[0][n][e], u = until * k1[0][n][e];
-        from = fmaf(qv, a, from);
-        from = fmaf(-kv, z, from);
-        to = fmaf(kv, u, to);
+        from = fmaf(qv[0][n][e], a, from);
+        from = fmaf(-kv[0][n][e], z, from);
+        to = fmaf(kv[0][n][e], u, to);
         dQ[0][n][e] += a;
         dK[0][n][e] += u - z;
       }
@@ -518,14 +510,13 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int row = top + e;
-        bf16 p[NV], r[NV];
-        split<NV>(w[e], p);
-        split<NV>(y[e], r);
+        bf16x2 p[NV];
+        split<NV>(w[e], y[e], p);
 #pragma unroll
         for (int n2 = 0; n2 < NV; ++n2) {
-          W[n2 * Room::kFlat + row * kRow + col] = p[n2];
-          if (col <= row) Y[n2 * Room::kFlat + row * kRow + col] = r[n2];
-          if (col < row) Y[n2 * Room::kFlat + col * kRow + row] = r[n2];
+          W[n2 * Room::kFlat + row * kRow + col] = p[n2][0];
+          if (col <= row) Y[n2 * Room::kFlat + row * kRow + col] = p[n2][1];
+          if (col < row) Y[n2 * Room::kFlat + col * kRow + row] = p[n2][1];
         }
       }
     }
@@ -537,8 +528,7 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
                      yf = plane_frag<NV>(Y + from, Room::kFlat);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const int64_t at = turned + (d0 + 16 * n + i) * kChunk + 32 * s + 8 * g;
-        const Frag<NI> kf = eight(kt + at), qf = eight(qt + at);
+        const Frag<NI> kf = own_frag(own.kt, d0 / 16 + n, s), qf = own_frag(own.qt, d0 / 16 + n, s);
         mma(dQ[0][n], wf, kf);
         mma(dK[0][n], wt, qf);
         mma(dK[0][n], yf, kf);
@@ -592,23 +582,22 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
 
 // The backward's workspace (bytes).
 struct Space {
-  int64_t squares, kt, qt, dstates, es, adds, starts, keys, grads, all;
+  int64_t squares, keys, dstates, es, adds, starts, padded, grads, all;
 };
 Space space_of(const Delta& d, const Cut& cut) {
-  const int64_t heads = d.r.B * d.r.heads, turned = d.r.B * d.r.key_heads * d.chunks * turned_bytes(d.r);
+  const int64_t heads = d.r.B * d.r.heads;
   const auto next = [](int64_t n) { return (n + 255) / 256 * 256; };
   Space w;
   w.squares = 0;
-  w.kt = next(heads * d.chunks * squares_bytes(d.r.dtype));
-  w.qt = w.kt + next(turned);
-  w.dstates = w.qt + next(turned);
+  w.keys = next(heads * d.chunks * squares_bytes(d.r.dtype));
+  w.dstates = w.keys + next(d.r.B * d.r.key_heads * d.chunks * keys_bytes(d.r));
   w.es = w.dstates + next(heads * d.chunks * d.r.dk * wide_of(d.r) * 4);
   w.adds = w.es + next(heads * d.r.T * wide_of(d.r) * 4);
   const int64_t segments = cut.segs > 1 ? next(heads * cut.segs * d.r.dk * d.r.dv * 4) : 0;
   w.starts = w.adds + segments;
-  w.keys = w.starts + segments;
-  w.grads = w.keys + next(padded_keys(d.r));
-  w.all = w.grads + (d.r.dv % 8 ? heads * d.r.T * wide_of(d.r) * (d.r.dtype == CPAB_F32 ? 4 : 2) : 0);
+  w.padded = w.starts + segments;
+  w.grads = w.padded + next(padded_keys(d.r));
+  w.all = w.grads + padded_values(d.r);
   return w;
 }
 
@@ -636,44 +625,38 @@ hipError_t launch_delta_rule_backward(const cpab_delta_rule& r, const float* kep
     e = launch_delta_pad(r.dtype, grad_o, strides, r.B, r.T, r.heads, r.dv, room + w.grads, st);
     grad_o = room + w.grads;
   }
-  if (e == hipSuccess && d.chunks > 0) e = pad_keys(&d, room + w.keys, st);
-  if (e == hipSuccess && d.chunks > 0) e = launch_delta_squares(d, room + w.squares, room + w.kt, room + w.qt, st);
+  if (e == hipSuccess && d.chunks > 0) e = pad_keys(&d, room + w.padded, st);
+  if (e == hipSuccess && d.chunks > 0) e = launch_delta_squares(d, room + w.squares, room + w.keys, true, st);
   if (e != hipSuccess) return e;
   with_key(d, [&](auto t, auto dp) {
     typedef decltype(t) T;
     constexpr int DP = decltype(dp)::value, NV = Parts<T>::kValue, NI = Parts<T>::kInput;
     const Squares<T>* squares = reinterpret_cast<const Squares<T>*>(room + w.squares);
-    const T *kt = reinterpret_cast<const T*>(room + w.kt), *qt = reinterpret_cast<const T*>(room + w.qt);
-    const auto run = [&](auto width, auto only_ends) {
-      constexpr int E = decltype(width)::value;
+    const Keys<T, DP>* keys = reinterpret_cast<const Keys<T, DP>*>(room + w.keys);
+    const auto run = [&](auto only_ends) {
       constexpr bool ENDS = decltype(only_ends)::value;
-      constexpr int kRoom = 2 * E * (NV * (DP + 8) + (3 * NV + NI) * kRow);
+      constexpr int kRoom = 2 * kWide * (NV * (DP + 8) + (3 * NV + NI) * kRow);
       static LdsAllowed allowed;
-      e = allow_lds(reinterpret_cast<const void*>(delta_back_chain_kernel<T, DP, E, ENDS>), kRoom, allowed);
+      e = allow_lds(reinterpret_cast<const void*>(delta_back_chain_kernel<T, DP, ENDS>), kRoom, allowed);
       if (e != hipSuccess) return;
-      delta_back_chain_kernel<T, DP, E, ENDS>
-          <<<(unsigned)((heads * cut.segs + 7) / 8 * 8 * ((r.dv + E - 1) / E)), 8 * E, kRoom, st>>>(
-              d, squares, kt, qt, cut, (const T*)grad_o, grad_h, starts, (T*)grad_v, grad_h0, dstates, es, adds);
+      delta_back_chain_kernel<T, DP, ENDS>
+          <<<(unsigned)((heads * cut.segs + 7) / 8 * 8 * ((r.dv + kWide - 1) / kWide)), kDeltaBlock, kRoom, st>>>(
+              d, squares, keys, cut, (const T*)grad_o, grad_h, starts, (T*)grad_v, grad_h0, dstates, es, adds);
       e = hipGetLastError();
     };
-    const auto both = [&](auto only_ends) {
-      if constexpr (sizeof(T) == 2)
-        if (r.dv > 32) return run(std::integral_constant<int, 64>(), only_ends);
-      run(std::integral_constant<int, 32>(), only_ends);
-    };
     if (cut.segs > 1) {
-      both(std::true_type());
+      run(std::true_type());
       if (e == hipSuccess) e = launch_delta_join(d, cut, false, kept + k.ends, adds, grad_h, starts, st);
       if (e != hipSuccess) return;
     }
-    both(std::false_type());
+    run(std::false_type());
     if (e != hipSuccess || d.chunks == 0 || !(grad_q || grad_k || grad_decay || grad_beta)) return;
     constexpr int kRoom = PartsRoom<T, DP>::kBytes;
     static LdsAllowed allowed;
     e = allow_lds(reinterpret_cast<const void*>(delta_parts_kernel<T, DP>), kRoom, allowed);
     if (e != hipSuccess) return;
     delta_parts_kernel<T, DP><<<(unsigned)(r.B * r.key_heads * d.chunks), kPartsBlock, kRoom, st>>>(
-        d, squares, kt, qt, kept + k.states, kept + k.xs, dstates, es, (const T*)grad_o, (T*)grad_q,
+        d, squares, keys, kept + k.states, kept + k.xs, dstates, es, (const T*)grad_o, (T*)grad_q,
         (T*)grad_k, grad_decay, grad_beta);
     e = hipGetLastError();
   });
