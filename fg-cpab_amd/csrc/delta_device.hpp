@@ -365,15 +365,16 @@ __device__ __forceinline__ Where where(int64_t heads, int segs, int blocks) {
   return Where{group % heads, (int)(group / heads), (int)(slot % blocks), group < heads * segs};
 }
 
-// What a forward keeps, in floats: the states before each chunk, X, and the segments' ends.
+// What a forward keeps, in floats: the states before each chunk, X, and the segments' maps,
+// transposed.
 struct Kept {
-  int64_t states, xs, ends, all;
+  int64_t states, xs, maps, all;
 };
 Kept kept_of(const Delta& d, const Cut& cut);
 
 // squares: of each chunk of each head; keys: of each of each key's head.
 hipError_t launch_delta_squares(const Delta& d, void* squares, void* keys, bool backward, hipStream_t s);
-hipError_t launch_delta_join(const Delta& d, const Cut& cut, bool forward, const float* ends, const float* adds,
+hipError_t launch_delta_join(const Delta& d, const Cut& cut, bool forward, const float* maps, const float* adds,
                              const float* given, float* to, hipStream_t s);
 int64_t delta_backward_workspace(const Delta& d);   // bytes
 

@@ -203,7 +203,7 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, Squ
 template <typename T, int DP, bool ENDS>
 __global__ __launch_bounds__(kDeltaBlock, 2) void delta_chain_kernel(
     Delta d, const Squares<T>* squares, const Keys<T, DP>* keys, const float* starts, Cut cut, T* o,
-    float* h_out, float* states, float* xs, float* ends, int segs) {
+    float* h_out, float* states, float* xs, float* adds, float* maps, float* turned, int segs) {
   typedef Shares<DP> Sh;
   constexpr int E = kWide, kPitch = DP + 8, kSteps = DP / 32;
   constexpr int NV = Parts<T>::kValue, NI = Parts<T>::kInput, NO = Parts<T>::kOut;
@@ -215,12 +215,12 @@ __global__ __launch_bounds__(kDeltaBlock, 2) void delta_chain_kernel(
   bf16* Ht = Ut + NO * kSamples;   // U until the chunk's end
   const int dk = (int)d.r.dk, dv = (int)d.r.dv, blocks_v = (dv + E - 1) / E, wide = (dv + 7) / 8 * 8;
   const int64_t heads = d.r.B * d.r.heads;
-  const Where at = where(heads, segs, blocks_v + (ENDS ? (dk + E - 1) / E : 0));
+  const Where at = where(heads, segs, blocks_v + (ENDS ? DP / E : 0));
   if (!at.in) return;
   const int64_t bh = at.bh, b = bh / d.r.heads;
   const int h = (int)(bh - b * d.r.heads), kh = h / d.group;
   const bool unit = ENDS && at.block >= blocks_v;
-  const int e0 = (unit ? at.block - blocks_v : at.block) * E, width = unit ? dk : dv;
+  const int e0 = (unit ? at.block - blocks_v : at.block) * E;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int64_t length = live_of(d, b);
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(kDeltaBlock, 2) void delta_chain_kernel(
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int row = d0 + 16 * m + 4 * g + e, col = e0 + s0 + 16 * n + i;
-          if (row < dk && col < width) to[row * pitch + col] = S[m][n][e];
+          if (row < dk && col < dv) to[row * pitch + col] = S[m][n][e];
         }
   };
   const int chunks = (int)((length + kChunk - 1) / kChunk);
@@ -420,7 +420,20 @@ __global__ __launch_bounds__(kDeltaBlock, 2) void delta_chain_kernel(
     }
   }
   if (ENDS) {
-    put_state(ends + (bh * cut.segs + at.seg) * dk * (dv + dk) + (unit ? dv : 0), dv + dk);
+    const int64_t segment = bh * cut.segs + at.seg;
+    if (!unit) {
+      put_state(adds + segment * dk * dv, dv);
+      return;
+    }
+    // the map [DP, DP], as the join takes its rows, and transposed for the backward's
+#pragma unroll
+    for (int m = 0; m < Sh::MT; ++m)
+#pragma unroll
+      for (int n = 0; n < Sh::NT; ++n) {
+        const int row = d0 + 16 * m + 4 * g, col = e0 + s0 + 16 * n;
+        store4(maps + (segment * DP + row + (i & 3)) * DP + col + (i & 12), across(S[m][n]));
+        if (turned) store4(turned + (segment * DP + col + i) * DP + row, S[m][n]);
+      }
     return;
   }
   if (at.seg == (chunks > 0 ? (chunks - 1) / cut.each : 0)) put_state(h_out + bh * dk * dv, dv);
@@ -433,74 +446,72 @@ __global__ __launch_bounds__(kDeltaBlock, 2) void delta_chain_kernel(
 }
 
 // The states that the segments begin with, one after another: 16 columns to a workgroup.
-// FORWARD: starts[s + 1] = what segment s makes of starts[s] and what it adds.  Else the
-// gradients that they end with: from[s - 1] = the transposed of from[s] and what s adds.
+// FORWARD: to[s + 1] = what segment s makes of to[s] and what it adds.  Else the gradients
+// that they end with: to[s - 1] = the transposed map of s on to[s], and what s adds.  The map
+// and what is added are fetched a segment ahead.
 template <int DP, bool FORWARD>
-__global__ __launch_bounds__(kDeltaBlock) void delta_join_kernel(Delta d, Cut cut, const float* ends,
+__global__ __launch_bounds__(kDeltaBlock) void delta_join_kernel(Delta d, Cut cut, const float* maps,
                                                                const float* adds, const float* given, float* to) {
   constexpr int kPitch = DP + 8, kPlane = 16 * kPitch, kSteps = DP / 32, kTiles = (DP / 16 + 3) / 4;
   __shared__ __align__(16) bf16 St[3 * kPlane];
-  const int dk = (int)d.r.dk, dv = (int)d.r.dv, wide = dv + dk;
+  const int dk = (int)d.r.dk, dv = (int)d.r.dv;
   const int64_t heads = d.r.B * d.r.heads, bh = blockIdx.x % heads, b = bh / d.r.heads;
   const int col = (int)(blockIdx.x / heads) * 16 + (threadIdx.x & 15);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int chunks = (int)((live_of(d, b) + kChunk - 1) / kChunk);
   const int live = min((chunks + cut.each - 1) / cut.each, cut.segs);   // segments with samples
-  f32x4 S[kTiles];
+  const auto at = [&](int m) { return min(16 * (wave + 4 * m), DP - 16); };   // a wave's tile; waves beyond repeat the last
+  f32x4 S[kTiles], added[kTiles];
+  Raw<float> map[kTiles][kSteps];
+  const auto fetch = [&](int n) {
+    const int64_t s = bh * cut.segs + (FORWARD ? n : live - 1 - n);
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) {
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) map[m][k].fetch(maps + (s * DP + at(m) + i) * DP + 32 * k + 8 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        added[m][e] = adds[(s * dk + min(at(m) + 4 * g + e, dk - 1)) * dv + min(col, dv - 1)];
+    }
+  };
 #pragma unroll
   for (int m = 0; m < kTiles; ++m)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int row = 16 * (wave + 4 * m) + 4 * g + e;
+      const int row = at(m) + 4 * g + e;
       S[m][e] = given && row < dk && col < dv ? given[(bh * dk + row) * dv + col] : 0.0f;
     }
+  loaded();
+  if (live > 1) fetch(0);
   for (int n = 0; n + 1 < live; ++n) {
     const int s = FORWARD ? n : live - 1 - n;
-    const float* end = ends + (bh * cut.segs + s) * dk * wide;
-    const float* add = FORWARD ? end : adds + (bh * cut.segs + s) * dk * dv;
-    const int64_t pitch = FORWARD ? wide : dv;
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m) put4<3>(St + i * kPitch + at(m) + 4 * g, kPlane, S[m]);
     Frag<3> a[kTiles][kSteps];
-    f32x4 acc[kTiles];
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) {
-      const int tile = 16 * (wave + 4 * m);
+      S[m] = added[m];
 #pragma unroll
-      for (int k = 0; k < kSteps; ++k) {
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int row = FORWARD ? tile + i : 32 * k + 8 * g + e, c = FORWARD ? 32 * k + 8 * g + e : tile + i;
-          v[e] = row < dk && c < dk ? end[row * (int64_t)wide + dv + c] : 0.0f;
-        }
-        a[m][k] = frag_of<3>(v);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int row = tile + 4 * g + e;
-        acc[m][e] = row < dk && col < dv ? add[row * pitch + col] : 0.0f;
-      }
+      for (int k = 0; k < kSteps; ++k) a[m][k] = map[m][k].frag();
     }
-    __syncthreads();
-#pragma unroll
-    for (int m = 0; m < kTiles; ++m)
-      if (16 * (wave + 4 * m) < DP) put4<3>(St + i * kPitch + 16 * (wave + 4 * m) + 4 * g, kPlane, S[m]);
+    fetch(min(n + 1, live - 2));
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
       const Frag<3> st = plane_frag<3>(St + i * kPitch + 32 * k + 8 * g, kPlane);
 #pragma unroll
-      for (int m = 0; m < kTiles; ++m) mma(acc[m], a[m][k], st);
+      for (int m = 0; m < kTiles; ++m) mma(S[m], a[m][k], st);
     }
+    __syncthreads();
     float* out = to + (bh * cut.segs + (FORWARD ? s + 1 : s - 1)) * dk * dv;
 #pragma unroll
-    for (int m = 0; m < kTiles; ++m) {
-      S[m] = acc[m];
+    for (int m = 0; m < kTiles; ++m)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int row = 16 * (wave + 4 * m) + 4 * g + e;
-        if (row < dk && col < dv) out[(int64_t)row * dv + col] = acc[m][e];
+        const int row = at(m) + 4 * g + e;
+        if (row < dk && col < dv) out[(int64_t)row * dv + col] = S[m][e];
+        else S[m][e] = 0.0f;
       }
-    }
   }
 }
 
@@ -683,15 +694,15 @@ hipError_t launch_delta_squares(const Delta& d, void* squares, void* keys, bool 
   return hipGetLastError();
 }
 
-hipError_t launch_delta_join(const Delta& d, const Cut& cut, bool forward, const float* ends, const float* adds,
+hipError_t launch_delta_join(const Delta& d, const Cut& cut, bool forward, const float* maps, const float* adds,
                              const float* given, float* to, hipStream_t st) {
   with_key(d, [&](auto, auto dp) {
     constexpr int DP = decltype(dp)::value;
     const unsigned blocks = (unsigned)(d.r.B * d.r.heads * ((d.r.dv + 15) / 16));
     if (forward)
-      delta_join_kernel<DP, true><<<blocks, kDeltaBlock, 0, st>>>(d, cut, ends, adds, given, to);
+      delta_join_kernel<DP, true><<<blocks, kDeltaBlock, 0, st>>>(d, cut, maps, adds, given, to);
     else
-      delta_join_kernel<DP, false><<<blocks, kDeltaBlock, 0, st>>>(d, cut, ends, adds, given, to);
+      delta_join_kernel<DP, false><<<blocks, kDeltaBlock, 0, st>>>(d, cut, maps, adds, given, to);
   });
   return hipGetLastError();
 }
@@ -710,8 +721,8 @@ Kept kept_of(const Delta& d, const Cut& cut) {
   Kept k;
   k.states = 0;
   k.xs = heads * d.chunks * d.r.dk * wide_of(d.r);
-  k.ends = k.xs + heads * d.r.T * wide_of(d.r);
-  k.all = k.ends + (cut.segs > 1 ? heads * cut.segs * d.r.dk * (d.r.dv + d.r.dk) : 0);
+  k.maps = k.xs + heads * d.r.T * wide_of(d.r);
+  k.all = k.maps + (cut.segs > 1 ? heads * cut.segs * key_rows(d.r) * key_rows(d.r) : 0);
   return k;
 }
 int64_t delta_rule_kept(const cpab_delta_rule& r) {
@@ -723,17 +734,19 @@ namespace {
 
 // The forward's workspace (bytes).
 struct Room {
-  int64_t squares, keys, starts, ends, padded, values, all;
+  int64_t squares, keys, starts, adds, maps, padded, values, all;
 };
-Room room_of(const Delta& d, const Cut& cut, bool keep) {
+Room room_of(const Delta& d, const Cut& cut) {
   const int64_t heads = d.r.B * d.r.heads;
   const auto next = [](int64_t n) { return (n + 255) / 256 * 256; };
   Room w;
   w.squares = 0;
   w.keys = next(heads * d.chunks * squares_bytes(d.r.dtype));
   w.starts = w.keys + next(d.r.B * d.r.key_heads * d.chunks * keys_bytes(d.r));
-  w.ends = w.starts + (cut.segs > 1 ? next(heads * cut.segs * d.r.dk * d.r.dv * 4) : 0);
-  w.padded = w.ends + (cut.segs > 1 && !keep ? next(heads * cut.segs * d.r.dk * (d.r.dv + d.r.dk) * 4) : 0);
+  const int64_t segments = cut.segs > 1 ? heads * cut.segs : 0;
+  w.adds = w.starts + next(segments * d.r.dk * d.r.dv * 4);
+  w.maps = w.adds + next(segments * d.r.dk * d.r.dv * 4);
+  w.padded = w.maps + next(segments * key_rows(d.r) * key_rows(d.r) * 4);
   w.values = w.padded + next(padded_keys(d.r));
   w.all = w.values + padded_values(d.r);
   return w;
@@ -744,7 +757,7 @@ Room room_of(const Delta& d, const Cut& cut, bool keep) {
 int64_t delta_rule_workspace(const cpab_delta_rule& r, bool keep, bool backward) {
   const Delta d = delta_of(r);
   if (backward) return delta_backward_workspace(d);
-  return steps(r, keep) ? 0 : room_of(d, cut_of(d), keep).all;
+  return steps(r, keep) ? 0 : room_of(d, cut_of(d)).all;
 }
 
 hipError_t launch_delta_rule_forward(const cpab_delta_rule& r, void* o, float* h, float* kept,
@@ -760,11 +773,12 @@ hipError_t launch_delta_rule_forward(const cpab_delta_rule& r, void* o, float* h
     return hipGetLastError();
   }
   const Cut cut = cut_of(d);
-  const Room w = room_of(d, cut, kept != nullptr);
+  const Room w = room_of(d, cut);
   const Kept k = kept_of(d, cut);
   char* room = static_cast<char*>(workspace);
   float* starts = reinterpret_cast<float*>(room + w.starts);
-  float* ends = kept ? kept + k.ends : reinterpret_cast<float*>(room + w.ends);
+  float* adds = reinterpret_cast<float*>(room + w.adds);
+  float* maps = reinterpret_cast<float*>(room + w.maps);
   hipError_t e = pad_keys(&d, room + w.padded, st);
   if (e == hipSuccess && r.dv % 8 != 0) {
     e = launch_delta_pad(r.dtype, r.v, r.v_strides, r.B, r.T, r.heads, r.dv, room + w.values, st);
@@ -786,15 +800,16 @@ hipError_t launch_delta_rule_forward(const cpab_delta_rule& r, void* o, float* h
       static LdsAllowed allowed;
       e = allow_lds(reinterpret_cast<const void*>(delta_chain_kernel<T, DP, ENDS>), kRoom, allowed);
       if (e != hipSuccess) return;
-      const int64_t blocks = (r.dv + kWide - 1) / kWide + (ENDS ? (r.dk + kWide - 1) / kWide : 0);
+      const int64_t blocks = (r.dv + kWide - 1) / kWide + (ENDS ? DP / kWide : 0);
       delta_chain_kernel<T, DP, ENDS><<<(unsigned)((heads * segs + 7) / 8 * 8 * blocks), kDeltaBlock, kRoom, st>>>(
-          d, squares, keys, starts, cut, (T*)o, h, kept, kept ? kept + k.xs : nullptr, ends, segs);
+          d, squares, keys, starts, cut, (T*)o, h, kept, kept ? kept + k.xs : nullptr, adds, maps,
+          kept ? kept + k.maps : nullptr, segs);
       e = hipGetLastError();
     };
     if (cut.segs > 1) {
       // the backward takes what the last segment makes of the state too
       run(std::true_type(), kept ? cut.segs : cut.segs - 1);
-      if (e == hipSuccess) e = launch_delta_join(d, cut, true, ends, nullptr, r.h0, starts, st);
+      if (e == hipSuccess) e = launch_delta_join(d, cut, true, maps, adds, r.h0, starts, st);
       if (e != hipSuccess) return;
     }
     run(std::false_type(), cut.segs);

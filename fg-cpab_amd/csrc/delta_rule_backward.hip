@@ -262,38 +262,43 @@ __device__ __forceinline__ f32x4 masked(f32x4 v, bool in) {
   return v;
 }
 
-constexpr int kPartsBlock = 512;
 constexpr int kWidePitch = kWide + 8;
 
-template <typename T, int DP>
+// NP: the parts that a value goes as: two where every output has 16 bits.
+template <typename T, int DP, int NP>
 struct PartsRoom {
-  static constexpr int NV = Parts<T>::kValue;
+  // groups of waves over the columns: with 32-bit inputs four would leave too few registers
+  static constexpr int kGroups = DP == 32 || sizeof(T) == 4 ? 2 : 4, kBlock = 256 * kGroups;
   static constexpr int kState = DP * kWidePitch, kSamples = kChunk * kWidePitch, kFlat = kChunk * kRow;
-  // S, its gradient and U, then in their place W, its transpose and the other square
-  static constexpr int kLoop = NV * (2 * kState + kSamples), kAfter = 3 * NV * kFlat;
+  // S, its gradient, U and Z, then in their place W, its transpose and the other square
+  static constexpr int kLoop = NP * (2 * kState + 2 * kSamples), kAfter = 3 * NP * kFlat;
   static constexpr int kParts = kLoop > kAfter ? kLoop : kAfter;   // 16-bit values
   static constexpr int kBytes = 2 * kParts + 4 * kChunk * (kChunk + 1);
 };
 
 // A chunk of a key's head: the gradients of its queries and keys, added up over the heads
-// that share them, and of those heads' gates.  Of the eight waves four share the samples and
-// two the columns.
-template <typename T, int DP>
-__global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
+// that share them, and of those heads' gates.  Four waves share the samples, and groups of
+// four the columns.
+template <typename T, int DP, int NP>
+__global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_kernel(
     Delta d, const Squares<T>* squares, const Keys<T, DP>* keys, const float* states, const float* xs,
     const float* dstates, const float* es, const T* grad_o, T* grad_q, T* grad_k, void* grad_decay,
     void* grad_beta) {
-  typedef PartsRoom<T, DP> Room;
-  constexpr int NV = Parts<T>::kValue, NI = Parts<T>::kInput, kSteps = DP / 32, NT = DP / 32;
+  typedef PartsRoom<T, DP, NP> Room;
+  constexpr int kGroups = Room::kGroups, kBlock = Room::kBlock, kWaves = kBlock / 64;
+  constexpr int NI = Parts<T>::kInput, kSteps = DP / 32;
+  constexpr int NT = DP / 16 / kGroups, NJ = 4 / kGroups;   // tiles of DP and of the 64 to a wave
   extern __shared__ __align__(16) bf16 lds[];
   __shared__ double G[kChunk];
-  __shared__ float betas[kChunk], dbeta[kChunk], before[2][kChunk], after[2][kChunk], whole[8], sums[8][kChunk];
+  __shared__ float betas[kChunk], dbeta[kChunk], before[kGroups][kChunk], after[kGroups][kChunk], whole[kWaves],
+      sums[kWaves][kChunk];
   bf16* S = lds;                              // [DP][32]
-  bf16* L = S + NV * Room::kState;            // the gradient, [DP][32]
-  bf16* U = L + NV * Room::kState;            // [64][32]
+  bf16* L = S + NP * Room::kState;            // the gradient, [DP][32]
+  bf16* U = L + NP * Room::kState;            // [64][32]
+  bf16* Z = U + NP * Room::kSamples;
   bf16* W = lds;                              // scale D dP, [64][64]
-  bf16* Wt = W + NV * Room::kFlat;
-  bf16* Y = Wt + NV * Room::kFlat;            // D dA + (D dA)^T
+  bf16* Wt = W + NP * Room::kFlat;
+  bf16* Y = Wt + NP * Room::kFlat;            // D dA + (D dA)^T
   float* H = reinterpret_cast<float*>(lds + Room::kParts);   // dP P + dA A, [64][65]
   const int c = blockIdx.x % d.chunks;
   const int64_t rest = blockIdx.x / d.chunks, b = rest / d.r.key_heads;
@@ -301,16 +306,15 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
   const int dk = (int)d.r.dk, dv = (int)d.r.dv, wide = (dv + 7) / 8 * 8;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   int i = lane & 15, g = lane >> 4;
-  const int w0 = 16 * (wave & 3), half = wave >> 2;   // samples; columns of DP and of 64
-  const int d0 = half * (DP / 2), j0 = half * 32;
+  const int tile = wave & 3, w0 = 16 * tile, group = wave >> 2;   // samples; columns of DP and of 64
+  const int d0 = group * NT, j0 = group * NJ;                     // tiles
   const int64_t t0 = (int64_t)c * kChunk;
   const int live = (int)min(max(live_of(d, b) - t0, (int64_t)0), (int64_t)kChunk);
   const int rows = (int)min(d.r.T - t0, (int64_t)kChunk);   // that there are
   const Keys<T, DP>& own = keys[(b * d.r.key_heads + kh) * d.chunks + c];
-  const Frag<1> eye[2] = {unit_frag(0), unit_frag(1)};
-  const auto own_frag = [&](const auto& of, int tile, int step) {
+  const auto own_frag = [&](const auto& of, int row, int step) {
     Raw<T> r;
-    r.fetch(of[tile][step][threadIdx.x & 63]);
+    r.fetch(of[row][step][threadIdx.x & 63]);
     return r.frag();
   };
   f32x4 dQ[1][NT], dK[1][NT];
@@ -344,7 +348,7 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
     }
     const float* state = states + (bh * d.chunks + c) * dk * wide;
     const float* dstate = dstates + (bh * d.chunks + c) * dk * wide;
-    f32x4 qs[1][NT], k1[1][NT], k2[1][NT], P[1][2], ZU[1][2];
+    f32x4 qs[1][NT], k1[1][NT], k2[1][NT], P[1][NJ], ZU[1][NJ];
     clear(qs);
     clear(k1);
     clear(k2);
@@ -352,16 +356,16 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
     clear(ZU);
     float dot = 0.0f;
     const int64_t token = (b * d.r.T + t0) * d.r.heads + h;
-    const int across = (int)d.r.heads * wide;
-    const Rows<T> orows{(grad_o ? grad_o : reinterpret_cast<const T*>(es)) + token * wide, across, live, wide};
+    const int next_row = (int)d.r.heads * wide;
+    const Rows<T> orows{(grad_o ? grad_o : reinterpret_cast<const T*>(es)) + token * wide, next_row, live, wide};
     // the library's own: rows of whole eights, zeros beyond dv
     const Rows<float> srows{state, wide, dk, wide}, lrows{dstate, wide, dk, wide};
-    const Rows<float> xrows{xs + token * wide, across, live, wide}, erows{es + token * wide, across, live, wide};
+    const Rows<float> xrows{xs + token * wide, next_row, live, wide}, erows{es + token * wide, next_row, live, wide};
     // A block of columns is fetched while the matrix unit has the one before.
-    constexpr int kQuads = (DP * (kWide / 4) + kPartsBlock - 1) / kPartsBlock;
-    static_assert(kChunk * (kWide / 4) == kPartsBlock, "a quad of X to a lane");
+    constexpr int kAll = DP * (kWide / 4), kQuads = (kAll + kBlock - 1) / kBlock, kValues = kChunk * (kWide / 4);
+    static_assert(kValues <= kBlock, "a quad of X to a lane");
     int tid = threadIdx.x;
-    f32x4 sq4[kQuads], lq4[kQuads], xq, eq, zq[2];
+    f32x4 sq4[kQuads], lq4[kQuads], xq, eq;
     Raw<T> oraw;
     const auto load4 = [](const Rows<float>& r, int row, int col) {
       float w[4];
@@ -371,17 +375,14 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
     const auto fetch = [&](int e0) {
 #pragma unroll
       for (int n = 0; n < kQuads; ++n) {
-        const int at = tid + n * kPartsBlock, row = at / (kWide / 4), col = at % (kWide / 4) * 4;
+        const int at = tid + n * kBlock, row = at / (kWide / 4), col = at % (kWide / 4) * 4;
         sq4[n] = load4(srows, row, e0 + col);
         lq4[n] = load4(lrows, row, e0 + col);
       }
       const int t = tid / (kWide / 4), col = tid % (kWide / 4) * 4;
       xq = load4(xrows, t, e0 + col);
       eq = load4(erows, t, e0 + col);
-      // this wave's own samples of dO and Z
-      oraw.fetch(orows.template place<8>(w0 + i, e0 + 8 * g));
-      zq[0] = load4(erows, w0 + i, e0 + 8 * g);
-      zq[1] = load4(erows, w0 + i, e0 + 8 * g + 4);
+      oraw.fetch(orows.template place<8>(w0 + i, e0 + 8 * g));   // this wave's own samples of dO
     };
     __syncthreads();
     fetch(0);
@@ -391,21 +392,22 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
       i = tid & 15, g = tid >> 4 & 3;
 #pragma unroll
       for (int n = 0; n < kQuads; ++n) {
-        const int at = tid + n * kPartsBlock, row = at / (kWide / 4), col = at % (kWide / 4) * 4;
-        const bool in = row < dk && e0 + col < wide;
-        const f32x4 s = masked(sq4[n], in), l = masked(lq4[n], in);
-        if (DP * (kWide / 4) % kPartsBlock == 0 || at < DP * (kWide / 4)) {
-          put4<NV>(S + row * kWidePitch + col, Room::kState, s);
-          put4<NV>(L + row * kWidePitch + col, Room::kState, l);
-        }
+        const int at = tid + n * kBlock, row = at / (kWide / 4), col = at % (kWide / 4) * 4;
+        if (kAll % kBlock == 0 || at < kAll) {
+          const bool in = row < dk && e0 + col < wide;
+          const f32x4 s = masked(sq4[n], in), l = masked(lq4[n], in);
+          put4<NP>(S + row * kWidePitch + col, Room::kState, s);
+          put4<NP>(L + row * kWidePitch + col, Room::kState, l);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dot = fmaf(s[e], l[e], dot);
+          for (int e = 0; e < 4; ++e) dot = fmaf(s[e], l[e], dot);
+        }
       }
-      {
+      if (kValues == kBlock || tid < kValues) {
         const int t = tid / (kWide / 4), col = tid % (kWide / 4) * 4;
         const bool in = t < live && e0 + col < wide;
         const f32x4 x = masked(xq, in), ev = masked(eq, in);
-        put4<NV>(U + t * kWidePitch + col, Room::kSamples, betas[t] * x);
+        put4<NP>(U + t * kWidePitch + col, Room::kSamples, betas[t] * x);
+        put4<NP>(Z + t * kWidePitch + col, Room::kSamples, betas[t] * ev);
         float part = x[0] * ev[0];
 #pragma unroll
         for (int e = 1; e < 4; ++e) part = fmaf(x[e], ev[e], part);
@@ -414,44 +416,38 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
         part += __shfl_xor(part, 4);
         if (col == 0) dbeta[t] += part;
       }
-      const int row = w0 + i, col = 8 * g;
-      const bool in = row < live && e0 + col < wide;
-      oraw.keep(grad_o && in);
+      oraw.keep(grad_o && orows.in(w0 + i, e0 + 8 * g));
       const Frag<NI> of = oraw.frag();
-      float z[8];
-      const f32x4 z0 = masked(zq[0], in), z1 = masked(zq[1], in);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) z[e] = betas[row] * z0[e], z[4 + e] = betas[row] * z1[e];
-      const Frag<NV> zf = frag_of<NV>(z);
       fetch(min(e0 + kWide, (dv - 1) / kWide * kWide));
       __syncthreads();
-      const Frag<NV> uf = plane_frag<NV>(U + row * kWidePitch + col, Room::kSamples);
+      const int mine = (w0 + i) * kWidePitch + 8 * g;
+      const Frag<NP> uf = plane_frag<NP>(U + mine, Room::kSamples), zf = plane_frag<NP>(Z + mine, Room::kSamples);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const int at = (d0 + 16 * n + i) * kWidePitch + col;
-        const Frag<NV> s = plane_frag<NV>(S + at, Room::kState), l = plane_frag<NV>(L + at, Room::kState);
+        const int at = (16 * (d0 + n) + i) * kWidePitch + 8 * g;
+        const Frag<NP> s = plane_frag<NP>(S + at, Room::kState), l = plane_frag<NP>(L + at, Room::kState);
         mma(qs[0][n], of, s);
         mma(k2[0][n], zf, s);
         mma(k1[0][n], uf, l);
       }
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const Frag<NV> u = plane_frag<NV>(U + (j0 + 16 * n + i) * kWidePitch + col, Room::kSamples);
+      for (int n = 0; n < NJ; ++n) {
+        const Frag<NP> u = plane_frag<NP>(U + (16 * (j0 + n) + i) * kWidePitch + 8 * g, Room::kSamples);
         mma(P[0][n], of, u);
         mma(ZU[0][n], zf, u);
       }
       __syncthreads();
     }
     // the products that M and P were made of
-    f32x4 kk[1][2], qk[1][2];
+    f32x4 kk[1][NJ], qk[1][NJ];
     clear(kk);
     clear(qk);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      const Frag<NI> ak = own_frag(own.k, wave & 3, s), aq = own_frag(own.q, wave & 3, s);
+      const Frag<NI> ak = own_frag(own.k, tile, s), aq = own_frag(own.q, tile, s);
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const Frag<NI> bk = own_frag(own.k, 2 * half + n, s);
+      for (int n = 0; n < NJ; ++n) {
+        const Frag<NI> bk = own_frag(own.k, j0 + n, s);
         mma(kk[0][n], ak, bk);
         mma(qk[0][n], aq, bk);
       }
@@ -462,10 +458,9 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
     clear(kv);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int step = (d0 + 16 * n) / 32;
-      const Frag<1> one = NT == 1 && half ? eye[1] : eye[n & 1];   // tiles of both halves of a step
-      mma(qv[0][n], own_frag(own.q, wave & 3, step), one);
-      mma(kv[0][n], own_frag(own.k, wave & 3, step), one);
+      const Frag<1> one = unit_frag((d0 + n) & 1);   // tiles of both halves of a step
+      mma(qv[0][n], own_frag(own.q, tile, (d0 + n) / 2), one);
+      mma(kv[0][n], own_frag(own.k, tile, (d0 + n) / 2), one);
     }
     // what passes a sample's decay from the state before the chunk, and to the one after
 #pragma unroll
@@ -487,14 +482,14 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
         from += __shfl_xor(from, n);
         to += __shfl_xor(to, n);
       }
-      if (i == 0) before[half][row] = from, after[half][row] = to;
+      if (i == 0) before[group][row] = from, after[group][row] = to;
     }
 #pragma unroll
     for (int n = 1; n < 64; n *= 2) dot += __shfl_xor(dot, n);
     if (lane == 0) whole[wave] = dot;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int col = j0 + 16 * n + i;
+    for (int n = 0; n < NJ; ++n) {
+      const int other = j0 + n, col = 16 * other + i, flat = Room::kFlat;
       f32x4 w, y;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -504,19 +499,24 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
         y[e] = col < row ? -decay * ZU[0][n][e] : 0.0f;
         H[row * (kChunk + 1) + col] = w[e] * qk[0][n][e] + y[e] * kk[0][n][e];
       }
-      put4<NV>(Wt + col * kRow + w0 + 4 * g, Room::kFlat, w);
-      // both halves of Y: above the diagonal its mirror image
-      const int top = w0 + 4 * g;
+      const int row4 = (w0 + 4 * g + (i & 3)) * kRow + 16 * other + (i & 12);
+      put4<NP>(Wt + col * kRow + w0 + 4 * g, flat, w);
+      put4<NP>(W + row4, flat, across(w));
+      // Y: a tile below the diagonal, and its mirror image above it
+      if (other < tile) {
+        put4<NP>(Y + col * kRow + w0 + 4 * g, flat, y);
+        put4<NP>(Y + row4, flat, across(y));
+      } else if (other == tile) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int row = top + e;
-        bf16x2 p[NV];
-        split<NV>(w[e], y[e], p);
+        for (int e = 0; e < 4; ++e) {
+          const int row = w0 + 4 * g + e;
+          bf16x2 p[NP];
+          split<NP>(y[e], y[e], p);
 #pragma unroll
-        for (int n2 = 0; n2 < NV; ++n2) {
-          W[n2 * Room::kFlat + row * kRow + col] = p[n2][0];
-          if (col <= row) Y[n2 * Room::kFlat + row * kRow + col] = p[n2][1];
-          if (col < row) Y[n2 * Room::kFlat + col * kRow + row] = p[n2][1];
+          for (int k = 0; k < NP; ++k) {
+            if (col <= row) Y[k * flat + row * kRow + col] = p[k][0];
+            if (col < row) Y[k * flat + col * kRow + row] = p[k][0];
+          }
         }
       }
     }
@@ -524,23 +524,23 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int from = (w0 + i) * kRow + 32 * s + 8 * g;
-      const Frag<NV> wf = plane_frag<NV>(W + from, Room::kFlat), wt = plane_frag<NV>(Wt + from, Room::kFlat),
-                     yf = plane_frag<NV>(Y + from, Room::kFlat);
+      const Frag<NP> wf = plane_frag<NP>(W + from, Room::kFlat), wt = plane_frag<NP>(Wt + from, Room::kFlat),
+                     yf = plane_frag<NP>(Y + from, Room::kFlat);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const Frag<NI> kf = own_frag(own.kt, d0 / 16 + n, s), qf = own_frag(own.qt, d0 / 16 + n, s);
+        const Frag<NI> kf = own_frag(own.kt, d0 + n, s), qf = own_frag(own.qt, d0 + n, s);
         mma(dQ[0][n], wf, kf);
         mma(dK[0][n], wt, qf);
         mma(dK[0][n], yf, kf);
       }
     }
-    // the decays: a wave has 8 of the rows, a lane a sample; what crosses it from the columns
-    // before, for each row from it on
+    // the decays: the waves share the rows, a lane has a sample; what crosses it from the
+    // columns before, for each row from it on
     {
       float sum = 0.0f;
-      for (int n = 0; n < 8; ++n) {
-        const int row = 8 * wave + n;
-        float v = H[row * (kChunk + 1) + lane];
+      for (int n = 0; n < kChunk / kWaves; ++n) {
+        const int row = kChunk / kWaves * wave + n;
+        float v = H[row * (kChunk + 1) + lane], from = 0.0f, to = 0.0f;
 #pragma unroll
         for (int m = 1; m < 64; m *= 2) {
           const float prior = __shfl_up(v, m);
@@ -548,8 +548,9 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
         }
         v = __shfl_up(v, 1);   // of the columns before
         if (lane == 0) v = 0.0f;
-        if (row >= lane) sum += v + (before[0][row] + before[1][row]);
-        else sum += after[0][row] + after[1][row];
+#pragma unroll
+        for (int m = 0; m < kGroups; ++m) from += before[m][row], to += after[m][row];
+        sum += row >= lane ? v + from : to;
       }
       sums[wave][lane] = sum;
     }
@@ -558,7 +559,7 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
       const int t = threadIdx.x;
       float dots = 0.0f, sum = 0.0f;
 #pragma unroll
-      for (int n = 0; n < 8; ++n) dots += whole[n], sum += sums[n][t];
+      for (int n = 0; n < kWaves; ++n) dots += whole[n], sum += sums[n][t];
       sum = fmaf(sq.gates.since[kChunk - 1], dots, sum);
       if (t < rows) {
         const int64_t at = (b * d.r.T + t0 + t) * d.r.heads + h;
@@ -572,7 +573,7 @@ __global__ __launch_bounds__(kPartsBlock) void delta_parts_kernel(
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int t = w0 + 4 * g + e, col = d0 + 16 * n + i;
+      const int t = w0 + 4 * g + e, col = 16 * (d0 + n) + i;
       if (t >= rows || col >= dk) continue;
       const int64_t at = ((b * d.r.T + t0 + t) * d.r.key_heads + kh) * dk + col;
       if (grad_q) grad_q[at] = from_float<T>(dQ[0][n][e]);
@@ -646,19 +647,25 @@ hipError_t launch_delta_rule_backward(const cpab_delta_rule& r, const float* kep
     };
     if (cut.segs > 1) {
       run(std::true_type());
-      if (e == hipSuccess) e = launch_delta_join(d, cut, false, kept + k.ends, adds, grad_h, starts, st);
+      if (e == hipSuccess) e = launch_delta_join(d, cut, false, kept + k.maps, adds, grad_h, starts, st);
       if (e != hipSuccess) return;
     }
     run(std::false_type());
     if (e != hipSuccess || d.chunks == 0 || !(grad_q || grad_k || grad_decay || grad_beta)) return;
-    constexpr int kRoom = PartsRoom<T, DP>::kBytes;
-    static LdsAllowed allowed;
-    e = allow_lds(reinterpret_cast<const void*>(delta_parts_kernel<T, DP>), kRoom, allowed);
-    if (e != hipSuccess) return;
-    delta_parts_kernel<T, DP><<<(unsigned)(r.B * r.key_heads * d.chunks), kPartsBlock, kRoom, st>>>(
-        d, squares, keys, kept + k.states, kept + k.xs, dstates, es, (const T*)grad_o, (T*)grad_q,
-        (T*)grad_k, grad_decay, grad_beta);
-    e = hipGetLastError();
+    const auto parts = [&](auto np) {
+      constexpr int NP = decltype(np)::value;
+      typedef PartsRoom<T, DP, NP> Room;
+      static LdsAllowed allowed;
+      e = allow_lds(reinterpret_cast<const void*>(delta_parts_kernel<T, DP, NP>), Room::kBytes, allowed);
+      if (e != hipSuccess) return;
+      delta_parts_kernel<T, DP, NP><<<(unsigned)(r.B * r.key_heads * d.chunks), Room::kBlock, Room::kBytes, st>>>(
+          d, squares, keys, kept + k.states, kept + k.xs, dstates, es, (const T*)grad_o, (T*)grad_q,
+          (T*)grad_k, grad_decay, grad_beta);
+      e = hipGetLastError();
+    };
+    if constexpr (sizeof(T) == 2)
+      if (r.gate_dtype == CPAB_BF16) return parts(std::integral_constant<int, 2>());
+    parts(std::integral_constant<int, 3>());
   });
   return e;
 }
