@@ -103,7 +103,22 @@ __device__ __forceinline__ Frag<N> frag_of(const float v[8]) {
   }
   return f;
 }
-// acc += A B^T: 16 x 16, over 32 of the summed index.
+// acc[m][n] += A[m] B[n]^T: 16 x 16 each, over 32 of the summed index.  The tiles in turn for
+// each pair of parts: a product waits for the one before it in its own sums.
+template <int MT, int NT, int NA, int NB>
+__device__ __forceinline__ void mma(f32x4 (&acc)[MT][NT], const Frag<NA> (&a)[MT], const Frag<NB> (&b)[NT]) {
+  constexpr int kLast = (NA > NB ? NA : NB) - 1;
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      if (i + j <= kLast)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m].p[i], b[n].p[j], acc[m][n], 0, 0, 0);
+}
 template <int NA, int NB>
 __device__ __forceinline__ void mma(f32x4& acc, const Frag<NA>& a, const Frag<NB>& b) {
   constexpr int kLast = (NA > NB ? NA : NB) - 1;

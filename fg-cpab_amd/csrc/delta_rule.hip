@@ -123,13 +123,12 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, Squ
       rk.put(own.k[wave][s][lane]);
       rq.put(own.q[wave][s][lane]);
     }
-    const Frag<NI> ak = rk.frag(), aq = rq.frag();
+    const Frag<NI> ak[1] = {rk.frag()}, aq[1] = {rq.frag()};
+    Frag<NI> bk[4];
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const Frag<NI> bk = krows.at(16 * n + i, col);
-      mma(kk[0][n], ak, bk);
-      mma(qk[0][n], aq, bk);
-    }
+    for (int n = 0; n < 4; ++n) bk[n] = krows.at(16 * n + i, col);
+    mma(kk, ak, bk);
+    mma(qk, aq, bk);
   }
   __syncthreads();
   float* Ab = room;                   // A beta
@@ -338,13 +337,12 @@ __global__ __launch_bounds__(kDeltaBlock, 2) void delta_chain_kernel(
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         if (s + 1 < kSteps) read(s + 1);
-        const Frag<NI> kv = kf[s].frag();
-#pragma unroll
-        for (int n = 0; n < 2; ++n) mma(R[0][n], kv, st[s & 1][n]);
+        const Frag<NI> kv[1] = {kf[s].frag()};
+        mma(R, kv, st[s & 1]);
         if (!ENDS) {
-          const Frag<NI> qv = qf[s].frag();
-#pragma unroll
-          for (int n = 0; n < 2; ++n) mma(O[n][0], first_of<NO>(st[s & 1][n]), qv);
+          const Frag<NI> qv[1] = {qf[s].frag()};
+          const Frag<NO> so[2] = {first_of<NO>(st[s & 1][0]), first_of<NO>(st[s & 1][1])};
+          mma(O, so, qv);
         }
       }
     }
@@ -366,9 +364,10 @@ __global__ __launch_bounds__(kDeltaBlock, 2) void delta_chain_kernel(
 #pragma unroll
         for (int n = 0; n < 2; ++n) rt[s][n] = plane_frag<NV>(Rt + (16 * n + i) * kRow + 32 * s + 8 * g, kSamples);
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int n = 0; n < 2; ++n) mma(X[0][n], mf[s], rt[s][n]);
+      for (int s = 0; s < 2; ++s) {
+        const Frag<NV> mv[1] = {mf[s]};
+        mma(X, mv, rt[s]);
+      }
     }
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
@@ -396,20 +395,22 @@ __global__ __launch_bounds__(kDeltaBlock, 2) void delta_chain_kernel(
         for (int n = 0; n < Sh::NT; ++n)
           ht[s][n] = plane_frag<NV>(Ht + (s0 + 16 * n + i) * kRow + 32 * s + 8 * g, kSamples);
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < 2; ++s) {
+        Frag<NI> kv[Sh::MT];
 #pragma unroll
-        for (int m = 0; m < Sh::MT; ++m) {
-          const Frag<NI> kv = ktf[m][s].frag();
-#pragma unroll
-          for (int n = 0; n < Sh::NT; ++n) mma(S[m][n], kv, ht[s][n]);
-        }
+        for (int m = 0; m < Sh::MT; ++m) kv[m] = ktf[m][s].frag();
+        mma(S, kv, ht[s]);
+      }
     }
     if (!ENDS) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < 2; ++s) {
+        Frag<NO> ut[2];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-          mma(O[n][0], plane_frag<NO>(Ut + (16 * n + i) * kRow + 32 * s + 8 * g, kSamples), pf[s]);
+        for (int n = 0; n < 2; ++n) ut[n] = plane_frag<NO>(Ut + (16 * n + i) * kRow + 32 * s + 8 * g, kSamples);
+        const Frag<NO> pv[1] = {pf[s]};
+        mma(O, ut, pv);
+      }
     }
     fetch_rest(next);
     if (ENDS) continue;

@@ -158,9 +158,8 @@ __global__ __launch_bounds__(kDeltaBlock, 2) void delta_back_chain_kernel(
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         if (s + 1 < kSteps) read(s + 1);
-        const Frag<NI> kv = kf[s].frag();
-#pragma unroll
-        for (int n = 0; n < 2; ++n) mma(U[0][n], kv, st[s & 1][n]);
+        const Frag<NI> kv[1] = {kf[s].frag()};
+        mma(U, kv, st[s & 1]);
       }
     }
     {
@@ -172,9 +171,10 @@ __global__ __launch_bounds__(kDeltaBlock, 2) void delta_back_chain_kernel(
 #pragma unroll
       for (int n = 0; n < 2; ++n) U[0][n] *= until;
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int n = 0; n < 2; ++n) mma(U[0][n], pf[s], ot[s][n]);
+      for (int s = 0; s < 2; ++s) {
+        const Frag<NV> pv[1] = {pf[s]};
+        mma(U, pv, ot[s]);
+      }
     }
 #pragma unroll
     for (int n = 0; n < 2; ++n) put4<NV>(Bt + (16 * n + i) * kRow + w0 + 4 * g, kSamples, beta * U[0][n]);
@@ -187,9 +187,10 @@ __global__ __launch_bounds__(kDeltaBlock, 2) void delta_back_chain_kernel(
 #pragma unroll
         for (int n = 0; n < 2; ++n) bt[s][n] = plane_frag<NV>(Bt + (16 * n + i) * kRow + 32 * s + 8 * g, kSamples);
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int n = 0; n < 2; ++n) mma(V[0][n], mf[s], bt[s][n]);
+      for (int s = 0; s < 2; ++s) {
+        const Frag<NV> mv[1] = {mf[s]};
+        mma(V, mv, bt[s]);
+      }
     }
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
@@ -220,15 +221,11 @@ __global__ __launch_bounds__(kDeltaBlock, 2) void delta_back_chain_kernel(
         gt[n] = plane_frag<NV>(Gt + from, kSamples);
         zt[n] = plane_frag<NV>(Zt + from, kSamples);
       }
+      Frag<NI> qv[Sh::MT], kv[Sh::MT];
 #pragma unroll
-      for (int m = 0; m < Sh::MT; ++m) {
-        const Frag<NI> qv = qtf[m][s].frag(), kv = ktf[m][s].frag();
-#pragma unroll
-        for (int n = 0; n < Sh::NT; ++n) {
-          mma(S[m][n], qv, gt[n]);
-          mma(S[m][n], kv, zt[n]);
-        }
-      }
+      for (int m = 0; m < Sh::MT; ++m) qv[m] = qtf[m][s].frag(), kv[m] = ktf[m][s].frag();
+      mma(S, qv, gt);
+      mma(S, kv, zt);
     }
     fetch_turned(next);
   }
@@ -417,25 +414,24 @@ __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_ke
         if (col == 0) dbeta[t] += part;
       }
       oraw.keep(grad_o && orows.in(w0 + i, e0 + 8 * g));
-      const Frag<NI> of = oraw.frag();
+      const Frag<NI> of[1] = {oraw.frag()};
       fetch(min(e0 + kWide, (dv - 1) / kWide * kWide));
       __syncthreads();
       const int mine = (w0 + i) * kWidePitch + 8 * g;
-      const Frag<NP> uf = plane_frag<NP>(U + mine, Room::kSamples), zf = plane_frag<NP>(Z + mine, Room::kSamples);
+      const Frag<NP> uf[1] = {plane_frag<NP>(U + mine, Room::kSamples)}, zf[1] = {plane_frag<NP>(Z + mine, Room::kSamples)};
+      Frag<NP> sf[NT], lf[NT], tf[NJ];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int at = (16 * (d0 + n) + i) * kWidePitch + 8 * g;
-        const Frag<NP> s = plane_frag<NP>(S + at, Room::kState), l = plane_frag<NP>(L + at, Room::kState);
-        mma(qs[0][n], of, s);
-        mma(k2[0][n], zf, s);
-        mma(k1[0][n], uf, l);
+        sf[n] = plane_frag<NP>(S + at, Room::kState), lf[n] = plane_frag<NP>(L + at, Room::kState);
       }
 #pragma unroll
-      for (int n = 0; n < NJ; ++n) {
-        const Frag<NP> u = plane_frag<NP>(U + (16 * (j0 + n) + i) * kWidePitch + 8 * g, Room::kSamples);
-        mma(P[0][n], of, u);
-        mma(ZU[0][n], zf, u);
-      }
+      for (int n = 0; n < NJ; ++n) tf[n] = plane_frag<NP>(U + (16 * (j0 + n) + i) * kWidePitch + 8 * g, Room::kSamples);
+      mma(qs, of, sf);
+      mma(k2, zf, sf);
+      mma(k1, uf, lf);
+      mma(P, of, tf);
+      mma(ZU, zf, tf);
       __syncthreads();
     }
     // the products that M and P were made of
@@ -444,13 +440,12 @@ __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_ke
     clear(qk);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      const Frag<NI> ak = own_frag(own.k, tile, s), aq = own_frag(own.q, tile, s);
+      const Frag<NI> ak[1] = {own_frag(own.k, tile, s)}, aq[1] = {own_frag(own.q, tile, s)};
+      Frag<NI> bk[NJ];
 #pragma unroll
-      for (int n = 0; n < NJ; ++n) {
-        const Frag<NI> bk = own_frag(own.k, j0 + n, s);
-        mma(kk[0][n], ak, bk);
-        mma(qk[0][n], aq, bk);
-      }
+      for (int n = 0; n < NJ; ++n) bk[n] = own_frag(own.k, j0 + n, s);
+      mma(kk, ak, bk);
+      mma(qk, aq, bk);
     }
     // keys and queries as the sums lie
     f32x4 qv[1][NT], kv[1][NT];
@@ -524,15 +519,14 @@ __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_ke
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int from = (w0 + i) * kRow + 32 * s + 8 * g;
-      const Frag<NP> wf = plane_frag<NP>(W + from, Room::kFlat), wt = plane_frag<NP>(Wt + from, Room::kFlat),
-                     yf = plane_frag<NP>(Y + from, Room::kFlat);
+      const Frag<NP> wf[1] = {plane_frag<NP>(W + from, Room::kFlat)}, wt[1] = {plane_frag<NP>(Wt + from, Room::kFlat)},
+                     yf[1] = {plane_frag<NP>(Y + from, Room::kFlat)};
+      Frag<NI> kf[NT], qf[NT];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const Frag<NI> kf = own_frag(own.kt, d0 + n, s), qf = own_frag(own.qt, d0 + n, s);
-        mma(dQ[0][n], wf, kf);
-        mma(dK[0][n], wt, qf);
-        mma(dK[0][n], yf, kf);
-      }
+      for (int n = 0; n < NT; ++n) kf[n] = own_frag(own.kt, d0 + n, s), qf[n] = own_frag(own.qt, d0 + n, s);
+      mma(dQ, wf, kf);
+      mma(dK, wt, qf);
+      mma(dK, yf, kf);
     }
     // the decays: the waves share the rows, a lane has a sample; what crosses it from the
     // columns before, for each row from it on
