@@ -19,6 +19,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "cpab_launch.hpp"
 #include "sequence_device.hpp"
 #include "sequence_launch.hpp"
 
@@ -32,6 +33,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kLanes = 256;
+constexpr int kSmallSide = 256;    // of the matrices whose products go in tiles of 64
 constexpr int kMatrices = 40;      // of a launch
 constexpr int kSpan = kLanes * 16; // values of a workgroup of the momentum's kernel
 constexpr float kUp = 1024.0f, kDown = 1.0f / 1024.0f, kLow = 2048.0f, kJoin = 1.0f / 2048.0f;
@@ -52,8 +54,12 @@ struct Batch {
   uint32_t first[kMatrices + 1];   // workgroups before each matrix's
 };
 
-constexpr int kPad = 64;
-__host__ __device__ __forceinline__ int64_t padded(int64_t n) { return (n + kPad - 1) / kPad * kPad; }
+// Tiles of a product: 128 x 128 where a matrix' shorter side is long enough that padding it
+// to whole tiles costs little, else 64 x 64.
+__host__ __device__ __forceinline__ int tile_of(int64_t rows, int64_t cols) {
+  return (rows < cols ? rows : cols) > kSmallSide ? 128 : 64;
+}
+__host__ __device__ __forceinline__ int64_t padded(int64_t n, int tile) { return (n + tile - 1) / tile * tile; }
 struct Places {
   int64_t m, n;   // padded
   int64_t sums, x0, x1, xt0, xt1, a, b, end;   // x: [m, n]; xt: [n, m]
@@ -62,8 +68,9 @@ struct Places {
 };
 __host__ __device__ __forceinline__ Places places(int64_t rows, int64_t cols) {
   Places p;
-  p.m = padded(rows < cols ? rows : cols);
-  p.n = padded(rows < cols ? cols : rows);
+  const int tile = tile_of(rows, cols);
+  p.m = padded(rows < cols ? rows : cols, tile);
+  p.n = padded(rows < cols ? cols : rows, tile);
   const int64_t spans = (rows * cols + kSpan - 1) / kSpan;
   p.sums = 0;
   p.x0 = (spans * 8 + 255) / 256 * 256;
@@ -205,11 +212,13 @@ struct Coefficients {
   int from;   // which of the two X
 };
 
-// One tile of a product.  64 x 64: a wave has 32 x 32 of it, in two sums.
-template <Product WHAT, typename T>
-__global__ __launch_bounds__(kLanes) void muon_product_kernel(Batch batch, int count, Coefficients c, char* room) {
-  constexpr int kTile = 64, kStepK = 32, kPitch = kStepK + 8;
-  __shared__ f16 lds[2][4][kTile][kPitch];   // twice: rows' hi and lo, columns' hi and lo
+// One tile of a product: a wave has a quarter of it, in two sums.  32 of the summed index lie
+// in LDS twice, as the matrix unit has the one and memory brings the other; rows of 64 bytes
+// begin 20 banks apart, so that a wave's wide reads meet no bank twice.
+template <Product WHAT, typename T, int TILE>
+__global__ __launch_bounds__(kLanes, 2) void muon_product_kernel(Batch batch, int count, Coefficients c, char* room) {
+  constexpr int kStepK = 32, kPitch = kStepK + 8, kEach = TILE / 64, MT = TILE / 64;
+  extern __shared__ __align__(16) f16 lds[];   // [2][4][TILE][kPitch]: rows' hi and lo, columns' hi and lo
   const int which = find(batch, count);
   const Matrix& t = batch.m[which];
   const Places p = places(t.rows, t.cols);
@@ -222,7 +231,7 @@ __global__ __launch_bounds__(kLanes) void muon_product_kernel(Batch batch, int c
     while ((tj + 1) * (tj + 2) / 2 <= tile) ++tj;
     ti = tile - tj * (tj + 1) / 2;
   } else {
-    const int64_t down = p.m / kTile;
+    const int64_t down = p.m / TILE;
     ti = tile % down;
     tj = tile / down;
   }
@@ -236,99 +245,122 @@ __global__ __launch_bounds__(kLanes) void muon_product_kernel(Batch batch, int c
   const f16* right = WHAT == kGram ? x : WHAT == kPolynomial ? a : xt;
   const int64_t left_plane = WHAT == kGram ? whole : square;
   const int64_t right_plane = WHAT == kPolynomial ? square : whole;
-  left += ti * kTile * K;
-  right += tj * kTile * K;
-  // a lane brings 16 bytes of each of the four arrays
+  left += ti * TILE * K;
+  right += tj * TILE * K;
+  // a lane brings 16 bytes of some rows of each of the four arrays
   const int row = threadIdx.x >> 2, part = (threadIdx.x & 3) * 8;
   const f16* from[4] = {left + row * K + part, left + left_plane + row * K + part,
                         right + row * K + part, right + right_plane + row * K + part};
-  u32x4 next[4];
+  u32x4 next[4][kEach];
+  const auto fetch = [&](int64_t k0) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) next[k] = *reinterpret_cast<const u32x4*>(from[k]);
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) next[k][e] = *reinterpret_cast<const u32x4*>(from[k] + 64 * e * K + k0);
+  };
+  fetch(0);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 31, g = lane >> 5;
-  const int wr = (wave >> 1) * 32, wc = (wave & 1) * 32;
-  f32x16 acc = {}, low = {};
+  const int wr = (wave >> 1) * (TILE / 2), wc = (wave & 1) * (TILE / 2);
+  f32x16 acc[MT][MT] = {}, low[MT][MT] = {};
   int buffer = 0;
   for (int64_t k0 = 0; k0 < K; k0 += kStepK, buffer ^= 1) {
+    f16* const now = lds + buffer * 4 * TILE * kPitch;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) *reinterpret_cast<u32x4*>(&lds[buffer][k][row][part]) = next[k];
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        *reinterpret_cast<u32x4*>(now + (k * TILE + row + 64 * e) * kPitch + part) = next[k][e];
     __syncthreads();
-    if (k0 + kStepK < K)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) next[k] = *reinterpret_cast<const u32x4*>(from[k] + k0 + kStepK);
+    if (k0 + kStepK < K) fetch(k0 + kStepK);
 #pragma unroll
     for (int k = 0; k < kStepK; k += 16) {
-      const f16x8 lh = *reinterpret_cast<const f16x8*>(&lds[buffer][0][wr + i][k + 8 * g]);
-      const f16x8 ll = *reinterpret_cast<const f16x8*>(&lds[buffer][1][wr + i][k + 8 * g]);
-      const f16x8 rh = *reinterpret_cast<const f16x8*>(&lds[buffer][2][wc + i][k + 8 * g]);
-      const f16x8 rl = *reinterpret_cast<const f16x8*>(&lds[buffer][3][wc + i][k + 8 * g]);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rh, acc, 0, 0, 0);
-      low = __builtin_amdgcn_mfma_f32_32x32x16_f16(lh, rl, low, 0, 0, 0);
-      low = __builtin_amdgcn_mfma_f32_32x32x16_f16(ll, rh, low, 0, 0, 0);
+      f16x8 l[2][MT], r[2][MT];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          l[h][m] = *reinterpret_cast<const f16x8*>(now + (h * TILE + wr + 32 * m + i) * kPitch + k + 8 * g);
+          r[h][m] = *reinterpret_cast<const f16x8*>(now + ((2 + h) * TILE + wc + 32 * m + i) * kPitch + k + 8 * g);
+        }
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < MT; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[0][m], r[0][n], acc[m][n], 0, 0, 0);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < MT; ++n) low[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[0][m], r[1][n], low[m][n], 0, 0, 0);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < MT; ++n) low[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[1][m], r[0][n], low[m][n], 0, 0, 0);
     }
   }
-  // a lane's column, and its 16 rows: four at a time, 8 apart
-  const int64_t col = tj * kTile + wc + i;
+  // a lane's column, and 16 rows of each 32: four at a time, 8 apart
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int64_t r0 = ti * kTile + wr + 8 * q + 4 * g;
-    float v[4];
+  for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = fmaf(low[4 * q + e], kJoin, acc[4 * q + e]) * (kDown * kDown);
-    if (WHAT == kPolynomial) {
+    for (int n = 0; n < MT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float av = fmaf((float)a[square + (r0 + e) * p.m + col], kJoin, (float)a[(r0 + e) * p.m + col]) * kDown;
-        v[e] = fmaf(c.c2, v[e], c.c1 * av);
+      for (int q = 0; q < 4; ++q) {
+        const int64_t col = tj * TILE + wc + 32 * n + i, r0 = ti * TILE + wr + 32 * m + 8 * q + 4 * g;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = fmaf(low[m][n][4 * q + e], kJoin, acc[m][n][4 * q + e]) * (kDown * kDown);
+        if (WHAT == kPolynomial) {   // A is its own transpose
+          const f16x4 hi = *reinterpret_cast<const f16x4*>(a + col * p.m + r0);
+          const f16x4 lo = *reinterpret_cast<const f16x4*>(a + square + col * p.m + r0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            v[e] = fmaf(c.c2, v[e], c.c1 * (fmaf((float)lo[e], kJoin, (float)hi[e]) * kDown));
+        }
+        if (WHAT == kStep || WHAT == kLast) {
+          const f16x4 hi = *reinterpret_cast<const f16x4*>(xt + col * p.m + r0);
+          const f16x4 lo = *reinterpret_cast<const f16x4*>(xt + whole + col * p.m + r0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(c.c0, fmaf((float)lo[e], kJoin, (float)hi[e]) * kDown, v[e]);
+        }
+        if (WHAT == kLast) {
+          const bool wide = t.rows <= t.cols;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int64_t pr = wide ? r0 + e : col, pc = wide ? col : r0 + e;
+            if (pr >= t.rows || pc >= t.cols) continue;
+            const int64_t at = pr * t.cols + pc;
+            T* to = static_cast<T*>(t.param) + at;
+            const float w = (t.master ? t.master[at] : to_float(*to)) * c.decay - t.rate * v[e];
+            *to = from_float<T>(w);
+            if (t.master) t.master[at] = w;
+          }
+          continue;
+        }
+        f16* out = WHAT == kGram ? a : WHAT == kPolynomial ? b : reinterpret_cast<f16*>(base + p.x(c.from ^ 1));
+        f16* turned = WHAT == kStep ? reinterpret_cast<f16*>(base + p.xt(c.from ^ 1)) : out;
+        const int64_t plane = WHAT == kStep ? whole : square, pitch = WHAT == kStep ? p.n : p.m;
+        f16x4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const Two w = two_of(v[e]);
+          hi[e] = w.hi, lo[e] = w.lo;
+          out[(r0 + e) * pitch + col] = w.hi;
+          out[plane + (r0 + e) * pitch + col] = w.lo;
+        }
+        if (WHAT == kStep || ti != tj) {
+          *reinterpret_cast<f16x4*>(turned + col * p.m + r0) = hi;
+          *reinterpret_cast<f16x4*>(turned + plane + col * p.m + r0) = lo;
+        }
       }
-    }
-    if (WHAT == kStep || WHAT == kLast) {
-      const f16x4 hi = *reinterpret_cast<const f16x4*>(xt + col * p.m + r0);
-      const f16x4 lo = *reinterpret_cast<const f16x4*>(xt + whole + col * p.m + r0);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        v[e] = fmaf(c.c0, fmaf((float)lo[e], kJoin, (float)hi[e]) * kDown, v[e]);
-    }
-    if (WHAT == kLast) {
-      const bool wide = t.rows <= t.cols;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t pr = wide ? r0 + e : col, pc = wide ? col : r0 + e;
-        if (pr >= t.rows || pc >= t.cols) continue;
-        const int64_t at = pr * t.cols + pc;
-        T* to = static_cast<T*>(t.param) + at;
-        const float w = (t.master ? t.master[at] : to_float(*to)) * c.decay - t.rate * v[e];
-        *to = from_float<T>(w);
-        if (t.master) t.master[at] = w;
-      }
-      continue;
-    }
-    f16* out = WHAT == kGram ? a : WHAT == kPolynomial ? b : reinterpret_cast<f16*>(base + p.x(c.from ^ 1));
-    f16* turned = WHAT == kStep ? reinterpret_cast<f16*>(base + p.xt(c.from ^ 1)) : out;
-    const int64_t plane = WHAT == kStep ? whole : square, pitch = WHAT == kStep ? p.n : p.m;
-    f16x4 hi, lo;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const Two w = two_of(v[e]);
-      hi[e] = w.hi, lo[e] = w.lo;
-      out[(r0 + e) * pitch + col] = w.hi;
-      out[plane + (r0 + e) * pitch + col] = w.lo;
-    }
-    if (WHAT == kStep || ti != tj) {
-      *reinterpret_cast<f16x4*>(turned + col * p.m + r0) = hi;
-      *reinterpret_cast<f16x4*>(turned + plane + col * p.m + r0) = lo;
-    }
-  }
 }
 
-// The matrices from k on that one launch takes, and their workspace.
-int64_t gather(int64_t n, const cpab_muon_matrix* matrices, const double* rates, int64_t* k, Batch* batch,
-               int* count) {
+// The matrices from k on, of those with this tile, that one launch takes, and their workspace.
+int64_t gather(int64_t n, const cpab_muon_matrix* matrices, const double* rates, int tile, int64_t* k,
+               Batch* batch, int* count) {
   int64_t bytes = 0;
   *count = 0;
   for (; *k < n && *count < kMatrices; ++*k) {
     const cpab_muon_matrix& t = matrices[*k];
-    if (t.rows == 0 || t.cols == 0) continue;
+    if (t.rows == 0 || t.cols == 0 || tile_of(t.rows, t.cols) != tile) continue;
     const int64_t need = (places(t.rows, t.cols).end + 255) / 256 * 256;
     if (*count > 0 && bytes + need > (1LL << 32)) break;   // a few GB of workspace are enough
     if (batch)
@@ -344,61 +376,73 @@ int64_t gather(int64_t n, const cpab_muon_matrix* matrices, const double* rates,
 
 int64_t muon_workspace(int64_t n, const cpab_muon_matrix* matrices) {
   int64_t most = 0;
-  for (int64_t k = 0; k < n;) {
-    int count = 0;
-    most = std::max(most, gather(n, matrices, nullptr, &k, nullptr, &count));
-  }
+  for (const int tile : {64, 128})
+    for (int64_t k = 0; k < n;) {
+      int count = 0;
+      most = std::max(most, gather(n, matrices, nullptr, tile, &k, nullptr, &count));
+    }
   return most;
 }
+
+namespace {
+
+// The step of one batch, whose products go in tiles of TILE.
+template <typename T, int TILE>
+hipError_t step(Batch& batch, int count, const Muon& s, char* room, hipStream_t st) {
+  constexpr int kRoom = 2 * 4 * TILE * 40 * 2;
+  const auto tiles = [&](auto each) {   // of all matrices
+    uint32_t total = 0;
+    for (int i = 0; i < count; ++i) {
+      batch.first[i] = total;
+      total += (uint32_t)each(batch.m[i], places(batch.m[i].rows, batch.m[i].cols));
+    }
+    return total;
+  };
+  const auto product = [&](auto what, uint32_t blocks, const Coefficients& c) {
+    constexpr Product WHAT = decltype(what)::value;
+    static LdsAllowed allowed;
+    const hipError_t e = allow_lds(reinterpret_cast<const void*>(muon_product_kernel<WHAT, T, TILE>), kRoom, allowed);
+    if (e != hipSuccess) return e;
+    muon_product_kernel<WHAT, T, TILE><<<blocks, kLanes, kRoom, st>>>(batch, count, c, room);
+    return hipGetLastError();
+  };
+  const Momentum m{s.momentum, s.rest, s.eps, s.nesterov};
+  uint32_t blocks = tiles([](const Matrix& a, const Places&) { return ((int64_t)a.rows * a.cols + kSpan - 1) / kSpan; });
+  muon_momentum_kernel<T><<<blocks, kLanes, 0, st>>>(batch, count, m, room);
+  blocks = tiles([](const Matrix&, const Places& p) { return p.m / 64 * (p.n / 64); });
+  muon_start_kernel<T><<<blocks, kLanes, 0, st>>>(batch, count, m, room);
+  hipError_t e = hipGetLastError();
+  for (int i = 0; i < s.steps && e == hipSuccess; ++i) {
+    const Coefficients c{s.c0, s.c1, s.c2, s.decay, i & 1};
+    blocks = tiles([](const Matrix&, const Places& p) { return p.m / TILE * (p.m / TILE + 1) / 2; });
+    e = product(std::integral_constant<Product, kGram>(), blocks, c);
+    if (e == hipSuccess) e = product(std::integral_constant<Product, kPolynomial>(), blocks, c);
+    if (e != hipSuccess) break;
+    blocks = tiles([](const Matrix&, const Places& p) { return p.m / TILE * (p.n / TILE); });
+    e = i + 1 < s.steps ? product(std::integral_constant<Product, kStep>(), blocks, c)
+                        : product(std::integral_constant<Product, kLast>(), blocks, c);
+  }
+  return e;
+}
+
+}  // namespace
 
 hipError_t launch_muon(int dtype, int64_t n, const cpab_muon_matrix* matrices, const double* rates,
                        const Muon& s, void* workspace, hipStream_t st) {
   char* room = static_cast<char*>(workspace);
-  for (int64_t k = 0; k < n;) {
-    Batch batch;
-    int count = 0;
-    gather(n, matrices, rates, &k, &batch, &count);
-    if (count == 0) break;
-    // a launch of `each` workgroups for each matrix
-    const auto launch = [&](auto each, auto kernel) {
-      uint32_t total = 0;
-      for (int i = 0; i < count; ++i) {
-        batch.first[i] = total;
-        total += (uint32_t)each(batch.m[i], places(batch.m[i].rows, batch.m[i].cols));
-      }
-      kernel(total);
-      return hipGetLastError();
-    };
-    const auto typed = [&](auto t) {
-      typedef decltype(t) T;
-      const Momentum m{s.momentum, s.rest, s.eps, s.nesterov};
-      hipError_t e = launch(
-          [](const Matrix& a, const Places&) { return ((int64_t)a.rows * a.cols + kSpan - 1) / kSpan; },
-          [&](uint32_t blocks) { muon_momentum_kernel<T><<<blocks, kLanes, 0, st>>>(batch, count, m, room); });
+  for (const int tile : {64, 128})
+    for (int64_t k = 0; k < n;) {
+      Batch batch;
+      int count = 0;
+      gather(n, matrices, rates, tile, &k, &batch, &count);
+      if (count == 0) break;
+      const auto typed = [&](auto t) {
+        typedef decltype(t) T;
+        return tile == 64 ? step<T, 64>(batch, count, s, room, st) : step<T, 128>(batch, count, s, room, st);
+      };
+      const hipError_t e = dtype == CPAB_F32 ? typed(0.0f) : typed(bf16());
       if (e != hipSuccess) return e;
-      e = launch([](const Matrix&, const Places& p) { return p.m / 64 * (p.n / 64); },
-                 [&](uint32_t blocks) { muon_start_kernel<T><<<blocks, kLanes, 0, st>>>(batch, count, m, room); });
-      for (int i = 0; i < s.steps && e == hipSuccess; ++i) {
-        const Coefficients c{s.c0, s.c1, s.c2, s.decay, i & 1};
-        const auto half = [](const Matrix&, const Places& p) { return p.m / 64 * (p.m / 64 + 1) / 2; };
-        const auto whole = [](const Matrix&, const Places& p) { return p.m / 64 * (p.n / 64); };
-        e = launch(half, [&](uint32_t blocks) {
-          muon_product_kernel<kGram, T><<<blocks, kLanes, 0, st>>>(batch, count, c, room);
-          muon_product_kernel<kPolynomial, T><<<blocks, kLanes, 0, st>>>(batch, count, c, room);
-        });
-        if (e != hipSuccess) break;
-        e = launch(whole, [&](uint32_t blocks) {
-          if (i + 1 < s.steps)
-            muon_product_kernel<kStep, T><<<blocks, kLanes, 0, st>>>(batch, count, c, room);
-          else
-            muon_product_kernel<kLast, T><<<blocks, kLanes, 0, st>>>(batch, count, c, room);
-        });
-      }
-      return e;
-    };
-    const hipError_t e = dtype == CPAB_F32 ? typed(0.0f) : typed(bf16());
-    if (e != hipSuccess) return e;
-  }
+    }
   return hipSuccess;
 }
 
