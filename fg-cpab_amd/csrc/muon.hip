@@ -36,7 +36,7 @@ constexpr int kLanes = 256;
 constexpr int kSmallSide = 256;    // of the matrices whose products go in tiles of 64
 constexpr int kMatrices = 40;      // of a launch
 constexpr int kSpan = kLanes * 16; // values of a workgroup of the momentum's kernel
-constexpr float kUp = 1024.0f, kDown = 1.0f / 1024.0f, kLow = 2048.0f, kJoin = 1.0f / 2048.0f;
+constexpr float kUp = 1024.0f, kDown = 1.0f / 1024.0f;
 
 // A matrix and where its parts lie in the workspace (bytes).  X is [m, n], m <= n, of
 // padded sizes; planes of 16-bit floats: hi, then lo.
@@ -57,8 +57,9 @@ struct Batch {
 // Tiles of a product: 128 x 128 where a matrix' shorter side is long enough that padding it
 // to whole tiles costs little, else 64 x 64.
 __host__ __device__ __forceinline__ int tile_of(int64_t rows, int64_t cols) {
-  return (rows < cols ? rows : cols) > kSmallSide ? 128 : 64;
+  return (rows < cols ? rows : cols) > 1024 ? 256 : (rows < cols ? rows : cols) > kSmallSide ? 128 : 64;
 }
+__host__ __device__ constexpr int lanes_of(int tile) { return tile > 128 ? 512 : 256; }
 __host__ __device__ __forceinline__ int64_t padded(int64_t n, int tile) { return (n + tile - 1) / tile * tile; }
 struct Places {
   int64_t m, n;   // padded
@@ -147,6 +148,12 @@ __global__ __launch_bounds__(kLanes) void muon_momentum_kernel(Batch batch, int 
     reinterpret_cast<double*>(room + t.at)[span] = (parts[0] + parts[1]) + (parts[2] + parts[3]);
 }
 
+// Where a matrix of so many (padded) rows has a value: 32 columns of all rows after another,
+// so that a tile's 32 of the summed index are one piece of memory.
+__host__ __device__ __forceinline__ int64_t place(int64_t row, int64_t col, int64_t rows) {
+  return (col / 32 * rows + row) * 32 + col % 32;
+}
+
 // 2^10 times a value in two 16-bit floats.
 struct Two {
   f16 hi, lo;
@@ -154,7 +161,7 @@ struct Two {
 __device__ __forceinline__ Two two_of(float x) {
   const float v = x * kUp;
   const f16 hi = (f16)v;
-  return Two{hi, (f16)((v - (float)hi) * kLow)};
+  return Two{hi, (f16)(v - (float)hi)};
 }
 
 // X and its transpose from the update, 64 x 64 values to a workgroup; zeros in the padding.
@@ -192,8 +199,9 @@ __global__ __launch_bounds__(kLanes) void muon_start_kernel(Batch batch, int cou
       x = update(s, t.momentum[at], to_float(static_cast<const T*>(t.grad)[at])) * by;
     }
     const Two v = two_of(x);
-    own[row * pcols + col] = v.hi;
-    own[plane + row * pcols + col] = v.lo;
+    const int64_t to = place(row, col, prows);
+    own[to] = v.hi;
+    own[plane + to] = v.lo;
     turn[0][c][r] = v.hi;
     turn[1][c][r] = v.lo;
   }
@@ -201,8 +209,9 @@ __global__ __launch_bounds__(kLanes) void muon_start_kernel(Batch batch, int cou
 #pragma unroll 4
   for (int k = 0; k < 16; ++k) {
     const int c = k * 4 + (threadIdx.x >> 6), r = threadIdx.x & 63;
-    other[(c0 + c) * prows + r0 + r] = turn[0][c][r];
-    other[plane + (c0 + c) * prows + r0 + r] = turn[1][c][r];
+    const int64_t to = place(c0 + c, r0 + r, pcols);
+    other[to] = turn[0][c][r];
+    other[plane + to] = turn[1][c][r];
   }
 }
 
@@ -216,14 +225,18 @@ struct Coefficients {
 // in LDS twice, as the matrix unit has the one and memory brings the other; rows of 64 bytes
 // begin 20 banks apart, so that a wave's wide reads meet no bank twice.
 template <Product WHAT, typename T, int TILE>
-__global__ __launch_bounds__(kLanes, 2) void muon_product_kernel(Batch batch, int count, Coefficients c, char* room) {
-  constexpr int kStepK = 32, kPitch = kStepK + 8, kEach = TILE / 64, MT = TILE / 64;
+__global__ __launch_bounds__((lanes_of(TILE)), 2) void muon_product_kernel(Batch batch, int count, Coefficients c, char* room) {
+  constexpr int kStepK = 32, kPitch = kStepK + 8, kThreads = lanes_of(TILE), kRows = kThreads / 4;
+  constexpr int kEach = TILE / kRows, kAcross = kThreads / 128, MT = TILE / 64, NT = TILE / 32 / kAcross;
   extern __shared__ __align__(16) f16 lds[];   // [2][4][TILE][kPitch]: rows' hi and lo, columns' hi and lo
   const int which = find(batch, count);
   const Matrix& t = batch.m[which];
   const Places p = places(t.rows, t.cols);
   char* const base = room + t.at;
-  const int64_t tile = blockIdx.x - batch.first[which];
+  // workgroups go to the eight dies in turn, each with a cache of its own: a die's tiles of a
+  // matrix follow one another
+  const uint32_t turn = blockIdx.x - batch.first[which], all = batch.first[which + 1] - batch.first[which];
+  const int64_t tile = turn % 8 * (all / 8) + min(turn % 8, all % 8) + turn / 8;
   int64_t ti, tj;
   if (WHAT == kGram || WHAT == kPolynomial) {   // tj >= ti
     tj = (int64_t)((sqrt(8.0 * (double)tile + 1.0) - 1.0) * 0.5);
@@ -245,23 +258,27 @@ __global__ __launch_bounds__(kLanes, 2) void muon_product_kernel(Batch batch, in
   const f16* right = WHAT == kGram ? x : WHAT == kPolynomial ? a : xt;
   const int64_t left_plane = WHAT == kGram ? whole : square;
   const int64_t right_plane = WHAT == kPolynomial ? square : whole;
-  left += ti * TILE * K;
-  right += tj * TILE * K;
+  const int64_t left_step = p.m * 32, right_step = WHAT == kStep || WHAT == kLast ? p.n * 32 : p.m * 32;
+  left += ti * TILE * 32 + threadIdx.x * 8;
+  right += tj * TILE * 32 + threadIdx.x * 8;
   // a lane brings 16 bytes of some rows of each of the four arrays
   const int row = threadIdx.x >> 2, part = (threadIdx.x & 3) * 8;
-  const f16* from[4] = {left + row * K + part, left + left_plane + row * K + part,
-                        right + row * K + part, right + right_plane + row * K + part};
   u32x4 next[4][kEach];
-  const auto fetch = [&](int64_t k0) {
+  const auto fetch = [&] {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) next[k][e] = *reinterpret_cast<const u32x4*>(from[k] + 64 * e * K + k0);
+    for (int e = 0; e < kEach; ++e) {
+      next[0][e] = *reinterpret_cast<const u32x4*>(left + kRows * e * 32);
+      next[1][e] = *reinterpret_cast<const u32x4*>(left + left_plane + kRows * e * 32);
+      next[2][e] = *reinterpret_cast<const u32x4*>(right + kRows * e * 32);
+      next[3][e] = *reinterpret_cast<const u32x4*>(right + right_plane + kRows * e * 32);
+    }
+    left += left_step;
+    right += right_step;
   };
-  fetch(0);
+  fetch();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 31, g = lane >> 5;
-  const int wr = (wave >> 1) * (TILE / 2), wc = (wave & 1) * (TILE / 2);
-  f32x16 acc[MT][MT] = {}, low[MT][MT] = {};
+  const int wr = wave / kAcross * (TILE / 2), wc = wave % kAcross * (32 * NT);
+  f32x16 acc[MT][NT] = {};
   int buffer = 0;
   for (int64_t k0 = 0; k0 < K; k0 += kStepK, buffer ^= 1) {
     f16* const now = lds + buffer * 4 * TILE * kPitch;
@@ -269,57 +286,59 @@ __global__ __launch_bounds__(kLanes, 2) void muon_product_kernel(Batch batch, in
     for (int k = 0; k < 4; ++k)
 #pragma unroll
       for (int e = 0; e < kEach; ++e)
-        *reinterpret_cast<u32x4*>(now + (k * TILE + row + 64 * e) * kPitch + part) = next[k][e];
+        *reinterpret_cast<u32x4*>(now + (k * TILE + row + kRows * e) * kPitch + part) = next[k][e];
     __syncthreads();
-    if (k0 + kStepK < K) fetch(k0 + kStepK);
+    if (k0 + kStepK < K) fetch();
 #pragma unroll
     for (int k = 0; k < kStepK; k += 16) {
-      f16x8 l[2][MT], r[2][MT];
+      f16x8 l[2][MT], r[2][NT];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
+        for (int m = 0; m < MT; ++m)
           l[h][m] = *reinterpret_cast<const f16x8*>(now + (h * TILE + wr + 32 * m + i) * kPitch + k + 8 * g);
-          r[h][m] = *reinterpret_cast<const f16x8*>(now + ((2 + h) * TILE + wc + 32 * m + i) * kPitch + k + 8 * g);
-        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          r[h][n] = *reinterpret_cast<const f16x8*>(now + ((2 + h) * TILE + wc + 32 * n + i) * kPitch + k + 8 * g);
+      }
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int n = 0; n < MT; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[0][m], r[0][n], acc[m][n], 0, 0, 0);
+        for (int n = 0; n < NT; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[0][m], r[0][n], acc[m][n], 0, 0, 0);
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int n = 0; n < MT; ++n) low[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[0][m], r[1][n], low[m][n], 0, 0, 0);
+        for (int n = 0; n < NT; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[0][m], r[1][n], acc[m][n], 0, 0, 0);
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int n = 0; n < MT; ++n) low[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[1][m], r[0][n], low[m][n], 0, 0, 0);
+        for (int n = 0; n < NT; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[1][m], r[0][n], acc[m][n], 0, 0, 0);
     }
   }
   // a lane's column, and 16 rows of each 32: four at a time, 8 apart
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int n = 0; n < MT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int64_t col = tj * TILE + wc + 32 * n + i, r0 = ti * TILE + wr + 32 * m + 8 * q + 4 * g;
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          v[e] = fmaf(low[m][n][4 * q + e], kJoin, acc[m][n][4 * q + e]) * (kDown * kDown);
+          v[e] = acc[m][n][4 * q + e] * (kDown * kDown);
         if (WHAT == kPolynomial) {   // A is its own transpose
-          const f16x4 hi = *reinterpret_cast<const f16x4*>(a + col * p.m + r0);
-          const f16x4 lo = *reinterpret_cast<const f16x4*>(a + square + col * p.m + r0);
+          const f16x4 hi = *reinterpret_cast<const f16x4*>(a + place(col, r0, p.m));
+          const f16x4 lo = *reinterpret_cast<const f16x4*>(a + square + place(col, r0, p.m));
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            v[e] = fmaf(c.c2, v[e], c.c1 * (fmaf((float)lo[e], kJoin, (float)hi[e]) * kDown));
+            v[e] = fmaf(c.c2, v[e], c.c1 * (((float)hi[e] + (float)lo[e]) * kDown));
         }
         if (WHAT == kStep || WHAT == kLast) {
-          const f16x4 hi = *reinterpret_cast<const f16x4*>(xt + col * p.m + r0);
-          const f16x4 lo = *reinterpret_cast<const f16x4*>(xt + whole + col * p.m + r0);
+          const f16x4 hi = *reinterpret_cast<const f16x4*>(xt + place(col, r0, p.n));
+          const f16x4 lo = *reinterpret_cast<const f16x4*>(xt + whole + place(col, r0, p.n));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = fmaf(c.c0, fmaf((float)lo[e], kJoin, (float)hi[e]) * kDown, v[e]);
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(c.c0, ((float)hi[e] + (float)lo[e]) * kDown, v[e]);
         }
         if (WHAT == kLast) {
           const bool wide = t.rows <= t.cols;
@@ -337,18 +356,19 @@ __global__ __launch_bounds__(kLanes, 2) void muon_product_kernel(Batch batch, in
         }
         f16* out = WHAT == kGram ? a : WHAT == kPolynomial ? b : reinterpret_cast<f16*>(base + p.x(c.from ^ 1));
         f16* turned = WHAT == kStep ? reinterpret_cast<f16*>(base + p.xt(c.from ^ 1)) : out;
-        const int64_t plane = WHAT == kStep ? whole : square, pitch = WHAT == kStep ? p.n : p.m;
+        const int64_t plane = WHAT == kStep ? whole : square, across = WHAT == kStep ? p.n : p.m;
+        const int64_t to = place(r0, col, p.m), over = place(col, r0, across);
         f16x4 hi, lo;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const Two w = two_of(v[e]);
           hi[e] = w.hi, lo[e] = w.lo;
-          out[(r0 + e) * pitch + col] = w.hi;
-          out[plane + (r0 + e) * pitch + col] = w.lo;
+          out[to + 32 * e] = w.hi;
+          out[plane + to + 32 * e] = w.lo;
         }
         if (WHAT == kStep || ti != tj) {
-          *reinterpret_cast<f16x4*>(turned + col * p.m + r0) = hi;
-          *reinterpret_cast<f16x4*>(turned + plane + col * p.m + r0) = lo;
+          *reinterpret_cast<f16x4*>(turned + over) = hi;
+          *reinterpret_cast<f16x4*>(turned + plane + over) = lo;
         }
       }
 }
@@ -376,7 +396,7 @@ int64_t gather(int64_t n, const cpab_muon_matrix* matrices, const double* rates,
 
 int64_t muon_workspace(int64_t n, const cpab_muon_matrix* matrices) {
   int64_t most = 0;
-  for (const int tile : {64, 128})
+  for (const int tile : {64, 128, 256})
     for (int64_t k = 0; k < n;) {
       int count = 0;
       most = std::max(most, gather(n, matrices, nullptr, tile, &k, nullptr, &count));
@@ -396,6 +416,7 @@ hipError_t step(Batch& batch, int count, const Muon& s, char* room, hipStream_t 
       batch.first[i] = total;
       total += (uint32_t)each(batch.m[i], places(batch.m[i].rows, batch.m[i].cols));
     }
+    batch.first[count] = total;
     return total;
   };
   const auto product = [&](auto what, uint32_t blocks, const Coefficients& c) {
@@ -403,7 +424,7 @@ hipError_t step(Batch& batch, int count, const Muon& s, char* room, hipStream_t 
     static LdsAllowed allowed;
     const hipError_t e = allow_lds(reinterpret_cast<const void*>(muon_product_kernel<WHAT, T, TILE>), kRoom, allowed);
     if (e != hipSuccess) return e;
-    muon_product_kernel<WHAT, T, TILE><<<blocks, kLanes, kRoom, st>>>(batch, count, c, room);
+    muon_product_kernel<WHAT, T, TILE><<<blocks, lanes_of(TILE), kRoom, st>>>(batch, count, c, room);
     return hipGetLastError();
   };
   const Momentum m{s.momentum, s.rest, s.eps, s.nesterov};
@@ -430,7 +451,7 @@ hipError_t step(Batch& batch, int count, const Muon& s, char* room, hipStream_t 
 hipError_t launch_muon(int dtype, int64_t n, const cpab_muon_matrix* matrices, const double* rates,
                        const Muon& s, void* workspace, hipStream_t st) {
   char* room = static_cast<char*>(workspace);
-  for (const int tile : {64, 128})
+  for (const int tile : {64, 128, 256})
     for (int64_t k = 0; k < n;) {
       Batch batch;
       int count = 0;
@@ -438,7 +459,8 @@ hipError_t launch_muon(int dtype, int64_t n, const cpab_muon_matrix* matrices, c
       if (count == 0) break;
       const auto typed = [&](auto t) {
         typedef decltype(t) T;
-        return tile == 64 ? step<T, 64>(batch, count, s, room, st) : step<T, 128>(batch, count, s, room, st);
+        return tile == 64 ? step<T, 64>(batch, count, s, room, st) : tile == 128 ? step<T, 128>(batch, count, s, room, st)
+                       : step<T, 256>(batch, count, s, room, st);
       };
       const hipError_t e = dtype == CPAB_F32 ? typed(0.0f) : typed(bf16());
       if (e != hipSuccess) return e;
