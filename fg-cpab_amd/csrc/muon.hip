@@ -29,11 +29,13 @@ namespace {
 typedef _Float16 f16;
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kLanes = 256;
-constexpr int kSmallSide = 256;    // of the matrices whose products go in tiles of 64
+constexpr int kWholeSide = 64, kWholeLong = 256;   // of the matrices that one workgroup keeps
+constexpr int kWholeLanes = 1024;
 constexpr int kMatrices = 40;      // of a launch
 constexpr int kSpan = kLanes * 16; // values of a workgroup of the momentum's kernel
 constexpr float kUp = 1024.0f, kDown = 1.0f / 1024.0f;
@@ -54,10 +56,12 @@ struct Batch {
   uint32_t first[kMatrices + 1];   // workgroups before each matrix's
 };
 
-// Tiles of a product: 128 x 128 where a matrix' shorter side is long enough that padding it
-// to whole tiles costs little, else 64 x 64.
+// How a matrix' products go: in one workgroup that keeps it in LDS where it fits (0), else in
+// tiles of 64, 128 or 256, the longer the shorter side, since padding it to whole tiles
+// costs less then.
 __host__ __device__ __forceinline__ int tile_of(int64_t rows, int64_t cols) {
-  return (rows < cols ? rows : cols) > 1024 ? 256 : (rows < cols ? rows : cols) > kSmallSide ? 128 : 64;
+  const int64_t m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+  return m <= kWholeSide && n <= kWholeLong ? 0 : m > 1024 ? 256 : m > 256 ? 128 : 64;
 }
 __host__ __device__ constexpr int lanes_of(int tile) { return tile > 128 ? 512 : 256; }
 __host__ __device__ __forceinline__ int64_t padded(int64_t n, int tile) { return (n + tile - 1) / tile * tile; }
@@ -215,11 +219,158 @@ __global__ __launch_bounds__(kLanes) void muon_start_kernel(Batch batch, int cou
   }
 }
 
-enum Product { kGram, kPolynomial, kStep, kLast };
 struct Coefficients {
   float c0, c1, c2, decay;
   int from;   // which of the two X
 };
+
+// The parameter's move, from the master weight where there is one.
+template <typename T>
+__device__ __forceinline__ void move(const Matrix& t, int64_t at, float decay, float v) {
+  T* to = static_cast<T*>(t.param) + at;
+  const float w = (t.master ? t.master[at] : to_float(*to)) * decay - t.rate * v;
+  *to = from_float<T>(w);
+  if (t.master) t.master[at] = w;
+}
+
+// As a sum of three products of two 16-bit floats each.
+__device__ __forceinline__ f32x4 mma(const f16x8 (&l)[2], const f16x8 (&r)[2], f32x4 acc) {
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[0], r[0], acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[0], r[1], acc, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(l[1], r[0], acc, 0, 0, 0);
+}
+
+// The whole step of a matrix of up to 64 x 256: X, its transpose and A, later B, lie in LDS;
+// a wave has 16 of X's columns in its registers, in 32 bits, and one 16 x 16 tile of A and B.
+// One launch instead of two and three to an iteration, which is what small matrices wait for.
+template <typename T>
+__global__ __launch_bounds__(kWholeLanes) void muon_whole_kernel(Batch batch, Momentum s, Coefficients c, int steps) {
+  constexpr int kP = kWholeSide + 8;   // pitch of A and of X's transpose
+  extern __shared__ __align__(16) f16 lds[];
+  __shared__ double parts[kWholeLanes / 64];
+  const Matrix& t = batch.m[blockIdx.x];
+  const bool wide = t.rows <= t.cols;
+  const int m = wide ? t.rows : t.cols, n = wide ? t.cols : t.rows, across = (n + 31) / 32 * 32, pitch = across + 8;
+  f16* const x = lds;                                   // [2][64][pitch]
+  f16* const xt = x + 2 * kWholeSide * pitch;           // [2][across][kP]
+  f16* const a = xt + 2 * across * kP;                  // [2][64][kP]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = lane & 15, g = lane >> 4, col = 16 * wave + i;
+  const bool busy = 16 * wave < across;
+  f32x4 own[4] = {};   // rows 16 k + 4 g .. of column col
+  double sum = 0.0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float grad[4], mom[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {   // the first value, unused, in place of those outside
+      const int row = 16 * k + 4 * g + e;
+      const uint32_t at = row < m && col < n ? wide ? row * n + col : col * m + row : 0;
+      grad[e] = to_float(static_cast<const T*>(t.grad)[at]);
+      mom[e] = t.momentum[at];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int row = 16 * k + 4 * g + e;
+      const bool in = row < m && col < n;
+      mom[e] = fmaf(s.mu, mom[e], s.rest * grad[e]);
+      if (in) t.momentum[wide ? row * n + col : col * m + row] = mom[e];
+      own[k][e] = in ? update(s, mom[e], grad[e]) : 0.0f;
+      sum = fma((double)own[k][e], (double)own[k][e], sum);
+    }
+  }
+  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  if (lane == 0) parts[wave] = sum;
+  __syncthreads();
+  sum = 0.0;
+  for (int k = 0; k < kWholeLanes / 64; ++k) sum += parts[k];
+  const double norm = sqrt(sum);
+  const float by = (float)(1.0 / (norm < (double)s.eps ? (double)s.eps : norm));
+#pragma unroll
+  for (int k = 0; k < 4; ++k) own[k] *= by;
+  const auto frag = [&](f16x8 (&to)[2], const f16* from, int plane) {
+    to[0] = *reinterpret_cast<const f16x8*>(from);
+    to[1] = *reinterpret_cast<const f16x8*>(from + plane);
+  };
+  const int tr = 16 * (wave >> 2), tc = 16 * (wave & 3);   // this wave's tile of A
+  const auto keep = [&](const f32x4& v) {                  // A is its own transpose
+    f16x4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const Two w = two_of(v[e]);
+      hi[e] = w.hi, lo[e] = w.lo;
+    }
+    f16* const to = a + (tc + i) * kP + tr + 4 * g;
+    *reinterpret_cast<f16x4*>(to) = hi;
+    *reinterpret_cast<f16x4*>(to + kWholeSide * kP) = lo;
+  };
+  for (int step = 0;; ++step) {
+    if (busy) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        f16x4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const Two w = two_of(own[k][e]);
+          hi[e] = w.hi, lo[e] = w.lo;
+          x[(16 * k + 4 * g + e) * pitch + col] = w.hi;
+          x[(kWholeSide + 16 * k + 4 * g + e) * pitch + col] = w.lo;
+        }
+        *reinterpret_cast<f16x4*>(xt + col * kP + 16 * k + 4 * g) = hi;
+        *reinterpret_cast<f16x4*>(xt + (across + col) * kP + 16 * k + 4 * g) = lo;
+      }
+    }
+    __syncthreads();
+    f16x8 l[2], r[2];
+    f32x4 gram = {};
+#pragma unroll 1
+    for (int k = 0; k < across; k += 32) {
+      frag(l, x + (tr + i) * pitch + k + 8 * g, kWholeSide * pitch);
+      frag(r, x + (tc + i) * pitch + k + 8 * g, kWholeSide * pitch);
+      gram = mma(l, r, gram);
+    }
+    gram *= kDown * kDown;
+    keep(gram);
+    __syncthreads();
+    f32x4 poly = {};
+#pragma unroll
+    for (int k = 0; k < kWholeSide; k += 32) {
+      frag(l, a + (tr + i) * kP + k + 8 * g, kWholeSide * kP);
+      frag(r, a + (tc + i) * kP + k + 8 * g, kWholeSide * kP);
+      poly = mma(l, r, poly);
+    }
+    __syncthreads();
+    keep(gram * c.c1 + poly * (c.c2 * kDown * kDown));
+    __syncthreads();
+    if (busy) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) own[k] *= c.c0 * (kUp * kUp);
+#pragma unroll
+      for (int k = 0; k < kWholeSide; k += 32) {
+        frag(r, xt + col * kP + k + 8 * g, across * kP);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          frag(l, a + (16 * u + i) * kP + k + 8 * g, kWholeSide * kP);
+          own[u] = mma(l, r, own[u]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) own[k] *= kDown * kDown;
+    }
+    if (step + 1 == steps) break;
+  }
+  int again = g;   // not the start's addresses, kept in registers all along
+  asm volatile("" : "+v"(again));
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int row = 16 * k + 4 * again + e;
+      if (row < m && col < n) move<T>(t, (uint32_t)(wide ? row * n + col : col * m + row), c.decay, own[k][e]);
+    }
+}
+
+enum Product { kGram, kPolynomial, kStep, kLast };
 
 // One tile of a product: a wave has a quarter of it, in two sums.  32 of the summed index lie
 // in LDS twice, as the matrix unit has the one and memory brings the other; rows of 64 bytes
@@ -345,12 +496,7 @@ __global__ __launch_bounds__((lanes_of(TILE)), 2) void muon_product_kernel(Batch
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int64_t pr = wide ? r0 + e : col, pc = wide ? col : r0 + e;
-            if (pr >= t.rows || pc >= t.cols) continue;
-            const int64_t at = pr * t.cols + pc;
-            T* to = static_cast<T*>(t.param) + at;
-            const float w = (t.master ? t.master[at] : to_float(*to)) * c.decay - t.rate * v[e];
-            *to = from_float<T>(w);
-            if (t.master) t.master[at] = w;
+            if (pr < t.rows && pc < t.cols) move<T>(t, pr * t.cols + pc, c.decay, v[e]);
           }
           continue;
         }
@@ -381,7 +527,7 @@ int64_t gather(int64_t n, const cpab_muon_matrix* matrices, const double* rates,
   for (; *k < n && *count < kMatrices; ++*k) {
     const cpab_muon_matrix& t = matrices[*k];
     if (t.rows == 0 || t.cols == 0 || tile_of(t.rows, t.cols) != tile) continue;
-    const int64_t need = (places(t.rows, t.cols).end + 255) / 256 * 256;
+    const int64_t need = tile == 0 ? 0 : (places(t.rows, t.cols).end + 255) / 256 * 256;
     if (*count > 0 && bytes + need > (1LL << 32)) break;   // a few GB of workspace are enough
     if (batch)
       batch->m[*count] = Matrix{t.param, t.grad, t.momentum, t.master, bytes, (int)t.rows, (int)t.cols,
@@ -389,6 +535,11 @@ int64_t gather(int64_t n, const cpab_muon_matrix* matrices, const double* rates,
     ++*count;
     bytes += need;
   }
+  // the longest products first, so that none begins when the others end
+  if (batch)
+    std::sort(batch->m, batch->m + *count, [](const Matrix& a, const Matrix& b) {
+      return std::make_pair(std::max(a.rows, a.cols), a.at) > std::make_pair(std::max(b.rows, b.cols), b.at);
+    });
   return bytes;
 }
 
@@ -396,7 +547,7 @@ int64_t gather(int64_t n, const cpab_muon_matrix* matrices, const double* rates,
 
 int64_t muon_workspace(int64_t n, const cpab_muon_matrix* matrices) {
   int64_t most = 0;
-  for (const int tile : {64, 128, 256})
+  for (const int tile : {0, 64, 128, 256})
     for (int64_t k = 0; k < n;) {
       int count = 0;
       most = std::max(most, gather(n, matrices, nullptr, tile, &k, nullptr, &count));
@@ -409,7 +560,6 @@ namespace {
 // The step of one batch, whose products go in tiles of TILE.
 template <typename T, int TILE>
 hipError_t step(Batch& batch, int count, const Muon& s, char* room, hipStream_t st) {
-  constexpr int kRoom = 2 * 4 * TILE * 40 * 2;
   const auto tiles = [&](auto each) {   // of all matrices
     uint32_t total = 0;
     for (int i = 0; i < count; ++i) {
@@ -419,13 +569,19 @@ hipError_t step(Batch& batch, int count, const Muon& s, char* room, hipStream_t 
     batch.first[count] = total;
     return total;
   };
-  const auto product = [&](auto what, uint32_t blocks, const Coefficients& c) {
+  const auto product = [&](auto what, auto side, uint32_t blocks, const Coefficients& c) {
     constexpr Product WHAT = decltype(what)::value;
+    constexpr int SIDE = decltype(side)::value, kRoom = 2 * 4 * SIDE * 40 * 2;
     static LdsAllowed allowed;
-    const hipError_t e = allow_lds(reinterpret_cast<const void*>(muon_product_kernel<WHAT, T, TILE>), kRoom, allowed);
+    const hipError_t e = allow_lds(reinterpret_cast<const void*>(muon_product_kernel<WHAT, T, SIDE>), kRoom, allowed);
     if (e != hipSuccess) return e;
-    muon_product_kernel<WHAT, T, TILE><<<blocks, lanes_of(TILE), kRoom, st>>>(batch, count, c, room);
+    muon_product_kernel<WHAT, T, SIDE><<<blocks, lanes_of(SIDE), kRoom, st>>>(batch, count, c, room);
     return hipGetLastError();
+  };
+  typedef std::integral_constant<int, TILE> Side;
+  typedef std::integral_constant<int, TILE == 256 ? 128 : TILE> Half;
+  const auto half = [&](int side) {   // the tiles on and above the diagonal
+    return tiles([side](const Matrix&, const Places& p) { return p.m / side * (p.m / side + 1) / 2; });
   };
   const Momentum m{s.momentum, s.rest, s.eps, s.nesterov};
   uint32_t blocks = tiles([](const Matrix& a, const Places&) { return ((int64_t)a.rows * a.cols + kSpan - 1) / kSpan; });
@@ -435,15 +591,37 @@ hipError_t step(Batch& batch, int count, const Muon& s, char* room, hipStream_t 
   hipError_t e = hipGetLastError();
   for (int i = 0; i < s.steps && e == hipSuccess; ++i) {
     const Coefficients c{s.c0, s.c1, s.c2, s.decay, i & 1};
-    blocks = tiles([](const Matrix&, const Places& p) { return p.m / TILE * (p.m / TILE + 1) / 2; });
-    e = product(std::integral_constant<Product, kGram>(), blocks, c);
-    if (e == hipSuccess) e = product(std::integral_constant<Product, kPolynomial>(), blocks, c);
+    e = product(std::integral_constant<Product, kGram>(), Side(), half(TILE), c);
+    if (e != hipSuccess) break;
+    // The polynomial's products are alike: tiles of 128, of which a compute unit has two at a
+    // time, where they fill its rounds better.
+    blocks = half(TILE);
+    if (TILE == 256 && (half(128) + 511) / 512 * 2 < (blocks + 255) / 256 * 4)
+      e = product(std::integral_constant<Product, kPolynomial>(), Half(), half(128), c);
+    else
+      e = product(std::integral_constant<Product, kPolynomial>(), Side(), half(TILE), c);
     if (e != hipSuccess) break;
     blocks = tiles([](const Matrix&, const Places& p) { return p.m / TILE * (p.n / TILE); });
-    e = i + 1 < s.steps ? product(std::integral_constant<Product, kStep>(), blocks, c)
-                        : product(std::integral_constant<Product, kLast>(), blocks, c);
+    e = i + 1 < s.steps ? product(std::integral_constant<Product, kStep>(), Side(), blocks, c)
+                        : product(std::integral_constant<Product, kLast>(), Side(), blocks, c);
   }
   return e;
+}
+
+// The step of the matrices of one batch that are kept whole.
+template <typename T>
+hipError_t step_whole(const Batch& batch, int count, const Muon& s, hipStream_t st) {
+  int room = 0;
+  for (int i = 0; i < count; ++i) {
+    const int across = (std::max(batch.m[i].rows, batch.m[i].cols) + 31) / 32 * 32;
+    room = std::max(room, 2 * 2 * (kWholeSide * (across + 8) + (across + kWholeSide) * (kWholeSide + 8)));
+  }
+  static LdsAllowed allowed;
+  const hipError_t e = allow_lds(reinterpret_cast<const void*>(muon_whole_kernel<T>), room, allowed);
+  if (e != hipSuccess) return e;
+  const Momentum m{s.momentum, s.rest, s.eps, s.nesterov};
+  muon_whole_kernel<T><<<count, kWholeLanes, room, st>>>(batch, m, Coefficients{s.c0, s.c1, s.c2, s.decay, 0}, s.steps);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -451,7 +629,7 @@ hipError_t step(Batch& batch, int count, const Muon& s, char* room, hipStream_t 
 hipError_t launch_muon(int dtype, int64_t n, const cpab_muon_matrix* matrices, const double* rates,
                        const Muon& s, void* workspace, hipStream_t st) {
   char* room = static_cast<char*>(workspace);
-  for (const int tile : {64, 128, 256})
+  for (const int tile : {0, 64, 128, 256})
     for (int64_t k = 0; k < n;) {
       Batch batch;
       int count = 0;
@@ -459,8 +637,10 @@ hipError_t launch_muon(int dtype, int64_t n, const cpab_muon_matrix* matrices, c
       if (count == 0) break;
       const auto typed = [&](auto t) {
         typedef decltype(t) T;
-        return tile == 64 ? step<T, 64>(batch, count, s, room, st) : tile == 128 ? step<T, 128>(batch, count, s, room, st)
-                       : step<T, 256>(batch, count, s, room, st);
+        return tile == 0    ? step_whole<T>(batch, count, s, st)
+               : tile == 64 ? step<T, 64>(batch, count, s, room, st)
+               : tile == 128 ? step<T, 128>(batch, count, s, room, st)
+                             : step<T, 256>(batch, count, s, room, st);
       };
       const hipError_t e = dtype == CPAB_F32 ? typed(0.0f) : typed(bf16());
       if (e != hipSuccess) return e;
