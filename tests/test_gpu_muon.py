@@ -257,3 +257,26 @@ def test_refusals(cuda):
     with pytest.raises(RuntimeError, match="inference"):
         call(put("momenta", 0, lambda t: made))
     cpab.muon_step([], [], [])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_on_both_sides_of_each_way(cuda, dtype):
+    # one workgroup up to 64 x 256, then tiles of 64, of 128 past a shorter side of 256 and of
+    # 256 past one of 1024; each way's own launches, in one call
+    compare(cuda, dtype, [(64, 256), (256, 64), (1, 256), (64, 1), (50, 97), (130, 20)], seed=11)
+    compare(cuda, dtype, [(64, 257), (257, 64), (65, 65), (65, 256)], seed=12)
+    compare(cuda, dtype, [(256, 256), (256, 700), (257, 257), (1024, 1024), (1025, 1025), (48, 31)], seed=13,
+            masters=dtype == BF16)
+
+
+def test_whole_matrices_same_bits(cuda):
+    def run(shapes):
+        st = make(cuda, F32, shapes, seed=14)
+        cpab.muon_step(st["params"], st["grads"], st["momenta"])
+        return st["params"] + st["momenta"]
+    a, b = run([(60, 200)] * 50), run([(60, 200)] * 50)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    # the first alone, and beside one that goes in tiles
+    for shapes in ([(60, 200)], [(60, 200), (300, 300)]):
+        c = run(shapes)
+        assert torch.equal(c[0], a[0])
