@@ -207,6 +207,32 @@ struct Rows {
 // takes from it once, before the loop, and has no registers for them.
 __device__ __forceinline__ void renew(int& a) { asm volatile("" : "+v"(a)); }
 
+// A value of another lane, by the vector unit's own exchanges; 0 where there is none.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ float lane_at(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+}
+// The sum over 8 or 16 neighbouring lanes.
+__device__ __forceinline__ float over8(float v) {
+  v += lane_at<0xb1>(v);    // the pair's other
+  v += lane_at<0x4e>(v);    // of two pairs
+  return v + lane_at<0x141>(v);   // mirrored in eights
+}
+__device__ __forceinline__ float over16(float v) {
+  v = over8(v);
+  return v + lane_at<0x140>(v);   // mirrored in sixteens
+}
+// The sum over the lanes before.
+__device__ __forceinline__ float lanes_before(float v) {
+  v += lane_at<0x111>(v);   // from 1, 2, 4 and 8 lanes below in the sixteen
+  v += lane_at<0x112>(v);
+  v += lane_at<0x114>(v);
+  v += lane_at<0x118>(v);
+  v += lane_at<0x142, 0xa>(v);   // the last of the sixteen before, to the second and the fourth
+  v += lane_at<0x143, 0xc>(v);   // and of the half before
+  return lane_at<0x138>(v);
+}
+
 // Waits for what has been loaded.  Before a loop whose registers begin with loads: the
 // compiler, which does not tell its first round from the others, would wait in each of them,
 // for everything that is fetched ahead.
@@ -306,6 +332,7 @@ __device__ __forceinline__ void store_some(T* p, const f32x4& v, int left) {
 // chunk of a head: exp(G_i), exp(G_63 - G_i) and beta; M and P (their transposes for the
 // backward) in planes.
 struct Gates {
+  double log[kChunk];   // the decays' logarithms, added up
   float since[kChunk], until[kChunk], beta[kChunk];
 };
 template <typename T>

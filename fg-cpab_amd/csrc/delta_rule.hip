@@ -95,6 +95,7 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, Squ
     }
     G[t] = g;
     betas[t] = beta;
+    out.gates.log[t] = g;
     out.gates.since[t] = expf((float)g);
     out.gates.until[t] = expf((float)(__shfl(g, 63) - g));
     out.gates.beta[t] = beta;

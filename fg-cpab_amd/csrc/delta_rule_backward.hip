@@ -287,7 +287,7 @@ __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_ke
   constexpr int NT = DP / 16 / kGroups, NJ = 4 / kGroups;   // tiles of DP and of the 64 to a wave
   extern __shared__ __align__(16) bf16 lds[];
   __shared__ double G[kChunk];
-  __shared__ float betas[kChunk], dbeta[kChunk], before[kGroups][kChunk], after[kGroups][kChunk], whole[kWaves],
+  __shared__ float betas[kChunk], since[kChunk], until[kChunk], dbeta[kChunk], before[kGroups][kChunk], after[kGroups][kChunk], whole[kWaves],
       sums[kWaves][kChunk];
   bf16* S = lds;                              // [DP][32]
   bf16* L = S + NP * Room::kState;            // the gradient, [DP][32]
@@ -331,16 +331,10 @@ __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_ke
     const Squares<T>& sq = squares[bh * d.chunks + c];
     if (threadIdx.x < kChunk) {
       const int t = threadIdx.x;
-      double sum = 0.0;
-      if (t < live)
-        sum = (double)clamped(gate_at(d, d.r.decay, b * d.r.decay_strides[0] + (t0 + t) * d.r.decay_strides[1] +
-                                                        h * d.r.decay_strides[2]));
-      for (int n = 1; n < 64; n *= 2) {
-        const double prior = __shfl_up(sum, n);
-        if (t >= n) sum += prior;
-      }
-      G[t] = sum;
+      G[t] = sq.gates.log[t];
       betas[t] = sq.gates.beta[t];
+      since[t] = sq.gates.since[t];
+      until[t] = sq.gates.until[t];
       dbeta[t] = 0.0f;
     }
     const float* state = states + (bh * d.chunks + c) * dk * wide;
@@ -408,9 +402,7 @@ __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_ke
         float part = x[0] * ev[0];
 #pragma unroll
         for (int e = 1; e < 4; ++e) part = fmaf(x[e], ev[e], part);
-        part += __shfl_xor(part, 1);
-        part += __shfl_xor(part, 2);
-        part += __shfl_xor(part, 4);
+        part = over8(part);
         if (col == 0) dbeta[t] += part;
       }
       oraw.keep(grad_o && orows.in(w0 + i, e0 + 8 * g));
@@ -461,26 +453,24 @@ __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_ke
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int row = w0 + 4 * g + e;
-      const float since = sq.gates.since[row], until = sq.gates.until[row], ss = d.r.scale * since;
+      const float early = since[row], late = until[row], ss = d.r.scale * early;
       float from = 0.0f, to = 0.0f;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const float a = ss * qs[0][n][e], z = since * k2[0][n][e], u = until * k1[0][n][e];
+        const float a = ss * qs[0][n][e], z = early * k2[0][n][e], u = late * k1[0][n][e];
         from = fmaf(qv[0][n][e], a, from);
         from = fmaf(-kv[0][n][e], z, from);
         to = fmaf(kv[0][n][e], u, to);
         dQ[0][n][e] += a;
         dK[0][n][e] += u - z;
       }
-#pragma unroll
-      for (int n = 1; n < 16; n *= 2) {
-        from += __shfl_xor(from, n);
-        to += __shfl_xor(to, n);
-      }
+      from = over16(from);
+      to = over16(to);
       if (i == 0) before[group][row] = from, after[group][row] = to;
     }
-#pragma unroll
-    for (int n = 1; n < 64; n *= 2) dot += __shfl_xor(dot, n);
+    dot = over16(dot);
+    dot += __shfl_xor(dot, 16);
+    dot += __shfl_xor(dot, 32);
     if (lane == 0) whole[wave] = dot;
 #pragma unroll
     for (int n = 0; n < NJ; ++n) {
@@ -534,14 +524,8 @@ __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_ke
       float sum = 0.0f;
       for (int n = 0; n < kChunk / kWaves; ++n) {
         const int row = kChunk / kWaves * wave + n;
-        float v = H[row * (kChunk + 1) + lane], from = 0.0f, to = 0.0f;
-#pragma unroll
-        for (int m = 1; m < 64; m *= 2) {
-          const float prior = __shfl_up(v, m);
-          if (lane >= m) v += prior;
-        }
-        v = __shfl_up(v, 1);   // of the columns before
-        if (lane == 0) v = 0.0f;
+        const float v = lanes_before(H[row * (kChunk + 1) + lane]);
+        float from = 0.0f, to = 0.0f;
 #pragma unroll
         for (int m = 0; m < kGroups; ++m) from += before[m][row], to += after[m][row];
         sum += row >= lane ? v + from : to;
@@ -554,7 +538,7 @@ __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_ke
       float dots = 0.0f, sum = 0.0f;
 #pragma unroll
       for (int n = 0; n < kWaves; ++n) dots += whole[n], sum += sums[n][t];
-      sum = fmaf(sq.gates.since[kChunk - 1], dots, sum);
+      sum = fmaf(since[kChunk - 1], dots, sum);
       if (t < rows) {
         const int64_t at = (b * d.r.T + t0 + t) * d.r.heads + h;
         if (grad_decay) put_gate(d, grad_decay, at, t < live ? sum : 0.0f);
