@@ -150,6 +150,10 @@ struct Raw {
 #pragma unroll
     for (int k = 0; k < kWords; ++k) v[k] = reinterpret_cast<const Unit*>(p)[k];
   }
+  __device__ __forceinline__ void take(const T* p) {   // 16-byte aligned
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) v[k] = reinterpret_cast<const U4*>(p)[k];
+  }
   __device__ __forceinline__ void put(T* p) const {   // 16-byte aligned
 #pragma unroll
     for (int k = 0; k < kWords; ++k) reinterpret_cast<U4*>(p)[k] = v[k];

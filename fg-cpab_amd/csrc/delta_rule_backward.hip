@@ -270,7 +270,10 @@ struct PartsRoom {
   // S, its gradient, U and Z, then in their place W, its transpose and the other square
   static constexpr int kLoop = NP * (2 * kState + 2 * kSamples), kAfter = 3 * NP * kFlat;
   static constexpr int kParts = kLoop > kAfter ? kLoop : kAfter;   // 16-bit values
-  static constexpr int kBytes = 2 * kParts + 4 * kChunk * (kChunk + 1);
+  static constexpr int kSquares = 2 * kParts + 4 * kChunk * (kChunk + 1);
+  // keys and queries too where there is room, which leaves 12 KB to the rest
+  static constexpr bool kStaged = kSquares + sizeof(Keys<T, DP>) <= 148 * 1024;
+  static constexpr int kBytes = kSquares + (kStaged ? sizeof(Keys<T, DP>) : 0);
 };
 
 // A chunk of a key's head: the gradients of its queries and keys, added up over the heads
@@ -308,10 +311,23 @@ __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_ke
   const int64_t t0 = (int64_t)c * kChunk;
   const int live = (int)min(max(live_of(d, b) - t0, (int64_t)0), (int64_t)kChunk);
   const int rows = (int)min(d.r.T - t0, (int64_t)kChunk);   // that there are
-  const Keys<T, DP>& own = keys[(b * d.r.key_heads + kh) * d.chunks + c];
+  const Keys<T, DP>& theirs = keys[(b * d.r.key_heads + kh) * d.chunks + c];
+  Keys<T, DP>& here = *reinterpret_cast<Keys<T, DP>*>(reinterpret_cast<char*>(lds) + Room::kSquares);
+  const Keys<T, DP>& own = Room::kStaged ? here : theirs;
+  if (Room::kStaged && live > 0) {
+    typedef typename Raw<T>::U4 U4;
+    const U4* from = reinterpret_cast<const U4*>(&theirs);
+    U4* to = reinterpret_cast<U4*>(&here);
+    constexpr int kAll = sizeof(Keys<T, DP>) / 16 / kBlock;
+    U4 v[kAll];
+#pragma unroll
+    for (int n = 0; n < kAll; ++n) v[n] = from[n * kBlock + threadIdx.x];
+#pragma unroll
+    for (int n = 0; n < kAll; ++n) to[n * kBlock + threadIdx.x] = v[n];
+  }
   const auto own_frag = [&](const auto& of, int row, int step) {
     Raw<T> r;
-    r.fetch(of[row][step][threadIdx.x & 63]);
+    r.take(of[row][step][threadIdx.x & 63]);
     return r.frag();
   };
   f32x4 dQ[1][NT], dK[1][NT];
