@@ -330,20 +330,61 @@ __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_ke
     r.take(of[row][step][threadIdx.x & 63]);
     return r.frag();
   };
+  if (live == 0) {
+    for (int n = threadIdx.x; n < rows * d.group; n += kBlock) {
+      const int64_t at = (b * d.r.T + t0 + n / d.group) * d.r.heads + kh * d.group + n % d.group;
+      if (grad_decay) put_gate(d, grad_decay, at, 0.0f);
+      if (grad_beta) put_gate(d, grad_beta, at, 0.0f);
+    }
+    for (int n = threadIdx.x; n < rows * dk; n += kBlock) {
+      const int64_t at = ((b * d.r.T + t0 + n / dk) * d.r.key_heads + kh) * dk + n % dk;
+      if (grad_q) grad_q[at] = from_float<T>(0.0f);
+      if (grad_k) grad_k[at] = from_float<T>(0.0f);
+    }
+    return;
+  }
+  const int64_t token = (b * d.r.T + t0) * d.r.heads + kh * d.group;
+  const int64_t state = ((b * d.r.heads + kh * d.group) * d.chunks + c) * dk * wide;
+  const int next_row = (int)d.r.heads * wide;
+  Rows<T> orows{(grad_o ? grad_o : reinterpret_cast<const T*>(es)) + token * wide, next_row, live, wide};
+  // the library's own: rows of whole eights, zeros beyond dv
+  Rows<float> srows{states + state, wide, dk, wide}, lrows{dstates + state, wide, dk, wide};
+  Rows<float> xrows{xs + token * wide, next_row, live, wide}, erows{es + token * wide, next_row, live, wide};
+  // A block of columns is fetched while the matrix unit has the one before, the next head's
+  // first during the rest of this one's.
+  constexpr int kAll = DP * (kWide / 4), kQuads = (kAll + kBlock - 1) / kBlock, kValues = kChunk * (kWide / 4);
+  static_assert(kValues <= kBlock, "a quad of X to a lane");
+  int tid = threadIdx.x;
+  f32x4 sq4[kQuads], lq4[kQuads], xq, eq;
+  Raw<T> oraw;
+  const auto load4 = [](const Rows<float>& r, int row, int col) {
+    float w[4];
+    load<4>(r.template place<4>(row, col), w);
+    return f32x4{w[0], w[1], w[2], w[3]};
+  };
+  const auto fetch = [&](int e0) {
+#pragma unroll
+    for (int n = 0; n < kQuads; ++n) {
+      const int at = tid + n * kBlock, row = at / (kWide / 4), col = at % (kWide / 4) * 4;
+      sq4[n] = load4(srows, row, e0 + col);
+      lq4[n] = load4(lrows, row, e0 + col);
+    }
+    const int t = tid / (kWide / 4), col = tid % (kWide / 4) * 4;
+    xq = load4(xrows, t, e0 + col);
+    eq = load4(erows, t, e0 + col);
+    oraw.fetch(orows.template place<8>(w0 + i, e0 + 8 * g));   // this wave's own samples of dO
+  };
+  const auto next_head = [&] {
+    orows.p += wide, xrows.p += wide, erows.p += wide;
+    srows.p += (int64_t)d.chunks * dk * wide, lrows.p += (int64_t)d.chunks * dk * wide;
+  };
+  fetch(0);
   f32x4 dQ[1][NT], dK[1][NT];
   clear(dQ);
   clear(dK);
   for (int hh = 0; hh < d.group; ++hh) {
     const int h = kh * d.group + hh;
     const int64_t bh = b * d.r.heads + h;
-    if (live == 0) {
-      if ((int)threadIdx.x < rows) {
-        const int64_t at = (b * d.r.T + t0 + threadIdx.x) * d.r.heads + h;
-        if (grad_decay) put_gate(d, grad_decay, at, 0.0f);
-        if (grad_beta) put_gate(d, grad_beta, at, 0.0f);
-      }
-      continue;
-    }
     const Squares<T>& sq = squares[bh * d.chunks + c];
     if (threadIdx.x < kChunk) {
       const int t = threadIdx.x;
@@ -353,8 +394,6 @@ __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_ke
       until[t] = sq.gates.until[t];
       dbeta[t] = 0.0f;
     }
-    const float* state = states + (bh * d.chunks + c) * dk * wide;
-    const float* dstate = dstates + (bh * d.chunks + c) * dk * wide;
     f32x4 qs[1][NT], k1[1][NT], k2[1][NT], P[1][NJ], ZU[1][NJ];
     clear(qs);
     clear(k1);
@@ -362,37 +401,7 @@ __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_ke
     clear(P);
     clear(ZU);
     float dot = 0.0f;
-    const int64_t token = (b * d.r.T + t0) * d.r.heads + h;
-    const int next_row = (int)d.r.heads * wide;
-    const Rows<T> orows{(grad_o ? grad_o : reinterpret_cast<const T*>(es)) + token * wide, next_row, live, wide};
-    // the library's own: rows of whole eights, zeros beyond dv
-    const Rows<float> srows{state, wide, dk, wide}, lrows{dstate, wide, dk, wide};
-    const Rows<float> xrows{xs + token * wide, next_row, live, wide}, erows{es + token * wide, next_row, live, wide};
-    // A block of columns is fetched while the matrix unit has the one before.
-    constexpr int kAll = DP * (kWide / 4), kQuads = (kAll + kBlock - 1) / kBlock, kValues = kChunk * (kWide / 4);
-    static_assert(kValues <= kBlock, "a quad of X to a lane");
-    int tid = threadIdx.x;
-    f32x4 sq4[kQuads], lq4[kQuads], xq, eq;
-    Raw<T> oraw;
-    const auto load4 = [](const Rows<float>& r, int row, int col) {
-      float w[4];
-      load<4>(r.template place<4>(row, col), w);
-      return f32x4{w[0], w[1], w[2], w[3]};
-    };
-    const auto fetch = [&](int e0) {
-#pragma unroll
-      for (int n = 0; n < kQuads; ++n) {
-        const int at = tid + n * kBlock, row = at / (kWide / 4), col = at % (kWide / 4) * 4;
-        sq4[n] = load4(srows, row, e0 + col);
-        lq4[n] = load4(lrows, row, e0 + col);
-      }
-      const int t = tid / (kWide / 4), col = tid % (kWide / 4) * 4;
-      xq = load4(xrows, t, e0 + col);
-      eq = load4(erows, t, e0 + col);
-      oraw.fetch(orows.template place<8>(w0 + i, e0 + 8 * g));   // this wave's own samples of dO
-    };
     __syncthreads();
-    fetch(0);
 #pragma unroll 1
     for (int e0 = 0; e0 < dv; e0 += kWide) {
       renew(tid);
@@ -423,7 +432,12 @@ __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_ke
       }
       oraw.keep(grad_o && orows.in(w0 + i, e0 + 8 * g));
       const Frag<NI> of[1] = {oraw.frag()};
-      fetch(min(e0 + kWide, (dv - 1) / kWide * kWide));
+      int next = e0 + kWide;
+      if (next >= dv) {   // the last head's is not used
+        next = 0;
+        if (hh + 1 < d.group) next_head();
+      }
+      fetch(next);
       __syncthreads();
       const int mine = (w0 + i) * kWidePitch + 8 * g;
       const Frag<NP> uf[1] = {plane_frag<NP>(U + mine, Room::kSamples)}, zf[1] = {plane_frag<NP>(Z + mine, Room::kSamples)};
@@ -441,19 +455,6 @@ __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_ke
       mma(P, of, tf);
       mma(ZU, zf, tf);
       __syncthreads();
-    }
-    // the products that M and P were made of
-    f32x4 kk[1][NJ], qk[1][NJ];
-    clear(kk);
-    clear(qk);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const Frag<NI> ak[1] = {own_frag(own.k, tile, s)}, aq[1] = {own_frag(own.q, tile, s)};
-      Frag<NI> bk[NJ];
-#pragma unroll
-      for (int n = 0; n < NJ; ++n) bk[n] = own_frag(own.k, j0 + n, s);
-      mma(kk, ak, bk);
-      mma(qk, aq, bk);
     }
     // keys and queries as the sums lie
     f32x4 qv[1][NT], kv[1][NT];
@@ -483,6 +484,19 @@ __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_ke
       from = over16(from);
       to = over16(to);
       if (i == 0) before[group][row] = from, after[group][row] = to;
+    }
+    // the products that M and P were made of
+    f32x4 kk[1][NJ], qk[1][NJ];
+    clear(kk);
+    clear(qk);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const Frag<NI> ak[1] = {own_frag(own.k, tile, s)}, aq[1] = {own_frag(own.q, tile, s)};
+      Frag<NI> bk[NJ];
+#pragma unroll
+      for (int n = 0; n < NJ; ++n) bk[n] = own_frag(own.k, j0 + n, s);
+      mma(kk, ak, bk);
+      mma(qk, aq, bk);
     }
     dot = over16(dot);
     dot += __shfl_xor(dot, 16);
