@@ -226,6 +226,13 @@ __device__ __forceinline__ float over16(float v) {
   v = over8(v);
   return v + lane_at<0x140>(v);   // mirrored in sixteens
 }
+// The sum over the lanes 16, 32 and 48 on.
+__device__ __forceinline__ float over_rows(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
 // The sum over the lanes before.
 __device__ __forceinline__ float lanes_before(float v) {
   v += lane_at<0x111>(v);   // from 1, 2, 4 and 8 lanes below in the sixteen

@@ -157,8 +157,7 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, Squ
       float sum = a[0] * t[0];   // rows that are not there yet are 0
 #pragma unroll
       for (int e = 1; e < 4; ++e) sum = fmaf(a[e], t[e], sum);
-      sum += __shfl_xor(sum, 16);
-      sum += __shfl_xor(sum, 32);
+      sum = over_rows(sum);
       const float v = (i == r ? 1.0f : 0.0f) - sum;
       t[r & 3] = g == r >> 2 ? v : t[r & 3];
     }
@@ -582,13 +581,10 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_steps_kernel(Delta d, T* o,
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      sk[e] += __shfl_xor(sk[e], 16);
-      sk[e] += __shfl_xor(sk[e], 32);
-      sq[e] += __shfl_xor(sq[e], 16);
-      sq[e] += __shfl_xor(sq[e], 32);
+      sk[e] = over_rows(sk[e]);
+      sq[e] = over_rows(sq[e]);
     }
-    kq += __shfl_xor(kq, 16);
-    kq += __shfl_xor(kq, 32);
+    kq = over_rows(kq);
     __shared__ float kqs[4];
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) < 16) {

@@ -498,9 +498,7 @@ __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_ke
       mma(kk, ak, bk);
       mma(qk, aq, bk);
     }
-    dot = over16(dot);
-    dot += __shfl_xor(dot, 16);
-    dot += __shfl_xor(dot, 32);
+    dot = over_rows(over16(dot));
     if (lane == 0) whole[wave] = dot;
 #pragma unroll
     for (int n = 0; n < NJ; ++n) {
