@@ -643,8 +643,10 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_pad_kernel(const T* from, i
   }
 }
 
-// Sample by sample where there are so few of them.
-bool steps(const cpab_delta_rule& r, bool keep) { return r.T <= (keep ? 0 : 16); }
+// Sample by sample where there are so few of them (64 rows of 4 heads of 64 in bfloat16: 4
+// samples take 11 us and 21 in a chunk, 8 17 and 21, 16 28 and 21; 16 heads of 128: 8 50 and 82,
+// 16 85 and 85), but never where something is kept: the backward goes by chunks.
+bool steps(const cpab_delta_rule& r, bool keep) { return r.T <= (keep ? 0 : 8); }
 
 }  // namespace
 
@@ -705,10 +707,16 @@ hipError_t launch_delta_join(const Delta& d, const Cut& cut, bool forward, const
   return hipGetLastError();
 }
 
+// Two workgroups to a compute unit between them, in segments of at least 8 chunks, or 4 where
+// a head is short: the segments' ends and their joining are then paid for.  One head of 128 of
+// four in bfloat16, forward and with the backward, us: 8192 samples 364 and 978 in one piece,
+// 117 and 332 in 16 segments, 153 and 406 in 32; 1024 64 and 182 in one, 54 and 154 in 4; 131072
+// 5626 and 16203, 1020 and 3460 in 32 (16: 1023 and 3584).  Fewer than 4 segments cost more than they give: 64
+// rows of 4096 samples, 2 heads of 64, 320 and 1206 in one, 403 and 1508 in 2.
 Cut cut_of(const Delta& d) {
   const int64_t columns = d.r.B * d.r.heads * ((d.r.dv + 31) / 32);
   const int64_t want = columns > 0 ? 2 * compute_units() / columns : 1;
-  const int segs = (int)std::min<int64_t>(want, d.chunks / 4);
+  const int segs = (int)std::min<int64_t>(want, std::max(d.chunks / 8, std::min(d.chunks / 4, 8)));
   if (segs < 4) return Cut{1, std::max(d.chunks, 1)};
   const int each = (d.chunks + segs - 1) / segs;
   return Cut{(d.chunks + each - 1) / each, each};

@@ -17,6 +17,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "cpab_launch.hpp"
@@ -56,9 +57,10 @@ struct Batch {
   uint32_t first[kMatrices + 1];   // workgroups before each matrix's
 };
 
-// How a matrix' products go: in one workgroup that keeps it in LDS where it fits (0), else in
-// tiles of 64, 128 or 256, the longer the shorter side, since padding it to whole tiles
-// costs less then.
+// How a matrix' products go: in one workgroup that keeps it in LDS where it fits (0: 16
+// matrices of 64 x 64 take 21 us a step and 93 in tiles, of 256 x 64 58 and 113), else in
+// tiles of up to 64, 128 or 256, to which the matrix is padded: the longer its shorter side,
+// the less that costs.
 __host__ __device__ __forceinline__ int tile_of(int64_t rows, int64_t cols) {
   const int64_t m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
   return m <= kWholeSide && n <= kWholeLong ? 0 : m > 1024 ? 256 : m > 256 ? 128 : 64;
@@ -557,7 +559,22 @@ int64_t muon_workspace(int64_t n, const cpab_muon_matrix* matrices) {
 
 namespace {
 
-// The step of one batch, whose products go in tiles of TILE.
+// The time of a product in so many tiles of a side, in units of what a tile of 128 takes with a
+// compute unit's other one beside it.  A unit has four of 64, two of 128 or one of 256 at a
+// time; one alone waits for memory at each step (128: 1.4), and the larger tile reads less for
+// what it computes.  Measured, us a step in 64, 128 and 256: 8 of 512 x 512 262, 380, 711; 8 of
+// 1024 x 1024 1018, 977, 1305; 40 of them 4841, 4140, 4388; 2 of 6144 x 2048 4489, 3601, 4692.
+// Four layers of 6144 x 2048 and 2048 x 2048, X's step alone: 967 in 128 and 887 in 256, the
+// polynomial 302 and 372, where 256 leaves most units without a tile in the second round.
+double cost_of(int side, double tiles) {
+  const int64_t each = (int64_t)std::ceil(tiles / compute_units());   // of a unit
+  const double some[4] = {0.0, 0.6, 0.8, 1.1};
+  return side == 64    ? (double)(each / 4) * 1.33 + some[each % 4]
+         : side == 128 ? (double)(each / 2) * 2.0 + (double)(each % 2) * 1.4
+                       : (double)each * 3.3;
+}
+
+// The step of one batch, of matrices padded to tiles of TILE.
 template <typename T, int TILE>
 hipError_t step(Batch& batch, int count, const Muon& s, char* room, hipStream_t st) {
   const auto tiles = [&](auto each) {   // of all matrices
@@ -578,10 +595,34 @@ hipError_t step(Batch& batch, int count, const Muon& s, char* room, hipStream_t 
     muon_product_kernel<WHAT, T, SIDE><<<blocks, lanes_of(SIDE), kRoom, st>>>(batch, count, c, room);
     return hipGetLastError();
   };
-  typedef std::integral_constant<int, TILE> Side;
-  typedef std::integral_constant<int, TILE == 256 ? 128 : TILE> Half;
-  const auto half = [&](int side) {   // the tiles on and above the diagonal
-    return tiles([side](const Matrix&, const Places& p) { return p.m / side * (p.m / side + 1) / 2; });
+  // A product in the tiles that should take the least time for all matrices together.
+  const auto best = [&](auto what, const Coefficients& c) {
+    constexpr Product WHAT = decltype(what)::value;
+    const auto each = [](int side, const Places& p) {
+      const int64_t down = p.m / side;   // of a symmetric one the tiles on and above the diagonal
+      return WHAT == kGram || WHAT == kPolynomial ? down * (down + 1) / 2 : down * (p.n / side);
+    };
+    const auto cost = [&](int side) {
+      if (side > TILE) return HUGE_VAL;
+      double sum = 0.0, longest = 1.0;   // tiles of the longest summed index
+      for (int i = 0; i < count; ++i) {
+        const Places p = places(batch.m[i].rows, batch.m[i].cols);
+        const double k = (double)(WHAT == kGram ? p.n : p.m);
+        sum += k * (double)each(side, p);
+        longest = std::max(longest, k);
+      }
+      return cost_of(side, sum / longest);
+    };
+    const double by64 = cost(64), by128 = cost(128), by256 = cost(256);
+    const auto go = [&](auto side) {
+      constexpr int SIDE = decltype(side)::value;
+      return product(what, side, tiles([&](const Matrix&, const Places& p) { return each(SIDE, p); }), c);
+    };
+    if constexpr (TILE >= 256)
+      if (by256 <= by128 && by256 <= by64) return go(std::integral_constant<int, 256>());
+    if constexpr (TILE >= 128)
+      if (by128 <= by64) return go(std::integral_constant<int, 128>());
+    return go(std::integral_constant<int, 64>());
   };
   const Momentum m{s.momentum, s.rest, s.eps, s.nesterov};
   uint32_t blocks = tiles([](const Matrix& a, const Places&) { return ((int64_t)a.rows * a.cols + kSpan - 1) / kSpan; });
@@ -591,19 +632,11 @@ hipError_t step(Batch& batch, int count, const Muon& s, char* room, hipStream_t 
   hipError_t e = hipGetLastError();
   for (int i = 0; i < s.steps && e == hipSuccess; ++i) {
     const Coefficients c{s.c0, s.c1, s.c2, s.decay, i & 1};
-    e = product(std::integral_constant<Product, kGram>(), Side(), half(TILE), c);
+    e = best(std::integral_constant<Product, kGram>(), c);
+    if (e == hipSuccess) e = best(std::integral_constant<Product, kPolynomial>(), c);
     if (e != hipSuccess) break;
-    // The polynomial's products are alike: tiles of 128, of which a compute unit has two at a
-    // time, where they fill its rounds better.
-    blocks = half(TILE);
-    if (TILE == 256 && (half(128) + 511) / 512 * 2 < (blocks + 255) / 256 * 4)
-      e = product(std::integral_constant<Product, kPolynomial>(), Half(), half(128), c);
-    else
-      e = product(std::integral_constant<Product, kPolynomial>(), Side(), half(TILE), c);
-    if (e != hipSuccess) break;
-    blocks = tiles([](const Matrix&, const Places& p) { return p.m / TILE * (p.n / TILE); });
-    e = i + 1 < s.steps ? product(std::integral_constant<Product, kStep>(), Side(), blocks, c)
-                        : product(std::integral_constant<Product, kLast>(), Side(), blocks, c);
+    e = i + 1 < s.steps ? best(std::integral_constant<Product, kStep>(), c)
+                        : best(std::integral_constant<Product, kLast>(), c);
   }
   return e;
 }
