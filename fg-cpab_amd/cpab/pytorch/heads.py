@@ -18,7 +18,10 @@ def gated_delta_rule(q, k, v, decay, beta, h0=None, lengths=None, scale=None):
         S' = exp(decay_t) S_{t-1},   S_t = S' + beta_t k_t (v_t - S'^T k_t)^T,
         o_t = scale S_t^T q_t
 
-    The state is held in 32 bits, and so is what passes between samples.
+    The state is held in 32 bits, and so is what passes between samples.  What is not
+    finite in a sample reaches its row's head from the 64 samples around it on (the formula's
+    own reach is from the sample on), and, as a head's key or query, the heads that share
+    it; no other row and no other head.
 
     Arguments:
         q, k: [B, T, key heads, dk] of v's type, dk from 1 to 128.  Keys longer than 1 can

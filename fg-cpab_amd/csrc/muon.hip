@@ -5,15 +5,22 @@
 // then some times  A = X X^T,  B = c1 A + c2 A A,  X = c0 X + B X,  at last
 // p = p (1 - lr wd) - rate X.  X is taken with its shorter side first.
 //
-// Bound by the matrix unit.  Its 32-bit products run at a fourteenth of the 16-bit ones'
-// rate, so X, A and B are held as two 16-bit floats, the nearest to 2^10 times the value and
-// 2^11 times what is left, 22 bits together, and a product is three: hi hi in one sum and
-// hi lo + lo hi in another, 2^-11 of which joins it at the end; lo lo, 2^-22 of the whole,
-// is left out.  2^10: what is below 2^-24 of 1 falls under the normal 16-bit floats, what is
-// above 63 over them; X's values stay near 1 and the polynomial's near 5.
+// Bound by the matrix unit.  Its 32-bit products run at a seventh of the 16-bit ones' rate in a
+// large library product here (154 and 1113 TFLOP/s), so X, A and B are held as two 16-bit
+// floats, the nearest to 2^10 times the value and to what is left, and a product is three, hi
+// hi, hi lo and lo hi, in one sum of 32 bits; lo lo, 2^-22 of the whole, is left out.  2^10:
+// the second float's last place is 2^-34 of 1, which gives 22 bits to what is above 2^-12 and
+// 2^-35 to what is below; what is above 63 has none, but X's values stay near 1 and the
+// polynomial's near 5.  (The second float times 2^11, with a sum of its own, would hold
+// 22 bits to 2^-24, for twice the sums' registers: tiles of 128 had one workgroup less, and the
+// error against 64 bits was the same, 5e-8 of the whole and 6e-8.)
 // All products are of rows with rows, the summed index contiguous, since A and B are their
 // own transposes and X is kept both ways; of A and B the half above the diagonal is computed
 // and written twice.  Each step is one launch for all matrices together.
+//
+// Measured: four layers of 6144 x 2048 and 2048 x 2048 in 32 bits 9.0 ms a step, of which the
+// products' 2.4 TFLOP, threefold, would take 6.5 at the library's rate: X's step runs at 930
+// TFLOP/s (3 x 275 GFLOP in 887 us), X X^T at 780, the polynomial at 710; the momentum 133 us (6.0 TB/s) and X's making 257 (4.2 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -244,7 +251,9 @@ __device__ __forceinline__ f32x4 mma(const f16x8 (&l)[2], const f16x8 (&r)[2], f
 
 // The whole step of a matrix of up to 64 x 256: X, its transpose and A, later B, lie in LDS;
 // a wave has 16 of X's columns in its registers, in 32 bits, and one 16 x 16 tile of A and B.
-// One launch instead of two and three to an iteration, which is what small matrices wait for.
+// One launch instead of two and three to an iteration, which is what small matrices wait for:
+// 17 matrices of 192 x 64, 64 x 64 and 49 x 64 take 45 us, in tiles 103.  What is left is LDS: a
+// compute unit alone writes X twice and reads it for A some 20,000 cycles an iteration.
 template <typename T>
 __global__ __launch_bounds__(kWholeLanes) void muon_whole_kernel(Batch batch, Momentum s, Coefficients c, int steps) {
   constexpr int kP = kWholeSide + 8;   // pitch of A and of X's transpose
@@ -374,9 +383,11 @@ __global__ __launch_bounds__(kWholeLanes) void muon_whole_kernel(Batch batch, Mo
 
 enum Product { kGram, kPolynomial, kStep, kLast };
 
-// One tile of a product: a wave has a quarter of it, in two sums.  32 of the summed index lie
-// in LDS twice, as the matrix unit has the one and memory brings the other; rows of 64 bytes
-// begin 20 banks apart, so that a wave's wide reads meet no bank twice.
+// One tile of a product: a wave has a quarter of it, of a tile of 256 an eighth.  32 of the
+// summed index lie in LDS twice, as the matrix unit has the one and memory brings the other;
+// rows of 64 bytes begin 20 banks apart, so that a wave's wide reads meet no bank twice.  LDS
+// brings a wave of 128 x 64 what it multiplies in half the matrix unit's time, one of 64 x 64
+// in two thirds.  (Rows of K values apart instead of pieces of 32: X's step 1068 us for 886.)
 template <Product WHAT, typename T, int TILE>
 __global__ __launch_bounds__((lanes_of(TILE)), 2) void muon_product_kernel(Batch batch, int count, Coefficients c, char* room) {
   constexpr int kStepK = 32, kPitch = kStepK + 8, kThreads = lanes_of(TILE), kRows = kThreads / 4;
