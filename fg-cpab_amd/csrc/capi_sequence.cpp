@@ -99,16 +99,21 @@ class Once {
   }
   bool room() const { return mask_ < kFew || many_; }
   bool add(const void* p) {   // false: it came before
+    uintptr_t& at = place(p);
+    if (at) return false;
+    at = reinterpret_cast<uintptr_t>(p);
+    return true;
+  }
+  bool has(const void* p) { return place(p) != 0; }
+
+ private:
+  uintptr_t& place(const void* p) {   // its own, or where it would go
     const uintptr_t key = reinterpret_cast<uintptr_t>(p);
     uintptr_t* table = many_ ? many_.get() : few_;
     int64_t at = (int64_t)(key * 0x9E3779B97F4A7C15u >> 32) & mask_;
-    for (; table[at]; at = (at + 1) & mask_)
-      if (table[at] == key) return false;
-    table[at] = key;
-    return true;
+    while (table[at] && table[at] != key) at = (at + 1) & mask_;
+    return table[at];
   }
-
- private:
   static constexpr int64_t kFew = 1024;
   int64_t mask_ = 63;
   uintptr_t few_[kFew] = {};
@@ -370,6 +375,9 @@ int cpab_muon_step(int dtype, int64_t n_matrices, const cpab_muon_matrix* matric
                     (long long)k);
   }
   if (!any) return CPAB_OK;
+  for (int64_t k = 0; k < n_matrices; ++k)
+    if (matrices[k].rows > 0 && matrices[k].cols > 0 && once.has(matrices[k].grad))
+      return fail(CPAB_ERR_INVALID, "the gradient of matrix %lld is an array that the step writes", (long long)k);
   CPAB_REQUIRE(rates);
   for (int64_t k = 0; k < n_matrices; ++k)
     if (!std::isfinite(rates[k])) return fail(CPAB_ERR_INVALID, "rates must be finite");

@@ -557,7 +557,8 @@ int cpab_delta_rule_backward(const cpab_delta_rule* rule, const float* kept, con
 
 /* One matrix of a Muon step: rows x cols values, contiguous, of the parameter and its
  * gradient (of the step's dtype) and of the momentum (float32); master as for AdamW.  The
- * arrays that a step writes do not overlap; one that comes twice is refused. */
+ * arrays that a step writes do not overlap each other nor a gradient; one that comes twice
+ * is refused. */
 typedef struct {
   void* param;
   const void* grad;

@@ -517,3 +517,24 @@ def test_no_gradient_comes(cuda):
     o, h = cpab.gated_delta_rule(*leaves)
     (Nothing.apply(o) + Nothing.apply(h) + leaves[0].sum()).backward()
     assert leaves[1].grad is None and torch.equal(leaves[0].grad, torch.ones_like(leaves[0]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T", [7, 8, 9])
+def test_on_both_sides_of_sample_by_sample(cuda, dtype, T):
+    compare(cuda, dtype, 3, T, 4, 2, 40, 72, seed=31)
+
+
+@pytest.mark.parametrize("dtype,gates", [(F32, F32), (BF16, BF16), (BF16, F32)])
+@pytest.mark.parametrize("dk,dv", [(20, 70), (64, 96), (128, 130)])
+def test_many_heads_to_a_key(cuda, dtype, gates, dk, dv):
+    # three heads of several blocks of columns to each key, rows that end within a chunk or have none
+    args, n = make(cuda, dtype, 4, 140, 6, 2, dk, dv, gates=gates, lengths=[140, 0, 64, 77], seed=33)
+    compare(cuda, dtype, 4, 140, 6, 2, dk, dv, given=(args, n))
+
+
+@pytest.mark.parametrize("T", [1000, 1023, 1025, 2100])
+def test_segments(cuda, T):
+    # where a head's axis begins to be cut, in four to eight pieces
+    compare(cuda, F32, 1, T, 2, 1, 32, 40, seed=34)
+    compare(cuda, BF16, 2, T, 1, 1, 64, 64, seed=35)

@@ -188,6 +188,8 @@ def _check_muon():
                     (dict(momentum=P), "comes twice")):
         _refused(step([m]), word)
     _refused(step([{}, {}]), "comes twice")
+    _refused(step([dict(grad=P)]), "the gradient of matrix 0 is an array")
+    _refused(step([dict(param=1 << 12, momentum=1 << 13), dict(grad=1 << 13)]), "the gradient of matrix 1 is an array")
     _refused(lib.cpab_muon_step(0, 1, None, None, 0.1, 0.0, 0.9, 1, coefficients, 1e-7, 5, 256, 1 << 50, None), "matrices")
     assert step([dict(rows=0), dict(cols=0)], ws=None, room=0) == 0 and step([], n=0) == 0
     size = lib.cpab_muon_workspace_size
