@@ -65,7 +65,7 @@ struct Batch {
 };
 
 // How a matrix' products go: in one workgroup that keeps it in LDS where it fits (0: 16
-// matrices of 64 x 64 take 21 us a step and 93 in tiles, of 256 x 64 58 and 113), else in
+// matrices of 64 x 64 take 21 us a step and 93 in tiles, of 256 x 64 38 and 113), else in
 // tiles of up to 64, 128 or 256, to which the matrix is padded: the longer its shorter side,
 // the less that costs.
 __host__ __device__ __forceinline__ int tile_of(int64_t rows, int64_t cols) {
@@ -233,13 +233,15 @@ struct Coefficients {
   int from;   // which of the two X
 };
 
+template <typename T>
+__device__ __forceinline__ void put(const Matrix& t, int64_t at, float w) {
+  static_cast<T*>(t.param)[at] = from_float<T>(w);
+  if (t.master) t.master[at] = w;
+}
 // The parameter's move, from the master weight where there is one.
 template <typename T>
 __device__ __forceinline__ void move(const Matrix& t, int64_t at, float decay, float v) {
-  T* to = static_cast<T*>(t.param) + at;
-  const float w = (t.master ? t.master[at] : to_float(*to)) * decay - t.rate * v;
-  *to = from_float<T>(w);
-  if (t.master) t.master[at] = w;
+  put<T>(t, at, (t.master ? t.master[at] : to_float(static_cast<const T*>(t.param)[at])) * decay - t.rate * v);
 }
 
 // As a sum of three products of two 16-bit floats each.
@@ -252,8 +254,9 @@ __device__ __forceinline__ f32x4 mma(const f16x8 (&l)[2], const f16x8 (&r)[2], f
 // The whole step of a matrix of up to 64 x 256: X, its transpose and A, later B, lie in LDS;
 // a wave has 16 of X's columns in its registers, in 32 bits, and one 16 x 16 tile of A and B.
 // One launch instead of two and three to an iteration, which is what small matrices wait for:
-// 17 matrices of 192 x 64, 64 x 64 and 49 x 64 take 45 us, in tiles 103.  What is left is LDS: a
-// compute unit alone writes X twice and reads it for A some 20,000 cycles an iteration.
+// 17 matrices of 192 x 64, 64 x 64 and 49 x 64 take 31 us, in tiles 103.  What is left is 10 us
+// around the iterations and 4.2 for each of them at 192 x 64, 2.5 at 64 x 64: a compute unit alone
+// writes X twice to LDS and reads it for A, and four barriers stand between.
 template <typename T>
 __global__ __launch_bounds__(kWholeLanes) void muon_whole_kernel(Batch batch, Momentum s, Coefficients c, int steps) {
   constexpr int kP = kWholeSide + 8;   // pitch of A and of X's transpose
@@ -268,26 +271,45 @@ __global__ __launch_bounds__(kWholeLanes) void muon_whole_kernel(Batch batch, Mo
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, g = lane >> 4, col = 16 * wave + i;
   const bool busy = 16 * wave < across;
-  f32x4 own[4] = {};   // rows 16 k + 4 g .. of column col
+  // Memory's values in its own order, through LDS in X's: of a matrix whose longer side comes
+  // first a lane's values else lie 16 rows apart (45 us for 33).
+  constexpr int kEach = kWholeSide * kWholeLong / kWholeLanes, kTurn = kWholeSide + 1;
+  float* const stage = reinterpret_cast<float*>(lds);   // [n][kTurn]
+  const int all = m * n, short_side = wide ? n : m;     // a row of the parameter
+  struct Turned {   // of this lane's values, one after another
+    int r, c, down, right, across;
+    bool wide;
+    __device__ int next() {
+      const int at = wide ? c * kTurn + r : r * kTurn + c;
+      r += down, c += right;
+      if (c >= across) c -= across, ++r;
+      return at;
+    }
+  };
+  const auto turned = [&](int tid) {
+    const int r = tid / short_side;
+    return Turned{r, tid - r * short_side, kWholeLanes / short_side, kWholeLanes % short_side, short_side, wide};
+  };
   double sum = 0.0;
+  {
+    float grad[kEach], mom[kEach];
+    Turned to = turned(threadIdx.x);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    float grad[4], mom[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {   // the first value, unused, in place of those outside
-      const int row = 16 * k + 4 * g + e;
-      const uint32_t at = row < m && col < n ? wide ? row * n + col : col * m + row : 0;
-      grad[e] = to_float(static_cast<const T*>(t.grad)[at]);
-      mom[e] = t.momentum[at];
+    for (int k = 0; k < kEach; ++k) {
+      const int at = min(k * kWholeLanes + (int)threadIdx.x, all - 1);
+      grad[k] = to_float(static_cast<const T*>(t.grad)[at]);
+      mom[k] = t.momentum[at];
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int row = 16 * k + 4 * g + e;
-      const bool in = row < m && col < n;
-      mom[e] = fmaf(s.mu, mom[e], s.rest * grad[e]);
-      if (in) t.momentum[wide ? row * n + col : col * m + row] = mom[e];
-      own[k][e] = in ? update(s, mom[e], grad[e]) : 0.0f;
-      sum = fma((double)own[k][e], (double)own[k][e], sum);
+    for (int k = 0; k < kEach; ++k) {
+      const int at = k * kWholeLanes + (int)threadIdx.x;
+      if (at < all) {
+        mom[k] = fmaf(s.mu, mom[k], s.rest * grad[k]);
+        t.momentum[at] = mom[k];
+        const float u = update(s, mom[k], grad[k]);
+        sum = fma((double)u, (double)u, sum);
+        stage[to.next()] = u;
+      }
     }
   }
   for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
@@ -297,8 +319,15 @@ __global__ __launch_bounds__(kWholeLanes) void muon_whole_kernel(Batch batch, Mo
   for (int k = 0; k < kWholeLanes / 64; ++k) sum += parts[k];
   const double norm = sqrt(sum);
   const float by = (float)(1.0 / (norm < (double)s.eps ? (double)s.eps : norm));
+  f32x4 own[4];   // rows 16 k + 4 g .. of column col
 #pragma unroll
-  for (int k = 0; k < 4; ++k) own[k] *= by;
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int row = 16 * k + 4 * g + e;
+      own[k][e] = row < m && col < n ? stage[col * kTurn + row] * by : 0.0f;
+    }
+  __syncthreads();
   const auto frag = [&](f16x8 (&to)[2], const f16* from, int plane) {
     to[0] = *reinterpret_cast<const f16x8*>(from);
     to[1] = *reinterpret_cast<const f16x8*>(from + plane);
@@ -370,15 +399,29 @@ __global__ __launch_bounds__(kWholeLanes) void muon_whole_kernel(Batch batch, Mo
     }
     if (step + 1 == steps) break;
   }
-  int again = g;   // not the start's addresses, kept in registers all along
-  asm volatile("" : "+v"(again));
+  __syncthreads();
 #pragma unroll
   for (int k = 0; k < 4; ++k)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int row = 16 * k + 4 * again + e;
-      if (row < m && col < n) move<T>(t, (uint32_t)(wide ? row * n + col : col * m + row), c.decay, own[k][e]);
+      const int row = 16 * k + 4 * g + e;
+      if (row < m && col < n) stage[col * kTurn + row] = own[k][e];
     }
+  __syncthreads();
+  int tid = threadIdx.x;   // the places again, which else keep their registers all along
+  asm volatile("" : "+v"(tid));
+  float w[kEach];
+  Turned from = turned(tid);
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int at = min(k * kWholeLanes + tid, all - 1);
+    w[k] = (t.master ? t.master[at] : to_float(static_cast<const T*>(t.param)[at]));
+  }
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int at = k * kWholeLanes + tid;
+    if (at < all) put<T>(t, at, w[k] * c.decay - t.rate * stage[from.next()]);
+  }
 }
 
 enum Product { kGram, kPolynomial, kStep, kLast };
