@@ -100,11 +100,13 @@ int check_delta_sizes(const cpab_delta_rule* rule) {
   if (r.heads > 0 && (r.key_heads < 1 || r.heads % r.key_heads != 0))
     return fail(CPAB_ERR_INVALID, "heads must be a multiple of key_heads, got %lld and %lld",
                 (long long)r.heads, (long long)r.key_heads);
-  // a launch's workgroups: a chunk or 32 columns of a head each
-  const double heads = (double)r.B * (double)r.heads, blocks = (double)kMaxCount / 256;
+  // a launch's workgroups: a chunk, up to 1024 lanes, or 32 columns of a head, 256; the lanes
+  // are counted in 32 bits
+  const double heads = (double)r.B * (double)r.heads, blocks = (double)kMaxCount / 256,
+               chunks = (double)(kMaxCount / 512);
   if (r.heads * (r.dv + 8) > CPAB_DELTA_MOST_STRIDE || r.key_heads * (r.dk + 8) > CPAB_DELTA_MOST_STRIDE ||
       r.heads > kMaxHeads || r.B > kMaxCount || r.T > kMaxCount - 64 || r.dv > kMaxCount / 64 ||
-      heads * ((double)r.T / 64 + 1) > blocks || heads * ((double)r.dv / 32 + 1) > blocks ||
+      heads * ((double)r.T / 64 + 1) > chunks || heads * ((double)r.dv / 32 + 1) > blocks ||
       heads * (double)(r.T + 64) * (double)(r.dv + r.dk) >= (double)kMaxValues ||
       heads * ((double)r.T / 64 + 2) * (double)r.dk * (double)r.dv >= (double)kMaxValues)
     return fail(CPAB_ERR_INVALID, "delta rule of %lld x %lld x %lld heads of %lld x %lld is too large",

@@ -153,6 +153,10 @@ def _check_delta_rule():
         _refused(call(T=100, ws=None, n=need), "workspace")
         _refused(call(T=100, ws=72, n=need), "aligned")
     assert lib.cpab_delta_rule_workspace_size(delta_rule(dk=200), 0, 0) == 0
+    # 2^22 chunks of up to 1024 lanes would pass 2^32 lanes
+    one = dict(heads=1, key_heads=1, B=1 << 16)
+    assert lib.cpab_delta_rule_workspace_size(delta_rule(T=62 * 64, **one), 1, 1) > 0
+    _refused(forward(T=63 * 64, **one), "too large")
     assert lib.cpab_delta_rule_kept(delta_rule(T=100)) > 0 and lib.cpab_delta_rule_kept(delta_rule(B=0)) == 0
     assert lib.cpab_delta_rule_kept(None) == 0
     assert forward(B=0) == 0 and forward(heads=0, key_heads=0) == 0 and backward(B=0) == 0
