@@ -622,7 +622,7 @@ namespace {
 // polynomial 302 and 372, where 256 leaves most units without a tile in the second round.
 double cost_of(int side, double tiles) {
   const int64_t each = (int64_t)std::ceil(tiles / compute_units());   // of a unit
-  const double some[4] = {0.0, 0.6, 0.8, 1.1};
+  const double some[4] = {0.0, 0.7, 0.9, 1.15};
   return side == 64    ? (double)(each / 4) * 1.33 + some[each % 4]
          : side == 128 ? (double)(each / 2) * 2.0 + (double)(each % 2) * 1.4
                        : (double)each * 3.3;
