@@ -108,6 +108,7 @@ int check_delta_sizes(const cpab_delta_rule* rule) {
       r.heads > kMaxHeads || r.B > kMaxCount || r.T > kMaxCount - 64 || r.dv > kMaxCount / 64 ||
       heads * ((double)r.T / 64 + 1) > chunks || heads * ((double)r.dv / 32 + 1) > blocks ||
       heads * (double)(r.T + 64) * (double)(r.dv + r.dk) >= (double)kMaxValues ||
+      (double)r.B * (double)r.key_heads * (double)r.T * (double)r.dk >= (double)kMaxValues ||   // also without heads
       heads * ((double)r.T / 64 + 2) * (double)r.dk * (double)r.dv >= (double)kMaxValues)
     return fail(CPAB_ERR_INVALID, "delta rule of %lld x %lld x %lld heads of %lld x %lld is too large",
                 (long long)r.B, (long long)r.T, (long long)r.heads, (long long)r.dk, (long long)r.dv);
@@ -209,11 +210,12 @@ int cpab_delta_rule_backward(const cpab_delta_rule* rule, const float* kept, con
                              int64_t workspace_bytes, void* stream) {
   CPAB_TRY(check_delta(rule));
   const cpab_delta_rule& r = *rule;
-  if (!any_delta(r)) return CPAB_OK;
+  CPAB_ALIGNED(grad_q, size_of(r.dtype)); CPAB_ALIGNED(grad_k, size_of(r.dtype));
+  if (!any_delta(r))   // queries and keys may be there all the same
+    return check_hip(cpab::launch_delta_rule_unread(r, grad_q, grad_k, as_stream(stream)), "cpab_delta_rule_backward");
   if (r.T > 0) CPAB_REQUIRE(kept);
   CPAB_ALIGNED(kept, 4); CPAB_ALIGNED(grad_h, 4); CPAB_ALIGNED(grad_h0, 4);
-  CPAB_ALIGNED(grad_o, size_of(r.dtype)); CPAB_ALIGNED(grad_q, size_of(r.dtype));
-  CPAB_ALIGNED(grad_k, size_of(r.dtype)); CPAB_ALIGNED(grad_v, size_of(r.dtype));
+  CPAB_ALIGNED(grad_o, size_of(r.dtype)); CPAB_ALIGNED(grad_v, size_of(r.dtype));
   CPAB_ALIGNED(grad_decay, size_of(r.gate_dtype)); CPAB_ALIGNED(grad_beta, size_of(r.gate_dtype));
   CPAB_TRY(check_workspace(workspace, workspace_bytes, cpab::delta_rule_workspace(r, true, true)));
   return check_hip(cpab::launch_delta_rule_backward(r, kept, grad_o, grad_h, grad_q, grad_k, grad_v,

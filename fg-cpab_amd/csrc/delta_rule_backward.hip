@@ -592,6 +592,14 @@ __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_ke
     }
 }
 
+template <typename T>
+__global__ __launch_bounds__(kDeltaBlock) void delta_zero_kernel(T* a, T* b, int64_t n) {
+  for (int64_t at = (int64_t)blockIdx.x * kDeltaBlock + threadIdx.x; at < n; at += (int64_t)gridDim.x * kDeltaBlock) {
+    if (a) a[at] = (T)0.0f;
+    if (b) b[at] = (T)0.0f;
+  }
+}
+
 // The backward's workspace (bytes).
 struct Space {
   int64_t squares, keys, dstates, es, adds, starts, padded, grads, all;
@@ -614,6 +622,17 @@ Space space_of(const Delta& d, const Cut& cut) {
 }
 
 }  // namespace
+
+hipError_t launch_delta_rule_unread(const cpab_delta_rule& r, void* grad_q, void* grad_k, hipStream_t st) {
+  const int64_t n = r.B * r.T * r.key_heads * r.dk;
+  if (n == 0 || !(grad_q || grad_k)) return hipSuccess;
+  const unsigned blocks = (unsigned)std::min<int64_t>((n + kDeltaBlock - 1) / kDeltaBlock, 1 << 16);
+  if (r.dtype == CPAB_F32)
+    delta_zero_kernel<float><<<blocks, kDeltaBlock, 0, st>>>((float*)grad_q, (float*)grad_k, n);
+  else
+    delta_zero_kernel<bf16><<<blocks, kDeltaBlock, 0, st>>>((bf16*)grad_q, (bf16*)grad_k, n);
+  return hipGetLastError();
+}
 
 int64_t delta_backward_workspace(const Delta& d) { return space_of(d, cut_of(d)).all; }
 

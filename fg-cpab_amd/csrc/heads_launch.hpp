@@ -28,5 +28,7 @@ hipError_t launch_delta_rule_backward(const cpab_delta_rule& r, const float* kep
                                       const float* grad_h, void* grad_q, void* grad_k, void* grad_v,
                                       void* grad_decay, void* grad_beta, float* grad_h0,
                                       void* workspace, hipStream_t s);
+// The gradients of queries and keys that no head of values reads.
+hipError_t launch_delta_rule_unread(const cpab_delta_rule& r, void* grad_q, void* grad_k, hipStream_t s);
 
 }  // namespace cpab

@@ -549,7 +549,8 @@ int cpab_delta_rule_forward(const cpab_delta_rule* rule, void* o, float* h, floa
 /* Backward of cpab_delta_rule_forward with the same description and what it kept: grad_o
  * [B, T, heads, dv] contiguous and grad_h [B, heads, dk, dv] (either may be NULL: zeros)
  * give the gradients of q, k, v, decay and beta, contiguous and of their types, and of h0
- * (each may be NULL).  Behind a row's end they are 0. */
+ * (each may be NULL).  Behind a row's end they are 0, and so are those of queries and keys
+ * that no head reads (heads of 0). */
 int cpab_delta_rule_backward(const cpab_delta_rule* rule, const float* kept, const void* grad_o,
                              const float* grad_h, void* grad_q, void* grad_k, void* grad_v,
                              void* grad_decay, void* grad_beta, float* grad_h0, void* workspace,
