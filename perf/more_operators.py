@@ -279,8 +279,9 @@ def _own_muon(st):
 
 def _own_qk(st):
     c = st["case"]
-    args = dict(freqs=st.get("freqs"), positions=st.get("positions"), neighbours=c["neighbours"],
-                eps=EPS)
+    args = dict(neighbours=c["neighbours"], eps=EPS)
+    if c["turned"]:   # positions go with frequencies: without these nothing turns
+        args.update(freqs=st["freqs"], positions=st.get("positions"))
     given = [st[k] for k in ("q", "k", "q_weight", "k_weight")]
     if not c["train"]:
         with torch.no_grad():
