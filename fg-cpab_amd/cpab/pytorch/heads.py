@@ -64,9 +64,10 @@ def qk_norm(q, k, q_weight, k_weight, freqs=None, positions=None, neighbours=Fal
         k: [B, T, key heads, width] of q's type
         q_weight, k_weight: [width] float32 or bfloat16, both of one type
         freqs: float32, radians for each unit of position, at most width / 2 of them; no
-            gradient (default: nothing turns)
+            gradient (default, or no values: nothing turns)
         positions: [B, T] (or what broadcasts to it: [T], [B, 1]) int32, int64 or float32,
-            the samples' places or times; no gradient (default: 0 to T - 1)
+            the samples' places or times; no gradient (default: 0 to T - 1).  They are not
+            taken without freqs; freqs of no values leave them unread
         neighbours: bool, pairs are two values side by side, (0, 1), (2, 3), ...; else
             len(freqs) apart, (0, n), (1, n + 1), ...
         eps: float

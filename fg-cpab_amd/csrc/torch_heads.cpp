@@ -128,7 +128,7 @@ variable_list qk_norm(const Tensor& q, const Tensor& k, const Tensor& qw, const 
   }
   Maybe places;
   if (positions.defined()) {
-    if (!freqs.defined()) fail("qk_norm: positions without freqs");
+    if (!freqs.defined()) fail("qk_norm: positions without freqs (give freqs of no values where nothing turns)");
     const auto type = positions.scalar_type();
     const int64_t dims = positions.dim();
     if (positions.device() != q.device() ||
