@@ -18,10 +18,12 @@ def gated_delta_rule(q, k, v, decay, beta, h0=None, lengths=None, scale=None):
         S' = exp(decay_t) S_{t-1},   S_t = S' + beta_t k_t (v_t - S'^T k_t)^T,
         o_t = scale S_t^T q_t
 
-    The state is held in 32 bits, and so is what passes between samples.  What is not
-    finite in a sample reaches its row's head from the 64 samples around it on (the formula's
-    own reach is from the sample on), and, as a head's key or query, the heads that share
-    it; no other row and no other head.
+    The state is held in 32 bits, and so is what passes between samples.  Products take it
+    to 24 bits; those whose result is rounded to bfloat16 to 17 (outputs of bfloat16 inputs,
+    and their gradients where decay and beta are bfloat16 too): within 1e-5 of the whole
+    before that rounding.  What is not finite in a sample reaches its row's head from the 64
+    samples around it on (the formula's own reach is from the sample on), and, as a head's
+    key or query, the heads that share it; no other row and no other head.
 
     Arguments:
         q, k: [B, T, key heads, dk] of v's type, dk from 1 to 128.  Keys longer than 1 can

@@ -185,9 +185,10 @@ def muon_step(params, grads, momenta, lr=1e-3, weight_decay=0.1, momentum=0.95, 
         masters: contiguous float32 matrices in the parameters' shapes that the step moves
             in the parameters' place; each parameter becomes its master's rounding
 
-    X and A are held to 22 bits whatever the parameters' type.  The matrices that it writes
-    do not overlap; one that comes twice is refused.  The rates are part of the launch: a
-    step captured in a graph keeps them.
+    X and A are held to 22 bits whatever the parameters' type, values below 2^-12 to 2^-35
+    (of an update whose values are all of one size, 20 bits at 2^30 of them).  The matrices
+    that it writes do not overlap; one that comes twice is refused.  The rates are part of
+    the launch: a step captured in a graph keeps them.
     """
     assert adjust_lr_fn in (None, "original", "match_rms_adamw"), \
         'adjust_lr_fn must be None, "original" or "match_rms_adamw"'

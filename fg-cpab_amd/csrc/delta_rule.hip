@@ -66,9 +66,10 @@ __device__ __forceinline__ void multiply16(f32x4& acc, const float* A, int pitch
 // M by blocks of 16 rows, all in 32 bits: with T_b = (I + A_bb beta_b)^-1 of the blocks on the
 // diagonal, by rows, a wave each, M_b = T_b (A_b - sum over c < b of A_bc beta_c M_c); a wave
 // has 16 columns.
-// Bound by memory: 8 x 4096 samples of 16 heads of 128 in bfloat16, two to a key, take 230 us,
-// for 0.8 GB (M and P in their three parts each, the keys and queries as the products take
-// them); the backward, which makes all of it again rather than keep it, 265.
+// 8 x 4096 samples of 16 heads of 128 in bfloat16, two to a key, take 198 us for 0.66 GB (0.55
+// of them written: M and P in their parts, the keys and queries as the products take them),
+// 3.4 TB/s; the backward, which makes all of it again rather than keep it, 239 for 0.85.
+// Memory alone would take 130 and 166: the waves wait for two thirds of their cycles.
 template <typename T, int DP, bool BACKWARD>
 __global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, Squares<T>* squares, Keys<T, DP>* keys) {
   constexpr int kPitch = kChunk + 4, NV = Parts<T>::kValue, NI = Parts<T>::kInput;
@@ -203,10 +204,11 @@ __global__ __launch_bounds__(kDeltaBlock) void delta_squares_kernel(Delta d, Squ
 // own, from the unit matrix without values: what the segment adds and what it makes of the
 // state before it.
 // Bound by a chunk's chain of five products, each behind the other's LDS: 8 x 4096 samples of
-// 16 heads of 128 in bfloat16 take 565 us, 8.8 a chunk with two workgroups to a compute unit in
-// turn, of which the matrix unit has a fifth; 0.9 GB of states, X and outputs would take 180.
+// 16 heads of 128 in bfloat16 take 526 us, 8.2 a chunk with two workgroups to a compute unit in
+// turn, of which the matrix unit has a sixth; the 1.45 GB that they read and write would take
+// 285.  Half of the LDS' cycles are counted as conflicts of banks.
 // 32 columns: 64, with the same matrices read half as often but one workgroup to a unit, took
-// longer.  Operands in the order in which lanes take them: from rows of 256 bytes 755 us.
+// longer.  Operands in the order in which lanes take them: from rows of 256 bytes a third more.
 template <typename T, int DP, bool ENDS>
 __global__ __launch_bounds__(kDeltaBlock, 2) void delta_chain_kernel(
     Delta d, const Squares<T>* squares, const Keys<T, DP>* keys, const float* starts, Cut cut, T* o,

@@ -279,11 +279,12 @@ struct PartsRoom {
 // A chunk of a key's head: the gradients of its queries and keys, added up over the heads
 // that share them, and of those heads' gates.  Four waves share the samples, and groups of
 // four the columns.
-// 8 x 4096 samples of 16 heads of 128 in bfloat16 take 763 us: 1.7 GB of states, their
-// gradients, X, E and dO would take 340, and the products after them, where memory only brings
-// the next head's first columns, the rest.  Sixteen waves are one workgroup to a compute unit, and
-// the registers' limit; eight took longer.  Keys and queries in LDS 854 us for 963 from the
-// cache, the next head fetched ahead 763.
+// 8 x 4096 samples of 16 heads of 128 in bfloat16 take 667 us: the 1.65 GB of states, their
+// gradients, X, E, dO and results would take 325, and the products after them, where memory
+// only brings the next head's first columns, the rest; the waves wait for half of their cycles.
+// Sixteen waves are one workgroup to a compute unit, and the registers' limit; eight took
+// longer.  Keys and queries in LDS take 0.89 of the time from the cache, the next head fetched
+// ahead 0.89 of that.
 template <typename T, int DP, int NP>
 __global__ __launch_bounds__((PartsRoom<T, DP, NP>::kBlock)) void delta_parts_kernel(
     Delta d, const Squares<T>* squares, const Keys<T, DP>* keys, const float* states, const float* xs,

@@ -18,9 +18,11 @@
 // own transposes and X is kept both ways; of A and B the half above the diagonal is computed
 // and written twice.  Each step is one launch for all matrices together.
 //
-// Measured: four layers of 6144 x 2048 and 2048 x 2048 in 32 bits 9.0 ms a step, of which the
-// products' 2.4 TFLOP, threefold, would take 6.5 at the library's rate: X's step runs at 930
-// TFLOP/s (3 x 275 GFLOP in 887 us), X X^T at 780, the polynomial at 710; the momentum 133 us (6.0 TB/s) and X's making 257 (4.2 TB/s).
+// Measured: four layers of 6144 x 2048 and 2048 x 2048 and a matrix of 49 x 2048 in 32 bits 9.3 ms
+// a step, of which the products' 2.4 TFLOP, threefold, would take 6.5 at the library's rate:
+// X's step runs at 930 TFLOP/s (3 x 275 GFLOP in 883 us), X X^T at 800, the polynomial at 710;
+// the last step, which moves the parameters, takes 1088 us, the momentum 132 (6.1 TB/s) and X's
+// making 248 (4.4 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -616,8 +618,11 @@ namespace {
 // The time of a product in so many tiles of a side, in units of what a tile of 128 takes with a
 // compute unit's other one beside it.  A unit has four of 64, two of 128 or one of 256 at a
 // time; one alone waits for memory at each step (128: 1.4), and the larger tile reads less for
-// what it computes.  Measured, us a step in 64, 128 and 256: 8 of 512 x 512 262, 380, 711; 8 of
-// 1024 x 1024 1018, 977, 1305; 40 of them 4841, 4140, 4388; 2 of 6144 x 2048 4489, 3601, 4692.
+// what it computes.  Measured, us a step all in 64, 128 or 256, and as chosen: 16 of 257 x 257
+// 250, 340, -, 249; 8 of 512 x 512 269, 385, -, 267; 40 of them 926, 898, -, 896; 8 of 768 x 768
+// 542, 578, -, 543; 8 of 1024 x 1024 1036, 1001, -, 1000; 8 of 1025 x 1025 1689, 1478, 1855, 1414;
+// 8 of 3840 x 1280 4614, 3712, 4340, 3726; 2 of 6144 x 2048 4596, 3710, 5126, 3706; 8 of them
+// 17463, 13785, 13979, 12832.
 // Four layers of 6144 x 2048 and 2048 x 2048, X's step alone: 967 in 128 and 887 in 256, the
 // polynomial 302 and 372, where 256 leaves most units without a tile in the second round.
 double cost_of(int side, double tiles) {

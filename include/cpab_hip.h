@@ -518,10 +518,12 @@ int cpab_qk_norm_backward(const cpab_qk_norm* norm, const void* const* grads,
  * 0, the state stays, and nothing of the inputs is used.  Each `heads / key_heads`
  * neighbouring heads share a query and a key.  q, k: [B, T, key_heads, dk] and v
  * [B, T, heads, dv] of dtype, at strides over B, T and the heads (elements), that over T at
- * most CPAB_DELTA_MOST_STRIDE, their last dimension contiguous; decay, beta: [B, T, heads] of gate_dtype at three strides; o
- * [B, T, heads, dv] contiguous; h [B, heads, dk, dv] float32, the state after each row's
- * last sample.  dk is from 1 to CPAB_DELTA_MOST_KEY, dv at least 1.  decay is the decay's logarithm, at most
- * 0; below -128 it counts as -128, whose exponential is 0.
+ * most CPAB_DELTA_MOST_STRIDE, their last dimension contiguous; decay, beta: [B, T, heads]
+ * of gate_dtype at three strides; o [B, T, heads, dv] contiguous; h [B, heads, dk, dv]
+ * float32, the state after each row's last sample.  dk is from 1 to CPAB_DELTA_MOST_KEY, dv
+ * at least 1.  decay is the decay's logarithm, at most 0; below -128 it counts as -128,
+ * whose exponential is 0.  States are held in 32 bits and multiplied to 24; where dtype is
+ * CPAB_BF16, to 17 for what is rounded to it (outputs; gradients where gate_dtype is too).
  * kept: NULL, or cpab_delta_rule_kept(...) floats that the backward of the same sizes
  * takes.  workspace: cpab_delta_rule_workspace_size(...) bytes, 16-byte aligned.  The
  * description lies in host memory and is read before the call returns. */
@@ -573,8 +575,8 @@ typedef struct {
  *   X = u / max(|u|, eps) (Frobenius; transposed where rows > cols),
  *   ns_steps times: A = X X^T, X = c0 X + (c1 A + c2 A^2) X,
  *   p = p (1 - lr weight_decay) - rates[i] X,
- * rates: one for each matrix.  X and A are held to 22 bits and multiplied in three 16-bit
- * products, which are added in 32; coefficients that bring a value of X or of the
+ * rates: one for each matrix.  X and A are held to 22 bits, what is below 2^-12 to 2^-35,
+ * and multiplied in three 16-bit products, which are added in 32; coefficients that bring a value of X or of the
  * polynomial's factor past 60 give what is not finite.  workspace:
  * cpab_muon_workspace_size(...) bytes, 256-byte aligned. */
 int64_t cpab_muon_workspace_size(int64_t n_matrices, const cpab_muon_matrix* matrices);
